@@ -372,6 +372,93 @@ MA_API int ma_attentionForwardBackward_host(ma_host_pipeline* pl, const ma_bf16*
                                             float* dQ, ma_bf16* dK, ma_bf16* dV, uint32_t B,
                                             ma_stream_t stream);
 
+/* ---- Attention for long contexts: rotary positions, a sliding window with
+ * sinks, grouped K/V heads, padded batches, and a K/V cache.  No counterpart
+ * in the reference, whose attention is causal over one block without
+ * positions (attention.metal:56-299).  Further layouts, with the conventions
+ * above (NKV heads of K and V, a divisor of NH; query head h uses K/V head
+ * h / (NH/NKV)):
+ *   k, v, dK, dV     : bf16 [B][M][NKV*D]
+ *   k_cache, v_cache : bf16 [B][cap][NKV*D]
+ *   lens             : int32 [B], the valid rows of each sequence (the rows
+ *                      before them count, the rest is padding), or NULL: all
+ *   start            : int32 [B], rows a sequence's cache holds already, which
+ *                      is the position of its first new row
+ * lens and start are device arrays, whose values the host cannot check: lens
+ * is clamped to [0, M] and start to [0, cap]. */
+
+/* Rotary positions: columns 0 .. rot-1 of each head turn in pairs, pair i of a
+ * row at position t by the angle t * inv_freq[i], and are multiplied by
+ * `amplitude`; the other columns pass through. */
+typedef struct MaRotary {
+  const double* inv_freq; /* device, [rot/2], radians per position */
+  uint32_t rot;           /* even, 2 .. D */
+  uint32_t interleaved;   /* 0: column i pairs with i + rot/2; 1: 2i with 2i + 1 */
+  uint32_t NKV;           /* heads of k */
+  float amplitude;        /* 1 unless a scaling of the context asks for more */
+} MaRotary;
+
+/* q_out, k_out = q, k turned.  positions: device int32 [B][M], or NULL (a
+ * row's index in its sequence).  In place (q_out == q, k_out == k) is allowed;
+ * other overlaps of an input with an output are refused (MA_ERR_RANGE). */
+MA_API int ma_rotaryForward(const ma_bf16* q, const ma_bf16* k, ma_bf16* q_out, ma_bf16* k_out,
+                            const MaRotary* r, const int32_t* positions, const AttentionParams* p,
+                            uint32_t B, ma_stream_t stream);
+/* The gradient: dQ, dK turned back.  dQ and dQ_out are fp32 (dq_f32 = 1, as
+ * the attention backward accumulates it) or bf16 (0); dK is bf16. */
+MA_API int ma_rotaryBackward(const void* dQ, const ma_bf16* dK, void* dQ_out, ma_bf16* dK_out,
+                             uint32_t dq_f32, const MaRotary* r, const int32_t* positions,
+                             const AttentionParams* p, uint32_t B, ma_stream_t stream);
+/* p->M new rows of q, k and v per sequence, at positions start[b] + i: q_out =
+ * q turned (padding rows: 0), k turned and v as it is stored to rows start[b]
+ * + i of the caches.  Padding rows, and rows that would fall past the cache's
+ * end, are not stored, and the caches' other rows stay as they are. */
+MA_API int ma_rotaryCacheAppend(const ma_bf16* q, const ma_bf16* k, const ma_bf16* v, ma_bf16* q_out,
+                                ma_bf16* k_cache, ma_bf16* v_cache, const int32_t* start,
+                                const int32_t* lens, const MaRotary* r, const AttentionParams* p,
+                                uint32_t B, uint32_t cap, ma_stream_t stream);
+
+/* The mask: query at position t sees key j when j <= t and (t - j < window or
+ * j < sinks).  window >= 1 (any window >= the sequence is plain causal);
+ * sinks may be 0. */
+typedef struct MaWindow {
+  uint32_t NKV;    /* heads of K and V */
+  uint32_t window; /* keys a query sees, itself included */
+  uint32_t sinks;  /* first keys that stay visible */
+} MaWindow;
+
+/* out (bf16 [B][M][N]) and l (fp32 [B][M][NH]) as ma_flashAttentionForward
+ * over the visible keys.  A padding row sees nothing: out = 0, l = -inf.
+ * Whatever the padding rows of q, k and v hold, NaN included, does not reach
+ * the valid rows. */
+MA_API int ma_windowAttentionForward(const ma_bf16* q, const ma_bf16* k, const ma_bf16* v, ma_bf16* out,
+                                     float* l, const int32_t* lens, const MaWindow* w,
+                                     const AttentionParams* p, uint32_t B, ma_stream_t stream);
+/* dQ (fp32 or bf16: dq_f32), dK and dV (bf16) from dO and the forward's out
+ * and l; padding rows get 0.  D = rowsum(dO * out) is formed inside, in fp32.
+ * `workspace` is device memory, 16-byte aligned, of at least the bytes that
+ * ma_windowAttentionBackward_workspace gives; it holds nothing between calls,
+ * and calls that may overlap on the GPU need one each. */
+MA_API int ma_windowAttentionBackward(const ma_bf16* dO, const ma_bf16* out, const float* l, const ma_bf16* q,
+                                      const ma_bf16* k, const ma_bf16* v, void* dQ, ma_bf16* dK, ma_bf16* dV,
+                                      uint32_t dq_f32, const int32_t* lens, const MaWindow* w,
+                                      const AttentionParams* p, uint32_t B, void* workspace,
+                                      uint64_t workspace_bytes, ma_stream_t stream);
+MA_API int ma_windowAttentionBackward_workspace(uint32_t dq_f32, const MaWindow* w, const AttentionParams* p,
+                                                uint32_t B, uint64_t* bytes);
+/* The forward for p->M >= 1 new tokens per sequence over a cache that already
+ * holds their keys and values (ma_rotaryCacheAppend): row i is the query at
+ * position start[b] + i and sees the cache's rows under the mask above.
+ * start[b] + lens[b] must not exceed cap (a query past the cache's end is
+ * computed as though it stood on the last row).  Cache rows that no query
+ * sees may hold anything.  Workspace as for the backward. */
+MA_API int ma_windowAttentionCached(const ma_bf16* q, const ma_bf16* k_cache, const ma_bf16* v_cache,
+                                    ma_bf16* out, float* l, const int32_t* start, const int32_t* lens,
+                                    const MaWindow* w, const AttentionParams* p, uint32_t B, uint32_t cap,
+                                    void* workspace, uint64_t workspace_bytes, ma_stream_t stream);
+MA_API int ma_windowAttentionCached_workspace(const MaWindow* w, const AttentionParams* p, uint32_t B,
+                                              uint32_t cap, uint64_t* bytes);
+
 /* Library version as major*10000 + minor*100 + patch. */
 MA_API int ma_version(void);
 

@@ -34,6 +34,19 @@ class AttentionParams(ctypes.Structure):
                 ("D", ctypes.c_uint32), ("NH", ctypes.c_uint32)]
 
 
+class Rotary(ctypes.Structure):
+    """MaRotary of metalattn.h."""
+
+    _fields_ = [("inv_freq", ctypes.c_void_p), ("rot", ctypes.c_uint32), ("interleaved", ctypes.c_uint32),
+                ("NKV", ctypes.c_uint32), ("amplitude", ctypes.c_float)]
+
+
+class Window(ctypes.Structure):
+    """MaWindow of metalattn.h."""
+
+    _fields_ = [("NKV", ctypes.c_uint32), ("window", ctypes.c_uint32), ("sinks", ctypes.c_uint32)]
+
+
 class MetalAttnError(RuntimeError):
     def __init__(self, code: int, message: str, entry: str):
         self.code = code
@@ -43,7 +56,10 @@ class MetalAttnError(RuntimeError):
 
 _P = ctypes.c_void_p
 _U32 = ctypes.c_uint32
+_U64 = ctypes.c_uint64
 _PP = ctypes.POINTER(AttentionParams)
+_PR = ctypes.POINTER(Rotary)
+_PW = ctypes.POINTER(Window)
 
 # name -> argtypes (every entry returns int)
 SIGNATURES = {
@@ -71,6 +87,14 @@ SIGNATURES = {
     "ma_host_pipeline_destroy": [_P],
     "ma_flashAttentionForward_host": [_P, _P, _P, _P, _P, _P, _U32, _P],
     "ma_attentionForwardBackward_host": [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _U32, _P],
+    "ma_rotaryForward": [_P, _P, _P, _P, _PR, _P, _PP, _U32, _P],
+    "ma_rotaryBackward": [_P, _P, _P, _P, _U32, _PR, _P, _PP, _U32, _P],
+    "ma_rotaryCacheAppend": [_P, _P, _P, _P, _P, _P, _P, _P, _PR, _PP, _U32, _U32, _P],
+    "ma_windowAttentionForward": [_P, _P, _P, _P, _P, _P, _PW, _PP, _U32, _P],
+    "ma_windowAttentionBackward": [_P, _P, _P, _P, _P, _P, _P, _P, _P, _U32, _P, _PW, _PP, _U32, _P, _U64, _P],
+    "ma_windowAttentionBackward_workspace": [_U32, _PW, _PP, _U32, ctypes.POINTER(_U64)],
+    "ma_windowAttentionCached": [_P, _P, _P, _P, _P, _P, _P, _PW, _PP, _U32, _U32, _P, _U64, _P],
+    "ma_windowAttentionCached_workspace": [_PW, _PP, _U32, _U32, ctypes.POINTER(_U64)],
     "ma_device_status": [ctypes.POINTER(ctypes.c_uint32), _P],
     "ma_debug_expire_next_wait": [_U32, _U32],
     "ma_version": [],

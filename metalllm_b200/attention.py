@@ -12,10 +12,19 @@ Shapes (B sequences of length T = params.M, N = params.N = NH*D):
     dQ                          : fp32 [B, T, N]
     l                           : fp32 [B, T, NH]
     D                           : bf16 [B, T, NH]
+
+For long contexts (no counterpart in the reference): rotary positions
+(rotaryForward, rotaryBackward), attention with a sliding window and sinks
+(windowAttentionForward, windowAttentionBackward) and, for serving, the same
+two over a K/V cache (rotaryCacheAppend, windowAttentionCached).  They take
+grouped heads (k, v and their gradients [B, T, NKV*D], caches
+[B, cap, NKV*D]; query head h uses K/V head h // (NH // NKV)) and padded
+batches (lens, int32 [B]: rows from lens[b] on are padding).
 """
 from __future__ import annotations
 
 import ctypes
+import math
 from typing import Optional
 
 import torch
@@ -279,6 +288,222 @@ def flashAttentionBackward(dZ: torch.Tensor, d: torch.Tensor, l: torch.Tensor, q
     else:
         _lib.call(name + "_shard", *args, shard[0], shard[1], _stream(stream))
     return dQ, dK, dV
+
+
+# ------------------------------------------------------------ long contexts
+def rotaryFrequencies(rot: int, base: float = 10000.0, factor: float = 1.0, original_length: Optional[int] = None,
+                      low: float = 1.0, high: float = 32.0, device="cuda") -> torch.Tensor:
+    """Radians per position of a rotation's rot/2 pairs, float64 [rot/2]:
+    base^(-2i/rot).  factor > 1 stretches the context: every frequency divided
+    by it, or, given original_length, by parts: pairs that make at least
+    `high` turns within original_length keep their frequency, pairs with at
+    most `low` turns are divided by factor, and those between move linearly
+    from one to the other.  (A stretch by parts usually goes with an
+    amplitude of 0.1 ln(factor) + 1.)"""
+    if rot < 2 or rot % 2:
+        raise ValueError(f"rot must be even and at least 2, got {rot}")
+    if not base > 0 or not factor > 0 or not high > low:
+        raise ValueError("base and factor must be positive and high above low")
+    i = torch.arange(rot // 2, dtype=torch.float64)
+    f = base ** (-2.0 * i / rot)
+    if original_length is None:
+        return (f / factor).to(device)
+    keep = ((original_length * f / (2.0 * math.pi) - low) / (high - low)).clamp(0.0, 1.0)
+    return (f * (keep + (1.0 - keep) / factor)).to(device)
+
+
+def _groups(p: AttentionParams, NKV: Optional[int]) -> int:
+    NKV = p.NH if NKV is None else int(NKV)
+    if NKV < 1 or p.NH % NKV:
+        raise ValueError(f"NKV={NKV} must divide NH={p.NH}")
+    return NKV
+
+
+def _check_optional(t: Optional[torch.Tensor], name: str, dtype: torch.dtype, shape: tuple) -> None:
+    if t is not None:
+        _check(t, name, dtype, shape)
+
+
+def _rotary(inv_freq: torch.Tensor, NKV: int, interleaved: bool, amplitude: float) -> _lib.Rotary:
+    if not isinstance(inv_freq, torch.Tensor) or inv_freq.dim() != 1:
+        raise TypeError("inv_freq must be a one-dimensional tensor (rotaryFrequencies)")
+    _check(inv_freq, "inv_freq", torch.float64, tuple(inv_freq.shape))
+    return _lib.Rotary(_ptr(inv_freq), 2 * inv_freq.numel(), int(bool(interleaved)), NKV, float(amplitude))
+
+
+def _u32(x: int, name: str) -> int:
+    if x < 0:
+        raise ValueError(f"{name} must not be negative, got {x}")
+    return min(int(x), 0xFFFFFFFF)
+
+
+def _window(window: int, sinks: int, NKV: int) -> _lib.Window:
+    return _lib.Window(NKV, _u32(window, "window"), _u32(sinks, "sinks"))
+
+
+def _workspace(like: torch.Tensor, stream: Optional[torch.cuda.Stream], name: str, *args):
+    """Device memory of the size that entry point `name` gives, for a call on `stream`."""
+    need = ctypes.c_uint64()
+    _lib.call(name, *args, ctypes.byref(need))
+    ws = torch.empty(need.value, dtype=torch.uint8, device=like.device)
+    if stream is not None and stream != torch.cuda.current_stream():
+        ws.record_stream(stream)  # freed on return, while `stream` may still be using it
+    return ws
+
+
+def rotaryForward(q: torch.Tensor, k: torch.Tensor, inv_freq: torch.Tensor, p: AttentionParams, B: int,
+                  NKV: Optional[int] = None, positions: Optional[torch.Tensor] = None, interleaved: bool = False,
+                  amplitude: float = 1.0, q_out: Optional[torch.Tensor] = None,
+                  k_out: Optional[torch.Tensor] = None, stream: Optional[torch.cuda.Stream] = None):
+    """q_out, k_out = q, k (bf16) with the first 2*len(inv_freq) columns of
+    every head turned by positions * inv_freq (float64, rotaryFrequencies) and
+    multiplied by amplitude.  Pairs are columns i and i + rot/2, or with
+    interleaved 2i and 2i + 1.  positions: int32 [B, T], by default 0 .. T-1.
+    q_out may be q and k_out may be k (ma_rotaryForward)."""
+    NKV = _groups(p, NKV)
+    r = _rotary(inv_freq, NKV, interleaved, amplitude)
+    qs, ks = (B, p.M, p.N), (B, p.M, NKV * p.D)
+    _check(q, "q", torch.bfloat16, qs)
+    _check(k, "k", torch.bfloat16, ks)
+    _check_optional(positions, "positions", torch.int32, (B, p.M))
+    q_out = _out(q_out, q, qs, torch.bfloat16, "q_out")
+    k_out = _out(k_out, k, ks, torch.bfloat16, "k_out")
+    _lib.call("ma_rotaryForward", _ptr(q), _ptr(k), _ptr(q_out), _ptr(k_out), ctypes.byref(r), _ptr(positions),
+              ctypes.byref(p), B, _stream(stream))
+    return q_out, k_out
+
+
+def rotaryBackward(dQ: torch.Tensor, dK: torch.Tensor, inv_freq: torch.Tensor, p: AttentionParams, B: int,
+                   NKV: Optional[int] = None, positions: Optional[torch.Tensor] = None, interleaved: bool = False,
+                   amplitude: float = 1.0, dQ_out: Optional[torch.Tensor] = None,
+                   dK_out: Optional[torch.Tensor] = None, stream: Optional[torch.cuda.Stream] = None):
+    """The gradients of rotaryForward's inputs from those of its outputs: dQ
+    (fp32 or bf16, and dQ_out of the same type) and dK (bf16) turned back.
+    In place allowed (ma_rotaryBackward)."""
+    NKV = _groups(p, NKV)
+    r = _rotary(inv_freq, NKV, interleaved, amplitude)
+    qs, ks = (B, p.M, p.N), (B, p.M, NKV * p.D)
+    t = torch.float32 if isinstance(dQ, torch.Tensor) and dQ.dtype == torch.float32 else torch.bfloat16
+    _check(dQ, "dQ", t, qs)
+    _check(dK, "dK", torch.bfloat16, ks)
+    _check_optional(positions, "positions", torch.int32, (B, p.M))
+    dQ_out = _out(dQ_out, dQ, qs, t, "dQ_out")
+    dK_out = _out(dK_out, dK, ks, torch.bfloat16, "dK_out")
+    _lib.call("ma_rotaryBackward", _ptr(dQ), _ptr(dK), _ptr(dQ_out), _ptr(dK_out), int(t == torch.float32),
+              ctypes.byref(r), _ptr(positions), ctypes.byref(p), B, _stream(stream))
+    return dQ_out, dK_out
+
+
+def _cap(cache: torch.Tensor, name: str) -> int:
+    if not isinstance(cache, torch.Tensor) or cache.dim() != 3:
+        raise TypeError(f"{name} must be a [B, cap, NKV*D] tensor")
+    return cache.shape[1]
+
+
+def rotaryCacheAppend(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor,
+                      v_cache: torch.Tensor, start: torch.Tensor, inv_freq: torch.Tensor, p: AttentionParams, B: int,
+                      NKV: Optional[int] = None, lens: Optional[torch.Tensor] = None, interleaved: bool = False,
+                      amplitude: float = 1.0, q_out: Optional[torch.Tensor] = None,
+                      stream: Optional[torch.cuda.Stream] = None) -> torch.Tensor:
+    """p.M new tokens of each sequence enter the caches (bf16 [B, cap, NKV*D]):
+    k turned at its position start[b] + i (start: int32 [B]) and v are stored
+    in that row.  Returns q turned (rows from lens[b] on: 0); q_out may be q.
+    Padding rows, and rows past the caches' end, are not stored
+    (ma_rotaryCacheAppend)."""
+    NKV = _groups(p, NKV)
+    r = _rotary(inv_freq, NKV, interleaved, amplitude)
+    qs, ks, cap = (B, p.M, p.N), (B, p.M, NKV * p.D), _cap(k_cache, "k_cache")
+    _check(q, "q", torch.bfloat16, qs)
+    for t, n in ((k, "k"), (v, "v")):
+        _check(t, n, torch.bfloat16, ks)
+    for t, n in ((k_cache, "k_cache"), (v_cache, "v_cache")):
+        _check(t, n, torch.bfloat16, (B, cap, NKV * p.D))
+    _check(start, "start", torch.int32, (B,))
+    _check_optional(lens, "lens", torch.int32, (B,))
+    q_out = _out(q_out, q, qs, torch.bfloat16, "q_out")
+    _lib.call("ma_rotaryCacheAppend", _ptr(q), _ptr(k), _ptr(v), _ptr(q_out), _ptr(k_cache), _ptr(v_cache),
+              _ptr(start), _ptr(lens), ctypes.byref(r), ctypes.byref(p), B, cap, _stream(stream))
+    return q_out
+
+
+def windowAttentionForward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, p: AttentionParams, B: int,
+                           window: int, sinks: int = 0, NKV: Optional[int] = None,
+                           lens: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
+                           l: Optional[torch.Tensor] = None, stream: Optional[torch.cuda.Stream] = None):
+    """out, l as flashAttentionForward, where the query at i sees key j <= i
+    only if i - j < window or j < sinks.  Padding rows: out = 0, l = -inf
+    (ma_windowAttentionForward)."""
+    NKV = _groups(p, NKV)
+    w = _window(window, sinks, NKV)
+    qs, ks = (B, p.M, p.N), (B, p.M, NKV * p.D)
+    _check(q, "q", torch.bfloat16, qs)
+    for t, n in ((k, "k"), (v, "v")):
+        _check(t, n, torch.bfloat16, ks)
+    _check_optional(lens, "lens", torch.int32, (B,))
+    out = _out(out, q, qs, torch.bfloat16, "out")
+    l = _out(l, q, (B, p.M, p.NH), torch.float32, "l")
+    _lib.call("ma_windowAttentionForward", _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(l), _ptr(lens),
+              ctypes.byref(w), ctypes.byref(p), B, _stream(stream))
+    return out, l
+
+
+def windowAttentionBackward(dO: torch.Tensor, out: torch.Tensor, l: torch.Tensor, q: torch.Tensor, k: torch.Tensor,
+                            v: torch.Tensor, p: AttentionParams, B: int, window: int, sinks: int = 0,
+                            NKV: Optional[int] = None, lens: Optional[torch.Tensor] = None,
+                            dQ: Optional[torch.Tensor] = None, dK: Optional[torch.Tensor] = None,
+                            dV: Optional[torch.Tensor] = None, dQ_dtype: Optional[torch.dtype] = None,
+                            stream: Optional[torch.cuda.Stream] = None):
+    """dQ, dK, dV of windowAttentionForward from dO and its out and l (padding
+    rows: 0).  dQ is fp32 as flashAttentionBackward's (for computeGradDx and
+    computeGradDw), or bf16: by the dQ given, or by dQ_dtype
+    (ma_windowAttentionBackward)."""
+    NKV = _groups(p, NKV)
+    w = _window(window, sinks, NKV)
+    qs, ks = (B, p.M, p.N), (B, p.M, NKV * p.D)
+    for t, n in ((dO, "dO"), (out, "out"), (q, "q")):
+        _check(t, n, torch.bfloat16, qs)
+    _check(l, "l", torch.float32, (B, p.M, p.NH))
+    for t, n in ((k, "k"), (v, "v")):
+        _check(t, n, torch.bfloat16, ks)
+    _check_optional(lens, "lens", torch.int32, (B,))
+    if dQ_dtype is None:
+        dQ_dtype = dQ.dtype if isinstance(dQ, torch.Tensor) else torch.float32
+    if dQ_dtype not in (torch.float32, torch.bfloat16):
+        raise TypeError(f"dQ must be float32 or bfloat16, got {dQ_dtype}")
+    f32 = int(dQ_dtype == torch.float32)
+    dQ = _out(dQ, q, qs, dQ_dtype, "dQ")
+    dK = _out(dK, k, ks, torch.bfloat16, "dK")
+    dV = _out(dV, k, ks, torch.bfloat16, "dV")
+    ws = _workspace(q, stream, "ma_windowAttentionBackward_workspace", f32, ctypes.byref(w), ctypes.byref(p), B)
+    _lib.call("ma_windowAttentionBackward", _ptr(dO), _ptr(out), _ptr(l), _ptr(q), _ptr(k), _ptr(v), _ptr(dQ),
+              _ptr(dK), _ptr(dV), f32, _ptr(lens), ctypes.byref(w), ctypes.byref(p), B, _ptr(ws), ws.numel(),
+              _stream(stream))
+    return dQ, dK, dV
+
+
+def windowAttentionCached(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, start: torch.Tensor,
+                          p: AttentionParams, B: int, window: int, sinks: int = 0, NKV: Optional[int] = None,
+                          lens: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
+                          l: Optional[torch.Tensor] = None, stream: Optional[torch.cuda.Stream] = None):
+    """out, l of p.M >= 1 new queries of each sequence, at positions
+    start[b] + i, over caches that already hold their keys and values
+    (rotaryCacheAppend); window and sinks as in windowAttentionForward, rows
+    from lens[b] on are padding.  start[b] + lens[b] must not exceed the
+    caches' rows (ma_windowAttentionCached)."""
+    NKV = _groups(p, NKV)
+    w = _window(window, sinks, NKV)
+    qs, cap = (B, p.M, p.N), _cap(k_cache, "k_cache")
+    _check(q, "q", torch.bfloat16, qs)
+    for t, n in ((k_cache, "k_cache"), (v_cache, "v_cache")):
+        _check(t, n, torch.bfloat16, (B, cap, NKV * p.D))
+    _check(start, "start", torch.int32, (B,))
+    _check_optional(lens, "lens", torch.int32, (B,))
+    out = _out(out, q, qs, torch.bfloat16, "out")
+    l = _out(l, q, (B, p.M, p.NH), torch.float32, "l")
+    ws = _workspace(q, stream, "ma_windowAttentionCached_workspace", ctypes.byref(w), ctypes.byref(p), B, cap)
+    _lib.call("ma_windowAttentionCached", _ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(out), _ptr(l), _ptr(start),
+              _ptr(lens), ctypes.byref(w), ctypes.byref(p), B, cap, _ptr(ws), ws.numel(), _stream(stream))
+    return out, l
 
 
 def device_status(stream: Optional[torch.cuda.Stream] = None) -> int:

@@ -864,3 +864,319 @@ extern "C" int ma_attentionForwardBackward_host(ma_host_pipeline* pl, const ma_b
                                                 ma_stream_t stream) {
   return pipeline_run(pl, true, q, k, v, dO, out, l, dQ, dK, dV, B, stream);
 }
+
+// ------------------------------------------------------------- long contexts
+namespace {
+
+struct Range {
+  const char* name;
+  const void* p;
+  uint64_t bytes;
+  int may_equal;  // index of the input an output may be in place of, or -1
+};
+
+// Refuses an output that shares memory with an input or another output
+// (in place, the same range as its input, where may_equal allows it).
+template <int NI, int NO>
+int check_overlaps(const Range (&in)[NI], const Range (&out)[NO]) {
+  auto share = [](const Range& a, const Range& b) {
+    const auto x = reinterpret_cast<uintptr_t>(a.p), y = reinterpret_cast<uintptr_t>(b.p);
+    return x < y + b.bytes && y < x + a.bytes;
+  };
+  for (int j = 0; j < NO; ++j) {
+    for (int i = 0; i < NI; ++i)
+      if (share(in[i], out[j]) && !(out[j].may_equal == i && in[i].p == out[j].p && in[i].bytes == out[j].bytes))
+        return fail(MA_ERR_RANGE, "output '%s' overlaps input '%s'", out[j].name, in[i].name);
+    for (int i = 0; i < j; ++i)
+      if (share(out[i], out[j])) return fail(MA_ERR_RANGE, "outputs '%s' and '%s' overlap", out[i].name, out[j].name);
+  }
+  return MA_OK;
+}
+
+int check_groups(const AttentionParams* p, uint32_t NKV) {
+  if (NKV == 0 || p->NH % NKV != 0) return fail(MA_ERR_SHAPE, "NKV=%u must divide NH=%u", NKV, p->NH);
+  return MA_OK;
+}
+
+#define MA_REQUIRE_I32(ptr)                                                                            \
+  do {                                                                                                 \
+    if (reinterpret_cast<uintptr_t>(ptr) & 3u) return fail(MA_ERR_ALIGN, "pointer '%s' is not 4-byte aligned", #ptr); \
+  } while (0)
+
+int check_rotary(const MaRotary* r, const AttentionParams* p) {
+  if (!r) return fail(MA_ERR_NULL, "MaRotary pointer is NULL");
+  int rc = check_groups(p, r->NKV);
+  if (rc) return rc;
+  if (r->rot < 2 || r->rot > p->D || r->rot % 2)
+    return fail(MA_ERR_SHAPE, "rot=%u must be even and within 2 .. D=%u", r->rot, p->D);
+  if (r->interleaved > 1) return fail(MA_ERR_SHAPE, "interleaved=%u must be 0 or 1", r->interleaved);
+  if (!r->inv_freq) return fail(MA_ERR_NULL, "pointer 'inv_freq' is NULL");
+  if (reinterpret_cast<uintptr_t>(r->inv_freq) & 7u)
+    return fail(MA_ERR_ALIGN, "pointer 'inv_freq' is not 8-byte aligned");
+  return MA_OK;
+}
+
+int check_cap(const AttentionParams* p, uint32_t NKV, uint32_t B, uint32_t cap) {
+  if (cap == 0) return fail(MA_ERR_SHAPE, "empty cache: cap=0");
+  if (cap > (1u << 30) || (uint64_t)B * cap >= (1ull << 40) / ((uint64_t)NKV * p->D))
+    return fail(MA_ERR_LIMIT, "cache too large: B=%u cap=%u NKV*D=%u", B, cap, NKV * p->D);
+  return MA_OK;
+}
+
+int rotary_impl(const void* q, const ma_bf16* k, void* q_out, ma_bf16* k_out, bool q_f32, const MaRotary* r,
+                const int32_t* positions, const AttentionParams* p, uint32_t B, bool back, ma_stream_t stream) {
+  ma::AttnShape s;
+  int rc = check_shape(p, B, 0, 0, false, &s);
+  if (rc) return rc;
+  rc = check_rotary(r, p);
+  if (rc) return rc;
+  MA_REQUIRE_PTR(q);
+  MA_REQUIRE_PTR(k);
+  MA_REQUIRE_PTR(q_out);
+  MA_REQUIRE_PTR(k_out);
+  MA_REQUIRE_I32(positions);
+  const uint64_t rows = (uint64_t)B * p->M;
+  const uint64_t nq = rows * p->N * (q_f32 ? 4 : 2), nk = rows * r->NKV * p->D * 2;
+  const Range in[] = {{"q", q, nq, -1}, {"k", k, nk, -1}};
+  const Range out[] = {{"q_out", q_out, nq, 0}, {"k_out", k_out, nk, 1}};
+  rc = check_overlaps(in, out);
+  if (rc) return rc;
+  uint32_t* status = nullptr;
+  rc = device_status_word(&status);
+  if (rc) return rc;
+  cudaError_t e = ma::launch_rotary(q, q_f32, reinterpret_cast<bf16p>(k), q_out, reinterpret_cast<bf16m>(k_out), *r,
+                                    positions, s, (int)r->NKV, back, reinterpret_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, back ? "rotaryBackward launch" : "rotaryForward launch");
+  return ok();
+}
+
+// Validates what the window operators share and fills their arguments.
+// cap = 0: training, the keys are the queries' own rows.
+int window_args(const MaWindow* w, const AttentionParams* p, uint32_t B, uint32_t cap, ma::WindowArgs* a) {
+  ma::AttnShape s;
+  int rc = check_shape(p, B, 0, 0, false, &s);
+  if (rc) return rc;
+  if (!w) return fail(MA_ERR_NULL, "MaWindow pointer is NULL");
+  rc = check_groups(p, w->NKV);
+  if (rc) return rc;
+  if (w->window == 0) return fail(MA_ERR_SHAPE, "window=0: a query sees itself at least (window >= 1)");
+  *a = ma::WindowArgs{};
+  a->B = s.B;
+  a->M = s.T;
+  a->K = cap ? (int)cap : s.T;
+  a->NH = s.NH;
+  a->NKV = (int)w->NKV;
+  a->D = s.D;
+  const uint32_t most = 0x7fffffffu;
+  a->window = (int)(w->window < most ? w->window : most);
+  a->sinks = (int)(w->sinks < most ? w->sinks : most);
+  a->scale = s.D == 64 ? 0.125f : 0.08838834764831845f;  // 1/sqrt(D)
+  return MA_OK;
+}
+
+// Bytes of the tensors of a window operator: q and out, k and v, l.
+struct WindowBytes {
+  uint64_t q, k, l;
+  explicit WindowBytes(const ma::WindowArgs& a)
+      : q((uint64_t)a.B * a.M * a.NH * a.D * 2), k((uint64_t)a.B * a.K * a.NKV * a.D * 2),
+        l((uint64_t)a.B * a.M * a.NH * 4) {}
+};
+
+int check_workspace(const void* workspace, uint64_t have, uint64_t need) {
+  if (need == 0) return MA_OK;
+  MA_REQUIRE_PTR(workspace);
+  if (have < need)
+    return fail(MA_ERR_LIMIT, "workspace of %llu bytes, %llu needed", (unsigned long long)have,
+                (unsigned long long)need);
+  return MA_OK;
+}
+
+}  // namespace
+
+extern "C" int ma_rotaryForward(const ma_bf16* q, const ma_bf16* k, ma_bf16* q_out, ma_bf16* k_out,
+                                const MaRotary* r, const int32_t* positions, const AttentionParams* p, uint32_t B,
+                                ma_stream_t stream) {
+  return rotary_impl(q, k, q_out, k_out, false, r, positions, p, B, false, stream);
+}
+
+extern "C" int ma_rotaryBackward(const void* dQ, const ma_bf16* dK, void* dQ_out, ma_bf16* dK_out, uint32_t dq_f32,
+                                 const MaRotary* r, const int32_t* positions, const AttentionParams* p, uint32_t B,
+                                 ma_stream_t stream) {
+  return rotary_impl(dQ, dK, dQ_out, dK_out, dq_f32 != 0, r, positions, p, B, true, stream);
+}
+
+extern "C" int ma_rotaryCacheAppend(const ma_bf16* q, const ma_bf16* k, const ma_bf16* v, ma_bf16* q_out,
+                                    ma_bf16* k_cache, ma_bf16* v_cache, const int32_t* start, const int32_t* lens,
+                                    const MaRotary* r, const AttentionParams* p, uint32_t B, uint32_t cap,
+                                    ma_stream_t stream) {
+  ma::AttnShape s;
+  int rc = check_shape(p, B, 0, 0, false, &s);
+  if (rc) return rc;
+  rc = check_rotary(r, p);
+  if (rc) return rc;
+  rc = check_cap(p, r->NKV, B, cap);
+  if (rc) return rc;
+  MA_REQUIRE_PTR(q);
+  MA_REQUIRE_PTR(k);
+  MA_REQUIRE_PTR(v);
+  MA_REQUIRE_PTR(q_out);
+  MA_REQUIRE_PTR(k_cache);
+  MA_REQUIRE_PTR(v_cache);
+  if (!start) return fail(MA_ERR_NULL, "pointer 'start' is NULL");
+  MA_REQUIRE_I32(start);
+  MA_REQUIRE_I32(lens);
+  const uint64_t rows = (uint64_t)B * p->M, nq = rows * p->N * 2, nk = rows * r->NKV * p->D * 2;
+  const uint64_t nc = (uint64_t)B * cap * r->NKV * p->D * 2;
+  const Range in[] = {{"q", q, nq, -1}, {"k", k, nk, -1}, {"v", v, nk, -1}};
+  const Range out[] = {{"q_out", q_out, nq, 0}, {"k_cache", k_cache, nc, -1}, {"v_cache", v_cache, nc, -1}};
+  rc = check_overlaps(in, out);
+  if (rc) return rc;
+  uint32_t* status = nullptr;
+  rc = device_status_word(&status);
+  if (rc) return rc;
+  cudaError_t e = ma::launch_rotary_append(
+      reinterpret_cast<bf16p>(q), reinterpret_cast<bf16p>(k), reinterpret_cast<bf16p>(v),
+      reinterpret_cast<bf16m>(q_out), reinterpret_cast<bf16m>(k_cache), reinterpret_cast<bf16m>(v_cache), start, lens,
+      *r, s, (int)r->NKV, (int)cap, reinterpret_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, "rotaryCacheAppend launch");
+  return ok();
+}
+
+extern "C" int ma_windowAttentionForward(const ma_bf16* q, const ma_bf16* k, const ma_bf16* v, ma_bf16* out,
+                                         float* l, const int32_t* lens, const MaWindow* w, const AttentionParams* p,
+                                         uint32_t B, ma_stream_t stream) {
+  ma::WindowArgs a;
+  int rc = window_args(w, p, B, 0, &a);
+  if (rc) return rc;
+  MA_REQUIRE_PTR(q);
+  MA_REQUIRE_PTR(k);
+  MA_REQUIRE_PTR(v);
+  MA_REQUIRE_PTR(out);
+  MA_REQUIRE_PTR(l);
+  MA_REQUIRE_I32(lens);
+  const WindowBytes n(a);
+  const Range ins[] = {{"q", q, n.q, -1}, {"k", k, n.k, -1}, {"v", v, n.k, -1}};
+  const Range outs[] = {{"out", out, n.q, -1}, {"l", l, n.l, -1}};
+  rc = check_overlaps(ins, outs);
+  if (rc) return rc;
+  rc = device_status_word(&a.status);
+  if (rc) return rc;
+  a.q = reinterpret_cast<bf16p>(q);
+  a.k = reinterpret_cast<bf16p>(k);
+  a.v = reinterpret_cast<bf16p>(v);
+  a.out = reinterpret_cast<bf16m>(out);
+  a.l = l;
+  a.lens = lens;
+  cudaError_t e = ma::launch_window_fwd(a, reinterpret_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, "windowAttentionForward launch");
+  return ok();
+}
+
+extern "C" int ma_windowAttentionBackward_workspace(uint32_t dq_f32, const MaWindow* w, const AttentionParams* p,
+                                                    uint32_t B, uint64_t* bytes) {
+  ma::WindowArgs a;
+  int rc = window_args(w, p, B, 0, &a);
+  if (rc) return rc;
+  if (!bytes) return fail(MA_ERR_NULL, "pointer 'bytes' is NULL");
+  *bytes = ma::window_bwd_workspace(a, dq_f32 != 0);
+  return ok();
+}
+
+extern "C" int ma_windowAttentionBackward(const ma_bf16* dO, const ma_bf16* out, const float* l, const ma_bf16* q,
+                                          const ma_bf16* k, const ma_bf16* v, void* dQ, ma_bf16* dK, ma_bf16* dV,
+                                          uint32_t dq_f32, const int32_t* lens, const MaWindow* w,
+                                          const AttentionParams* p, uint32_t B, void* workspace,
+                                          uint64_t workspace_bytes, ma_stream_t stream) {
+  ma::WindowArgs a;
+  int rc = window_args(w, p, B, 0, &a);
+  if (rc) return rc;
+  MA_REQUIRE_PTR(dO);
+  MA_REQUIRE_PTR(out);
+  MA_REQUIRE_PTR(l);
+  MA_REQUIRE_PTR(q);
+  MA_REQUIRE_PTR(k);
+  MA_REQUIRE_PTR(v);
+  MA_REQUIRE_PTR(dQ);
+  MA_REQUIRE_PTR(dK);
+  MA_REQUIRE_PTR(dV);
+  MA_REQUIRE_I32(lens);
+  const uint64_t need = ma::window_bwd_workspace(a, dq_f32 != 0);
+  rc = check_workspace(workspace, workspace_bytes, need);
+  if (rc) return rc;
+  const WindowBytes n(a);
+  const Range ins[] = {{"dO", dO, n.q, -1}, {"out", out, n.q, -1}, {"l", l, n.l, -1},
+                       {"q", q, n.q, -1},   {"k", k, n.k, -1},     {"v", v, n.k, -1}};
+  const Range outs[] = {{"dQ", dQ, dq_f32 ? 2 * n.q : n.q, -1}, {"dK", dK, n.k, -1}, {"dV", dV, n.k, -1},
+                        {"workspace", workspace, need, -1}};
+  rc = check_overlaps(ins, outs);
+  if (rc) return rc;
+  rc = device_status_word(&a.status);
+  if (rc) return rc;
+  a.q = reinterpret_cast<bf16p>(q);
+  a.k = reinterpret_cast<bf16p>(k);
+  a.v = reinterpret_cast<bf16p>(v);
+  a.out = const_cast<bf16m>(reinterpret_cast<bf16p>(out));
+  a.l = const_cast<float*>(l);
+  a.lens = lens;
+  ma::WindowGrads g;
+  g.dO = reinterpret_cast<bf16p>(dO);
+  g.dQ = dQ;
+  g.dK = reinterpret_cast<bf16m>(dK);
+  g.dV = reinterpret_cast<bf16m>(dV);
+  g.dq_f32 = dq_f32 != 0;
+  g.workspace = workspace;
+  cudaError_t e = ma::launch_window_bwd(a, g, reinterpret_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, "windowAttentionBackward launch");
+  return ok();
+}
+
+extern "C" int ma_windowAttentionCached_workspace(const MaWindow* w, const AttentionParams* p, uint32_t B,
+                                                  uint32_t cap, uint64_t* bytes) {
+  ma::WindowArgs a;
+  int rc = window_args(w, p, B, cap, &a);
+  if (rc) return rc;
+  rc = check_cap(p, w->NKV, B, cap);
+  if (rc) return rc;
+  if (!bytes) return fail(MA_ERR_NULL, "pointer 'bytes' is NULL");
+  *bytes = ma::window_cached_workspace(a);
+  return ok();
+}
+
+extern "C" int ma_windowAttentionCached(const ma_bf16* q, const ma_bf16* k_cache, const ma_bf16* v_cache,
+                                        ma_bf16* out, float* l, const int32_t* start, const int32_t* lens,
+                                        const MaWindow* w, const AttentionParams* p, uint32_t B, uint32_t cap,
+                                        void* workspace, uint64_t workspace_bytes, ma_stream_t stream) {
+  ma::WindowArgs a;
+  int rc = window_args(w, p, B, cap, &a);
+  if (rc) return rc;
+  rc = check_cap(p, w->NKV, B, cap);
+  if (rc) return rc;
+  MA_REQUIRE_PTR(q);
+  MA_REQUIRE_PTR(k_cache);
+  MA_REQUIRE_PTR(v_cache);
+  MA_REQUIRE_PTR(out);
+  MA_REQUIRE_PTR(l);
+  if (!start) return fail(MA_ERR_NULL, "pointer 'start' is NULL");
+  MA_REQUIRE_I32(start);
+  MA_REQUIRE_I32(lens);
+  const uint64_t need = ma::window_cached_workspace(a);
+  rc = check_workspace(workspace, workspace_bytes, need);
+  if (rc) return rc;
+  const WindowBytes n(a);
+  const Range ins[] = {{"q", q, n.q, -1}, {"k_cache", k_cache, n.k, -1}, {"v_cache", v_cache, n.k, -1}};
+  const Range outs[] = {{"out", out, n.q, -1}, {"l", l, n.l, -1}, {"workspace", workspace, need, -1}};
+  rc = check_overlaps(ins, outs);
+  if (rc) return rc;
+  rc = device_status_word(&a.status);
+  if (rc) return rc;
+  a.q = reinterpret_cast<bf16p>(q);
+  a.k = reinterpret_cast<bf16p>(k_cache);
+  a.v = reinterpret_cast<bf16p>(v_cache);
+  a.out = reinterpret_cast<bf16m>(out);
+  a.l = l;
+  a.start = start;
+  a.lens = lens;
+  cudaError_t e = ma::launch_window_cached(a, workspace, reinterpret_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, "windowAttentionCached launch");
+  return ok();
+}

@@ -166,4 +166,42 @@ struct AdamSegment {
 };
 cudaError_t launch_adam_fused(const AdamSegment* segs, int nsegs, long long max_count, float* p,
                               __nv_bfloat16* m, __nv_bfloat16* v, float lr_t, cudaStream_t st);
+
+// Rotary positions (rotary.cu).  q is fp32 or bf16 (q_f32); NKV heads of k.
+cudaError_t launch_rotary(const void* q, bool q_f32, const __nv_bfloat16* k, void* q_out, __nv_bfloat16* k_out,
+                          const MaRotary& r, const int32_t* positions, const AttnShape& s, int NKV, bool back,
+                          cudaStream_t st);
+cudaError_t launch_rotary_append(const __nv_bfloat16* q, const __nv_bfloat16* k, const __nv_bfloat16* v,
+                                 __nv_bfloat16* q_out, __nv_bfloat16* k_cache, __nv_bfloat16* v_cache,
+                                 const int32_t* start, const int32_t* lens, const MaRotary& r, const AttnShape& s,
+                                 int NKV, int cap, cudaStream_t st);
+
+// Attention with a sliding window and sinks: M query rows and K key rows per
+// sequence (K = M in training, the cache's rows in serving).
+struct WindowArgs {
+  const __nv_bfloat16 *q, *k, *v;
+  __nv_bfloat16* out;
+  float* l;
+  const int32_t* lens;   // [B] valid query rows, or null (all)
+  const int32_t* start;  // [B] position of a sequence's first query, or null (0)
+  int B, M, K, NH, NKV, D, window, sinks;
+  float scale;
+  uint32_t* status;
+  // lens and start lie on the device, so the host cannot refuse what they
+  // hold: out of range they are clamped, and nothing outside a tensor is read
+  __device__ int len(int b) const { return lens ? min(max(lens[b], 0), M) : M; }
+  __device__ int pos(int b, int i) const { return start ? (int)min((long long)max(start[b], 0) + i, K - 1ll) : i; }
+};
+struct WindowGrads {
+  const __nv_bfloat16* dO;
+  void* dQ;  // fp32 or bf16
+  __nv_bfloat16 *dK, *dV;
+  bool dq_f32;
+  void* workspace;  // window_bwd_workspace bytes
+};
+cudaError_t launch_window_fwd(const WindowArgs& a, cudaStream_t st);
+size_t window_cached_workspace(const WindowArgs& a);
+cudaError_t launch_window_cached(const WindowArgs& a, void* workspace, cudaStream_t st);
+size_t window_bwd_workspace(const WindowArgs& a, bool dq_f32);
+cudaError_t launch_window_bwd(const WindowArgs& a, const WindowGrads& g, cudaStream_t st);
 }  // namespace ma

@@ -1,0 +1,284 @@
+// rotary.cu -- rotary positions: rotaryForward, rotaryBackward and
+// rotaryCacheAppend.
+//
+// A pair (a, b) of a head's first `rot` columns at position t turns by the
+// angle t * f_i of its frequency:
+//   forward   (a cos - b sin, a sin + b cos) * amplitude
+//   backward  the transpose: (a cos + b sin, b cos - a sin) * amplitude
+// Half layout pairs column i with i + rot/2, interleaved 2i with 2i + 1; the
+// columns from `rot` on pass through.  The products are fp32 and each output
+// rounds once.
+//
+// The angle is the only place where fp32 would lose: at position 10^6 an fp32
+// product is off by 0.03 rad.  It is formed in fp64 in whole turns, the whole
+// turns are dropped, and the rest (at most half a turn, 2^-25 exact) goes to
+// sincospif in fp32.
+//
+// HBM-bound: each element is read and written once.  A thread owns one unit
+// of a row's rotation (8 pairs of the half layout = two 16-byte vectors, 4
+// pairs of the interleaved one = one vector, or a single pair where `rot`
+// does not allow vectors) and walks heads with it, so a sine is computed once
+// for the heads of a thread and not once for each head.  Neighbouring lanes
+// take the units of one head and then the next head, so a warp reads whole
+// rows.  Heads are dealt to as many threads as fill the GPU twice: at few rows
+// every thread has one head (latency), at many rows the sines are shared.
+#include "common.cuh"
+
+namespace ma {
+namespace {
+
+constexpr int THREADS = 256;
+
+// What the kernel turns and copies.  Heads 0 .. hq-1 are q's, the next hk k's.
+struct RotArgs {
+  const void* q;
+  const __nv_bfloat16* k;
+  const __nv_bfloat16* v;  // append only: copied to the cache
+  void* q_out;
+  __nv_bfloat16* k_out;  // [B][T][hk*D], or the caches [B][cap][hk*D]
+  __nv_bfloat16* v_out;
+  const double* inv_freq;
+  const int32_t* positions;  // [B][T] or null (row index)
+  const int32_t* start;      // append: [B], position of a sequence's first new row
+  const int32_t* lens;       // append: [B] valid rows, or null
+  long long rows;
+  int T, cap;
+  int hq, hk, D, rot;
+  int hsplit;     // threads a row's heads are dealt to
+  int units;      // rotation units of one head
+  int cunits;     // copied units of one head: q's and k's columns from rot on
+  int vunits;     // append: copied units of one head of v
+  bool copy_q, copy_k;  // out of place, so the columns from rot on move too
+  float amp, sign;      // sign -1: the backward's negative angle
+};
+
+template <typename T, int N>
+struct alignas(sizeof(T) * N) Vec {
+  T x[N];
+};
+
+__device__ __forceinline__ float to_f(float x) { return x; }
+__device__ __forceinline__ float to_f(__nv_bfloat16 x) { return __bfloat162float(x); }
+__device__ __forceinline__ void from_f(float& y, float x) { y = x; }
+__device__ __forceinline__ void from_f(__nv_bfloat16& y, float x) { y = __float2bfloat16_rn(x); }
+
+// N elements of T as vectors of at most 16 bytes
+template <typename T, int N>
+__device__ __forceinline__ void load(const T* p, T (&x)[N]) {
+  constexpr int W = N * sizeof(T) > 16 ? 16 / sizeof(T) : N;
+#pragma unroll
+  for (int i = 0; i < N; i += W) {
+    const Vec<T, W> v = *reinterpret_cast<const Vec<T, W>*>(p + i);
+#pragma unroll
+    for (int j = 0; j < W; ++j) x[i + j] = v.x[j];
+  }
+}
+template <typename T, int N>
+__device__ __forceinline__ void store(T* p, const T (&x)[N]) {
+  constexpr int W = N * sizeof(T) > 16 ? 16 / sizeof(T) : N;
+#pragma unroll
+  for (int i = 0; i < N; i += W) {
+    Vec<T, W> v;
+#pragma unroll
+    for (int j = 0; j < W; ++j) v.x[j] = x[i + j];
+    *reinterpret_cast<Vec<T, W>*>(p + i) = v;
+  }
+}
+
+// One unit (P pairs) of one head.  zero: a row past its sequence's length.
+template <typename T, bool INTER, int P>
+__device__ __forceinline__ void turn(const T* in, T* out, int unit, int half, const float (&c)[P],
+                                     const float (&s)[P], bool zero) {
+  if constexpr (INTER) {
+    T x[2 * P];
+    const int at = unit * 2 * P;
+    load(in + at, x);
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      const float a = to_f(x[2 * i]), b = to_f(x[2 * i + 1]);
+      from_f(x[2 * i], zero ? 0.0f : a * c[i] - b * s[i]);
+      from_f(x[2 * i + 1], zero ? 0.0f : a * s[i] + b * c[i]);
+    }
+    store(out + at, x);
+  } else {
+    T x[P], y[P];
+    const int at = unit * P;
+    load(in + at, x);
+    load(in + at + half, y);
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      const float a = to_f(x[i]), b = to_f(y[i]);
+      from_f(x[i], zero ? 0.0f : a * c[i] - b * s[i]);
+      from_f(y[i], zero ? 0.0f : a * s[i] + b * c[i]);
+    }
+    store(out + at, x);
+    store(out + at + half, y);
+  }
+}
+
+// Where row `row` of the new tokens goes in a cache: its row there, or -1.
+__device__ __forceinline__ long long cache_row(const RotArgs& a, int b, int t, bool valid) {
+  const long long pos = (long long)a.start[b] + t;
+  return valid && pos >= 0 && pos < a.cap ? (long long)b * a.cap + pos : -1;
+}
+
+// P pairs a unit, C elements a copied unit.
+template <typename TQ, bool INTER, int P, int C, bool APPEND>
+__global__ void __launch_bounds__(THREADS) rotary_kernel(const RotArgs a) {
+  pdl_wait_and_release();
+  const int heads = a.hq + a.hk, D = a.D, half = a.rot / 2;
+  const long long nrot = a.rows * a.units * a.hsplit;
+  const int copies = heads * a.cunits + (APPEND ? a.hk * a.vunits : 0);
+  const long long total = nrot + a.rows * copies;
+  for (long long g = blockIdx.x * (long long)THREADS + threadIdx.x; g < total;
+       g += (long long)gridDim.x * THREADS) {
+    if (g < nrot) {
+      const int unit = (int)(g % a.units);
+      const long long r = g / a.units;
+      const int h0 = (int)(r % a.hsplit);
+      const long long row = r / a.hsplit;
+      const int b = (int)(row / a.T), t = (int)(row % a.T);
+      const bool valid = !APPEND || !a.lens || t < a.lens[b];
+      const long long pos = APPEND ? (long long)a.start[b] + t : a.positions ? a.positions[row] : t;
+      float c[P], s[P];
+#pragma unroll
+      for (int i = 0; i < P; ++i) {
+        const double turns = (double)pos * (a.inv_freq[unit * P + i] * 0.15915494309189533577);
+        sincospif(2.0f * (float)(turns - rint(turns)), &s[i], &c[i]);
+        c[i] *= a.amp;
+        s[i] *= a.amp * a.sign;
+      }
+      const long long krow = APPEND ? cache_row(a, b, t, valid) : row;
+      for (int h = h0; h < heads; h += a.hsplit) {
+        if (h < a.hq) {
+          const long long off = (row * a.hq + h) * D;
+          turn<TQ, INTER, P>(static_cast<const TQ*>(a.q) + off, static_cast<TQ*>(a.q_out) + off, unit, half, c, s,
+                             !valid);
+        } else if (krow >= 0) {
+          const int kh = h - a.hq;
+          turn<__nv_bfloat16, INTER, P>(a.k + (row * a.hk + kh) * D, a.k_out + (krow * a.hk + kh) * D, unit, half, c,
+                                        s, false);
+        }
+      }
+      continue;
+    }
+    // the columns that only move: q's and k's from rot on, and v
+    const long long r = g - nrot;
+    const long long row = r / copies;
+    int u = (int)(r % copies);
+    const int b = (int)(row / a.T), t = (int)(row % a.T);
+    const bool valid = !APPEND || !a.lens || t < a.lens[b];
+    if (u < heads * a.cunits) {
+      const int h = u / a.cunits, at = a.rot + (u % a.cunits) * C;
+      if (h < a.hq) {
+        if (!a.copy_q && valid) continue;
+        const long long off = (row * a.hq + h) * D + at;
+        TQ x[C];
+        load(static_cast<const TQ*>(a.q) + off, x);
+        if (!valid) {
+#pragma unroll
+          for (int i = 0; i < C; ++i) from_f(x[i], 0.0f);
+        }
+        store(static_cast<TQ*>(a.q_out) + off, x);
+      } else if (a.copy_k) {
+        const long long krow = APPEND ? cache_row(a, b, t, valid) : row;
+        if (krow < 0) continue;
+        const int kh = h - a.hq;
+        __nv_bfloat16 x[C];
+        load(a.k + (row * a.hk + kh) * D + at, x);
+        store(a.k_out + (krow * a.hk + kh) * D + at, x);
+      }
+    } else if constexpr (APPEND) {  // v, always in 16-byte pieces
+      u -= heads * a.cunits;
+      const long long krow = cache_row(a, b, t, valid);
+      if (krow < 0) continue;
+      const int at = u * 8;  // within the row's hk*D columns
+      __nv_bfloat16 x[8];
+      load(a.v + row * a.hk * D + at, x);
+      store(a.v_out + krow * a.hk * D + at, x);
+    }
+  }
+}
+
+template <typename TQ, bool INTER, int P, int C, bool APPEND>
+cudaError_t launch_as(RotArgs a, cudaStream_t st) {
+  int dev = 0, sms = 148;
+  cudaGetDevice(&dev);
+  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  const int heads = a.hq + a.hk;
+  a.units = a.rot / 2 / P;
+  const bool copied = APPEND || a.copy_q || a.copy_k;
+  a.cunits = copied ? (a.D - a.rot) / C : 0;
+  a.vunits = APPEND ? a.D / 8 : 0;
+  // threads enough to fill the GPU twice (2048 a SM), each at least one head
+  const long long fill = (long long)sms * 2048 * 2;
+  long long split = fill / (a.rows * a.units) + 1;
+  a.hsplit = (int)(split < heads ? split : heads);
+  const long long total = a.rows * a.units * a.hsplit +
+                          a.rows * ((long long)heads * a.cunits + (APPEND ? a.hk * a.vunits : 0));
+  const long long blocks = (total + THREADS - 1) / THREADS;
+  const long long most = 1ll << 30;
+  launch_pdl(rotary_kernel<TQ, INTER, P, C, APPEND>, (unsigned)(blocks < most ? blocks : most), THREADS, 0, st, a);
+  count_launches(1);
+  return cudaGetLastError();
+}
+
+// Vectors where `rot` is a whole number of them, else single pairs.
+template <typename TQ, bool APPEND>
+cudaError_t launch_type(const RotArgs& a, bool inter, cudaStream_t st) {
+  if (inter)
+    return a.rot % 8 == 0 ? launch_as<TQ, true, 4, 8, APPEND>(a, st) : launch_as<TQ, true, 1, 2, APPEND>(a, st);
+  return a.rot % 16 == 0 ? launch_as<TQ, false, 8, 8, APPEND>(a, st) : launch_as<TQ, false, 1, 2, APPEND>(a, st);
+}
+
+RotArgs rot_args(const AttnShape& s, int NKV, const MaRotary& r, bool back) {
+  RotArgs a{};
+  a.rows = (long long)s.B * s.T;
+  a.T = s.T;
+  a.hq = s.NH;
+  a.hk = NKV;
+  a.D = s.D;
+  a.rot = (int)r.rot;
+  a.inv_freq = r.inv_freq;
+  a.amp = r.amplitude;
+  a.sign = back ? -1.0f : 1.0f;
+  return a;
+}
+
+}  // namespace
+
+cudaError_t launch_rotary(const void* q, bool q_f32, const __nv_bfloat16* k, void* q_out, __nv_bfloat16* k_out,
+                          const MaRotary& r, const int32_t* positions, const AttnShape& s, int NKV, bool back,
+                          cudaStream_t st) {
+  RotArgs a = rot_args(s, NKV, r, back);
+  a.q = q;
+  a.k = k;
+  a.q_out = q_out;
+  a.k_out = k_out;
+  a.positions = positions;
+  a.copy_q = q != q_out;
+  a.copy_k = k != k_out;
+  return q_f32 ? launch_type<float, false>(a, r.interleaved, st)
+               : launch_type<__nv_bfloat16, false>(a, r.interleaved, st);
+}
+
+cudaError_t launch_rotary_append(const __nv_bfloat16* q, const __nv_bfloat16* k, const __nv_bfloat16* v,
+                                 __nv_bfloat16* q_out, __nv_bfloat16* k_cache, __nv_bfloat16* v_cache,
+                                 const int32_t* start, const int32_t* lens, const MaRotary& r, const AttnShape& s,
+                                 int NKV, int cap, cudaStream_t st) {
+  RotArgs a = rot_args(s, NKV, r, false);
+  a.q = q;
+  a.k = k;
+  a.v = v;
+  a.q_out = q_out;
+  a.k_out = k_cache;
+  a.v_out = v_cache;
+  a.start = start;
+  a.lens = lens;
+  a.cap = cap;
+  a.copy_q = q != q_out;
+  a.copy_k = true;
+  return launch_type<__nv_bfloat16, true>(a, r.interleaved, st);
+}
+
+}  // namespace ma
