@@ -32,6 +32,14 @@
 // stays fp32 (the reference rounds it to bf16); P is bf16 as in the reference
 // (attention.metal:139,153).
 //
+// WIN: the same kernel for windowAttentionForward and windowAttentionCached
+// (sliding window, sinks, grouped K/V heads, sequence lengths, queries that
+// start inside a cache).  A unit then visits the sink tiles and the tiles from
+// the first row's window on, the tiles that every row sees whole carry no
+// masking code, and a tile in which some row sees nothing is allowed.  Warp 2
+// zeroes the rows of a V tile that no query may see (padding, a cache's rows
+// past the end or out of the window): P is 0 there, but 0 * NaN is not.
+//
 // Every mbarrier wait is bounded (about 2 s); on time-out the CTA sets an
 // abort flag that all roles poll, winds down, frees its TMEM and sets
 // STATUS_FWD_TIMEOUT in the device status word.
@@ -58,7 +66,7 @@ constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LN2 = 0.6931471805599453f;
 constexpr float RESCALE_THRESHOLD = 8.0f;  // log2 units
 
-template <int HD, bool DYN = false>
+template <int HD, bool DYN = false, bool WIN = false>
 struct FwdCfg {
   static constexpr int KB = HD / 64;  // 64-column blocks per row
   static constexpr int QST = HD == 64 ? 2 : 1;  // Q-pair stages
@@ -84,7 +92,7 @@ struct FwdCfg {
   static constexpr uint32_t OFF_P = OFF_V + VST * KV_BYTES;      // [2 tiles] P / O staging
   // D=64: an all-zero fp32 tile (128 rows x 32 columns) that TMA stores copy
   // into dQ when the forward zeroes it for an accumulating backward
-  static constexpr uint32_t ZT_BYTES = P_TMEM ? BM * 32 * 4 : 0;
+  static constexpr uint32_t ZT_BYTES = P_TMEM && !WIN ? BM * 32 * 4 : 0;
   static constexpr uint32_t OFF_ZT = OFF_P + 2 * STG_BYTES;
   // the unit schedule: NSCHED 16-byte launch-control responses
   static constexpr int NSCHED = DYN ? (int)kSchedSlots : 0;  // dynamic schedule only
@@ -96,9 +104,9 @@ struct FwdCfg {
   static constexpr uint32_t OFF_BAR = OFF_SCHED + NSCHED * 16;
   // q_full/empty[QST], k_full/empty[KST], v_full/empty[VST], per tile X:
   // s_full, s_free, p_full, pv_done, o_free, do_full; then never (nothing
-  // arrives: the time-out test hook), fin (the UMMA issuer's wind-down) and
-  // sched_full/empty[NSCHED]
-  static constexpr int NBAR = 2 * QST + 2 * KST + 2 * VST + 2 * 6 + 2 + 2 * NSCHED;
+  // arrives: the time-out test hook), fin (the UMMA issuer's wind-down),
+  // sched_full/empty[NSCHED] and, for WIN, v_fixed[VST]
+  static constexpr int NBAR = 2 * QST + 2 * KST + 2 * VST + 2 * 6 + 2 + 2 * NSCHED + (WIN ? VST : 0);
   static constexpr uint32_t OFF_TSLOT = OFF_BAR + NBAR * 8;
   static constexpr uint32_t SMEM_BYTES = OFF_TSLOT + 16 + 1024;  // + alignment slack
   static constexpr uint32_t TCOL_S = 0;     // S_A, S_B at columns 0, 128
@@ -123,6 +131,7 @@ struct FwdParams {
   // then accumulates into dQ
   float* dQz;
   uint32_t expire_ns;  // time-out test hook (ma_debug_expire_next_wait), 0 = off
+  WindowArgs win;      // WIN only
 };
 
 // sum over 8 bf16 pairs of a[i] * b[i], fp32 (products of bf16 values are
@@ -179,6 +188,73 @@ __device__ __forceinline__ Unit decode_unit(const FwdParams& prm, int k) {
   return x;
 }
 
+// A unit under a window.  The key tiles it visits, by list index j: the sink
+// tiles 0 .. ns-1 before the window, then lo, lo+1, ...; tile A is active for
+// j < nA, tile B for j < nB except j == skip (the one tile that A's window
+// reaches and B's does not).
+struct WinUnit : Unit {
+  int n;     // valid rows of the sequence
+  int ns, lo, skip;
+  int t0A, t1A, t0B, t1B;  // positions of the first and the last valid row of A and B
+  int end;   // keys of the sequence: rows from here on are padding
+  bool cached;
+
+  __device__ int key_tile(int j) const { return j < ns ? j : lo + (j - ns); }
+  __device__ bool active(int x, int j) const { return x == 0 ? j < nA : j < nB && j != skip; }
+  // the first list index of a tile: its PV starts the sum
+  __device__ int first(int x) const { return x == 1 && skip == 0 ? 1 : 0; }
+  // every valid row of tile x sees every key of the tile at k0
+  __device__ bool whole(const WindowArgs& w, int x, int k0) const {
+    return k0 + BN - 1 <= (x == 0 ? t0A : t0B) &&
+           (k0 > (x == 0 ? t1A : t1B) - w.window || k0 + BN - 1 < w.sinks);
+  }
+  // rows [*a, *b) of the tile at k0 that no query sees: past the end
+  __device__ bool past_end(const WindowArgs& w, int k0, int* a) const {
+    *a = max(0, end - k0);
+    return k0 + BN > end && end < w.K && *a < BN;
+  }
+  // and, in a cache, between the sinks and the first row's window
+  __device__ bool out_of_window(const WindowArgs& w, int k0, int* a, int* b) const {
+    *a = min(max(w.sinks, k0) - k0, BN);
+    *b = min(max(0, t0A - w.window + 1) - k0, BN);
+    return cached && *a < *b;
+  }
+  __device__ bool fix(const WindowArgs& w, int k0) const {
+    int a, b;
+    return past_end(w, k0, &a) || out_of_window(w, k0, &a, &b);
+  }
+};
+
+template <int HB>
+__device__ __forceinline__ WinUnit decode_win_unit(const FwdParams& prm, int k) {
+  const WindowArgs& w = prm.win;
+  WinUnit x;
+  static_cast<Unit&>(x) = decode_unit<HB>(prm, k);
+  x.n = w.len(x.b);
+  x.cached = w.start != nullptr;
+  x.nA = x.nB = x.nkv = x.ns = x.lo = 0;
+  x.t0A = x.t1A = x.t0B = x.t1B = 0;
+  x.skip = -1;
+  x.end = x.n > 0 ? w.pos(x.b, x.n - 1) + 1 : 0;
+  const int r0 = 2 * x.pair * BM;
+  if (r0 >= x.n) return x;
+  const int nS = w.sinks / BN + (w.sinks % BN != 0);
+  const bool b = r0 + BM < x.n;
+  const int rB = min(r0 + BM, x.n - 1);
+  x.t0A = w.pos(x.b, r0);
+  x.t1A = w.pos(x.b, min(r0 + BM - 1, x.n - 1));
+  x.t0B = w.pos(x.b, rB);
+  x.t1B = w.pos(x.b, min(rB + BM - 1, x.n - 1));
+  const int loB = max(0, x.t0B - w.window + 1) / BN;
+  x.lo = max(0, x.t0A - w.window + 1) / BN;
+  x.ns = min(nS, x.lo);
+  x.nA = x.ns + x.t1A / BN - x.lo + 1;
+  x.nB = b ? x.ns + x.t1B / BN - x.lo + 1 : 0;
+  x.skip = b && loB > x.lo && x.lo >= nS ? x.ns : -1;
+  x.nkv = b ? x.nB : x.nA;
+  return x;
+}
+
 // Static schedule: the g-th unit of this CTA, or -1 when it has none left.
 __device__ __forceinline__ int unit_of_round(const FwdParams& prm, int g) {
   const int G = gridDim.x;
@@ -187,14 +263,14 @@ __device__ __forceinline__ int unit_of_round(const FwdParams& prm, int g) {
   return k < prm.nunits ? (int)k : -1;
 }
 
-template <int HD, bool DYN>
+template <int HD, bool DYN, bool WIN>
 __global__ void __launch_bounds__(NUM_THREADS, 1)
     flash_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                      const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmO,
                      const __grid_constant__ CUtensorMap tmdO, const __grid_constant__ CUtensorMap tmdQz,
                      const FwdParams prm) {
   pdl_wait_and_release();
-  using C = FwdCfg<HD, DYN>;
+  using C = FwdCfg<HD, DYN, WIN>;
   extern __shared__ uint8_t smem_raw[];
   __shared__ int abort_flag;
   const uint32_t raw = smem_u32(smem_raw);
@@ -221,10 +297,16 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   const uint32_t BAR_FIN = barX + 8u * 13;    // the UMMA issuer's last commit (wind-down)
   auto BAR_UF = [&](int s) { return barX + 8u * (14 + s); };              // response s landed
   auto BAR_UE = [&](int s) { return barX + 8u * (14 + C::NSCHED + s); };  // response s read by all
+  auto BAR_VZ = [&](int s) { return barX + 8u * (14 + 2 * C::NSCHED + s); };  // WIN: V slot s zeroed where it must be
   // dynamic schedule: unit g >= 1 of this CTA is the one launch-control
   // response g-1 names (requested by the TMA producer when it starts unit
-  // g-1); readers: the producer, the UMMA issuer and the 8 softmax warps
-  constexpr uint32_t SCHED_READERS = 10;
+  // g-1); readers: the producer, the UMMA issuer, the 8 softmax warps and,
+  // for WIN, the warp that zeroes V rows
+  constexpr uint32_t SCHED_READERS = WIN ? 11 : 10;
+  auto unit = [&](int k) {
+    if constexpr (WIN) return decode_win_unit<C::HB>(prm, k);
+    else return decode_unit<C::HB>(prm, k);
+  };
   const uint32_t tslot = sbase + C::OFF_TSLOT;
 
   if (threadIdx.x == 0) {
@@ -239,7 +321,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     }
     for (int s = 0; s < C::VST; ++s) {
       mbar_init(BAR_VF(s), 1);
-      mbar_init(BAR_VE(s), 1);
+      mbar_init(BAR_VE(s), WIN ? 2 : 1);  // WIN: the warp that zeroes rows, too
     }
     for (int x = 0; x < 2; ++x) {
       mbar_init(BAR_SF(x), 1);
@@ -255,6 +337,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       mbar_init(BAR_UF(u), 1);
       mbar_init(BAR_UE(u), SCHED_READERS);
     }
+    if constexpr (WIN)
+      for (int s = 0; s < C::VST; ++s) mbar_init(BAR_VZ(s), 1);
     fence_mbar_init();
   }
   if (warp == 1) {
@@ -293,8 +377,10 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
           if (!sched_request(sch, nreq)) break;
           ++nreq;
         }
-        const Unit un = decode_unit<C::HB>(prm, k);
+        const auto un = unit(k);
         const int col0 = un.h * HD;
+        const int kv0 = WIN ? un.h / (prm.win.NH / prm.win.NKV) * HD : col0;  // columns of the K/V head
+        if (WIN && un.nkv == 0) continue;  // only padding
         const int qs = qc % C::QST;
         if (qc >= C::QST && !mbar_wait(BAR_QE(qs), ((qc / C::QST) - 1) & 1, abort_p)) break;
         const int ntile = un.nB > 0 ? 2 : 1;
@@ -305,19 +391,21 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
                         BAR_QF(qs), col0 + kb * 64, (2 * un.pair + x) * BM, un.b);
         ++qc;
         for (int j = 0; j < un.nkv; ++j) {
+          int kt = j;
+          if constexpr (WIN) kt = un.key_tile(j);
           const int ks = kc % C::KST;
           if (kc >= C::KST && !mbar_wait(BAR_KE(ks), ((kc / C::KST) - 1) & 1, abort_p)) { ok = false; break; }
           mbar_arrive_expect_tx(BAR_KF(ks), C::KV_BYTES);
           for (int kb = 0; kb < C::KB; ++kb)
             tma_load_3d(sbase + C::OFF_K + ks * C::KV_BYTES + kb * BN * 128, &tmK, BAR_KF(ks),
-                        col0 + kb * 64, j * BN, un.b);
+                        kv0 + kb * 64, kt * BN, un.b);
           ++kc;
           const int vs = vc % C::VST;
           if (vc >= C::VST && !mbar_wait(BAR_VE(vs), ((vc / C::VST) - 1) & 1, abort_p)) { ok = false; break; }
           mbar_arrive_expect_tx(BAR_VF(vs), C::KV_BYTES);
           for (int kb = 0; kb < C::KB; ++kb)
             tma_load_3d(sbase + C::OFF_V + vs * C::KV_BYTES + kb * BN * 128, &tmV, BAR_VF(vs),
-                        col0 + kb * 64, j * BN, un.b);
+                        kv0 + kb * 64, kt * BN, un.b);
           ++vc;
         }
       }
@@ -335,14 +423,23 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       uint32_t sc[2] = {0, 0};   // S_X issued so far
       uint32_t pvc[2] = {0, 0};  // PV_X issued so far
       uint32_t uc[2] = {0, 0};   // units in which tile X was active
+      uint32_t vzp = 0;          // WIN: bit s = parity of v_fixed[s]'s next phase
       bool ok = true;
       for (int g = 0; ok; ++g) {
         int k;
         if constexpr (DYN) k = sched_unit<false>(sch, g);
         else k = unit_of_round(prm, g);
         if (k < 0) break;
-        const Unit un = decode_unit<C::HB>(prm, k);
+        const auto un = unit(k);
         const int n[2] = {un.nA, un.nB};
+        if (WIN && un.nkv == 0) continue;  // only padding
+        // tile x works on list index j; f[x] is the first it works on
+        auto act = [&](int x, int j) {
+          if constexpr (WIN) return un.active(x, j);
+          else return j < n[x];
+        };
+        int f[2] = {0, 0};
+        if constexpr (WIN) f[1] = un.first(1);
         const int qs = qc % C::QST;
         if (!mbar_wait(BAR_QF(qs), (qc / C::QST) & 1, abort_p)) break;
         // S_X(j) = Q_X K_j^T
@@ -364,7 +461,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         // O_X += P_X V_j
         auto issue_pv = [&](int x, int j) -> bool {
           if (!mbar_wait(BAR_PF(x), pvc[x] & 1, abort_p)) return false;
-          if (j == 0 && uc[x] >= 1 && !mbar_wait(BAR_OE(x), (uc[x] - 1) & 1, abort_p)) return false;
+          if (j == f[x] && uc[x] >= 1 && !mbar_wait(BAR_OE(x), (uc[x] - 1) & 1, abort_p)) return false;
           tc_fence_after();
           const uint32_t sp = sbase + C::OFF_P + x * C::STG_BYTES;
           const uint32_t sv = sbase + C::OFF_V + ((vc + j) % C::VST) * C::KV_BYTES;
@@ -373,10 +470,10 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
             const uint64_t bd = smem_desc_sw128(sv + kk * 2048, BN * 128, 1024);
             if (C::P_TMEM) {  // A = P_X from TMEM: 8 columns per 16 keys
               umma_bf16_ts(tmem + C::TCOL_O + x * HD, tmem + C::TCOL_P + x * (BN / 2) + kk * 8, bd,
-                           IDESC_O, (j > 0 || kk > 0) ? 1u : 0u);
+                           IDESC_O, (j > f[x] || kk > 0) ? 1u : 0u);
             } else {
               const uint64_t ad = smem_desc_sw128(sp + (kk >> 2) * (BM * 128) + (kk & 3) * 32, 16, 1024);
-              umma_bf16_ss(tmem + C::TCOL_O + x * HD, ad, bd, IDESC_O, (j > 0 || kk > 0) ? 1u : 0u);
+              umma_bf16_ss(tmem + C::TCOL_O + x * HD, ad, bd, IDESC_O, (j > f[x] || kk > 0) ? 1u : 0u);
             }
           }
           umma_commit(BAR_PV(x));
@@ -389,10 +486,18 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         };
         auto wait_v = [&](int j) {
           const uint32_t v = vc + j;
-          return mbar_wait(BAR_VF(v % C::VST), (v / C::VST) & 1, abort_p);
+          if (!mbar_wait(BAR_VF(v % C::VST), (v / C::VST) & 1, abort_p)) return false;
+          if constexpr (WIN) {
+            if (un.fix(prm.win, un.key_tile(j) * BN)) {  // warp 2 has zeroed its unseen rows
+              const uint32_t vs = v % C::VST;
+              if (!mbar_wait(BAR_VZ(vs), (vzp >> vs) & 1, abort_p)) return false;
+              vzp ^= 1u << vs;
+            }
+          }
+          return true;
         };
         // prologue: S_A(0), S_B(0); K_0 is consumed once both are done
-        ok = wait_k(0) && issue_s(0, 0) && (n[1] == 0 || issue_s(1, 0));
+        ok = wait_k(0) && issue_s(0, 0) && (!act(1, 0) || issue_s(1, 0));
         if (ok) umma_commit(BAR_KE(kc % C::KST));
         // time-out test hook: with the first products in flight, wait on a
         // barrier nothing arrives at until the hook's limit runs out
@@ -403,13 +508,13 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
             // that), so the next scores are ready before this tile's softmax ends
             if (j + 1 < un.nkv) {
               if (!wait_k(j + 1)) { ok = false; break; }
-              if (j + 1 < n[0] && !issue_s(0, j + 1)) { ok = false; break; }
-              if (j + 1 < n[1] && !issue_s(1, j + 1)) { ok = false; break; }
+              if (act(0, j + 1) && !issue_s(0, j + 1)) { ok = false; break; }
+              if (act(1, j + 1) && !issue_s(1, j + 1)) { ok = false; break; }
               umma_commit(BAR_KE((kc + j + 1) % C::KST));  // K_{j+1} consumed
             }
             if (!wait_v(j)) { ok = false; break; }
-            if (j < n[0] && !issue_pv(0, j)) { ok = false; break; }
-            if (j < n[1] && !issue_pv(1, j)) { ok = false; break; }
+            if (act(0, j) && !issue_pv(0, j)) { ok = false; break; }
+            if (act(1, j) && !issue_pv(1, j)) { ok = false; break; }
           } else {
             // PV_A(j) S_A(j+1) | PV_B(j) S_B(j+1)
             if (!wait_v(j)) { ok = false; break; }
@@ -418,7 +523,11 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
               if (!issue_pv(0, j)) { ok = false; break; }
               if (!lastA && (!wait_k(j + 1) || !issue_s(0, j + 1))) { ok = false; break; }
             }
-            if (j < n[1]) {
+            if constexpr (WIN) {
+              // B may start one tile after A (skip), so its next S does not hang on its PV
+              if (act(1, j) && !issue_pv(1, j)) { ok = false; break; }
+              if (act(1, j + 1) && ((lastA && !wait_k(j + 1)) || !issue_s(1, j + 1))) { ok = false; break; }
+            } else if (j < n[1]) {
               if (!issue_pv(1, j)) { ok = false; break; }
               if (j + 1 < n[1] && ((lastA && !wait_k(j + 1)) || !issue_s(1, j + 1))) { ok = false; break; }
             }
@@ -436,6 +545,47 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       if (*abort_p) {  // wind-down: every UMMA issued must complete before TMEM is freed
         umma_commit(BAR_FIN);
         mbar_wait_for(BAR_FIN, 0, kDrainLimitNs);
+      }
+    } else if (WIN && warp == 2) {
+      // ------------------------------------------------ unseen rows of V
+      if constexpr (WIN) {
+        uint32_t vc = 0;
+        bool ok = true;
+        for (int g = 0; ok; ++g) {
+          const int k = sched_unit<true>(sch, g);
+          if (k < 0) break;
+          const auto un = unit(k);
+          for (int j = 0; ok && j < un.nkv; ++j) {
+            // every tile is waited for and released, so that this warp stays
+            // within one phase of each slot's barriers
+            const int k0 = un.key_tile(j) * BN;
+            const uint32_t v = vc + j, vs = v % C::VST;
+            ok = mbar_wait_warp(BAR_VF(vs), (v / C::VST) & 1, abort_p);
+            if (!ok) break;
+            if (!un.fix(prm.win, k0)) {
+              if (lane == 0) mbar_arrive(BAR_VE(vs));
+              continue;
+            }
+            // rows [a, b) are contiguous in each 64-column block (the swizzle
+            // permutes the chunks of a row within its 128 bytes)
+            auto zero = [&](int a, int b) {
+              for (int kb = 0; kb < C::KB; ++kb) {
+                uint4* blk = reinterpret_cast<uint4*>(gbase + C::OFF_V + vs * C::KV_BYTES + kb * BN * 128);
+                for (int i = a * 8 + lane; i < b * 8; i += 32) blk[i] = make_uint4(0u, 0u, 0u, 0u);
+              }
+            };
+            int a, b;
+            if (un.past_end(prm.win, k0, &a)) zero(a, BN);
+            if (un.out_of_window(prm.win, k0, &a, &b)) zero(a, b);
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              mbar_arrive(BAR_VZ(vs));
+              mbar_arrive(BAR_VE(vs));
+            }
+          }
+          vc += un.nkv;
+        }
       }
     }
   } else {
@@ -459,10 +609,33 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       if constexpr (DYN) k = sched_unit<true>(sch, g);
       else k = unit_of_round(prm, g);
       if (k < 0) break;
-      const Unit un = decode_unit<C::HB>(prm, k);
+      const auto un = unit(k);
       const int nt = x == 0 ? un.nA : un.nB;
-      if (nt == 0) continue;
       const int qtile = 2 * un.pair + x;
+      if constexpr (WIN) {
+        if (nt == 0) {  // only padding: O = 0, l = -inf (rows past T are clipped)
+          if (qtile * BM >= prm.T) continue;
+          if (wg_leader) bulk_wait_read<0>();
+          bar_sync_named(wg_bar, 128);
+          for (int kb = 0; kb < C::KB; ++kb)
+#pragma unroll
+            for (int ch = 0; ch < 8; ++ch)
+              *reinterpret_cast<uint4*>(pbuf + kb * (BM * 128) + row * 128 + ch * 16) = make_uint4(0u, 0u, 0u, 0u);
+          fence_proxy_async_smem();
+          const int grow = qtile * BM + row;
+          if (grow < prm.T) prm.lse[((long long)un.b * prm.T + grow) * prm.NH + un.h] = -INFINITY;
+          bar_sync_named(wg_bar, 128);
+          if (wg_leader) {
+            for (int kb = 0; kb < C::KB; ++kb)
+              tma_store_3d(&tmO, sbase + C::OFF_P + x * C::STG_BYTES + kb * BM * 128, un.h * HD + kb * 64,
+                           qtile * BM, un.b);
+            bulk_commit();
+          }
+          continue;
+        }
+      } else {
+        if (nt == 0) continue;
+      }
       if (C::ZT_BYTES && prm.dQz && wg_leader) {
         // this query tile's dQ slab (128 rows x HD fp32; rows past T are
         // clipped) from the zero tile, by TMA stores that need no waiting for
@@ -484,7 +657,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       // Instantiated twice so that the other tiles carry no masking code.
       auto tile = [&](auto diag_tag, int j) -> bool {
         constexpr bool DIAG = decltype(diag_tag)::value;
-        if constexpr (DIAG && C::P_TMEM) {
+        if constexpr (DIAG && C::P_TMEM && !WIN) {
           // the unit's last key tile: the dO tile of X goes by TMA into the O
           // staging (idle until the epilogue; rows past T read as zero); the
           // epilogue reads each chunk back before writing O over it
@@ -514,7 +687,18 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         }
         tc_fence_before();
         mbar_arrive(BAR_SE(x));
-        if constexpr (DIAG) {
+        if constexpr (WIN) {
+          if constexpr (DIAG) {
+            // key k0 + i is visible up to the row's own position, and from its
+            // window's first key on or among the sinks
+            const int k0 = un.key_tile(j) * BN;
+            const int t = prm.win.pos(un.b, qtile * BM + row);
+            const int up = t - k0, from = t - prm.win.window + 1 - k0, sink = prm.win.sinks - k0;
+#pragma unroll
+            for (int i = 0; i < BN; ++i)
+              if (i > up || (i < from && i >= sink)) s[i] = -INFINITY;
+          }
+        } else if constexpr (DIAG) {
 #pragma unroll
           for (int i = 0; i < BN; ++i)
             if (i > row) s[i] = -INFINITY;
@@ -534,7 +718,9 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         // m_used; O_X is rescaled below, once PV_X(j-1) has completed
         bool rescale = false;
         float alpha = 1.0f;
-        if (j == 0) {
+        bool first = j == 0;
+        if constexpr (WIN) first = j == un.first(x);
+        if (first) {
           m_used = m_new;
         } else {
           const bool need = m_new > m_used + RESCALE_THRESHOLD;
@@ -546,7 +732,9 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
           }
         }
         // P = 2^(S*c - m) with packed fp32x2 FMAs; row sum in 4 packed partials
-        const float2 c2 = make_float2(c, c), nm2 = make_float2(-m_used, -m_used);
+        // (WIN: a row that has seen no key yet has m = -inf and P = 2^-inf = 0)
+        const float base = WIN && m_used == -INFINITY ? 0.0f : m_used;
+        const float2 c2 = make_float2(c, c), nm2 = make_float2(-base, -base);
         float2 ps[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f),
                         make_float2(0.f, 0.f)};
         uint32_t pk[BN / 2];  // P as bf16 pairs, even key in the low half
@@ -561,7 +749,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
                  (ps[3].x + ps[3].y);
         // PV_X(j-1) must be complete before O_X is rescaled and before P_X(j)
         // overwrites P_X (waited for only now, so the exponentials overlap it)
-        if (j >= 1) {
+        if (!first) {
           if (!mbar_wait_warp(BAR_PV(x), (sc - 1) & 1, abort_p)) return false;
           tc_fence_after();
         }
@@ -604,14 +792,20 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         ++sc;
         return true;
       };
-      for (int j = 0; ok && j < nt; ++j)
-        ok = (j == qtile) ? tile(std::true_type{}, j) : tile(std::false_type{}, j);
+      for (int j = 0; ok && j < nt; ++j) {
+        if constexpr (WIN) {
+          if (!un.active(x, j)) continue;
+          ok = un.whole(prm.win, x, un.key_tile(j) * BN) ? tile(std::false_type{}, j) : tile(std::true_type{}, j);
+        } else {
+          ok = (j == qtile) ? tile(std::true_type{}, j) : tile(std::false_type{}, j);
+        }
+      }
       // --------------------------------------------- epilogue of tile X
       const bool epi = ok && mbar_wait_warp(BAR_PV(x), (sc - 1) & 1, abort_p);
       if constexpr (C::P_TMEM) {
         // without dO the epilogue is the staging's first writer in this unit
         // (with dO the warpgroup waits for the dO load, issued after the wait)
-        if (!prm.dO) {
+        if (WIN || !prm.dO) {
           if (wg_leader) bulk_wait_read<0>();
           bar_sync_named(wg_bar, 128);
         }
@@ -620,7 +814,9 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         tc_fence_after();
         const float inv = 1.0f / l_sum;
         const int grow = qtile * BM + row;
-        const bool fuse_d = C::P_TMEM && prm.dO;
+        bool valid = true;
+        if constexpr (WIN) valid = grow < un.n;
+        const bool fuse_d = C::P_TMEM && !WIN && prm.dO;
         bool dok = true;
         if (fuse_d) dok = mbar_wait_warp(BAR_DO(x), nd & 1, abort_p);
         float dsum = 0.0f;
@@ -645,6 +841,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
             v1.y = pack_bf16(__uint_as_float(r[10]) * inv, __uint_as_float(r[11]) * inv);
             v1.z = pack_bf16(__uint_as_float(r[12]) * inv, __uint_as_float(r[13]) * inv);
             v1.w = pack_bf16(__uint_as_float(r[14]) * inv, __uint_as_float(r[15]) * inv);
+            if (WIN && !valid) v0 = v1 = make_uint4(0u, 0u, 0u, 0u);  // a padding row, whatever it computed
             const int kb = cc / 64, ch = (cc % 64) / 8;
             uint8_t* blk = pbuf + kb * (BM * 128) + row * 128;
             uint4* p0 = reinterpret_cast<uint4*>(blk + ((ch ^ (row & 7)) * 16));
@@ -659,7 +856,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         fence_proxy_async_smem();
         if (grow < prm.T) {
           const long long ri = ((long long)un.b * prm.T + grow) * prm.NH + un.h;
-          prm.lse[ri] = (m_used + log2f(l_sum)) * LN2;
+          prm.lse[ri] = WIN && !valid ? -INFINITY : (m_used + log2f(l_sum)) * LN2;
           if (fuse_d && dok) prm.D[ri] = __float2bfloat16_rn(dsum);
         }
         if (fuse_d) ++nd;
@@ -692,21 +889,21 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
 
 // Launches the instantiation DYN (dynamic schedule: one CTA per unit, else
 // one per SM).
-template <int HD, bool DYN>
+template <int HD, bool DYN, bool WIN = false>
 cudaError_t launch_fwd_kernel(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
                               const CUtensorMap& to, const CUtensorMap& tdo, const CUtensorMap& tdqz,
                               const FwdParams& prm, cudaStream_t st) {
-  using C = FwdCfg<HD, DYN>;
+  using C = FwdCfg<HD, DYN, WIN>;
   // The setmaxnreg split assumes the kernel was compiled to exactly
   // LAUNCH_REGS registers per thread; refuse to launch otherwise.
   static const cudaError_t reg_check = [] {
     cudaFuncAttributes a;
-    cudaError_t e = cudaFuncGetAttributes(&a, flash_fwd_kernel<HD, DYN>);
+    cudaError_t e = cudaFuncGetAttributes(&a, flash_fwd_kernel<HD, DYN, WIN>);
     if (e != cudaSuccess) return e;
     return a.numRegs == LAUNCH_REGS ? cudaSuccess : cudaErrorInvalidKernelImage;
   }();
   if (reg_check != cudaSuccess) return reg_check;
-  cudaError_t e = cudaFuncSetAttribute(flash_fwd_kernel<HD, DYN>,
+  cudaError_t e = cudaFuncSetAttribute(flash_fwd_kernel<HD, DYN, WIN>,
                                        cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES);
   if (e != cudaSuccess) return e;
   int grid = prm.nunits;  // dynamic: one CTA per unit (see decode_unit)
@@ -716,7 +913,7 @@ cudaError_t launch_fwd_kernel(const CUtensorMap& tq, const CUtensorMap& tk, cons
     cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
     grid = prm.nunits < sms ? prm.nunits : sms;
   }
-  launch_pdl(flash_fwd_kernel<HD, DYN>, grid, NUM_THREADS, C::SMEM_BYTES, st, tq, tk, tv, to, tdo, tdqz, prm);
+  launch_pdl(flash_fwd_kernel<HD, DYN, WIN>, grid, NUM_THREADS, C::SMEM_BYTES, st, tq, tk, tv, to, tdo, tdqz, prm);
   count_launches(1);
   return cudaGetLastError();
 }
@@ -766,7 +963,36 @@ cudaError_t launch_fwd(const __nv_bfloat16* q, const __nv_bfloat16* k, const __n
   return launch_fwd_kernel<HD, false>(tq, tk, tv, to, tdo, tdqz, prm, st);
 }
 
+template <int HD>
+cudaError_t launch_win(const WindowArgs& a, cudaStream_t st) {
+  CUtensorMap tq, tk, tv, to;
+  const CUtensorMapDataType bf = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  const CUtensorMapSwizzle sw = CU_TENSOR_MAP_SWIZZLE_128B;
+  const uint64_t n = (uint64_t)a.NH * HD, nkv = (uint64_t)a.NKV * HD;
+  if (!make_tmap_3d(&tq, a.q, bf, 2, n, a.M, a.B, 64, BM, sw) ||
+      !make_tmap_3d(&tk, a.k, bf, 2, nkv, a.K, a.B, 64, BN, sw) ||
+      !make_tmap_3d(&tv, a.v, bf, 2, nkv, a.K, a.B, 64, BN, sw) ||
+      !make_tmap_3d(&to, a.out, bf, 2, n, a.M, a.B, 64, BM, sw))
+    return cudaErrorInvalidValue;
+  FwdParams prm{};
+  prm.T = a.M;
+  prm.NH = a.NH;
+  prm.nbh = a.B * a.NH;
+  prm.nqt = (a.M + BM - 1) / BM;
+  prm.npairs = (prm.nqt + 1) / 2;
+  prm.nunits = prm.npairs * prm.nbh;
+  prm.scale_log2 = LOG2E / sqrtf((float)HD);
+  prm.lse = a.l;
+  prm.status = a.status;
+  prm.win = a;
+  return launch_fwd_kernel<HD, true, true>(tq, tk, tv, to, tq, tq, prm, st);
+}
+
 }  // namespace
+
+cudaError_t launch_window_fwd(const WindowArgs& a, cudaStream_t st) {
+  return a.D == 64 ? launch_win<64>(a, st) : launch_win<128>(a, st);
+}
 
 cudaError_t launch_flash_fwd(const __nv_bfloat16* q, const __nv_bfloat16* k,
                              const __nv_bfloat16* v, __nv_bfloat16* out, float* lse,

@@ -37,46 +37,6 @@ __device__ __forceinline__ float dot(const float (&a)[E], const float (&b)[E]) {
   return warp_sum(s);
 }
 
-template <int HD>
-__global__ void __launch_bounds__(256) window_fwd_rows(const WindowArgs a) {
-  pdl_wait_and_release();
-  constexpr int E = HD / 32;
-  const int lane = threadIdx.x % 32;
-  const long long items = (long long)a.B * a.M * a.NH;
-  for (long long it = blockIdx.x * 8ll + threadIdx.x / 32; it < items; it += gridDim.x * 8ll) {
-    const int h = (int)(it % a.NH);
-    const long long row = it / a.NH;
-    const int b = (int)(row / a.M), i = (int)(row % a.M);
-    const int kh = h / (a.NH / a.NKV);
-    float q[E], o[E] = {};
-    load_row<E>(a.q + it * HD, lane, q);
-    float m = -INFINITY, l = 0.0f;
-    if (i < a.len(b)) {
-      const int pos = a.pos(b, i);
-      const int low = max(0, pos - a.window + 1);
-      const int ns = min(a.sinks, low);
-      for (int n = 0; n < ns + pos + 1 - low; ++n) {
-        const int j = n < ns ? n : low + n - ns;
-        const long long off = (((long long)b * a.K + j) * a.NKV + kh) * HD;
-        float k[E], v[E];
-        load_row<E>(a.k + off, lane, k);
-        load_row<E>(a.v + off, lane, v);
-        const float s = dot<E>(q, k) * a.scale;
-        const float mn = fmaxf(m, s);
-        const float alpha = exp2f((m - mn) * LOG2E), p = exp2f((s - mn) * LOG2E);
-        m = mn;
-        l = l * alpha + p;
-#pragma unroll
-        for (int e = 0; e < E; ++e) o[e] = o[e] * alpha + p * v[e];
-      }
-    }
-    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-#pragma unroll
-    for (int e = 0; e < E; ++e) a.out[it * HD + lane + 32 * e] = __float2bfloat16_rn(o[e] * inv);
-    if (lane == 0) a.l[it] = l > 0.0f ? m + logf(l) : -INFINITY;
-  }
-}
-
 // delta and dQ of a row
 template <int HD>
 __global__ void __launch_bounds__(256) window_bwd_dq_rows(const WindowArgs a, const WindowGrads g) {
@@ -164,13 +124,6 @@ unsigned row_blocks(long long items) {
 }
 
 }  // namespace
-
-cudaError_t launch_window_fwd(const WindowArgs& a, cudaStream_t st) {
-  const unsigned grid = row_blocks((long long)a.B * a.M * a.NH);
-  launch_pdl(a.D == 64 ? window_fwd_rows<64> : window_fwd_rows<128>, grid, 256, 0, st, a);
-  count_launches(1);
-  return cudaGetLastError();
-}
 
 size_t window_cached_workspace(const WindowArgs&) { return 0; }
 
