@@ -68,9 +68,24 @@
 // here S, dP, dQ and dK/dV stay fp32 until their single store, and P, dS are
 // bf16 (the UMMA operand type).
 //
+// WIN: the same kernel for windowAttentionBackward (sliding window, sinks,
+// grouped K/V heads, sequence lengths).  A unit is a key tile of a K/V head;
+// its steps are the query tiles that can see it, for each query head of the
+// group, so shared heads' gradients are summed in the accumulators.  A sink
+// tile is seen by every later query: what lies past its window is cut into
+// units of their own where that chain would be the longest (WinBwd), whose
+// partial dK/dV the launcher's last kernel adds up in a fixed order.  The
+// statistics come ready from a kernel before this one, [B][NH][T], and the
+// warp that stages them also zeroes the padding rows of Q, dO and K tiles
+// (their P and dS are 0, but 0 * NaN is not).  A unit or chunk without a
+// valid row runs one step in which everything is masked and so writes zeros.
+//
 // All mbarrier waits are bounded (about 2 s); on time-out the CTA winds down,
 // frees its TMEM and sets STATUS_BWD_TIMEOUT.  Warps meet only at mbarriers
 // (no named barriers), so a failed wait cannot leave a warp stuck at one.
+#include <algorithm>
+#include <type_traits>
+
 #include "common.cuh"
 #include "sm100.cuh"
 #include "tmap.h"
@@ -86,7 +101,7 @@ constexpr int PERSIST_MAX_NKT = 16;  // static schedule when T/128 <= this (D=64
 constexpr float LOG2E = 1.4426950408889634f;
 
 
-template <int HD, bool PERSIST>
+template <int HD, bool PERSIST, bool WIN = false>
 struct BwdCfg {
   static constexpr int KB = HD / 64;
   static constexpr bool D64 = HD == 64;
@@ -163,8 +178,9 @@ struct BwdCfg {
   // kv_full/empty[KVB], qd_full/empty[S], st_full/empty[8], then s_full,
   // s_free, p_ready, p_free, dq_full, dq_free, dqs_full, dqs_free, done,
   // acc_free, never (nothing arrives: the time-out test hook), fin (the
-  // UMMA issuer's wind-down), sched_full/empty[NSCHED]
-  static constexpr int NBAR = 2 * KVB + 2 * STAGES + 2 * SSTG + 12 + 2 * (DQSB - 1) + 2 * NSCHED;
+  // UMMA issuer's wind-down), sched_full/empty[NSCHED] and, for WIN,
+  // qd_fixed[S] (padding rows zeroed)
+  static constexpr int NBAR = 2 * KVB + 2 * STAGES + 2 * SSTG + 12 + 2 * (DQSB - 1) + 2 * NSCHED + (WIN ? STAGES : 0);
   static constexpr uint32_t OFF_TSLOT = OFF_BAR + NBAR * 8;
   static constexpr uint32_t SMEM_BYTES = OFF_TSLOT + 16 + 1024;
   static constexpr uint32_t TCOL_S = 0;
@@ -175,6 +191,20 @@ struct BwdCfg {
   static constexpr uint32_t TCOL_PT = 256 + 3 * HD;  // D=64 only: 64 columns of bf16 pairs
 };
 
+// What the window adds.  Sink tiles 0 .. nsplit-1 are split: their query
+// tiles past the window go, far_tiles at a time, to nfar units each; unit
+// `slot`s of part hold 2 x 128 x D fp32 partial sums (dV, dK), slot 0 of a
+// tile its window's.
+struct WinBwd {
+  const int32_t* lens;
+  int G, window, sinks;
+  int nsplit, nfar, far_tiles;
+  int nfar_units;              // nsplit * nfar * (batch, K/V head) pairs, dealt first
+  int rows;                    // rows of a (batch, head) in the statistics
+  const float *neg_l, *neg_d;  // -l*log2e, -D/sqrt(D)
+  float* part;
+};
+
 struct BwdParams {
   int T, N, NH, bh_begin, nbh, nkt, nunits;
   float scale, scale_log2;
@@ -182,6 +212,7 @@ struct BwdParams {
   const __nv_bfloat16* Dv;
   uint32_t* status;
   uint32_t expire_ns;  // time-out test hook (ma_debug_expire_next_wait), 0 = off
+  WinBwd win;          // WIN only
 };
 
 // Unit k -> (batch, head, key tile); its query tiles are kt .. nkt-1.  Block
@@ -189,6 +220,27 @@ struct BwdParams {
 // block), key tile-major; HB = 1 is (batch, head)-major.
 struct BUnit {
   int b, h, kt, nq;
+  __device__ int q_tile(int i) const { return kt + i; }
+  __device__ int q_head(int) const { return h; }
+};
+
+// A unit under a window: nt query tiles from q0 on, for each query head.
+struct WinBUnit {
+  int b, h, kt, nq;
+  int q0, nt, head0;
+  int n;     // valid rows; 0 where the unit has none: everything is masked
+  int slot;  // partial sums go to this slot, or -1: straight to dK, dV
+  __device__ int q_tile(int i) const { return q0 + i % nt; }
+  __device__ int q_head(int i) const { return head0 + i / nt; }
+  // key `key` sees queries [*from, *to) of the query tile at row0
+  __device__ void seen(const WinBwd& w, int key, int row0, int* from, int* to) const {
+    *from = key - row0;
+    *to = (key < w.sinks ? n : min(n, key + w.window)) - row0;
+  }
+  __device__ bool whole(const WinBwd& w, int row0) const {
+    const int k0 = kt * BK;
+    return k0 + BK - 1 <= row0 && (row0 + BQ - 1 - k0 < w.window || k0 + BK - 1 < w.sinks) && row0 + BQ <= n;
+  }
 };
 
 template <int HB>
@@ -211,6 +263,51 @@ __device__ __forceinline__ BUnit bwd_unit(const BwdParams& prm, int k) {
   return u;
 }
 
+template <int HB>
+__device__ __forceinline__ WinBUnit bwd_win_unit(const BwdParams& prm, int k) {
+  const WinBwd& w = prm.win;
+  WinBUnit u;
+  const bool far = k < w.nfar_units;
+  int c = 0;
+  if (far) {
+    const int bh = k % prm.nbh, r = k / prm.nbh;
+    u.b = bh / prm.NH;
+    u.h = bh % prm.NH;
+    u.kt = r % w.nsplit;
+    c = r / w.nsplit;
+  } else {
+    const BUnit p = bwd_unit<HB>(prm, k - w.nfar_units);
+    u.b = p.b;
+    u.h = p.h;
+    u.kt = p.kt;
+  }
+  u.head0 = u.h * w.G;
+  u.n = w.lens ? min(max(__ldg(w.lens + u.b), 0), prm.T) : prm.T;
+  const bool split = u.kt < w.nsplit;
+  u.slot = split ? ((u.b * prm.NH + u.h) * w.nsplit + u.kt) * (1 + w.nfar) + (far ? 1 + c : 0) : -1;
+  const int k0 = u.kt * BK;
+  const int last = (u.n - 1) / BQ;                     // the last query tile with a valid row
+  const int win_last = (k0 + BK - 1 + w.window - 1) / BQ;  // and the last in the window
+  u.q0 = far ? win_last + 1 + c * w.far_tiles : u.kt;
+  int end = last;
+  if (far) end = min(last, u.q0 + w.far_tiles - 1);
+  else if (split || k0 >= w.sinks) end = min(last, win_last);
+  u.nt = end - u.q0 + 1;
+  u.nq = u.nt * w.G;
+  if (u.nt <= 0 || u.n <= k0) {
+    u.n = 0;
+    u.q0 = u.kt;
+    u.nt = u.nq = 1;
+  }
+  return u;
+}
+
+template <int HB, bool WIN>
+__device__ __forceinline__ auto decode_bwd_unit(const BwdParams& prm, int k) {
+  if constexpr (WIN) return bwd_win_unit<HB>(prm, k);
+  else return bwd_unit<HB>(prm, k);
+}
+
 // Static schedule: the unit of this CTA in round g, -1 when rounds are
 // exhausted, -2 when this CTA has none in round g (last, partial round).
 __device__ __forceinline__ int bwd_unit_of_round(const BwdParams& prm, int g) {
@@ -223,21 +320,22 @@ __device__ __forceinline__ int bwd_unit_of_round(const BwdParams& prm, int g) {
 
 // Walks this CTA's (unit, query tile) steps in order.  t counts steps over
 // all units, uc counts units.
+template <bool WIN>
 struct StepIter {
   int g;        // dynamic: units fetched; static: next round to look at
-  BUnit u;
-  int i;        // query tile index within the unit
+  std::conditional_t<WIN, WinBUnit, BUnit> u;
+  int i;        // step within the unit
   uint32_t t;   // global step
   uint32_t uc;  // unit counter
   bool valid;
 };
 
-template <bool DYN, int HB, bool WARP>
-__device__ __forceinline__ bool next_unit(const BwdParams& prm, StepIter& s, const Sched& sc) {
+template <bool DYN, int HB, bool WIN, bool WARP>
+__device__ __forceinline__ bool next_unit(const BwdParams& prm, StepIter<WIN>& s, const Sched& sc) {
   if constexpr (DYN) {
     const int k = sched_unit<WARP>(sc, (uint32_t)s.g++);
     if (k < 0 || k >= prm.nunits) return false;
-    s.u = bwd_unit<HB>(prm, k);
+    s.u = decode_bwd_unit<HB, WIN>(prm, k);
     return true;
   } else {
     for (;;) {
@@ -245,26 +343,26 @@ __device__ __forceinline__ bool next_unit(const BwdParams& prm, StepIter& s, con
       if (k == -1) return false;
       ++s.g;
       if (k >= 0) {
-        s.u = bwd_unit<HB>(prm, k);
+        s.u = decode_bwd_unit<HB, WIN>(prm, k);
         return true;
       }
     }
   }
 }
 
-template <bool DYN, int HB, bool WARP>
-__device__ __forceinline__ StepIter first_step(const BwdParams& prm, const Sched& sc) {
-  StepIter s;
+template <bool DYN, int HB, bool WIN, bool WARP>
+__device__ __forceinline__ StepIter<WIN> first_step(const BwdParams& prm, const Sched& sc) {
+  StepIter<WIN> s;
   s.g = 0;
   s.i = 0;
   s.t = 0;
   s.uc = 0;
-  s.valid = next_unit<DYN, HB, WARP>(prm, s, sc);
+  s.valid = next_unit<DYN, HB, WIN, WARP>(prm, s, sc);
   return s;
 }
 
-template <bool DYN, int HB, bool WARP>
-__device__ __forceinline__ void advance(const BwdParams& prm, StepIter& s, const Sched& sc) {
+template <bool DYN, int HB, bool WIN, bool WARP>
+__device__ __forceinline__ void advance(const BwdParams& prm, StepIter<WIN>& s, const Sched& sc) {
   ++s.t;
   if (s.i + 1 < s.u.nq) {
     ++s.i;
@@ -272,7 +370,7 @@ __device__ __forceinline__ void advance(const BwdParams& prm, StepIter& s, const
   }
   s.i = 0;
   ++s.uc;
-  s.valid = next_unit<DYN, HB, WARP>(prm, s, sc);
+  s.valid = next_unit<DYN, HB, WIN, WARP>(prm, s, sc);
 }
 
 // P^T and dS^T for N query columns of one key row.  s[] holds S^T on entry
@@ -311,6 +409,27 @@ __device__ __forceinline__ void p_ds_row(float (&s)[N], float (&dp)[N], const fl
   }
 }
 
+// The window's masked form: query column qcol0 + j is seen when from <= it <
+// to, else P and dS are 0 whatever the products hold.
+template <int N>
+__device__ __forceinline__ void p_ds_row_window(float (&s)[N], float (&dp)[N], const float* nl, const float* nd,
+                                                float c, float sc, int from, int to) {
+#pragma unroll
+  for (int j = 0; j < N; j += 4) {
+    const float4 L = *reinterpret_cast<const float4*>(nl + j);
+    const float4 Dn = *reinterpret_cast<const float4*>(nd + j);
+    const float l[4] = {L.x, L.y, L.z, L.w}, d[4] = {Dn.x, Dn.y, Dn.z, Dn.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const bool see = j + e >= from && j + e < to;
+      const float p = ex2(fmaf(s[j + e], c, l[e]));
+      const float r = p * fmaf(dp[j + e], sc, d[e]);
+      s[j + e] = see ? p : 0.0f;
+      dp[j + e] = see ? r : 0.0f;
+    }
+  }
+}
+
 // N bf16 values of one row as N/8 swizzled 16-byte chunks of a K-major SW128
 // row, starting at chunk ch0 (row base `rowp`, swizzle phase `row & 7`).
 template <int N>
@@ -327,14 +446,14 @@ __device__ __forceinline__ void store_row_sw128(uint8_t* rowp, int row, const fl
   }
 }
 
-template <int HD, bool PERSIST>
-__global__ void __launch_bounds__(BwdCfg<HD, PERSIST>::NUM_THREADS, 1)
+template <int HD, bool PERSIST, bool WIN>
+__global__ void __launch_bounds__(BwdCfg<HD, PERSIST, WIN>::NUM_THREADS, 1)
     flash_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                      const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmdO,
                      const __grid_constant__ CUtensorMap tmdQ, __nv_bfloat16* __restrict__ dK,
                      __nv_bfloat16* __restrict__ dV, const BwdParams prm) {
   pdl_wait_and_release();
-  using C = BwdCfg<HD, PERSIST>;
+  using C = BwdCfg<HD, PERSIST, WIN>;
   extern __shared__ uint8_t smem_raw[];
   __shared__ int abort_flag;
   const uint32_t raw = smem_u32(smem_raw);
@@ -364,6 +483,7 @@ __global__ void __launch_bounds__(BwdCfg<HD, PERSIST>::NUM_THREADS, 1)
   const uint32_t BAR_FIN = BAR_SF + 88;   // the UMMA issuer's last commit (wind-down)
   const uint32_t BAR_UF = BAR_SF + 96 + 16u * (C::DQSB - 1);  // sched_full[NSCHED], then sched_empty
   const uint32_t BAR_UE = BAR_UF + 8u * C::NSCHED;
+  auto BAR_QZ = [&](int s) { return BAR_UE + 8u * (C::NSCHED + s); };  // WIN: padding rows of stage s zeroed
   const uint32_t tslot = sbase + C::OFF_TSLOT;
   float* stat_base = reinterpret_cast<float*>(gbase + C::OFF_STAT);
 
@@ -371,11 +491,12 @@ __global__ void __launch_bounds__(BwdCfg<HD, PERSIST>::NUM_THREADS, 1)
     abort_flag = 0;
     for (int s = 0; s < C::KVB; ++s) {
       mbar_init(BAR_KF(s), 1);
-      mbar_init(BAR_KE(s), 1);
+      mbar_init(BAR_KE(s), WIN ? 2 : 1);  // WIN: the warp that zeroes rows, too
     }
     for (int s = 0; s < C::STAGES; ++s) {
       mbar_init(BAR_QF(s), 1);
-      mbar_init(BAR_QE(s), 1);
+      mbar_init(BAR_QE(s), WIN ? 2 : 1);
+      if constexpr (WIN) mbar_init(BAR_QZ(s), 1);
     }
     for (int s = 0; s < C::SSTG; ++s) {
       mbar_init(BAR_TF(s), 32);
@@ -412,6 +533,17 @@ __global__ void __launch_bounds__(BwdCfg<HD, PERSIST>::NUM_THREADS, 1)
   volatile int* abort_p = &abort_flag;
   const Sched sch{sbase + C::OFF_SCHED, BAR_UF, BAR_UE, abort_p};  // the unit schedule
 
+  // WIN: whether step s brings tiles with padding rows (a unit's first step:
+  // its K tile too); past the tensor's end TMA has filled in zeros itself
+  auto fix_q = [&](const StepIter<WIN>& s) {
+    if constexpr (WIN) return s.u.n < prm.T && s.u.q_tile(s.i) * BQ + BQ > s.u.n;
+    else return false;
+  };
+  auto fix_k = [&](const StepIter<WIN>& s) {
+    if constexpr (WIN) return s.i == 0 && s.u.n < prm.T && s.u.kt * BK + BK > s.u.n;
+    else return false;
+  };
+
   if (warp < 4) {
     reg_dealloc<C::REGS_PRODUCER>();
     if (warp == 0) {
@@ -421,8 +553,8 @@ __global__ void __launch_bounds__(BwdCfg<HD, PERSIST>::NUM_THREADS, 1)
         tma_prefetch_desc(&tmdO);
         uint32_t kv_armed = 0, q_armed = 0;  // loads issued into each ring
         uint32_t nreq = 0;                   // launch-control requests issued
-        for (StepIter s = first_step<C::DYN, C::HB, false>(prm, sch); s.valid; advance<C::DYN, C::HB, false>(prm, s, sch)) {
-          const int col0 = s.u.h * HD;
+        for (StepIter<WIN> s = first_step<C::DYN, C::HB, WIN, false>(prm, sch); s.valid; advance<C::DYN, C::HB, WIN, false>(prm, s, sch)) {
+          const int kv0 = s.u.h * HD, col0 = s.u.q_head(s.i) * HD;
           if (s.i == 0) {  // K/V of a new unit
             const int kvs = s.uc % C::KVB;
             if (s.uc >= C::KVB && !mbar_wait(BAR_KE(kvs), ((s.uc / C::KVB) - 1) & 1, abort_p)) break;
@@ -430,14 +562,14 @@ __global__ void __launch_bounds__(BwdCfg<HD, PERSIST>::NUM_THREADS, 1)
             ++kv_armed;
             for (int kb = 0; kb < C::KB; ++kb) {
               tma_load_3d(sbase + C::OFF_K + kvs * C::KV_BYTES + kb * BK * 128, &tmK, BAR_KF(kvs),
-                          col0 + kb * 64, s.u.kt * BK, s.u.b);
+                          kv0 + kb * 64, s.u.kt * BK, s.u.b);
               tma_load_3d(sbase + C::OFF_V + kvs * C::KV_BYTES + kb * BK * 128, &tmV, BAR_KF(kvs),
-                          col0 + kb * 64, s.u.kt * BK, s.u.b);
+                          kv0 + kb * 64, s.u.kt * BK, s.u.b);
             }
           }
           const int st = s.t % C::STAGES;
           if (s.t >= C::STAGES && !mbar_wait(BAR_QE(st), ((s.t / C::STAGES) - 1) & 1, abort_p)) break;
-          const int qt = s.u.kt + s.i;
+          const int qt = s.u.q_tile(s.i);
           mbar_arrive_expect_tx(BAR_QF(st), 2 * C::QD_BYTES);
           ++q_armed;
           for (int kb = 0; kb < C::KB; ++kb) {
@@ -466,12 +598,19 @@ __global__ void __launch_bounds__(BwdCfg<HD, PERSIST>::NUM_THREADS, 1)
         constexpr uint32_t IDESC_KV = idesc_bf16_f32(BK, HD, 0, 1);  // dV, dK
         constexpr uint32_t IDESC_Q = idesc_bf16_f32(BQ, HD, 1, 1);   // dQ
         const uint32_t spt = sbase + C::OFF_PT, sdst = sbase + C::OFF_DST;
+        uint32_t qzp = 0;  // WIN: bit s = parity of qd_fixed[s]'s next phase
         // S^T and dP^T of step s into their TMEM columns
-        auto issue_s = [&](const StepIter& s) -> bool {
+        auto issue_s = [&](const StepIter<WIN>& s) -> bool {
           const int st = s.t % C::STAGES;
           const int kvs = s.uc % C::KVB;
           if (s.i == 0 && !mbar_wait(BAR_KF(kvs), (s.uc / C::KVB) & 1, abort_p)) return false;
           if (!mbar_wait(BAR_QF(st), (s.t / C::STAGES) & 1, abort_p)) return false;
+          if constexpr (WIN) {
+            if (fix_q(s) || fix_k(s)) {  // warp 2 has zeroed the padding rows
+              if (!mbar_wait(BAR_QZ(st), (qzp >> st) & 1, abort_p)) return false;
+              qzp ^= 1u << st;
+            }
+          }
           if (s.t >= 1 && !mbar_wait(BAR_SE, (s.t - 1) & 1, abort_p)) return false;
           if (C::DQ_ALIAS && s.t >= 1 && !mbar_wait(BAR_DQE, (s.t - 1) & 1, abort_p)) return false;
           tc_fence_after();
@@ -494,24 +633,24 @@ __global__ void __launch_bounds__(BwdCfg<HD, PERSIST>::NUM_THREADS, 1)
           umma_commit(BAR_SF);
           return true;
         };
-        StepIter cur = first_step<C::DYN, C::HB, false>(prm, sch);
-        StepIter la = cur;  // next step whose S^T/dP^T is to be issued
+        StepIter<WIN> cur = first_step<C::DYN, C::HB, WIN, false>(prm, sch);
+        StepIter<WIN> la = cur;  // next step whose S^T/dP^T is to be issued
         bool ok = true;
         if (la.valid) {
           ok = issue_s(la);
-          advance<C::DYN, C::HB, false>(prm, la, sch);
+          advance<C::DYN, C::HB, WIN, false>(prm, la, sch);
         }
         // time-out test hook: with the first products in flight, wait on a
         // barrier nothing arrives at until the hook's limit runs out
         if (ok && prm.expire_ns) ok = mbar_wait(BAR_NEVER, 0, abort_p, prm.expire_ns);
-        for (; ok && cur.valid; advance<C::DYN, C::HB, false>(prm, cur, sch)) {
+        for (; ok && cur.valid; advance<C::DYN, C::HB, WIN, false>(prm, cur, sch)) {
           // the next step's S^T/dP^T ahead of this step's products, except
           // where it starts a unit whose K/V can only be loaded into the
           // single K/V buffer once this step's products are done with it
           const bool early = C::EARLY_S && la.valid && (C::KVB > 1 || la.uc == cur.uc);
           if (early) {
             if (!issue_s(la)) break;
-            advance<C::DYN, C::HB, false>(prm, la, sch);
+            advance<C::DYN, C::HB, WIN, false>(prm, la, sch);
           }
           const int st = cur.t % C::STAGES;
           const int kvs = cur.uc % C::KVB;
@@ -558,7 +697,7 @@ __global__ void __launch_bounds__(BwdCfg<HD, PERSIST>::NUM_THREADS, 1)
           // (after them: D=128, or a unit start with a single K/V buffer)
           if ((!C::EARLY_S || C::KVB == 1) && !early && la.valid) {
             if (!issue_s(la)) break;
-            advance<C::DYN, C::HB, false>(prm, la, sch);
+            advance<C::DYN, C::HB, WIN, false>(prm, la, sch);
           }
         }
         if (*abort_p) {  // wind-down: every UMMA issued must complete before TMEM is freed
@@ -572,29 +711,69 @@ __global__ void __launch_bounds__(BwdCfg<HD, PERSIST>::NUM_THREADS, 1)
       // are loaded into registers one step ahead, so the ring slot is filled
       // as soon as the compute warps free it, whatever the load latency.
       float nl[4], nd[4];
-      auto load_stats = [&](const StepIter& s) {
-        const int qt = s.u.kt + s.i;
-        const long long rbase = (long long)s.u.b * prm.T;
+      auto load_stats = [&](const StepIter<WIN>& s) {
+        const int qt = s.u.q_tile(s.i);
+        if constexpr (WIN) {  // prepared, padded to whole tiles
+          const int heads = prm.NH * prm.win.G;
+          const long long si = ((long long)s.u.b * heads + s.u.q_head(s.i)) * prm.win.rows + qt * BQ + lane * 4;
+          const float4 L = __ldg(reinterpret_cast<const float4*>(prm.win.neg_l + si));
+          const float4 D4 = __ldg(reinterpret_cast<const float4*>(prm.win.neg_d + si));
+          nl[0] = L.x, nl[1] = L.y, nl[2] = L.z, nl[3] = L.w;
+          nd[0] = D4.x, nd[1] = D4.y, nd[2] = D4.z, nd[3] = D4.w;
+        } else {
+          const long long rbase = (long long)s.u.b * prm.T;
 #pragma unroll
-        for (int v = 0; v < 4; ++v) {
-          const int q = qt * BQ + lane * 4 + v;
-          nl[v] = 0.0f;
-          nd[v] = 0.0f;
-          if (q < prm.T) {
-            const long long si = (rbase + q) * prm.NH + s.u.h;
-            nl[v] = -__ldg(prm.lse + si) * LOG2E;
-            nd[v] = -__bfloat162float(prm.Dv[si]) * prm.scale;
+          for (int v = 0; v < 4; ++v) {
+            const int q = qt * BQ + lane * 4 + v;
+            nl[v] = 0.0f;
+            nd[v] = 0.0f;
+            if (q < prm.T) {
+              const long long si = (rbase + q) * prm.NH + s.u.h;
+              nl[v] = -__ldg(prm.lse + si) * LOG2E;
+              nd[v] = -__bfloat162float(prm.Dv[si]) * prm.scale;
+            }
           }
         }
       };
-      StepIter s = first_step<C::DYN, C::HB, true>(prm, sch);
+      // WIN: rows [a, 128) of a tile are contiguous in each 64-column block
+      // (the swizzle permutes the chunks of a row within its 128 bytes)
+      auto zero_rows = [&](uint32_t off, int a) {
+        for (int kb = 0; kb < C::KB; ++kb) {
+          uint4* blk = reinterpret_cast<uint4*>(gbase + off + kb * BQ * 128);
+          for (int i = a * 8 + lane; i < BQ * 8; i += 32) blk[i] = make_uint4(0u, 0u, 0u, 0u);
+        }
+      };
+      StepIter<WIN> s = first_step<C::DYN, C::HB, WIN, true>(prm, sch);
       if (s.valid) load_stats(s);
       while (s.valid) {
         const float cl[4] = {nl[0], nl[1], nl[2], nl[3]};
         const float cd[4] = {nd[0], nd[1], nd[2], nd[3]};
-        StepIter nx = s;
-        advance<C::DYN, C::HB, true>(prm, nx, sch);
+        StepIter<WIN> nx = s;
+        advance<C::DYN, C::HB, WIN, true>(prm, nx, sch);
         if (nx.valid) load_stats(nx);  // the next step's, in flight while this one waits
+        if constexpr (WIN) {
+          // every stage (and a unit's K/V) is waited for and released, so that
+          // this warp stays within one phase of each slot's barriers
+          const int qs = s.t % C::STAGES, kvs = s.uc % C::KVB;
+          if (s.i == 0 && !mbar_wait_warp(BAR_KF(kvs), (s.uc / C::KVB) & 1, abort_p)) break;
+          if (!mbar_wait_warp(BAR_QF(qs), (s.t / C::STAGES) & 1, abort_p)) break;
+          const bool fq = fix_q(s), fk = fix_k(s);
+          if (fk) zero_rows(C::OFF_K + kvs * C::KV_BYTES, max(0, s.u.n - s.u.kt * BK));
+          if (fq) {
+            const int a = max(0, s.u.n - s.u.q_tile(s.i) * BQ);
+            zero_rows(C::OFF_Q + qs * C::QD_BYTES, a);
+            zero_rows(C::OFF_DO + qs * C::QD_BYTES, a);
+          }
+          if (fq || fk) {
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(BAR_QZ(qs));
+          }
+          if (lane == 0) {
+            mbar_arrive(BAR_QE(qs));
+            if (s.i == 0) mbar_arrive(BAR_KE(kvs));
+          }
+        }
         const int st = s.t % C::SSTG;
         if (s.t >= C::SSTG && !mbar_wait_warp(BAR_TE(st), ((s.t / C::SSTG) - 1) & 1, abort_p)) break;
         float* stt = stat_base + st * (2 * BQ);
@@ -609,12 +788,12 @@ __global__ void __launch_bounds__(BwdCfg<HD, PERSIST>::NUM_THREADS, 1)
     } else {
       // ------------------------------------------------- dQ reduce issuer
       if (lane == 0) {
-        for (StepIter s = first_step<C::DYN, C::HB, false>(prm, sch); s.valid; advance<C::DYN, C::HB, false>(prm, s, sch)) {
+        for (StepIter<WIN> s = first_step<C::DYN, C::HB, WIN, false>(prm, sch); s.valid; advance<C::DYN, C::HB, WIN, false>(prm, s, sch)) {
           const int b = s.t % C::DQSB;
           if (!mbar_wait(BAR_DSF(b), (s.t / C::DQSB) & 1, abort_p)) break;
           for (int box = 0; box < HD / 32; ++box)
             tma_reduce_add_3d(&tmdQ, sbase + C::OFF_DQS + b * C::DQS_BYTES + box * (BQ * 128),
-                              s.u.h * HD + box * 32, (s.u.kt + s.i) * BQ, s.u.b);
+                              s.u.q_head(s.i) * HD + box * 32, s.u.q_tile(s.i) * BQ, s.u.b);
           bulk_commit();
           // the reduction DQSB-1 steps back has read its buffer, which may
           // now be rewritten (with one buffer: this step's)
@@ -671,7 +850,7 @@ __global__ void __launch_bounds__(BwdCfg<HD, PERSIST>::NUM_THREADS, 1)
     // registers; frees the accumulators (BAR_ACC) for the next unit, then
     // converts to bf16 and stores this thread's row slice straight to global
     // memory (rows past T are not stored)
-    auto epilogue = [&](const BUnit& v, uint32_t vuc) {
+    auto epilogue = [&](const auto& v, uint32_t vuc) {
       if (ok) ok = mbar_wait_warp(BAR_DONE, vuc & 1, abort_p);
       if (!ok) return;
       tc_fence_after();
@@ -692,6 +871,20 @@ __global__ void __launch_bounds__(BwdCfg<HD, PERSIST>::NUM_THREADS, 1)
       tc_fence_before();
       mbar_arrive(BAR_ACC);  // the next unit may overwrite dK/dV in TMEM
       const int key = v.kt * BK + krow;
+      if constexpr (WIN) {
+        if (v.slot >= 0) {  // partial sums, fp32
+#pragma unroll
+          for (int which = 0; which < 2; ++which) {
+            float4* dst = reinterpret_cast<float4*>(
+                prm.win.part + (((long long)v.slot * 2 + which) * BK + krow) * HD + part * CPH);
+#pragma unroll
+            for (int cc = 0; cc < CPH; cc += 4)
+              dst[cc / 4] = make_float4(__uint_as_float(acc[which][cc + 0]), __uint_as_float(acc[which][cc + 1]),
+                                        __uint_as_float(acc[which][cc + 2]), __uint_as_float(acc[which][cc + 3]));
+          }
+          return;
+        }
+      }
       if (key < prm.T) {
         const long long off = ((long long)v.b * prm.T + key) * prm.N + v.h * HD + part * CPH;
 #pragma unroll
@@ -713,11 +906,11 @@ __global__ void __launch_bounds__(BwdCfg<HD, PERSIST>::NUM_THREADS, 1)
     // A unit's last dQ drain and its dK/dV epilogue run after the first step
     // of the next unit has been handed to the tensor core (or after the last
     // step of the last unit), so they overlap the next unit's UMMAs.
-    BUnit prev{};
+    decltype(StepIter<WIN>::u) prev{};
     uint32_t t = 0, uc = 0;
     bool have_prev = false;
-    for (StepIter st_it = first_step<C::DYN, C::HB, true>(prm, sch); ok && st_it.valid; advance<C::DYN, C::HB, true>(prm, st_it, sch)) {
-      const BUnit& u = st_it.u;
+    for (StepIter<WIN> st_it = first_step<C::DYN, C::HB, WIN, true>(prm, sch); ok && st_it.valid; advance<C::DYN, C::HB, WIN, true>(prm, st_it, sch)) {
+      const auto& u = st_it.u;
       const int i = st_it.i;
       t = st_it.t;
       uc = st_it.uc;
@@ -761,8 +954,20 @@ __global__ void __launch_bounds__(BwdCfg<HD, PERSIST>::NUM_THREADS, 1)
       ok = mbar_wait_warp(BAR_TF(ss), (t / C::SSTG) & 1, abort_p);
       if (!ok) break;
       const float* stt = stat_base + ss * (2 * BQ) + part * CPP;
-      if (i == 0) p_ds_row<true, CPP>(s, dp, stt, stt + BQ, c, sc, krow, part * CPP);
-      else p_ds_row<false, CPP>(s, dp, stt, stt + BQ, c, sc, krow, part * CPP);
+      if constexpr (WIN) {
+        const int row0 = u.q_tile(i) * BQ;
+        if (u.whole(prm.win, row0)) {
+          p_ds_row<false, CPP>(s, dp, stt, stt + BQ, c, sc, krow, part * CPP);
+        } else {
+          int from, to;
+          u.seen(prm.win, u.kt * BK + krow, row0 + part * CPP, &from, &to);
+          p_ds_row_window<CPP>(s, dp, stt, stt + BQ, c, sc, from, to);
+        }
+      } else if (i == 0) {
+        p_ds_row<true, CPP>(s, dp, stt, stt + BQ, c, sc, krow, part * CPP);
+      } else {
+        p_ds_row<false, CPP>(s, dp, stt, stt + BQ, c, sc, krow, part * CPP);
+      }
       mbar_arrive(BAR_TE(ss));
       // the previous step's UMMAs must be done with P^T/dS^T, and when the dQ
       // staging shares their smem its reduction must have read it
@@ -814,7 +1019,7 @@ __global__ void __launch_bounds__(BwdCfg<HD, PERSIST>::NUM_THREADS, 1)
     const int row = quarter * 32 + lane;
     const uint32_t tl = tmem + ((uint32_t)(quarter * 32) << 16);
     bool ok = true;
-    for (StepIter s = first_step<C::DYN, C::HB, true>(prm, sch); ok && s.valid; advance<C::DYN, C::HB, true>(prm, s, sch)) {
+    for (StepIter<WIN> s = first_step<C::DYN, C::HB, WIN, true>(prm, sch); ok && s.valid; advance<C::DYN, C::HB, WIN, true>(prm, s, sch)) {
       const uint32_t t = s.t;
       const int b = t % C::DQSB;
       uint8_t* dqs = gbase + C::OFF_DQS + b * C::DQS_BYTES;
@@ -869,17 +1074,18 @@ __global__ void zero_dq_shard_kernel(float4* __restrict__ dQ, int T, int N, int 
   }
 }
 
-template <int HD, bool PERSIST>
+// T rows of queries and keys, nq and nkv columns.
+template <int HD, bool PERSIST, bool WIN = false>
 cudaError_t launch_bwd_kernel(const __nv_bfloat16* dO, const __nv_bfloat16* q,
                               const __nv_bfloat16* k, const __nv_bfloat16* v, float* dQ,
-                              __nv_bfloat16* dK, __nv_bfloat16* dV, const AttnShape& s,
+                              __nv_bfloat16* dK, __nv_bfloat16* dV, int T, int B, uint64_t nq, uint64_t nkv,
                               const BwdParams& prm, int grid, cudaStream_t st) {
-  using C = BwdCfg<HD, PERSIST>;
+  using C = BwdCfg<HD, PERSIST, WIN>;
   // The setmaxnreg split assumes the kernel was compiled to exactly
   // LAUNCH_REGS registers per thread; refuse to launch otherwise.
   static const cudaError_t reg_check = [] {
     cudaFuncAttributes a;
-    cudaError_t e = cudaFuncGetAttributes(&a, flash_bwd_kernel<HD, PERSIST>);
+    cudaError_t e = cudaFuncGetAttributes(&a, flash_bwd_kernel<HD, PERSIST, WIN>);
     if (e != cudaSuccess) return e;
     return a.numRegs == C::LAUNCH_REGS ? cudaSuccess : cudaErrorInvalidKernelImage;
   }();
@@ -887,17 +1093,17 @@ cudaError_t launch_bwd_kernel(const __nv_bfloat16* dO, const __nv_bfloat16* q,
   CUtensorMap tq, tk, tv, tdo, tdq;
   const CUtensorMapDataType bf = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   const CUtensorMapSwizzle sw = CU_TENSOR_MAP_SWIZZLE_128B;
-  if (!make_tmap_3d(&tq, q, bf, 2, s.N, s.T, s.B, 64, BQ, sw) ||
-      !make_tmap_3d(&tk, k, bf, 2, s.N, s.T, s.B, 64, BK, sw) ||
-      !make_tmap_3d(&tv, v, bf, 2, s.N, s.T, s.B, 64, BK, sw) ||
-      !make_tmap_3d(&tdo, dO, bf, 2, s.N, s.T, s.B, 64, BQ, sw) ||
-      !make_tmap_3d(&tdq, dQ, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, s.N, s.T, s.B, 32, BQ, sw))
+  if (!make_tmap_3d(&tq, q, bf, 2, nq, T, B, 64, BQ, sw) ||
+      !make_tmap_3d(&tk, k, bf, 2, nkv, T, B, 64, BK, sw) ||
+      !make_tmap_3d(&tv, v, bf, 2, nkv, T, B, 64, BK, sw) ||
+      !make_tmap_3d(&tdo, dO, bf, 2, nq, T, B, 64, BQ, sw) ||
+      !make_tmap_3d(&tdq, dQ, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, nq, T, B, 32, BQ, sw))
     return cudaErrorInvalidValue;
-  cudaError_t e = cudaFuncSetAttribute(flash_bwd_kernel<HD, PERSIST>,
+  cudaError_t e = cudaFuncSetAttribute(flash_bwd_kernel<HD, PERSIST, WIN>,
                                        cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES);
   if (e != cudaSuccess) return e;
-  launch_pdl(flash_bwd_kernel<HD, PERSIST>, grid, C::NUM_THREADS, C::SMEM_BYTES, st, tq, tk, tv, tdo, tdq, dK,
-                                                                        dV, prm);
+  launch_pdl(flash_bwd_kernel<HD, PERSIST, WIN>, grid, C::NUM_THREADS, C::SMEM_BYTES, st, tq, tk, tv, tdo, tdq, dK,
+             dV, prm);
   count_launches(1);
   return cudaGetLastError();
 }
@@ -914,7 +1120,7 @@ cudaError_t launch_bwd(const __nv_bfloat16* dO, const __nv_bfloat16* Dv, const f
     const cudaError_t e = launch_zero_dq(dQ, s, st);
     if (e != cudaSuccess) return e;
   }
-  BwdParams prm;
+  BwdParams prm{};
   prm.T = s.T;
   prm.N = s.N;
   prm.NH = s.NH;
@@ -936,12 +1142,195 @@ cudaError_t launch_bwd(const __nv_bfloat16* dO, const __nv_bfloat16* Dv, const f
     cudaGetDevice(&dev);
     cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
     const int grid = prm.nunits < sms ? prm.nunits : sms;
-    return launch_bwd_kernel<HD, true>(dO, q, k, v, dQ, dK, dV, s, prm, grid, st);
+    return launch_bwd_kernel<HD, true>(dO, q, k, v, dQ, dK, dV, s.T, s.B, s.N, s.N, prm, grid, st);
   }
-  return launch_bwd_kernel<HD, false>(dO, q, k, v, dQ, dK, dV, s, prm, prm.nunits, st);
+  return launch_bwd_kernel<HD, false>(dO, q, k, v, dQ, dK, dV, s.T, s.B, s.N, s.N, prm, prm.nunits, st);
+}
+
+// ------------------------------------------------------- windowed backward
+// How a call's workspace is laid out, and how its sink tiles are split.
+struct WinPlan {
+  int nqt, rows, nsplit, nfar, far_tiles;
+  size_t stat, part, dq;  // bytes: one statistic, the partial sums, dQ in fp32
+  size_t total() const { return 2 * stat + part + dq; }
+};
+
+WinPlan win_plan(const WindowArgs& a, bool dq_f32) {
+  WinPlan p{};
+  p.nqt = (a.M + BQ - 1) / BQ;
+  p.rows = p.nqt * BQ;
+  const int nbh = a.B * a.NKV;
+  const int ns = (int)std::min<long long>(((long long)a.sinks + BK - 1) / BK, p.nqt);
+  const int window = std::min(a.window, 1 << 25);
+  const int near = (BK - 1 + window - 1) / BQ + 1;  // query tiles of tile 0's window
+  const int far = p.nqt - near;
+  // A sink tile's far queries are a chain of `far` steps a head where other
+  // units have `near`.  Where the sink tiles alone would not keep the GPU busy
+  // twice over, the chain is cut into pieces of a window's length, of 8 tiles
+  // at least (a piece costs 2 x 128 x D fp32 written and read) and 16 at most.
+  if (far > near && far > 8 && (long long)ns * nbh < 2 * 148) {
+    p.nsplit = ns;
+    p.far_tiles = std::max({near, 8, (far + 15) / 16});
+    p.nfar = ns > 0 ? (far + p.far_tiles - 1) / p.far_tiles : 0;
+  }
+  auto up = [](size_t x) { return (x + 255) & ~(size_t)255; };
+  p.stat = up((size_t)a.B * a.NH * p.rows * sizeof(float));
+  p.part = up((size_t)nbh * p.nsplit * (1 + p.nfar) * 2 * BK * a.D * sizeof(float));
+  p.dq = dq_f32 ? 0 : up((size_t)a.B * a.M * a.NH * a.D * sizeof(float));
+  return p;
+}
+
+__device__ __forceinline__ float dot8(uint4 a, uint4 b) {
+  const __nv_bfloat162* x = reinterpret_cast<const __nv_bfloat162*>(&a);
+  const __nv_bfloat162* y = reinterpret_cast<const __nv_bfloat162*>(&b);
+  float s = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 u = __bfloat1622float2(x[i]), v = __bfloat1622float2(y[i]);
+    s = fmaf(u.x, v.x, s);
+    s = fmaf(u.y, v.y, s);
+  }
+  return s;
+}
+
+// The statistics -l*log2e and -(dO . O)/sqrt(D), [B][NH][rows] (0 for padding
+// and past the end), and zeros for dQ.  HBM-bound: dO, O read and dQ written
+// once.  A warp takes 32 rows of a head, D/8 lanes a row with 16-byte loads,
+// and writes 32 neighbouring statistics.
+template <int HD>
+__global__ void __launch_bounds__(256) window_stats_kernel(const WindowArgs a, const __nv_bfloat16* __restrict__ dO,
+                                                           float* __restrict__ neg_l, float* __restrict__ neg_d,
+                                                           float* __restrict__ dQ, int rows) {
+  pdl_wait_and_release();
+  constexpr int G = HD / 8, RPI = 32 / G;  // lanes a row, rows an instruction
+  const int lane = threadIdx.x % 32;
+  const int tiles = rows / 32;
+  const long long items = (long long)a.B * tiles * a.NH;
+  for (long long it = blockIdx.x * 8ll + threadIdx.x / 32; it < items; it += gridDim.x * 8ll) {
+    const int h = (int)(it % a.NH);
+    const long long r = it / a.NH;
+    const int b = (int)(r / tiles), row0 = (int)(r % tiles) * 32;
+    const int n = a.len(b);
+    float mine = 0.0f;  // of row row0 + lane
+#pragma unroll
+    for (int i = 0; i < 32; i += RPI) {
+      const int row = row0 + i + lane / G;
+      const long long off = (((long long)b * a.M + row) * a.NH + h) * HD;
+      float s = 0.0f;
+      if (row < n)
+        s = dot8(__ldcs(reinterpret_cast<const uint4*>(dO + off) + lane % G),
+                 __ldcs(reinterpret_cast<const uint4*>(a.out + off) + lane % G));
+      if (row < a.M) {
+        float4* z = reinterpret_cast<float4*>(dQ + off) + lane % G;
+        z[0] = z[G] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      }
+#pragma unroll
+      for (int m = G / 2; m >= 1; m >>= 1) s += __shfl_xor_sync(0xffffffffu, s, m);
+      const float got = __shfl_sync(0xffffffffu, s, (lane - i) * G & 31);
+      if (lane >= i && lane < i + RPI) mine = got;
+    }
+    const int row = row0 + lane;
+    const bool valid = row < n;
+    const long long at = ((long long)b * a.NH + h) * rows + row;
+    neg_l[at] = valid ? -a.l[((long long)b * a.M + row) * a.NH + h] * LOG2E : 0.0f;
+    neg_d[at] = valid ? -mine * a.scale : 0.0f;
+  }
+}
+
+// dQ rounded to bf16, and the split sink tiles' partial dV, dK added up in
+// slot order and rounded.
+__global__ void __launch_bounds__(256) window_finish_kernel(const float* __restrict__ dQ, __nv_bfloat16* __restrict__ dQ16,
+                                                            long long nq4, const float* __restrict__ part, int slots,
+                                                            int nsplit, int D, int NKV, int T, long long npart4,
+                                                            __nv_bfloat16* __restrict__ dK, __nv_bfloat16* __restrict__ dV) {
+  pdl_wait_and_release();
+  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < nq4 + npart4; i += gridDim.x * 256ll) {
+    if (i < npart4) {
+      const int d4 = D / 4;
+      const int c = (int)(i % d4);
+      long long r = i / d4;
+      const int row = (int)(r % BK);
+      r /= BK;
+      const int which = (int)(r % 2);
+      r /= 2;  // (batch, K/V head, sink tile)
+      const int tile = (int)(r % nsplit);
+      const long long bh = r / nsplit;
+      const int key = tile * BK + row;
+      if (key >= T) continue;
+      float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      for (int k = 0; k < slots; ++k) {
+        const float4 x = __ldg(reinterpret_cast<const float4*>(part) + (((r * slots + k) * 2 + which) * BK + row) * d4 + c);
+        s.x += x.x, s.y += x.y, s.z += x.z, s.w += x.w;
+      }
+      __nv_bfloat16* to = (which == 0 ? dV : dK) + ((bh / NKV * T + key) * NKV + bh % NKV) * D + c * 4;
+      *reinterpret_cast<uint2*>(to) = make_uint2(pack_bf16(s.x, s.y), pack_bf16(s.z, s.w));
+    } else {
+      const long long j = i - npart4;
+      const float4 x = __ldcs(reinterpret_cast<const float4*>(dQ) + j);
+      reinterpret_cast<uint2*>(dQ16)[j] = make_uint2(pack_bf16(x.x, x.y), pack_bf16(x.z, x.w));
+    }
+  }
+}
+
+template <int HD>
+cudaError_t launch_win_bwd(const WindowArgs& a, const WindowGrads& g, cudaStream_t st) {
+  const WinPlan p = win_plan(a, g.dq_f32);
+  char* ws = static_cast<char*>(g.workspace);
+  float* neg_l = reinterpret_cast<float*>(ws);
+  float* neg_d = reinterpret_cast<float*>(ws + p.stat);
+  float* part = reinterpret_cast<float*>(ws + 2 * p.stat);
+  float* dQ = g.dq_f32 ? static_cast<float*>(g.dQ) : reinterpret_cast<float*>(ws + 2 * p.stat + p.part);
+  int dev = 0, sms = 148;
+  cudaGetDevice(&dev);
+  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  auto blocks = [&](long long n, int per) { return (unsigned)std::min<long long>((n + per - 1) / per, sms * 16ll); };
+  launch_pdl(window_stats_kernel<HD>, blocks((long long)a.B * a.NH * (p.rows / 32), 8), 256, 0, st, a, g.dO, neg_l,
+             neg_d, dQ, p.rows);
+  count_launches(1);
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return e;
+  BwdParams prm{};
+  prm.T = a.M;
+  prm.N = a.NKV * HD;
+  prm.NH = a.NKV;
+  prm.nbh = a.B * a.NKV;
+  prm.nkt = p.nqt;
+  prm.scale = 1.0f / sqrtf((float)HD);
+  prm.scale_log2 = LOG2E / sqrtf((float)HD);
+  prm.status = a.status;
+  WinBwd& w = prm.win;
+  w.lens = a.lens;
+  w.G = a.NH / a.NKV;
+  w.window = std::min(a.window, 1 << 25);  // M <= 2^24: the same mask, and sums of positions stay in range
+  w.sinks = a.sinks;
+  w.nsplit = p.nsplit;
+  w.nfar = p.nfar;
+  w.far_tiles = p.far_tiles;
+  w.nfar_units = p.nsplit * p.nfar * prm.nbh;
+  w.rows = p.rows;
+  w.neg_l = neg_l;
+  w.neg_d = neg_d;
+  w.part = part;
+  prm.nunits = w.nfar_units + prm.nkt * prm.nbh;
+  e = launch_bwd_kernel<HD, false, true>(g.dO, a.q, a.k, a.v, dQ, g.dK, g.dV, a.M, a.B, (uint64_t)a.NH * HD,
+                                         (uint64_t)a.NKV * HD, prm, prm.nunits, st);
+  if (e != cudaSuccess) return e;
+  const long long nq4 = g.dq_f32 ? 0 : (long long)a.B * a.M * a.NH * HD / 4;
+  const long long npart4 = (long long)prm.nbh * p.nsplit * 2 * BK * HD / 4;
+  if (nq4 + npart4 == 0) return cudaSuccess;
+  launch_pdl(window_finish_kernel, blocks(nq4 + npart4, 256), 256, 0, st, dQ,
+             static_cast<__nv_bfloat16*>(g.dQ), nq4, part, 1 + p.nfar, p.nsplit, HD, a.NKV, a.M, npart4, g.dK, g.dV);
+  count_launches(1);
+  return cudaGetLastError();
 }
 
 }  // namespace
+
+size_t window_bwd_workspace(const WindowArgs& a, bool dq_f32) { return win_plan(a, dq_f32).total(); }
+
+cudaError_t launch_window_bwd(const WindowArgs& a, const WindowGrads& g, cudaStream_t st) {
+  return a.D == 64 ? launch_win_bwd<64>(a, g, st) : launch_win_bwd<128>(a, g, st);
+}
 
 cudaError_t launch_zero_dq(float* dQ, const AttnShape& s, cudaStream_t st) {
   if (s.bh_begin == 0 && s.bh_end == s.B * s.NH)
