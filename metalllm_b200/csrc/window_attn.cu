@@ -17,7 +17,7 @@
 // 16 keys of every block with its own m, l and O in registers, joined at the
 // end.  Few rows on a long axis leave most SMs idle, so the blocks are split
 // over CTAs until the GPU is full, and a second kernel joins the splits'
-// (m, l, O) in split order.
+// (m, l, O) in a fixed order.
 //
 // Cache rows that no query sees may hold anything: their scores are replaced
 // by -inf and their V rows zeroed in shared memory, since 0 * NaN is NaN.
@@ -322,40 +322,52 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM)
   if (threadIdx.x == 0 && abort_flag) atomicOr(a.status, STATUS_FWD_TIMEOUT);
 }
 
-// Joins the splits of a row, in split order.  A row's D/4 threads each sum 4
-// columns; latency-bound (a few KB a row).
+// Joins the splits of a row.  A block a row: D/4 threads across the columns,
+// JOIN / (D/4) slices of the splits, each slice in split order and then the
+// slices in theirs, so the order of the sums is fixed.  Latency-bound (a few
+// hundred KB in all), so the slices' loads go out together.
+constexpr int JOIN = 256;
+
 template <int HD>
-__global__ void __launch_bounds__(256) window_join_kernel(const DecodeParams prm) {
+__global__ void __launch_bounds__(JOIN) window_join_kernel(const DecodeParams prm) {
+  constexpr int LANES = HD / 4, SLICES = JOIN / LANES;
+  __shared__ float4 so[SLICES][LANES];
+  __shared__ float2 sml[SLICES];
   pdl_wait_and_release();
   const WindowArgs& a = prm.a;
   const int G = a.NH / a.NKV, R = a.M * G;
-  const long long rows = (long long)a.B * a.NKV * R;
-  const long long it = (blockIdx.x * 256ll + threadIdx.x) / (HD / 4);
-  if (it >= rows) return;
-  const int d = (threadIdx.x % (HD / 4)) * 4;
-  const int row = (int)(it % R);
-  const long long bk = it / R;
-  const int b = (int)(bk / a.NKV), kh = (int)(bk % a.NKV);
-  const long long at0 = ((bk * prm.groups + row / ROWS) * prm.nsplit) * ROWS + row % ROWS;
-  float top = -INFINITY;
-  for (int s = 0; s < prm.nsplit; ++s) top = fmaxf(top, __ldg(prm.part_ml + (at0 + (long long)s * ROWS) * 2));
-  const float base = top == -INFINITY ? 0.0f : top;
-  float sum = 0.0f;
+  const int row = blockIdx.x % R;
+  const int bk = blockIdx.x / R;
+  const int b = bk / a.NKV, kh = bk % a.NKV;
+  const int lane = threadIdx.x % LANES, slice = threadIdx.x / LANES;
+  const long long at0 = (((long long)bk * prm.groups + row / ROWS) * prm.nsplit) * ROWS + row % ROWS;
+  float top = -INFINITY, sum = 0.0f;
   float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  for (int s = 0; s < prm.nsplit; ++s) {
+  auto add = [&](float2 ml, float4 y) {
+    const float m = fmaxf(top, ml.x), base = m == -INFINITY ? 0.0f : m;
+    const float f = ex2(top - base), h = ex2(ml.x - base);
+    top = m;
+    sum = sum * f + ml.y * h;
+    x.x = x.x * f + y.x * h, x.y = x.y * f + y.y * h, x.z = x.z * f + y.z * h, x.w = x.w * f + y.w * h;
+  };
+#pragma unroll 4
+  for (int s = slice; s < prm.nsplit; s += SLICES) {
     const long long at = at0 + (long long)s * ROWS;
-    const float2 ml = __ldg(reinterpret_cast<const float2*>(prm.part_ml) + at);
-    const float f = ex2(ml.x - base);
-    const float4 y = __ldg(reinterpret_cast<const float4*>(prm.part_o + at * HD + d));
-    sum = fmaf(f, ml.y, sum);
-    x.x = fmaf(f, y.x, x.x), x.y = fmaf(f, y.y, x.y), x.z = fmaf(f, y.z, x.z), x.w = fmaf(f, y.w, x.w);
+    add(__ldg(reinterpret_cast<const float2*>(prm.part_ml) + at),
+        __ldg(reinterpret_cast<const float4*>(prm.part_o + at * HD) + lane));
   }
+  so[slice][lane] = x;
+  if (lane == 0) sml[slice] = make_float2(top, sum);
+  __syncthreads();
+  if (slice > 0) return;
+#pragma unroll
+  for (int s = 1; s < SLICES; ++s) add(sml[s], so[s][lane]);
   const bool valid = row / G < a.len(b);
   const float inv = valid ? 1.0f / sum : 0.0f;
   const long long item = ((long long)b * a.M + row / G) * a.NH + kh * G + row % G;
-  *reinterpret_cast<uint2*>(a.out + item * HD + d) =
+  *reinterpret_cast<uint2*>(a.out + item * HD + lane * 4) =
       valid ? make_uint2(pack_bf16(x.x * inv, x.y * inv), pack_bf16(x.z * inv, x.w * inv)) : make_uint2(0u, 0u);
-  if (d == 0) a.l[item] = valid ? (top + log2f(sum)) * LN2 : -INFINITY;
+  if (lane == 0) a.l[item] = valid ? (top + log2f(sum)) * LN2 : -INFINITY;
 }
 
 // Few query rows a K/V head take the kernel of this file, more the tiled
@@ -401,8 +413,7 @@ cudaError_t launch_decode(const WindowArgs& a, void* workspace, cudaStream_t st)
   count_launches(1);
   e = cudaGetLastError();
   if (e != cudaSuccess || p.nsplit == 1) return e;
-  const long long threads = (long long)a.B * a.M * a.NH * (HD / 4);
-  launch_pdl(window_join_kernel<HD>, (unsigned)((threads + 255) / 256), 256, 0, st, prm);
+  launch_pdl(window_join_kernel<HD>, (unsigned)(a.B * a.M * a.NH), JOIN, 0, st, prm);
   count_launches(1);
   return cudaGetLastError();
 }
