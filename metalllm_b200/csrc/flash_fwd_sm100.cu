@@ -56,6 +56,7 @@ using namespace sm100;
 
 constexpr int BM = 128;  // query rows per tile
 constexpr int BN = 128;  // keys per tile
+constexpr int NARROW = 32;  // columns of a sink tile with at most that many sinks
 constexpr int NUM_THREADS = 384;
 constexpr int LAUNCH_REGS = 168;    // 65536 / 384, rounded down to a multiple of 8
 constexpr int REGS_PRODUCER = 120;  // warpgroup 0 after setmaxnreg.dec
@@ -134,6 +135,11 @@ struct FwdParams {
   WindowArgs win;      // WIN only
 };
 
+// bits 0 .. n-1 (none for n <= 0, all from 32 on)
+__device__ __forceinline__ uint32_t bits_below(int n) {
+  return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1u;
+}
+
 // sum over 8 bf16 pairs of a[i] * b[i], fp32 (products of bf16 values are
 // exact in fp32)
 __device__ __forceinline__ float dot_bf16x8(uint4 a, uint4 b) {
@@ -203,6 +209,9 @@ struct WinUnit : Unit {
   __device__ bool active(int x, int j) const { return x == 0 ? j < nA : j < nB && j != skip; }
   // the first list index of a tile: its PV starts the sum
   __device__ int first(int x) const { return x == 1 && skip == 0 ? 1 : 0; }
+  // only the sinks of this tile are visible, and they fill a quarter at most:
+  // its products and exponentials stop there
+  __device__ bool narrow(const WindowArgs& w, int j) const { return j < ns && w.sinks - j * BN <= NARROW; }
   // every valid row of tile x sees every key of the tile at k0
   __device__ bool whole(const WindowArgs& w, int x, int k0) const {
     return k0 + BN - 1 <= (x == 0 ? t0A : t0B) &&
@@ -418,6 +427,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     } else if (warp == 1 && lane == 0) {
       // ----------------------------------------------------------- MMA
       constexpr uint32_t IDESC_S = idesc_bf16_f32(BM, BN, 0, 0);
+      constexpr uint32_t IDESC_SN = idesc_bf16_f32(BM, NARROW, 0, 0);
       constexpr uint32_t IDESC_O = idesc_bf16_f32(BM, HD, 0, 1);
       uint32_t qc = 0, kc = 0, vc = 0;
       uint32_t sc[2] = {0, 0};   // S_X issued so far
@@ -448,11 +458,14 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
           tc_fence_after();
           const uint32_t sq = sbase + C::OFF_Q + (qs * 2 + x) * C::QT_BYTES;
           const uint32_t sk = sbase + C::OFF_K + ((kc + j) % C::KST) * C::KV_BYTES;
+          uint32_t idesc = IDESC_S;
+          if constexpr (WIN)
+            if (un.narrow(prm.win, j)) idesc = IDESC_SN;
 #pragma unroll
           for (int kk = 0; kk < HD / 16; ++kk) {
             const uint32_t off = (kk >> 2) * (BM * 128) + (kk & 3) * 32;
             umma_bf16_ss(tmem + C::TCOL_S + x * BN, smem_desc_sw128(sq + off, 16, 1024),
-                         smem_desc_sw128(sk + off, 16, 1024), IDESC_S, kk > 0 ? 1u : 0u);
+                         smem_desc_sw128(sk + off, 16, 1024), idesc, kk > 0 ? 1u : 0u);
           }
           umma_commit(BAR_SF(x));
           ++sc[x];
@@ -465,8 +478,12 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
           tc_fence_after();
           const uint32_t sp = sbase + C::OFF_P + x * C::STG_BYTES;
           const uint32_t sv = sbase + C::OFF_V + ((vc + j) % C::VST) * C::KV_BYTES;
+          int steps = BN / 16;
+          if constexpr (WIN)
+            if (un.narrow(prm.win, j)) steps = NARROW / 16;
 #pragma unroll
           for (int kk = 0; kk < BN / 16; ++kk) {
+            if (WIN && kk >= steps) break;
             const uint64_t bd = smem_desc_sw128(sv + kk * 2048, BN * 128, 1024);
             if (C::P_TMEM) {  // A = P_X from TMEM: 8 columns per 16 keys
               umma_bf16_ts(tmem + C::TCOL_O + x * HD, tmem + C::TCOL_P + x * (BN / 2) + kk * 8, bd,
@@ -655,8 +672,10 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       float m_used = -INFINITY, l_sum = 0.0f;
       // one key tile; DIAG: the diagonal tile (keys after the query masked).
       // Instantiated twice so that the other tiles carry no masking code.
-      auto tile = [&](auto diag_tag, int j) -> bool {
+      // NC: the tile's first columns that matter (all 128, or a sink tile's 32).
+      auto tile = [&](auto diag_tag, auto nc_tag, int j) -> bool {
         constexpr bool DIAG = decltype(diag_tag)::value;
+        constexpr int NC = decltype(nc_tag)::value;
         if constexpr (DIAG && C::P_TMEM && !WIN) {
           // the unit's last key tile: the dO tile of X goes by TMA into the O
           // staging (idle until the epilogue; rows past T read as zero); the
@@ -672,17 +691,25 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         }
         if (!mbar_wait_warp(BAR_SF(x), sc & 1, abort_p)) return false;
         tc_fence_after();
-        float s[BN];
+        float s[NC];
+        if constexpr (NC == 32) {
+          uint32_t ra[32];
+          tmem_ld32(trow + tcol_s, ra);
+          tmem_wait_ld_dep(ra);
 #pragma unroll
-        for (int cc = 0; cc < BN; cc += 64) {
-          uint32_t ra[32], rb[32];
-          tmem_ld32(trow + tcol_s + cc, ra);
-          tmem_ld32(trow + tcol_s + cc + 32, rb);
-          tmem_wait_ld_dep(ra, rb);
+          for (int i = 0; i < 32; ++i) s[i] = __uint_as_float(ra[i]);
+        } else {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            s[cc + i] = __uint_as_float(ra[i]);
-            s[cc + 32 + i] = __uint_as_float(rb[i]);
+          for (int cc = 0; cc < NC; cc += 64) {
+            uint32_t ra[32], rb[32];
+            tmem_ld32(trow + tcol_s + cc, ra);
+            tmem_ld32(trow + tcol_s + cc + 32, rb);
+            tmem_wait_ld_dep(ra, rb);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              s[cc + i] = __uint_as_float(ra[i]);
+              s[cc + 32 + i] = __uint_as_float(rb[i]);
+            }
           }
         }
         tc_fence_before();
@@ -690,13 +717,18 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         if constexpr (WIN) {
           if constexpr (DIAG) {
             // key k0 + i is visible up to the row's own position, and from its
-            // window's first key on or among the sinks
+            // window's first key on or among the sinks; 32 keys to a word of
+            // bits, one test and one select a key
             const int k0 = un.key_tile(j) * BN;
             const int t = prm.win.pos(un.b, qtile * BM + row);
             const int up = t - k0, from = t - prm.win.window + 1 - k0, sink = prm.win.sinks - k0;
 #pragma unroll
-            for (int i = 0; i < BN; ++i)
-              if (i > up || (i < from && i >= sink)) s[i] = -INFINITY;
+            for (int w = 0; w < NC; w += 32) {
+              const uint32_t see = bits_below(up + 1 - w) & (~bits_below(from - w) | bits_below(sink - w));
+#pragma unroll
+              for (int i = 0; i < 32; ++i)
+                if (!(see & (1u << i))) s[w + i] = -INFINITY;
+            }
           }
         } else if constexpr (DIAG) {
 #pragma unroll
@@ -708,7 +740,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
 #pragma unroll
         for (int q = 0; q < 8; ++q) pm[q] = fmaxf(s[q], s[8 + q]);
 #pragma unroll
-        for (int i = 16; i < BN; i += 16)
+        for (int i = 16; i < NC; i += 16)
 #pragma unroll
           for (int q = 0; q < 8; ++q) pm[q] = fmax3(pm[q], s[i + q], s[i + 8 + q]);
         const float mx = fmax3(fmax3(pm[0], pm[1], pm[2]), fmax3(pm[3], pm[4], pm[5]),
@@ -737,9 +769,9 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         const float2 c2 = make_float2(c, c), nm2 = make_float2(-base, -base);
         float2 ps[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f),
                         make_float2(0.f, 0.f)};
-        uint32_t pk[BN / 2];  // P as bf16 pairs, even key in the low half
+        uint32_t pk[NC / 2];  // P as bf16 pairs, even key in the low half
 #pragma unroll
-        for (int i = 0; i < BN; i += 2) {
+        for (int i = 0; i < NC; i += 2) {
           const float2 t = __ffma2_rn(make_float2(s[i], s[i + 1]), c2, nm2);
           const float e0 = ex2(t.x), e1 = ex2(t.y);
           ps[(i >> 1) & 3] = __fadd2_rn(ps[(i >> 1) & 3], make_float2(e0, e1));
@@ -768,7 +800,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         if constexpr (C::P_TMEM) {
           // this lane's P row into P_X
 #pragma unroll
-          for (int q = 0; q < BN / 32; ++q) {
+          for (int q = 0; q < NC / 32; ++q) {
             uint32_t r[16];
 #pragma unroll
             for (int i = 0; i < 16; ++i) r[i] = pk[q * 16 + i];
@@ -777,9 +809,9 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
           tmem_wait_st();
         } else {
 #pragma unroll
-          for (int kb = 0; kb < BN / 64; ++kb) {
+          for (int kb = 0; kb < (NC + 63) / 64; ++kb) {
 #pragma unroll
-            for (int ch = 0; ch < 8; ++ch) {
+            for (int ch = 0; ch < (NC < 64 ? NC / 8 : 8); ++ch) {
               const int c0 = (kb * 64 + ch * 8) / 2;
               const uint4 v = make_uint4(pk[c0], pk[c0 + 1], pk[c0 + 2], pk[c0 + 3]);
               *reinterpret_cast<uint4*>(pbuf + kb * (BM * 128) + row * 128 + ((ch ^ (row & 7)) * 16)) = v;
@@ -792,12 +824,15 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         ++sc;
         return true;
       };
+      using All = std::integral_constant<int, BN>;
       for (int j = 0; ok && j < nt; ++j) {
         if constexpr (WIN) {
           if (!un.active(x, j)) continue;
-          ok = un.whole(prm.win, x, un.key_tile(j) * BN) ? tile(std::false_type{}, j) : tile(std::true_type{}, j);
+          if (un.narrow(prm.win, j)) ok = tile(std::true_type{}, std::integral_constant<int, NARROW>{}, j);
+          else if (un.whole(prm.win, x, un.key_tile(j) * BN)) ok = tile(std::false_type{}, All{}, j);
+          else ok = tile(std::true_type{}, All{}, j);
         } else {
-          ok = (j == qtile) ? tile(std::true_type{}, j) : tile(std::false_type{}, j);
+          ok = (j == qtile) ? tile(std::true_type{}, All{}, j) : tile(std::false_type{}, All{}, j);
         }
       }
       // --------------------------------------------- epilogue of tile X
