@@ -376,9 +376,12 @@ __device__ __forceinline__ void advance(const BwdParams& prm, StepIter<WIN>& s, 
 // P^T and dS^T for N query columns of one key row.  s[] holds S^T on entry
 // and P^T on exit; dp[] holds dP^T on entry and dS^T on exit.  nl = -l*log2e
 // and nd = -D/sqrt(D) per query column (shared memory, broadcast reads).
-template <bool DIAG, int N>
+// SEEN (a window's masked step): bit j of see[] says whether query column j is
+// visible; else P and dS are 0 whatever the products hold.
+template <bool DIAG, int N, bool SEEN = false>
 __device__ __forceinline__ void p_ds_row(float (&s)[N], float (&dp)[N], const float* nl,
-                                         const float* nd, float c, float sc, int krow, int qcol0) {
+                                         const float* nd, float c, float sc, int krow, int qcol0,
+                                         const uint32_t* see = nullptr) {
   const float2 c2 = make_float2(c, c), sc2 = make_float2(sc, sc);
 #pragma unroll
   for (int j = 0; j < N; j += 4) {
@@ -406,26 +409,10 @@ __device__ __forceinline__ void p_ds_row(float (&s)[N], float (&dp)[N], const fl
     dp[j + 1] = r0.y;
     dp[j + 2] = r1.x;
     dp[j + 3] = r1.y;
-  }
-}
-
-// The window's masked form: query column qcol0 + j is seen when from <= it <
-// to, else P and dS are 0 whatever the products hold.
-template <int N>
-__device__ __forceinline__ void p_ds_row_window(float (&s)[N], float (&dp)[N], const float* nl, const float* nd,
-                                                float c, float sc, int from, int to) {
+    if constexpr (SEEN) {
 #pragma unroll
-  for (int j = 0; j < N; j += 4) {
-    const float4 L = *reinterpret_cast<const float4*>(nl + j);
-    const float4 Dn = *reinterpret_cast<const float4*>(nd + j);
-    const float l[4] = {L.x, L.y, L.z, L.w}, d[4] = {Dn.x, Dn.y, Dn.z, Dn.w};
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const bool see = j + e >= from && j + e < to;
-      const float p = ex2(fmaf(s[j + e], c, l[e]));
-      const float r = p * fmaf(dp[j + e], sc, d[e]);
-      s[j + e] = see ? p : 0.0f;
-      dp[j + e] = see ? r : 0.0f;
+      for (int e = j; e < j + 4; ++e)
+        if (!(see[e / 32] & (1u << (e % 32)))) s[e] = dp[e] = 0.0f;
     }
   }
 }
@@ -961,7 +948,10 @@ __global__ void __launch_bounds__(BwdCfg<HD, PERSIST, WIN>::NUM_THREADS, 1)
         } else {
           int from, to;
           u.seen(prm.win, u.kt * BK + krow, row0 + part * CPP, &from, &to);
-          p_ds_row_window<CPP>(s, dp, stt, stt + BQ, c, sc, from, to);
+          uint32_t see[CPP / 32];
+#pragma unroll
+          for (int w = 0; w < CPP / 32; ++w) see[w] = bits_below(to - 32 * w) & ~bits_below(from - 32 * w);
+          p_ds_row<false, CPP, true>(s, dp, stt, stt + BQ, c, sc, krow, part * CPP, see);
         }
       } else if (i == 0) {
         p_ds_row<true, CPP>(s, dp, stt, stt + BQ, c, sc, krow, part * CPP);

@@ -135,11 +135,6 @@ struct FwdParams {
   WindowArgs win;      // WIN only
 };
 
-// bits 0 .. n-1 (none for n <= 0, all from 32 on)
-__device__ __forceinline__ uint32_t bits_below(int n) {
-  return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1u;
-}
-
 // sum over 8 bf16 pairs of a[i] * b[i], fp32 (products of bf16 values are
 // exact in fp32)
 __device__ __forceinline__ float dot_bf16x8(uint4 a, uint4 b) {

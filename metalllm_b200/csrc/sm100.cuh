@@ -497,6 +497,11 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+// bits 0 .. n-1 (none for n <= 0, all from 32 on)
+__device__ __forceinline__ uint32_t bits_below(int n) {
+  return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1u;
+}
+
 // max(a, b, c) in one instruction (three-source max.f32, sm_100).
 __device__ __forceinline__ float fmax3(float a, float b, float c) {
   float r;
