@@ -20,14 +20,17 @@
 // does not allow vectors) and walks heads with it, so a sine is computed once
 // for the heads of a thread and not once for each head.  Neighbouring lanes
 // take the units of one head and then the next head, so a warp reads whole
-// rows.  Heads are dealt to as many threads as fill the GPU twice: at few rows
-// every thread has one head (latency), at many rows the sines are shared.
+// rows.  A thread loads BATCH heads before it turns the first.  Heads are dealt
+// to as many threads as fill half of the GPU: at few rows every thread has one
+// head (latency), at many rows the sines are shared.
 #include "common.cuh"
+#include "sm100.cuh"
 
 namespace ma {
 namespace {
 
 constexpr int THREADS = 256;
+constexpr int BATCH = 4;
 
 // What the kernel turns and copies.  Heads 0 .. hq-1 are q's, the next hk k's.
 struct RotArgs {
@@ -52,67 +55,124 @@ struct RotArgs {
   float amp, sign;      // sign -1: the backward's negative angle
 };
 
+// N elements as they lie in memory: 16-byte vectors where N fills them, kept
+// packed in registers (a bf16 element of its own would take a whole one).
 template <typename T, int N>
-struct alignas(sizeof(T) * N) Vec {
-  T x[N];
+struct Piece;
+
+template <int N>
+struct Piece<float, N> {
+  float x[N];
+  __device__ __forceinline__ void load(const float* p) {
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+      if constexpr (N % 4 == 0) *reinterpret_cast<float4*>(x + i) = *reinterpret_cast<const float4*>(p + i);
+      else if constexpr (N == 2) *reinterpret_cast<float2*>(x) = *reinterpret_cast<const float2*>(p);
+      else x[0] = p[0];
+    }
+  }
+  __device__ __forceinline__ void store(float* p) const {
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+      if constexpr (N % 4 == 0) *reinterpret_cast<float4*>(p + i) = *reinterpret_cast<const float4*>(x + i);
+      else if constexpr (N == 2) *reinterpret_cast<float2*>(p) = *reinterpret_cast<const float2*>(x);
+      else p[0] = x[0];
+    }
+  }
+  __device__ __forceinline__ float get(int i) const { return x[i]; }
+  __device__ __forceinline__ void set2(int i, float u, float v) { x[i] = u, x[i + 1] = v; }  // i even
+  __device__ __forceinline__ void set(float u) { x[0] = u; }                                 // N = 1
 };
 
-__device__ __forceinline__ float to_f(float x) { return x; }
-__device__ __forceinline__ float to_f(__nv_bfloat16 x) { return __bfloat162float(x); }
-__device__ __forceinline__ void from_f(float& y, float x) { y = x; }
-__device__ __forceinline__ void from_f(__nv_bfloat16& y, float x) { y = __float2bfloat16_rn(x); }
-
-// N elements of T as vectors of at most 16 bytes
-template <typename T, int N>
-__device__ __forceinline__ void load(const T* p, T (&x)[N]) {
-  constexpr int W = N * sizeof(T) > 16 ? 16 / sizeof(T) : N;
-#pragma unroll
-  for (int i = 0; i < N; i += W) {
-    const Vec<T, W> v = *reinterpret_cast<const Vec<T, W>*>(p + i);
-#pragma unroll
-    for (int j = 0; j < W; ++j) x[i + j] = v.x[j];
+template <int N>
+struct Piece<__nv_bfloat16, N> {
+  static constexpr int W = N < 2 ? 1 : N / 2;
+  uint32_t w[W];
+  __device__ __forceinline__ void load(const __nv_bfloat16* p) {
+    if constexpr (N == 8) {
+      const uint4 v = *reinterpret_cast<const uint4*>(p);
+      w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+    } else if constexpr (N == 4) {
+      const uint2 v = *reinterpret_cast<const uint2*>(p);
+      w[0] = v.x, w[1] = v.y;
+    } else if constexpr (N == 2) {
+      w[0] = *reinterpret_cast<const uint32_t*>(p);
+    } else {
+      w[0] = *reinterpret_cast<const uint16_t*>(p);
+    }
   }
-}
-template <typename T, int N>
-__device__ __forceinline__ void store(T* p, const T (&x)[N]) {
-  constexpr int W = N * sizeof(T) > 16 ? 16 / sizeof(T) : N;
-#pragma unroll
-  for (int i = 0; i < N; i += W) {
-    Vec<T, W> v;
-#pragma unroll
-    for (int j = 0; j < W; ++j) v.x[j] = x[i + j];
-    *reinterpret_cast<Vec<T, W>*>(p + i) = v;
+  __device__ __forceinline__ void store(__nv_bfloat16* p) const {
+    if constexpr (N == 8) *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+    else if constexpr (N == 4) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+    else if constexpr (N == 2) *reinterpret_cast<uint32_t*>(p) = w[0];
+    else *reinterpret_cast<uint16_t*>(p) = (uint16_t)w[0];
   }
-}
+  __device__ __forceinline__ float get(int i) const {
+    return __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
+  }
+  __device__ __forceinline__ void set2(int i, float u, float v) { w[i / 2] = sm100::pack_bf16(u, v); }
+  __device__ __forceinline__ void set(float u) { w[0] = sm100::pack_bf16(u, 0.0f) & 0xffffu; }
+};
 
-// One unit (P pairs) of one head.  zero: a row past its sequence's length.
-template <typename T, bool INTER, int P>
-__device__ __forceinline__ void turn(const T* in, T* out, int unit, int half, const float (&c)[P],
-                                     const float (&s)[P], bool zero) {
+// The two pieces of a unit turned: half layout, pair i is (x[i], y[i]);
+// interleaved, (x[2i], x[2i + 1]) and y is empty.
+template <bool INTER, typename T, int P>
+__device__ __forceinline__ void turn_unit(Piece<T, INTER ? 2 * P : P>& x, Piece<T, P>& y, const float (&c)[P],
+                                          const float (&s)[P], bool zero) {
+  auto one = [&](float a, float b, int i, float& u, float& v) {
+    u = zero ? 0.0f : a * c[i] - b * s[i];
+    v = zero ? 0.0f : a * s[i] + b * c[i];
+  };
   if constexpr (INTER) {
-    T x[2 * P];
-    const int at = unit * 2 * P;
-    load(in + at, x);
 #pragma unroll
     for (int i = 0; i < P; ++i) {
-      const float a = to_f(x[2 * i]), b = to_f(x[2 * i + 1]);
-      from_f(x[2 * i], zero ? 0.0f : a * c[i] - b * s[i]);
-      from_f(x[2 * i + 1], zero ? 0.0f : a * s[i] + b * c[i]);
+      float u, v;
+      one(x.get(2 * i), x.get(2 * i + 1), i, u, v);
+      x.set2(2 * i, u, v);
     }
-    store(out + at, x);
+  } else if constexpr (P == 1) {
+    float u, v;
+    one(x.get(0), y.get(0), 0, u, v);
+    x.set(u);
+    y.set(v);
   } else {
-    T x[P], y[P];
-    const int at = unit * P;
-    load(in + at, x);
-    load(in + at + half, y);
 #pragma unroll
-    for (int i = 0; i < P; ++i) {
-      const float a = to_f(x[i]), b = to_f(y[i]);
-      from_f(x[i], zero ? 0.0f : a * c[i] - b * s[i]);
-      from_f(y[i], zero ? 0.0f : a * s[i] + b * c[i]);
+    for (int i = 0; i < P; i += 2) {
+      float u0, v0, u1, v1;
+      one(x.get(i), y.get(i), i, u0, v0);
+      one(x.get(i + 1), y.get(i + 1), i + 1, u1, v1);
+      x.set2(i, u0, u1);
+      y.set2(i, v0, v1);
     }
-    store(out + at, x);
-    store(out + at + half, y);
+  }
+}
+
+// One unit (P pairs) of heads h0, h0 + step, ... below `heads`; in and out are
+// the row's first head.  zero: a row past its sequence's length.
+template <typename T, bool INTER, int P>
+__device__ __forceinline__ void turn(const T* in, T* out, int h0, int step, int heads, int D, int unit, int half,
+                                     const float (&c)[P], const float (&s)[P], bool zero) {
+  const int at = INTER ? unit * 2 * P : unit * P;
+  for (int h = h0; h < heads; h += BATCH * step) {
+    Piece<T, INTER ? 2 * P : P> x[BATCH];
+    Piece<T, P> y[BATCH];
+#pragma unroll
+    for (int j = 0; j < BATCH; ++j) {
+      const int g = h + j * step;
+      if (g < heads) {
+        x[j].load(in + (long long)g * D + at);
+        if constexpr (!INTER) y[j].load(in + (long long)g * D + at + half);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < BATCH; ++j) {
+      const int g = h + j * step;
+      if (g < heads) {
+        turn_unit<INTER, T, P>(x[j], y[j], c, s, zero);
+        x[j].store(out + (long long)g * D + at);
+        if constexpr (!INTER) y[j].store(out + (long long)g * D + at + half);
+      }
+    }
   }
 }
 
@@ -149,16 +209,14 @@ __global__ void __launch_bounds__(THREADS) rotary_kernel(const RotArgs a) {
         s[i] *= a.amp * a.sign;
       }
       const long long krow = APPEND ? cache_row(a, b, t, valid) : row;
-      for (int h = h0; h < heads; h += a.hsplit) {
-        if (h < a.hq) {
-          const long long off = (row * a.hq + h) * D;
-          turn<TQ, INTER, P>(static_cast<const TQ*>(a.q) + off, static_cast<TQ*>(a.q_out) + off, unit, half, c, s,
-                             !valid);
-        } else if (krow >= 0) {
-          const int kh = h - a.hq;
-          turn<__nv_bfloat16, INTER, P>(a.k + (row * a.hk + kh) * D, a.k_out + (krow * a.hk + kh) * D, unit, half, c,
-                                        s, false);
-        }
+      const long long qoff = row * a.hq * D;
+      turn<TQ, INTER, P>(static_cast<const TQ*>(a.q) + qoff, static_cast<TQ*>(a.q_out) + qoff, h0, a.hsplit, a.hq, D,
+                         unit, half, c, s, !valid);
+      if (krow >= 0) {
+        // k's heads go on where q's ended
+        const int k0 = a.hq <= h0 ? h0 - a.hq : (a.hsplit - (a.hq - h0) % a.hsplit) % a.hsplit;
+        turn<__nv_bfloat16, INTER, P>(a.k + row * a.hk * D, a.k_out + krow * a.hk * D, k0, a.hsplit, a.hk, D, unit, half,
+                                      c, s, false);
       }
       continue;
     }
@@ -173,29 +231,29 @@ __global__ void __launch_bounds__(THREADS) rotary_kernel(const RotArgs a) {
       if (h < a.hq) {
         if (!a.copy_q && valid) continue;
         const long long off = (row * a.hq + h) * D + at;
-        TQ x[C];
-        load(static_cast<const TQ*>(a.q) + off, x);
+        Piece<TQ, C> x;
+        x.load(static_cast<const TQ*>(a.q) + off);
         if (!valid) {
 #pragma unroll
-          for (int i = 0; i < C; ++i) from_f(x[i], 0.0f);
+          for (int i = 0; i < C; i += 2) x.set2(i, 0.0f, 0.0f);
         }
-        store(static_cast<TQ*>(a.q_out) + off, x);
+        x.store(static_cast<TQ*>(a.q_out) + off);
       } else if (a.copy_k) {
         const long long krow = APPEND ? cache_row(a, b, t, valid) : row;
         if (krow < 0) continue;
         const int kh = h - a.hq;
-        __nv_bfloat16 x[C];
-        load(a.k + (row * a.hk + kh) * D + at, x);
-        store(a.k_out + (krow * a.hk + kh) * D + at, x);
+        Piece<__nv_bfloat16, C> x;
+        x.load(a.k + (row * a.hk + kh) * D + at);
+        x.store(a.k_out + (krow * a.hk + kh) * D + at);
       }
     } else if constexpr (APPEND) {  // v, always in 16-byte pieces
       u -= heads * a.cunits;
       const long long krow = cache_row(a, b, t, valid);
       if (krow < 0) continue;
       const int at = u * 8;  // within the row's hk*D columns
-      __nv_bfloat16 x[8];
-      load(a.v + row * a.hk * D + at, x);
-      store(a.v_out + krow * a.hk * D + at, x);
+      Piece<__nv_bfloat16, 8> x;
+      x.load(a.v + row * a.hk * D + at);
+      x.store(a.v_out + krow * a.hk * D + at);
     }
   }
 }
@@ -210,8 +268,8 @@ cudaError_t launch_as(RotArgs a, cudaStream_t st) {
   const bool copied = APPEND || a.copy_q || a.copy_k;
   a.cunits = copied ? (a.D - a.rot) / C : 0;
   a.vunits = APPEND ? a.D / 8 : 0;
-  // threads enough to fill the GPU twice (2048 a SM), each at least one head
-  const long long fill = (long long)sms * 2048 * 2;
+  // threads enough for half of what a SM holds, each at least one head
+  const long long fill = (long long)sms * 1024;
   long long split = fill / (a.rows * a.units) + 1;
   a.hsplit = (int)(split < heads ? split : heads);
   const long long total = a.rows * a.units * a.hsplit +
