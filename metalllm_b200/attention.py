@@ -332,16 +332,22 @@ def _groups(p: AttentionParams, NKV: Optional[int]) -> int:
     return NKV
 
 
-def _check_optional(t: Optional[torch.Tensor], name: str, dtype: torch.dtype, shape: tuple) -> None:
-    if t is not None:
+def _check_all(*specs) -> None:
+    """_check for each (tensor, name, dtype, shape), and for each (tensor,
+    name, dtype, shape, True) that is not None."""
+    cur = torch.cuda.current_device() if torch.cuda.is_initialized() else -1
+    for t, name, dtype, shape, *optional in specs:
+        if type(t) is torch.Tensor and t.dtype is dtype and t.shape == shape and t.is_contiguous() and t.is_cuda and \
+                t.get_device() == cur or (t is None and optional):
+            continue
         _check(t, name, dtype, shape)
 
 
 def _rotary(inv_freq: torch.Tensor, NKV: int, interleaved: bool, amplitude: float) -> _lib.Rotary:
     if not isinstance(inv_freq, torch.Tensor) or inv_freq.dim() != 1:
         raise TypeError("inv_freq must be a one-dimensional tensor (rotaryFrequencies)")
-    _check(inv_freq, "inv_freq", torch.float64, tuple(inv_freq.shape))
-    return _lib.Rotary(_ptr(inv_freq), 2 * inv_freq.numel(), int(bool(interleaved)), NKV, float(amplitude))
+    _check(inv_freq, "inv_freq", torch.float64, inv_freq.shape)
+    return _lib.Rotary(inv_freq.data_ptr(), 2 * inv_freq.numel(), bool(interleaved), NKV, amplitude)
 
 
 def _u32(x: int, name: str) -> int:
@@ -376,9 +382,8 @@ def rotaryForward(q: torch.Tensor, k: torch.Tensor, inv_freq: torch.Tensor, p: A
     NKV = _groups(p, NKV)
     r = _rotary(inv_freq, NKV, interleaved, amplitude)
     qs, ks = (B, p.M, p.N), (B, p.M, NKV * p.D)
-    _check(q, "q", torch.bfloat16, qs)
-    _check(k, "k", torch.bfloat16, ks)
-    _check_optional(positions, "positions", torch.int32, (B, p.M))
+    _check_all((q, "q", torch.bfloat16, qs), (k, "k", torch.bfloat16, ks),
+               (positions, "positions", torch.int32, (B, p.M), True))
     q_out = _out(q_out, q, qs, torch.bfloat16, "q_out")
     k_out = _out(k_out, k, ks, torch.bfloat16, "k_out")
     _lib.call("ma_rotaryForward", _ptr(q), _ptr(k), _ptr(q_out), _ptr(k_out), ctypes.byref(r), _ptr(positions),
@@ -397,9 +402,7 @@ def rotaryBackward(dQ: torch.Tensor, dK: torch.Tensor, inv_freq: torch.Tensor, p
     r = _rotary(inv_freq, NKV, interleaved, amplitude)
     qs, ks = (B, p.M, p.N), (B, p.M, NKV * p.D)
     t = torch.float32 if isinstance(dQ, torch.Tensor) and dQ.dtype == torch.float32 else torch.bfloat16
-    _check(dQ, "dQ", t, qs)
-    _check(dK, "dK", torch.bfloat16, ks)
-    _check_optional(positions, "positions", torch.int32, (B, p.M))
+    _check_all((dQ, "dQ", t, qs), (dK, "dK", torch.bfloat16, ks), (positions, "positions", torch.int32, (B, p.M), True))
     dQ_out = _out(dQ_out, dQ, qs, t, "dQ_out")
     dK_out = _out(dK_out, dK, ks, torch.bfloat16, "dK_out")
     _lib.call("ma_rotaryBackward", _ptr(dQ), _ptr(dK), _ptr(dQ_out), _ptr(dK_out), int(t == torch.float32),
@@ -426,13 +429,10 @@ def rotaryCacheAppend(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache
     NKV = _groups(p, NKV)
     r = _rotary(inv_freq, NKV, interleaved, amplitude)
     qs, ks, cap = (B, p.M, p.N), (B, p.M, NKV * p.D), _cap(k_cache, "k_cache")
-    _check(q, "q", torch.bfloat16, qs)
-    for t, n in ((k, "k"), (v, "v")):
-        _check(t, n, torch.bfloat16, ks)
-    for t, n in ((k_cache, "k_cache"), (v_cache, "v_cache")):
-        _check(t, n, torch.bfloat16, (B, cap, NKV * p.D))
-    _check(start, "start", torch.int32, (B,))
-    _check_optional(lens, "lens", torch.int32, (B,))
+    cs = (B, cap, NKV * p.D)
+    _check_all((q, "q", torch.bfloat16, qs), (k, "k", torch.bfloat16, ks), (v, "v", torch.bfloat16, ks),
+               (k_cache, "k_cache", torch.bfloat16, cs), (v_cache, "v_cache", torch.bfloat16, cs),
+               (start, "start", torch.int32, (B,)), (lens, "lens", torch.int32, (B,), True))
     q_out = _out(q_out, q, qs, torch.bfloat16, "q_out")
     _lib.call("ma_rotaryCacheAppend", _ptr(q), _ptr(k), _ptr(v), _ptr(q_out), _ptr(k_cache), _ptr(v_cache),
               _ptr(start), _ptr(lens), ctypes.byref(r), ctypes.byref(p), B, cap, _stream(stream))
@@ -449,10 +449,8 @@ def windowAttentionForward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, p:
     NKV = _groups(p, NKV)
     w = _window(window, sinks, NKV)
     qs, ks = (B, p.M, p.N), (B, p.M, NKV * p.D)
-    _check(q, "q", torch.bfloat16, qs)
-    for t, n in ((k, "k"), (v, "v")):
-        _check(t, n, torch.bfloat16, ks)
-    _check_optional(lens, "lens", torch.int32, (B,))
+    _check_all((q, "q", torch.bfloat16, qs), (k, "k", torch.bfloat16, ks), (v, "v", torch.bfloat16, ks),
+               (lens, "lens", torch.int32, (B,), True))
     out = _out(out, q, qs, torch.bfloat16, "out")
     l = _out(l, q, (B, p.M, p.NH), torch.float32, "l")
     _lib.call("ma_windowAttentionForward", _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(l), _ptr(lens),
@@ -473,12 +471,9 @@ def windowAttentionBackward(dO: torch.Tensor, out: torch.Tensor, l: torch.Tensor
     NKV = _groups(p, NKV)
     w = _window(window, sinks, NKV)
     qs, ks = (B, p.M, p.N), (B, p.M, NKV * p.D)
-    for t, n in ((dO, "dO"), (out, "out"), (q, "q")):
-        _check(t, n, torch.bfloat16, qs)
-    _check(l, "l", torch.float32, (B, p.M, p.NH))
-    for t, n in ((k, "k"), (v, "v")):
-        _check(t, n, torch.bfloat16, ks)
-    _check_optional(lens, "lens", torch.int32, (B,))
+    _check_all((dO, "dO", torch.bfloat16, qs), (out, "out", torch.bfloat16, qs), (q, "q", torch.bfloat16, qs),
+               (l, "l", torch.float32, (B, p.M, p.NH)), (k, "k", torch.bfloat16, ks), (v, "v", torch.bfloat16, ks),
+               (lens, "lens", torch.int32, (B,), True))
     if dQ_dtype is None:
         dQ_dtype = dQ.dtype if isinstance(dQ, torch.Tensor) else torch.float32
     if dQ_dtype not in (torch.float32, torch.bfloat16):
@@ -506,11 +501,10 @@ def windowAttentionCached(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch
     NKV = _groups(p, NKV)
     w = _window(window, sinks, NKV)
     qs, cap = (B, p.M, p.N), _cap(k_cache, "k_cache")
-    _check(q, "q", torch.bfloat16, qs)
-    for t, n in ((k_cache, "k_cache"), (v_cache, "v_cache")):
-        _check(t, n, torch.bfloat16, (B, cap, NKV * p.D))
-    _check(start, "start", torch.int32, (B,))
-    _check_optional(lens, "lens", torch.int32, (B,))
+    cs = (B, cap, NKV * p.D)
+    _check_all((q, "q", torch.bfloat16, qs), (k_cache, "k_cache", torch.bfloat16, cs),
+               (v_cache, "v_cache", torch.bfloat16, cs), (start, "start", torch.int32, (B,)),
+               (lens, "lens", torch.int32, (B,), True))
     out = _out(out, q, qs, torch.bfloat16, "out")
     l = _out(l, q, (B, p.M, p.NH), torch.float32, "l")
     ws = _workspace(q, stream, "ma_windowAttentionCached_workspace", ctypes.byref(w), ctypes.byref(p), B, cap)

@@ -439,7 +439,7 @@ __global__ void __launch_bounds__(BwdCfg<HD, PERSIST, WIN>::NUM_THREADS, 1)
                      const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmdO,
                      const __grid_constant__ CUtensorMap tmdQ, __nv_bfloat16* __restrict__ dK,
                      __nv_bfloat16* __restrict__ dV, const BwdParams prm) {
-  pdl_wait_and_release();
+  if constexpr (!WIN) pdl_wait_and_release();  // WIN: after the set-up below
   using C = BwdCfg<HD, PERSIST, WIN>;
   extern __shared__ uint8_t smem_raw[];
   __shared__ int abort_flag;
@@ -516,6 +516,9 @@ __global__ void __launch_bounds__(BwdCfg<HD, PERSIST, WIN>::NUM_THREADS, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  // nothing before here touches global memory, so the barriers and TMEM are set
+  // up while the kernel before is still draining
+  if constexpr (WIN) pdl_wait_and_release();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(gbase + C::OFF_TSLOT);
   volatile int* abort_p = &abort_flag;
   const Sched sch{sbase + C::OFF_SCHED, BAR_UF, BAR_UE, abort_p};  // the unit schedule
@@ -1202,22 +1205,38 @@ __global__ void __launch_bounds__(256) window_stats_kernel(const WindowArgs a, c
     const int b = (int)(r / tiles), row0 = (int)(r % tiles) * 32;
     const int n = a.len(b);
     float mine = 0.0f;  // of row row0 + lane
+    // loads before stores: 8 rows of a lane in flight at once
+#pragma unroll
+    for (int i0 = 0; i0 < 32; i0 += 8 * RPI < 32 ? 8 * RPI : 32) {
+      constexpr int N = 8 * RPI < 32 ? 8 : 32 / RPI;
+      uint4 x[N], y[N];
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        const int row = row0 + i0 + k * RPI + lane / G;
+        const long long off = (((long long)b * a.M + row) * a.NH + h) * HD;
+        x[k] = y[k] = make_uint4(0u, 0u, 0u, 0u);
+        if (row < n) {
+          x[k] = __ldcs(reinterpret_cast<const uint4*>(dO + off) + lane % G);
+          y[k] = __ldcs(reinterpret_cast<const uint4*>(a.out + off) + lane % G);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        const int i = i0 + k * RPI;
+        float s = dot8(x[k], y[k]);
+#pragma unroll
+        for (int m = G / 2; m >= 1; m >>= 1) s += __shfl_xor_sync(0xffffffffu, s, m);
+        const float got = __shfl_sync(0xffffffffu, s, (lane - i) * G & 31);
+        if (lane >= i && lane < i + RPI) mine = got;
+      }
+    }
 #pragma unroll
     for (int i = 0; i < 32; i += RPI) {
       const int row = row0 + i + lane / G;
-      const long long off = (((long long)b * a.M + row) * a.NH + h) * HD;
-      float s = 0.0f;
-      if (row < n)
-        s = dot8(__ldcs(reinterpret_cast<const uint4*>(dO + off) + lane % G),
-                 __ldcs(reinterpret_cast<const uint4*>(a.out + off) + lane % G));
       if (row < a.M) {
-        float4* z = reinterpret_cast<float4*>(dQ + off) + lane % G;
+        float4* z = reinterpret_cast<float4*>(dQ + (((long long)b * a.M + row) * a.NH + h) * HD) + lane % G;
         z[0] = z[G] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
       }
-#pragma unroll
-      for (int m = G / 2; m >= 1; m >>= 1) s += __shfl_xor_sync(0xffffffffu, s, m);
-      const float got = __shfl_sync(0xffffffffu, s, (lane - i) * G & 31);
-      if (lane >= i && lane < i + RPI) mine = got;
     }
     const int row = row0 + lane;
     const bool valid = row < n;

@@ -133,6 +133,7 @@ struct FwdParams {
   float* dQz;
   uint32_t expire_ns;  // time-out test hook (ma_debug_expire_next_wait), 0 = off
   WindowArgs win;      // WIN only
+  bool single;         // WIN: a unit is one query tile (A), not a pair
 };
 
 // sum over 8 bf16 pairs of a[i] * b[i], fp32 (products of bf16 values are
@@ -194,6 +195,7 @@ __device__ __forceinline__ Unit decode_unit(const FwdParams& prm, int k) {
 // j < nA, tile B for j < nB except j == skip (the one tile that A's window
 // reaches and B's does not).
 struct WinUnit : Unit {
+  int tile0; // query tile of A; B's is the next
   int n;     // valid rows of the sequence
   int ns, lo, skip;
   int t0A, t1A, t0B, t1B;  // positions of the first and the last valid row of A and B
@@ -234,16 +236,17 @@ __device__ __forceinline__ WinUnit decode_win_unit(const FwdParams& prm, int k) 
   const WindowArgs& w = prm.win;
   WinUnit x;
   static_cast<Unit&>(x) = decode_unit<HB>(prm, k);
+  x.tile0 = prm.single ? x.pair : 2 * x.pair;
   x.n = w.len(x.b);
   x.cached = w.start != nullptr;
   x.nA = x.nB = x.nkv = x.ns = x.lo = 0;
   x.t0A = x.t1A = x.t0B = x.t1B = 0;
   x.skip = -1;
   x.end = x.n > 0 ? w.pos(x.b, x.n - 1) + 1 : 0;
-  const int r0 = 2 * x.pair * BM;
+  const int r0 = x.tile0 * BM;
   if (r0 >= x.n) return x;
   const int nS = w.sinks / BN + (w.sinks % BN != 0);
-  const bool b = r0 + BM < x.n;
+  const bool b = !prm.single && r0 + BM < x.n;
   const int rB = min(r0 + BM, x.n - 1);
   x.t0A = w.pos(x.b, r0);
   x.t1A = w.pos(x.b, min(r0 + BM - 1, x.n - 1));
@@ -273,7 +276,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
                      const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmO,
                      const __grid_constant__ CUtensorMap tmdO, const __grid_constant__ CUtensorMap tmdQz,
                      const FwdParams prm) {
-  pdl_wait_and_release();
+  if constexpr (!WIN) pdl_wait_and_release();  // WIN: after the set-up below
   using C = FwdCfg<HD, DYN, WIN>;
   extern __shared__ uint8_t smem_raw[];
   __shared__ int abort_flag;
@@ -357,6 +360,9 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  // nothing before here touches global memory, so the barriers and TMEM are set
+  // up while the kernel before is still draining
+  if constexpr (WIN) pdl_wait_and_release();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(gbase + C::OFF_TSLOT);
   volatile int* abort_p = &abort_flag;
   const Sched sch{sbase + C::OFF_SCHED, BAR_UF(0), BAR_UE(0), abort_p};
@@ -385,6 +391,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         const int col0 = un.h * HD;
         const int kv0 = WIN ? un.h / (prm.win.NH / prm.win.NKV) * HD : col0;  // columns of the K/V head
         if (WIN && un.nkv == 0) continue;  // only padding
+        int tile0 = 2 * un.pair;
+        if constexpr (WIN) tile0 = un.tile0;
         const int qs = qc % C::QST;
         if (qc >= C::QST && !mbar_wait(BAR_QE(qs), ((qc / C::QST) - 1) & 1, abort_p)) break;
         const int ntile = un.nB > 0 ? 2 : 1;
@@ -392,7 +400,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         for (int x = 0; x < ntile; ++x)
           for (int kb = 0; kb < C::KB; ++kb)
             tma_load_3d(sbase + C::OFF_Q + (qs * 2 + x) * C::QT_BYTES + kb * BM * 128, &tmQ,
-                        BAR_QF(qs), col0 + kb * 64, (2 * un.pair + x) * BM, un.b);
+                        BAR_QF(qs), col0 + kb * 64, (tile0 + x) * BM, un.b);
         ++qc;
         for (int j = 0; j < un.nkv; ++j) {
           int kt = j;
@@ -623,10 +631,11 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       if (k < 0) break;
       const auto un = unit(k);
       const int nt = x == 0 ? un.nA : un.nB;
-      const int qtile = 2 * un.pair + x;
+      int qtile = 2 * un.pair + x;
       if constexpr (WIN) {
+        qtile = un.tile0 + x;
         if (nt == 0) {  // only padding: O = 0, l = -inf (rows past T are clipped)
-          if (qtile * BM >= prm.T) continue;
+          if ((prm.single && x == 1) || qtile * BM >= prm.T) continue;
           if (wg_leader) bulk_wait_read<0>();
           bar_sync_named(wg_bar, 128);
           for (int kb = 0; kb < C::KB; ++kb)
@@ -1009,7 +1018,14 @@ cudaError_t launch_win(const WindowArgs& a, cudaStream_t st) {
   prm.NH = a.NH;
   prm.nbh = a.B * a.NH;
   prm.nqt = (a.M + BM - 1) / BM;
-  prm.npairs = (prm.nqt + 1) / 2;
+  // pairs share their K/V tiles, but a few of them leave most SMs idle: then a
+  // unit is one tile (2 x 500 queries of 16 heads over a cache, 64 pairs or 128
+  // tiles for 148 SMs)
+  int dev = 0, sms = 148;
+  cudaGetDevice(&dev);
+  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  prm.single = (long long)prm.nqt * prm.nbh <= sms;
+  prm.npairs = prm.single ? prm.nqt : (prm.nqt + 1) / 2;
   prm.nunits = prm.npairs * prm.nbh;
   prm.scale_log2 = LOG2E / sqrtf((float)HD);
   prm.lse = a.l;

@@ -187,6 +187,8 @@ def test_python_layer_refuses():
         A.windowAttentionForward(q, k, k, p, 1, 4, NKV=2)
     with pytest.raises(TypeError, match="inv_freq"):
         A.rotaryForward(q, k, [1.0], p, 1, NKV=2)
+    with pytest.raises(TypeError, match="'?q'? must"):
+        A.windowAttentionForward(None, k, k, p, 1, 4, NKV=2)
     with pytest.raises(TypeError, match="cap"):
         A.windowAttentionCached(q, k[0], k[0], None, p, 1, 4, NKV=2)
     with pytest.raises(ValueError, match="even"):
