@@ -138,7 +138,7 @@ struct BwdCfg {
   // prefetch the next unit (under launch control too, where a CTA also runs
   // many units: C4 backward 3.75 -> 3.64 ms against one K/V buffer and three
   // Q/dO stages); D=128 has room for one of each
-  static constexpr int STAGES = D64 ? 2 : 1;
+  static constexpr int STAGES = D64 ? (WIN ? 3 : 2) : 1;
   static constexpr int KVB = D64 ? 2 : 1;
   static constexpr bool P_IN_TMEM = D64;         // P^T in TMEM (else smem)
   static constexpr bool EARLY_S = D64;           // next S^T before dV/dK/dQ
@@ -150,7 +150,7 @@ struct BwdCfg {
   // ring stages: the statistics warp loads a step's values into registers a
   // step ahead, so one stage suffices where the shared memory is tight.
   static constexpr int DQSB = 1;
-  static constexpr int SSTG = (D64 && PERSIST) ? 1 : 8;
+  static constexpr int SSTG = D64 && (PERSIST || WIN) ? 1 : 8;
   static constexpr uint32_t KV_BYTES = BK * HD * 2;
   static constexpr uint32_t QD_BYTES = BQ * HD * 2;
   static constexpr uint32_t PT_BYTES = BK * BQ * 2;
@@ -174,13 +174,18 @@ struct BwdCfg {
   static constexpr int NSCHED = DYN ? (int)kSchedSlots : 0;
   static constexpr uint32_t SCHED_READERS = 5 + NCOMP / 32 + (DRAIN_WG ? 4 : 0);
   static constexpr uint32_t OFF_SCHED = OFF_STAT + SSTG * STAT_BYTES;
-  static constexpr uint32_t OFF_BAR = OFF_SCHED + NSCHED * 16;
+  // WIN: the units' descriptors (unit 0's after those of the responses' slots),
+  // decoded once, by the producer
+  static constexpr int NDESC = WIN ? NSCHED + 1 : 0;
+  static constexpr uint32_t DESC_BYTES = 48;
+  static constexpr uint32_t OFF_DESC = OFF_SCHED + NSCHED * 16;
+  static constexpr uint32_t OFF_BAR = OFF_DESC + NDESC * DESC_BYTES;
   // kv_full/empty[KVB], qd_full/empty[S], st_full/empty[8], then s_full,
   // s_free, p_ready, p_free, dq_full, dq_free, dqs_full, dqs_free, done,
   // acc_free, never (nothing arrives: the time-out test hook), fin (the
   // UMMA issuer's wind-down), sched_full/empty[NSCHED] and, for WIN,
-  // qd_fixed[S] (padding rows zeroed)
-  static constexpr int NBAR = 2 * KVB + 2 * STAGES + 2 * SSTG + 12 + 2 * (DQSB - 1) + 2 * NSCHED + (WIN ? STAGES : 0);
+  // qd_fixed[S] (padding rows zeroed) and desc_full[NDESC]
+  static constexpr int NBAR = 2 * KVB + 2 * STAGES + 2 * SSTG + 12 + 2 * (DQSB - 1) + 2 * NSCHED + (WIN ? STAGES : 0) + NDESC;
   static constexpr uint32_t OFF_TSLOT = OFF_BAR + NBAR * 8;
   static constexpr uint32_t SMEM_BYTES = OFF_TSLOT + 16 + 1024;
   static constexpr uint32_t TCOL_S = 0;
@@ -225,21 +230,20 @@ struct BUnit {
 };
 
 // A unit under a window: nt query tiles from q0 on, for each query head.
-struct WinBUnit {
+// (48 bytes: it is passed on through shared memory.)
+struct alignas(16) WinBUnit {
   int b, h, kt, nq;
   int q0, nt, head0;
   int n;     // valid rows; 0 where the unit has none: everything is masked
   int slot;  // partial sums go to this slot, or -1: straight to dK, dV
+  int valid; // 0: no unit is left
+  int pad[2];
   __device__ int q_tile(int i) const { return q0 + i % nt; }
   __device__ int q_head(int i) const { return head0 + i / nt; }
   // key `key` sees queries [*from, *to) of the query tile at row0
   __device__ void seen(const WinBwd& w, int key, int row0, int* from, int* to) const {
     *from = key - row0;
     *to = (key < w.sinks ? n : min(n, key + w.window)) - row0;
-  }
-  __device__ bool whole(const WinBwd& w, int row0) const {
-    const int k0 = kt * BK;
-    return k0 + BK - 1 <= row0 && (row0 + BQ - 1 - k0 < w.window || k0 + BK - 1 < w.sinks) && row0 + BQ <= n;
   }
 };
 
@@ -302,11 +306,12 @@ __device__ __forceinline__ WinBUnit bwd_win_unit(const BwdParams& prm, int k) {
   return u;
 }
 
-template <int HB, bool WIN>
-__device__ __forceinline__ auto decode_bwd_unit(const BwdParams& prm, int k) {
-  if constexpr (WIN) return bwd_win_unit<HB>(prm, k);
-  else return bwd_unit<HB>(prm, k);
-}
+// The descriptors' ring: unit 0 in slot kSchedSlots, unit g in the slot of the
+// response that named it, which the readers release together.
+struct UnitRing {
+  WinBUnit* desc;
+  uint32_t full;  // slot 0's barrier
+};
 
 // Static schedule: the unit of this CTA in round g, -1 when rounds are
 // exhausted, -2 when this CTA has none in round g (last, partial round).
@@ -330,12 +335,37 @@ struct StepIter {
   bool valid;
 };
 
-template <bool DYN, int HB, bool WIN, bool WARP>
-__device__ __forceinline__ bool next_unit(const BwdParams& prm, StepIter<WIN>& s, const Sched& sc) {
-  if constexpr (DYN) {
+// PUBLISH (WIN's producer): decodes the unit and passes it on; WIN's other
+// roles read it (the code of twenty decodings would not fit the instruction
+// cache).
+template <bool DYN, int HB, bool WIN, bool WARP, bool PUBLISH = false>
+__device__ __forceinline__ bool next_unit(const BwdParams& prm, StepIter<WIN>& s, const Sched& sc, const UnitRing& ur) {
+  if constexpr (WIN && PUBLISH) {
+    const uint32_t g = (uint32_t)s.g++;
+    const int k = sched_unit<WARP>(sc, g);
+    const bool some = k >= 0 && k < prm.nunits;
+    if (some) s.u = bwd_win_unit<HB>(prm, k);
+    s.u.valid = some;
+    const uint32_t slot = g == 0 ? kSchedSlots : (g - 1) % kSchedSlots;
+    ur.desc[slot] = s.u;
+    mbar_arrive(ur.full + 8u * slot);
+    return some;
+  } else if constexpr (WIN) {
+    const uint32_t g = (uint32_t)s.g++;
+    const uint32_t slot = g == 0 ? kSchedSlots : (g - 1) % kSchedSlots;
+    const uint32_t ph = g == 0 ? 0u : ((g - 1) / kSchedSlots) & 1u;
+    if (!(WARP ? mbar_wait_warp(ur.full + 8u * slot, ph, sc.abort) : mbar_wait(ur.full + 8u * slot, ph, sc.abort)))
+      return false;
+    s.u = ur.desc[slot];
+    if (g > 0) {
+      if (WARP) __syncwarp();
+      if (!WARP || (threadIdx.x & 31) == 0) mbar_arrive(sc.empty + 8u * slot);
+    }
+    return s.u.valid != 0;
+  } else if constexpr (DYN) {
     const int k = sched_unit<WARP>(sc, (uint32_t)s.g++);
     if (k < 0 || k >= prm.nunits) return false;
-    s.u = decode_bwd_unit<HB, WIN>(prm, k);
+    s.u = bwd_unit<HB>(prm, k);
     return true;
   } else {
     for (;;) {
@@ -343,26 +373,26 @@ __device__ __forceinline__ bool next_unit(const BwdParams& prm, StepIter<WIN>& s
       if (k == -1) return false;
       ++s.g;
       if (k >= 0) {
-        s.u = decode_bwd_unit<HB, WIN>(prm, k);
+        s.u = bwd_unit<HB>(prm, k);
         return true;
       }
     }
   }
 }
 
-template <bool DYN, int HB, bool WIN, bool WARP>
-__device__ __forceinline__ StepIter<WIN> first_step(const BwdParams& prm, const Sched& sc) {
+template <bool DYN, int HB, bool WIN, bool WARP, bool PUBLISH = false>
+__device__ __forceinline__ StepIter<WIN> first_step(const BwdParams& prm, const Sched& sc, const UnitRing& ur) {
   StepIter<WIN> s;
   s.g = 0;
   s.i = 0;
   s.t = 0;
   s.uc = 0;
-  s.valid = next_unit<DYN, HB, WIN, WARP>(prm, s, sc);
+  s.valid = next_unit<DYN, HB, WIN, WARP, PUBLISH>(prm, s, sc, ur);
   return s;
 }
 
-template <bool DYN, int HB, bool WIN, bool WARP>
-__device__ __forceinline__ void advance(const BwdParams& prm, StepIter<WIN>& s, const Sched& sc) {
+template <bool DYN, int HB, bool WIN, bool WARP, bool PUBLISH = false>
+__device__ __forceinline__ void advance(const BwdParams& prm, StepIter<WIN>& s, const Sched& sc, const UnitRing& ur) {
   ++s.t;
   if (s.i + 1 < s.u.nq) {
     ++s.i;
@@ -370,7 +400,7 @@ __device__ __forceinline__ void advance(const BwdParams& prm, StepIter<WIN>& s, 
   }
   s.i = 0;
   ++s.uc;
-  s.valid = next_unit<DYN, HB, WIN, WARP>(prm, s, sc);
+  s.valid = next_unit<DYN, HB, WIN, WARP, PUBLISH>(prm, s, sc, ur);
 }
 
 // P^T and dS^T for N query columns of one key row.  s[] holds S^T on entry
@@ -507,6 +537,7 @@ __global__ void __launch_bounds__(BwdCfg<HD, PERSIST, WIN>::NUM_THREADS, 1)
       mbar_init(BAR_UF + 8u * u, 1);
       mbar_init(BAR_UE + 8u * u, C::SCHED_READERS);
     }
+    for (int u = 0; u < C::NDESC; ++u) mbar_init(BAR_QZ(C::STAGES + u), 1);  // desc_full
     fence_mbar_init();
   }
   if (warp == 1) {
@@ -522,6 +553,7 @@ __global__ void __launch_bounds__(BwdCfg<HD, PERSIST, WIN>::NUM_THREADS, 1)
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(gbase + C::OFF_TSLOT);
   volatile int* abort_p = &abort_flag;
   const Sched sch{sbase + C::OFF_SCHED, BAR_UF, BAR_UE, abort_p};  // the unit schedule
+  const UnitRing ring{reinterpret_cast<WinBUnit*>(gbase + C::OFF_DESC), BAR_QZ(C::STAGES)};
 
   // WIN: whether step s brings tiles with padding rows (a unit's first step:
   // its K tile too); past the tensor's end TMA has filled in zeros itself
@@ -543,7 +575,7 @@ __global__ void __launch_bounds__(BwdCfg<HD, PERSIST, WIN>::NUM_THREADS, 1)
         tma_prefetch_desc(&tmdO);
         uint32_t kv_armed = 0, q_armed = 0;  // loads issued into each ring
         uint32_t nreq = 0;                   // launch-control requests issued
-        for (StepIter<WIN> s = first_step<C::DYN, C::HB, WIN, false>(prm, sch); s.valid; advance<C::DYN, C::HB, WIN, false>(prm, s, sch)) {
+        for (StepIter<WIN> s = first_step<C::DYN, C::HB, WIN, false, true>(prm, sch, ring); s.valid; advance<C::DYN, C::HB, WIN, false, true>(prm, s, sch, ring)) {
           const int kv0 = s.u.h * HD, col0 = s.u.q_head(s.i) * HD;
           if (s.i == 0) {  // K/V of a new unit
             const int kvs = s.uc % C::KVB;
@@ -623,24 +655,24 @@ __global__ void __launch_bounds__(BwdCfg<HD, PERSIST, WIN>::NUM_THREADS, 1)
           umma_commit(BAR_SF);
           return true;
         };
-        StepIter<WIN> cur = first_step<C::DYN, C::HB, WIN, false>(prm, sch);
+        StepIter<WIN> cur = first_step<C::DYN, C::HB, WIN, false>(prm, sch, ring);
         StepIter<WIN> la = cur;  // next step whose S^T/dP^T is to be issued
         bool ok = true;
         if (la.valid) {
           ok = issue_s(la);
-          advance<C::DYN, C::HB, WIN, false>(prm, la, sch);
+          advance<C::DYN, C::HB, WIN, false>(prm, la, sch, ring);
         }
         // time-out test hook: with the first products in flight, wait on a
         // barrier nothing arrives at until the hook's limit runs out
         if (ok && prm.expire_ns) ok = mbar_wait(BAR_NEVER, 0, abort_p, prm.expire_ns);
-        for (; ok && cur.valid; advance<C::DYN, C::HB, WIN, false>(prm, cur, sch)) {
+        for (; ok && cur.valid; advance<C::DYN, C::HB, WIN, false>(prm, cur, sch, ring)) {
           // the next step's S^T/dP^T ahead of this step's products, except
           // where it starts a unit whose K/V can only be loaded into the
           // single K/V buffer once this step's products are done with it
           const bool early = C::EARLY_S && la.valid && (C::KVB > 1 || la.uc == cur.uc);
           if (early) {
             if (!issue_s(la)) break;
-            advance<C::DYN, C::HB, WIN, false>(prm, la, sch);
+            advance<C::DYN, C::HB, WIN, false>(prm, la, sch, ring);
           }
           const int st = cur.t % C::STAGES;
           const int kvs = cur.uc % C::KVB;
@@ -687,7 +719,7 @@ __global__ void __launch_bounds__(BwdCfg<HD, PERSIST, WIN>::NUM_THREADS, 1)
           // (after them: D=128, or a unit start with a single K/V buffer)
           if ((!C::EARLY_S || C::KVB == 1) && !early && la.valid) {
             if (!issue_s(la)) break;
-            advance<C::DYN, C::HB, WIN, false>(prm, la, sch);
+            advance<C::DYN, C::HB, WIN, false>(prm, la, sch, ring);
           }
         }
         if (*abort_p) {  // wind-down: every UMMA issued must complete before TMEM is freed
@@ -733,13 +765,13 @@ __global__ void __launch_bounds__(BwdCfg<HD, PERSIST, WIN>::NUM_THREADS, 1)
           for (int i = a * 8 + lane; i < BQ * 8; i += 32) blk[i] = make_uint4(0u, 0u, 0u, 0u);
         }
       };
-      StepIter<WIN> s = first_step<C::DYN, C::HB, WIN, true>(prm, sch);
+      StepIter<WIN> s = first_step<C::DYN, C::HB, WIN, true>(prm, sch, ring);
       if (s.valid) load_stats(s);
       while (s.valid) {
         const float cl[4] = {nl[0], nl[1], nl[2], nl[3]};
         const float cd[4] = {nd[0], nd[1], nd[2], nd[3]};
         StepIter<WIN> nx = s;
-        advance<C::DYN, C::HB, WIN, true>(prm, nx, sch);
+        advance<C::DYN, C::HB, WIN, true>(prm, nx, sch, ring);
         if (nx.valid) load_stats(nx);  // the next step's, in flight while this one waits
         if constexpr (WIN) {
           // every stage (and a unit's K/V) is waited for and released, so that
@@ -778,7 +810,7 @@ __global__ void __launch_bounds__(BwdCfg<HD, PERSIST, WIN>::NUM_THREADS, 1)
     } else {
       // ------------------------------------------------- dQ reduce issuer
       if (lane == 0) {
-        for (StepIter<WIN> s = first_step<C::DYN, C::HB, WIN, false>(prm, sch); s.valid; advance<C::DYN, C::HB, WIN, false>(prm, s, sch)) {
+        for (StepIter<WIN> s = first_step<C::DYN, C::HB, WIN, false>(prm, sch, ring); s.valid; advance<C::DYN, C::HB, WIN, false>(prm, s, sch, ring)) {
           const int b = s.t % C::DQSB;
           if (!mbar_wait(BAR_DSF(b), (s.t / C::DQSB) & 1, abort_p)) break;
           for (int box = 0; box < HD / 32; ++box)
@@ -899,7 +931,7 @@ __global__ void __launch_bounds__(BwdCfg<HD, PERSIST, WIN>::NUM_THREADS, 1)
     decltype(StepIter<WIN>::u) prev{};
     uint32_t t = 0, uc = 0;
     bool have_prev = false;
-    for (StepIter<WIN> st_it = first_step<C::DYN, C::HB, WIN, true>(prm, sch); ok && st_it.valid; advance<C::DYN, C::HB, WIN, true>(prm, st_it, sch)) {
+    for (StepIter<WIN> st_it = first_step<C::DYN, C::HB, WIN, true>(prm, sch, ring); ok && st_it.valid; advance<C::DYN, C::HB, WIN, true>(prm, st_it, sch, ring)) {
       const auto& u = st_it.u;
       const int i = st_it.i;
       t = st_it.t;
@@ -946,16 +978,14 @@ __global__ void __launch_bounds__(BwdCfg<HD, PERSIST, WIN>::NUM_THREADS, 1)
       const float* stt = stat_base + ss * (2 * BQ) + part * CPP;
       if constexpr (WIN) {
         const int row0 = u.q_tile(i) * BQ;
-        if (u.whole(prm.win, row0)) {
-          p_ds_row<false, CPP>(s, dp, stt, stt + BQ, c, sc, krow, part * CPP);
-        } else {
-          int from, to;
-          u.seen(prm.win, u.kt * BK + krow, row0 + part * CPP, &from, &to);
-          uint32_t see[CPP / 32];
+        // one form for masked and whole steps (a second would cost more in
+        // instruction fetches than it saves)
+        int from, to;
+        u.seen(prm.win, u.kt * BK + krow, row0 + part * CPP, &from, &to);
+        uint32_t see[CPP / 32];
 #pragma unroll
-          for (int w = 0; w < CPP / 32; ++w) see[w] = bits_below(to - 32 * w) & ~bits_below(from - 32 * w);
-          p_ds_row<false, CPP, true>(s, dp, stt, stt + BQ, c, sc, krow, part * CPP, see);
-        }
+        for (int w = 0; w < CPP / 32; ++w) see[w] = bits_below(to - 32 * w) & ~bits_below(from - 32 * w);
+        p_ds_row<false, CPP, true>(s, dp, stt, stt + BQ, c, sc, krow, part * CPP, see);
       } else if (i == 0) {
         p_ds_row<true, CPP>(s, dp, stt, stt + BQ, c, sc, krow, part * CPP);
       } else {
@@ -1012,7 +1042,7 @@ __global__ void __launch_bounds__(BwdCfg<HD, PERSIST, WIN>::NUM_THREADS, 1)
     const int row = quarter * 32 + lane;
     const uint32_t tl = tmem + ((uint32_t)(quarter * 32) << 16);
     bool ok = true;
-    for (StepIter<WIN> s = first_step<C::DYN, C::HB, WIN, true>(prm, sch); ok && s.valid; advance<C::DYN, C::HB, WIN, true>(prm, s, sch)) {
+    for (StepIter<WIN> s = first_step<C::DYN, C::HB, WIN, true>(prm, sch, ring); ok && s.valid; advance<C::DYN, C::HB, WIN, true>(prm, s, sch, ring)) {
       const uint32_t t = s.t;
       const int b = t % C::DQSB;
       uint8_t* dqs = gbase + C::OFF_DQS + b * C::DQS_BYTES;
