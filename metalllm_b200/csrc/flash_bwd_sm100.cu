@@ -76,8 +76,8 @@
 // units of their own where that chain would be the longest (WinBwd), whose
 // partial dK/dV the launcher's last kernel adds up in a fixed order.  The
 // statistics come ready from a kernel before this one, [B][NH][T], and the
-// warp that stages them also zeroes the padding rows of Q, dO and K tiles
-// (their P and dS are 0, but 0 * NaN is not).  A unit or chunk without a
+// warp that stages them also zeroes the padding rows of Q, dO, K and V tiles
+// (their P is 0, but 0 * NaN is not).  A unit or chunk without a
 // valid row runs one step in which everything is masked and so writes zeros.
 //
 // All mbarrier waits are bounded (about 2 s); on time-out the CTA winds down,
@@ -151,6 +151,9 @@ struct BwdCfg {
   // step ahead, so one stage suffices where the shared memory is tight.
   static constexpr int DQSB = 1;
   static constexpr int SSTG = D64 && (PERSIST || WIN) ? 1 : 8;
+  // WIN has more code in flight, and fetching it stalls the warps more than
+  // the UMMA issuer's loops do
+  static constexpr int UMMA_UNROLL = WIN && D64 ? 2 : 8;
   static constexpr uint32_t KV_BYTES = BK * HD * 2;
   static constexpr uint32_t QD_BYTES = BQ * HD * 2;
   static constexpr uint32_t PT_BYTES = BK * BQ * 2;
@@ -406,8 +409,8 @@ __device__ __forceinline__ void advance(const BwdParams& prm, StepIter<WIN>& s, 
 // P^T and dS^T for N query columns of one key row.  s[] holds S^T on entry
 // and P^T on exit; dp[] holds dP^T on entry and dS^T on exit.  nl = -l*log2e
 // and nd = -D/sqrt(D) per query column (shared memory, broadcast reads).
-// SEEN (a window's masked step): bit j of see[] says whether query column j is
-// visible; else P and dS are 0 whatever the products hold.
+// SEEN (a window's step): bit j of see[] says whether query column j is visible;
+// else P and with it dS are 0 (padding rows hold zeros, so dP is finite).
 template <bool DIAG, int N, bool SEEN = false>
 __device__ __forceinline__ void p_ds_row(float (&s)[N], float (&dp)[N], const float* nl,
                                          const float* nd, float c, float sc, int krow, int qcol0,
@@ -420,6 +423,13 @@ __device__ __forceinline__ void p_ds_row(float (&s)[N], float (&dp)[N], const fl
     const float2 t0 = __ffma2_rn(make_float2(s[j], s[j + 1]), c2, make_float2(L.x, L.y));
     const float2 t1 = __ffma2_rn(make_float2(s[j + 2], s[j + 3]), c2, make_float2(L.z, L.w));
     float p0 = ex2(t0.x), p1 = ex2(t0.y), p2 = ex2(t1.x), p3 = ex2(t1.y);
+    if constexpr (SEEN) {
+      const uint32_t m = see[j / 32] >> (j % 32);
+      if (!(m & 1u)) p0 = 0.0f;
+      if (!(m & 2u)) p1 = 0.0f;
+      if (!(m & 4u)) p2 = 0.0f;
+      if (!(m & 8u)) p3 = 0.0f;
+    }
     if (DIAG) {  // key after query: P = 0 (attention.metal:282)
       const int q = qcol0 + j;
       if (krow > q) p0 = 0.0f;
@@ -439,11 +449,6 @@ __device__ __forceinline__ void p_ds_row(float (&s)[N], float (&dp)[N], const fl
     dp[j + 1] = r0.y;
     dp[j + 2] = r1.x;
     dp[j + 3] = r1.y;
-    if constexpr (SEEN) {
-#pragma unroll
-      for (int e = j; e < j + 4; ++e)
-        if (!(see[e / 32] & (1u << (e % 32)))) s[e] = dp[e] = 0.0f;
-    }
   }
 }
 
@@ -640,13 +645,13 @@ __global__ void __launch_bounds__(BwdCfg<HD, PERSIST, WIN>::NUM_THREADS, 1)
           const uint32_t sv = sbase + C::OFF_V + kvs * C::KV_BYTES;
           const uint32_t sq = sbase + C::OFF_Q + st * C::QD_BYTES;
           const uint32_t sdo = sbase + C::OFF_DO + st * C::QD_BYTES;
-#pragma unroll
+#pragma unroll C::UMMA_UNROLL
           for (int kk = 0; kk < HD / 16; ++kk) {
             const uint32_t off = (kk >> 2) * (BK * 128) + (kk & 3) * 32;
             umma_bf16_ss(tmem + C::TCOL_S, smem_desc_sw128(sk + off, 16, 1024),
                          smem_desc_sw128(sq + off, 16, 1024), IDESC_S, kk > 0 ? 1u : 0u);
           }
-#pragma unroll
+#pragma unroll C::UMMA_UNROLL
           for (int kk = 0; kk < HD / 16; ++kk) {
             const uint32_t off = (kk >> 2) * (BK * 128) + (kk & 3) * 32;
             umma_bf16_ss(tmem + C::TCOL_DP, smem_desc_sw128(sv + off, 16, 1024),
@@ -683,7 +688,7 @@ __global__ void __launch_bounds__(BwdCfg<HD, PERSIST, WIN>::NUM_THREADS, 1)
           // the previous unit's epilogue must have read dK/dV out of TMEM
           if (cur.i == 0 && cur.uc >= 1 && !mbar_wait(BAR_ACC, (cur.uc - 1) & 1, abort_p)) break;
           tc_fence_after();
-#pragma unroll
+#pragma unroll C::UMMA_UNROLL
           for (int kk = 0; kk < BQ / 16; ++kk) {  // dV += P^T dO_i
             const uint64_t bd = smem_desc_sw128(sdo + kk * 2048, BQ * 128, 1024);
             if (C::P_IN_TMEM) {
@@ -694,7 +699,7 @@ __global__ void __launch_bounds__(BwdCfg<HD, PERSIST, WIN>::NUM_THREADS, 1)
               umma_bf16_ss(tmem + C::TCOL_DV, ad, bd, IDESC_KV, (cur.i > 0 || kk > 0) ? 1u : 0u);
             }
           }
-#pragma unroll
+#pragma unroll C::UMMA_UNROLL
           for (int kk = 0; kk < BQ / 16; ++kk) {  // dK += dS^T Q_i
             const uint64_t ad = smem_desc_sw128(sdst + (kk >> 2) * (BK * 128) + (kk & 3) * 32, 16, 1024);
             const uint64_t bd = smem_desc_sw128(sq + kk * 2048, BQ * 128, 1024);
@@ -704,7 +709,7 @@ __global__ void __launch_bounds__(BwdCfg<HD, PERSIST, WIN>::NUM_THREADS, 1)
           // the dQ columns must have been drained (previous step)
           if (cur.t >= 1 && !mbar_wait(BAR_DQE, (cur.t - 1) & 1, abort_p)) break;
           tc_fence_after();
-#pragma unroll
+#pragma unroll C::UMMA_UNROLL
           for (int kk = 0; kk < BK / 16; ++kk) {  // dQ_i = dS K (A = dS^T as MN-major)
             const uint64_t ad = smem_desc_sw128(sdst + kk * 2048, BK * 128, 1024);
             const uint64_t bd = smem_desc_sw128(sk + kk * 2048, BK * 128, 1024);
@@ -780,7 +785,10 @@ __global__ void __launch_bounds__(BwdCfg<HD, PERSIST, WIN>::NUM_THREADS, 1)
           if (s.i == 0 && !mbar_wait_warp(BAR_KF(kvs), (s.uc / C::KVB) & 1, abort_p)) break;
           if (!mbar_wait_warp(BAR_QF(qs), (s.t / C::STAGES) & 1, abort_p)) break;
           const bool fq = fix_q(s), fk = fix_k(s);
-          if (fk) zero_rows(C::OFF_K + kvs * C::KV_BYTES, max(0, s.u.n - s.u.kt * BK));
+          if (fk) {
+            zero_rows(C::OFF_K + kvs * C::KV_BYTES, max(0, s.u.n - s.u.kt * BK));
+            zero_rows(C::OFF_V + kvs * C::KV_BYTES, max(0, s.u.n - s.u.kt * BK));
+          }
           if (fq) {
             const int a = max(0, s.u.n - s.u.q_tile(s.i) * BQ);
             zero_rows(C::OFF_Q + qs * C::QD_BYTES, a);
@@ -929,16 +937,15 @@ __global__ void __launch_bounds__(BwdCfg<HD, PERSIST, WIN>::NUM_THREADS, 1)
     // of the next unit has been handed to the tensor core (or after the last
     // step of the last unit), so they overlap the next unit's UMMAs.
     decltype(StepIter<WIN>::u) prev{};
-    uint32_t t = 0, uc = 0;
     bool have_prev = false;
-    for (StepIter<WIN> st_it = first_step<C::DYN, C::HB, WIN, true>(prm, sch, ring); ok && st_it.valid; advance<C::DYN, C::HB, WIN, true>(prm, st_it, sch, ring)) {
+    // Step st: P^T and dS^T formed and handed to the UMMA issuer.
+    auto form = [&](const StepIter<WIN>& st_it) {
       const auto& u = st_it.u;
       const int i = st_it.i;
-      t = st_it.t;
-      uc = st_it.uc;
+      const uint32_t t = st_it.t;
       const int ss = t % C::SSTG;
       ok = mbar_wait_warp(BAR_SF, t & 1, abort_p);
-      if (!ok) break;
+      if (!ok) return;
       tc_fence_after();
       float s[CPP], dp[CPP];
       if constexpr (CPP == 64) {
@@ -974,7 +981,7 @@ __global__ void __launch_bounds__(BwdCfg<HD, PERSIST, WIN>::NUM_THREADS, 1)
       tc_fence_before();
       mbar_arrive(BAR_SE);
       ok = mbar_wait_warp(BAR_TF(ss), (t / C::SSTG) & 1, abort_p);
-      if (!ok) break;
+      if (!ok) return;
       const float* stt = stat_base + ss * (2 * BQ) + part * CPP;
       if constexpr (WIN) {
         const int row0 = u.q_tile(i) * BQ;
@@ -996,7 +1003,7 @@ __global__ void __launch_bounds__(BwdCfg<HD, PERSIST, WIN>::NUM_THREADS, 1)
       // staging shares their smem its reduction must have read it
       if (t >= 1) ok = mbar_wait_warp(BAR_PE, (t - 1) & 1, abort_p);
       if (ok && C::DQS_ALIAS && t >= 1) ok = mbar_wait_warp(BAR_DSE(0), (t - 1) & 1, abort_p);
-      if (!ok) break;
+      if (!ok) return;
       // this part's columns of the key row: P^T (bf16 pairs in TMEM, or smem),
       // dS^T (smem); chunk (part*CPP % 64) / 8 of 64-column block part*CPP / 64
       const int blk = (part * CPP) / 64, ch0 = ((part * CPP) % 64) / 8;
@@ -1014,25 +1021,32 @@ __global__ void __launch_bounds__(BwdCfg<HD, PERSIST, WIN>::NUM_THREADS, 1)
       fence_proxy_async_smem();
       tc_fence_before();
       mbar_arrive(BAR_PR);
+    };
+    for (StepIter<WIN> st_it = first_step<C::DYN, C::HB, WIN, true>(prm, sch, ring); ok;
+         advance<C::DYN, C::HB, WIN, true>(prm, st_it, sch, ring)) {
+      if (st_it.valid) form(st_it);
+      if (!ok) break;
       // on a unit's first step the previous unit's dK/dV epilogue comes
       // first: the UMMA issuer waits for it before this step's products,
-      // the dQ product that drain_dq(t) waits for among them
+      // the dQ product that drain_dq(t) waits for among them.  The last
+      // unit's follows its last step.
       if constexpr (C::EPI_COMPUTE) {
-        if (i == 0 && have_prev) epilogue(prev, uc - 1);
-        prev = u;
+        if (have_prev && (!st_it.valid || st_it.i == 0)) {
+          if constexpr (!C::DRAIN_WG && C::EARLY_S)
+            if (!st_it.valid) drain_dq(st_it.t - 1);
+          epilogue(prev, st_it.uc - 1);
+        }
+        if (!st_it.valid) break;
+        prev = st_it.u;
         have_prev = true;
       }
       if constexpr (!C::DRAIN_WG) {
         if (C::EARLY_S) {
-          if (t >= 1) drain_dq(t - 1);
+          if (st_it.t >= 1) drain_dq(st_it.t - 1);
         } else {
-          drain_dq(t);
+          drain_dq(st_it.t);
         }
       }
-    }
-    if (ok && have_prev) {  // the last unit of this CTA
-      if constexpr (!C::DRAIN_WG && C::EARLY_S) drain_dq(t);
-      if constexpr (C::EPI_COMPUTE) epilogue(prev, uc);
     }
   } else {
     reg_dealloc<C::REGS_DRAIN>();
