@@ -151,9 +151,9 @@ struct BwdCfg {
   // step ahead, so one stage suffices where the shared memory is tight.
   static constexpr int DQSB = 1;
   static constexpr int SSTG = D64 && (PERSIST || WIN) ? 1 : 8;
-  // WIN has more code in flight, and fetching it stalls the warps more than
-  // the UMMA issuer's loops do
-  static constexpr int UMMA_UNROLL = WIN && D64 ? 2 : 8;
+  // WIN at D=64 has the most code in flight, and fetching it stalls the warps
+  // more than the UMMA issuer's loops do
+  static constexpr int UMMA_UNROLL = WIN && D64 ? 1 : 8;
   static constexpr uint32_t KV_BYTES = BK * HD * 2;
   static constexpr uint32_t QD_BYTES = BQ * HD * 2;
   static constexpr uint32_t PT_BYTES = BK * BQ * 2;
@@ -645,17 +645,17 @@ __global__ void __launch_bounds__(BwdCfg<HD, PERSIST, WIN>::NUM_THREADS, 1)
           const uint32_t sv = sbase + C::OFF_V + kvs * C::KV_BYTES;
           const uint32_t sq = sbase + C::OFF_Q + st * C::QD_BYTES;
           const uint32_t sdo = sbase + C::OFF_DO + st * C::QD_BYTES;
+          const uint64_t dk = smem_desc_sw128(sk, 16, 1024), dv = smem_desc_sw128(sv, 16, 1024);
+          const uint64_t dq = smem_desc_sw128(sq, 16, 1024), ddo = smem_desc_sw128(sdo, 16, 1024);
 #pragma unroll C::UMMA_UNROLL
           for (int kk = 0; kk < HD / 16; ++kk) {
             const uint32_t off = (kk >> 2) * (BK * 128) + (kk & 3) * 32;
-            umma_bf16_ss(tmem + C::TCOL_S, smem_desc_sw128(sk + off, 16, 1024),
-                         smem_desc_sw128(sq + off, 16, 1024), IDESC_S, kk > 0 ? 1u : 0u);
+            umma_bf16_ss(tmem + C::TCOL_S, desc_at(dk, off), desc_at(dq, off), IDESC_S, kk > 0 ? 1u : 0u);
           }
 #pragma unroll C::UMMA_UNROLL
           for (int kk = 0; kk < HD / 16; ++kk) {
             const uint32_t off = (kk >> 2) * (BK * 128) + (kk & 3) * 32;
-            umma_bf16_ss(tmem + C::TCOL_DP, smem_desc_sw128(sv + off, 16, 1024),
-                         smem_desc_sw128(sdo + off, 16, 1024), IDESC_S, kk > 0 ? 1u : 0u);
+            umma_bf16_ss(tmem + C::TCOL_DP, desc_at(dv, off), desc_at(ddo, off), IDESC_S, kk > 0 ? 1u : 0u);
           }
           umma_commit(BAR_SF);
           return true;
@@ -688,33 +688,30 @@ __global__ void __launch_bounds__(BwdCfg<HD, PERSIST, WIN>::NUM_THREADS, 1)
           // the previous unit's epilogue must have read dK/dV out of TMEM
           if (cur.i == 0 && cur.uc >= 1 && !mbar_wait(BAR_ACC, (cur.uc - 1) & 1, abort_p)) break;
           tc_fence_after();
+          const uint64_t bdo = smem_desc_sw128(sdo, BQ * 128, 1024), bq = smem_desc_sw128(sq, BQ * 128, 1024);
+          const uint64_t apt = smem_desc_sw128(spt, 16, 1024), adst = smem_desc_sw128(sdst, 16, 1024);
 #pragma unroll C::UMMA_UNROLL
           for (int kk = 0; kk < BQ / 16; ++kk) {  // dV += P^T dO_i
-            const uint64_t bd = smem_desc_sw128(sdo + kk * 2048, BQ * 128, 1024);
-            if (C::P_IN_TMEM) {
-              umma_bf16_ts(tmem + C::TCOL_DV, tmem + C::TCOL_PT + kk * 8, bd, IDESC_KV,
-                           (cur.i > 0 || kk > 0) ? 1u : 0u);
-            } else {
-              const uint64_t ad = smem_desc_sw128(spt + (kk >> 2) * (BK * 128) + (kk & 3) * 32, 16, 1024);
-              umma_bf16_ss(tmem + C::TCOL_DV, ad, bd, IDESC_KV, (cur.i > 0 || kk > 0) ? 1u : 0u);
-            }
+            const uint32_t acc = (cur.i > 0 || kk > 0) ? 1u : 0u;
+            if (C::P_IN_TMEM)
+              umma_bf16_ts(tmem + C::TCOL_DV, tmem + C::TCOL_PT + kk * 8, desc_at(bdo, kk * 2048), IDESC_KV, acc);
+            else
+              umma_bf16_ss(tmem + C::TCOL_DV, desc_at(apt, (kk >> 2) * (BK * 128) + (kk & 3) * 32),
+                           desc_at(bdo, kk * 2048), IDESC_KV, acc);
           }
 #pragma unroll C::UMMA_UNROLL
           for (int kk = 0; kk < BQ / 16; ++kk) {  // dK += dS^T Q_i
-            const uint64_t ad = smem_desc_sw128(sdst + (kk >> 2) * (BK * 128) + (kk & 3) * 32, 16, 1024);
-            const uint64_t bd = smem_desc_sw128(sq + kk * 2048, BQ * 128, 1024);
-            umma_bf16_ss(tmem + C::TCOL_DK, ad, bd, IDESC_KV, (cur.i > 0 || kk > 0) ? 1u : 0u);
+            umma_bf16_ss(tmem + C::TCOL_DK, desc_at(adst, (kk >> 2) * (BK * 128) + (kk & 3) * 32),
+                         desc_at(bq, kk * 2048), IDESC_KV, (cur.i > 0 || kk > 0) ? 1u : 0u);
           }
           umma_commit(BAR_QE(st));
           // the dQ columns must have been drained (previous step)
           if (cur.t >= 1 && !mbar_wait(BAR_DQE, (cur.t - 1) & 1, abort_p)) break;
           tc_fence_after();
+          const uint64_t aq = smem_desc_sw128(sdst, BK * 128, 1024), bk = smem_desc_sw128(sk, BK * 128, 1024);
 #pragma unroll C::UMMA_UNROLL
-          for (int kk = 0; kk < BK / 16; ++kk) {  // dQ_i = dS K (A = dS^T as MN-major)
-            const uint64_t ad = smem_desc_sw128(sdst + kk * 2048, BK * 128, 1024);
-            const uint64_t bd = smem_desc_sw128(sk + kk * 2048, BK * 128, 1024);
-            umma_bf16_ss(tmem + C::TCOL_DQ, ad, bd, IDESC_Q, kk > 0 ? 1u : 0u);
-          }
+          for (int kk = 0; kk < BK / 16; ++kk)  // dQ_i = dS K (A = dS^T as MN-major)
+            umma_bf16_ss(tmem + C::TCOL_DQ, desc_at(aq, kk * 2048), desc_at(bk, kk * 2048), IDESC_Q, kk > 0 ? 1u : 0u);
           umma_commit(BAR_DQF);
           umma_commit(BAR_PE);
           if (cur.i + 1 == cur.u.nq) {  // the unit's last UMMA

@@ -383,6 +383,11 @@ __device__ __forceinline__ uint64_t smem_desc_sw128(uint32_t addr, uint32_t lbo,
   return d;
 }
 
+// The descriptor of an operand `bytes` further on (a multiple of 16; shared
+// memory's addresses do not reach the field's end, so it is one addition
+// where encoding anew takes a dozen instructions of the one issuing thread).
+__device__ __forceinline__ uint64_t desc_at(uint64_t desc, uint32_t bytes) { return desc + (bytes >> 4); }
+
 // Instruction descriptor of tcgen05.mma kind::f16: bf16 A/B, fp32 D.
 // a_mn / b_mn select MN-major (1) instead of K-major (0) operands.
 __host__ __device__ constexpr uint32_t idesc_bf16_f32(int M, int N, int a_mn, int b_mn) {
