@@ -68,24 +68,9 @@
 // here S, dP, dQ and dK/dV stay fp32 until their single store, and P, dS are
 // bf16 (the UMMA operand type).
 //
-// WIN: the same kernel for windowAttentionBackward (sliding window, sinks,
-// grouped K/V heads, sequence lengths).  A unit is a key tile of a K/V head;
-// its steps are the query tiles that can see it, for each query head of the
-// group, so shared heads' gradients are summed in the accumulators.  A sink
-// tile is seen by every later query: what lies past its window is cut into
-// units of their own where that chain would be the longest (WinBwd), whose
-// partial dK/dV the launcher's last kernel adds up in a fixed order.  The
-// statistics come ready from a kernel before this one, [B][NH][T], and the
-// warp that stages them also zeroes the padding rows of Q, dO, K and V tiles
-// (their P is 0, but 0 * NaN is not).  A unit or chunk without a
-// valid row runs one step in which everything is masked and so writes zeros.
-//
 // All mbarrier waits are bounded (about 2 s); on time-out the CTA winds down,
 // frees its TMEM and sets STATUS_BWD_TIMEOUT.  Warps meet only at mbarriers
 // (no named barriers), so a failed wait cannot leave a warp stuck at one.
-#include <algorithm>
-#include <type_traits>
-
 #include "common.cuh"
 #include "sm100.cuh"
 #include "tmap.h"
@@ -101,7 +86,7 @@ constexpr int PERSIST_MAX_NKT = 16;  // static schedule when T/128 <= this (D=64
 constexpr float LOG2E = 1.4426950408889634f;
 
 
-template <int HD, bool PERSIST, bool WIN = false>
+template <int HD, bool PERSIST>
 struct BwdCfg {
   static constexpr int KB = HD / 64;
   static constexpr bool D64 = HD == 64;
@@ -138,7 +123,7 @@ struct BwdCfg {
   // prefetch the next unit (under launch control too, where a CTA also runs
   // many units: C4 backward 3.75 -> 3.64 ms against one K/V buffer and three
   // Q/dO stages); D=128 has room for one of each
-  static constexpr int STAGES = D64 ? (WIN ? 3 : 2) : 1;
+  static constexpr int STAGES = D64 ? 2 : 1;
   static constexpr int KVB = D64 ? 2 : 1;
   static constexpr bool P_IN_TMEM = D64;         // P^T in TMEM (else smem)
   static constexpr bool EARLY_S = D64;           // next S^T before dV/dK/dQ
@@ -150,10 +135,7 @@ struct BwdCfg {
   // ring stages: the statistics warp loads a step's values into registers a
   // step ahead, so one stage suffices where the shared memory is tight.
   static constexpr int DQSB = 1;
-  static constexpr int SSTG = D64 && (PERSIST || WIN) ? 1 : 8;
-  // WIN at D=64 has the most code in flight, and fetching it stalls the warps
-  // more than the UMMA issuer's loops do
-  static constexpr int UMMA_UNROLL = WIN && D64 ? 1 : 8;
+  static constexpr int SSTG = (D64 && PERSIST) ? 1 : 8;
   static constexpr uint32_t KV_BYTES = BK * HD * 2;
   static constexpr uint32_t QD_BYTES = BQ * HD * 2;
   static constexpr uint32_t PT_BYTES = BK * BQ * 2;
@@ -177,18 +159,12 @@ struct BwdCfg {
   static constexpr int NSCHED = DYN ? (int)kSchedSlots : 0;
   static constexpr uint32_t SCHED_READERS = 5 + NCOMP / 32 + (DRAIN_WG ? 4 : 0);
   static constexpr uint32_t OFF_SCHED = OFF_STAT + SSTG * STAT_BYTES;
-  // WIN: the units' descriptors (unit 0's after those of the responses' slots),
-  // decoded once, by the producer
-  static constexpr int NDESC = WIN ? NSCHED + 1 : 0;
-  static constexpr uint32_t DESC_BYTES = 48;
-  static constexpr uint32_t OFF_DESC = OFF_SCHED + NSCHED * 16;
-  static constexpr uint32_t OFF_BAR = OFF_DESC + NDESC * DESC_BYTES;
+  static constexpr uint32_t OFF_BAR = OFF_SCHED + NSCHED * 16;
   // kv_full/empty[KVB], qd_full/empty[S], st_full/empty[8], then s_full,
   // s_free, p_ready, p_free, dq_full, dq_free, dqs_full, dqs_free, done,
   // acc_free, never (nothing arrives: the time-out test hook), fin (the
-  // UMMA issuer's wind-down), sched_full/empty[NSCHED] and, for WIN,
-  // qd_fixed[S] (padding rows zeroed) and desc_full[NDESC]
-  static constexpr int NBAR = 2 * KVB + 2 * STAGES + 2 * SSTG + 12 + 2 * (DQSB - 1) + 2 * NSCHED + (WIN ? STAGES : 0) + NDESC;
+  // UMMA issuer's wind-down), sched_full/empty[NSCHED]
+  static constexpr int NBAR = 2 * KVB + 2 * STAGES + 2 * SSTG + 12 + 2 * (DQSB - 1) + 2 * NSCHED;
   static constexpr uint32_t OFF_TSLOT = OFF_BAR + NBAR * 8;
   static constexpr uint32_t SMEM_BYTES = OFF_TSLOT + 16 + 1024;
   static constexpr uint32_t TCOL_S = 0;
@@ -199,20 +175,6 @@ struct BwdCfg {
   static constexpr uint32_t TCOL_PT = 256 + 3 * HD;  // D=64 only: 64 columns of bf16 pairs
 };
 
-// What the window adds.  Sink tiles 0 .. nsplit-1 are split: their query
-// tiles past the window go, far_tiles at a time, to nfar units each; unit
-// `slot`s of part hold 2 x 128 x D fp32 partial sums (dV, dK), slot 0 of a
-// tile its window's.
-struct WinBwd {
-  const int32_t* lens;
-  int G, window, sinks;
-  int nsplit, nfar, far_tiles;
-  int nfar_units;              // nsplit * nfar * (batch, K/V head) pairs, dealt first
-  int rows;                    // rows of a (batch, head) in the statistics
-  const float *neg_l, *neg_d;  // -l*log2e, -D/sqrt(D)
-  float* part;
-};
-
 struct BwdParams {
   int T, N, NH, bh_begin, nbh, nkt, nunits;
   float scale, scale_log2;
@@ -220,7 +182,6 @@ struct BwdParams {
   const __nv_bfloat16* Dv;
   uint32_t* status;
   uint32_t expire_ns;  // time-out test hook (ma_debug_expire_next_wait), 0 = off
-  WinBwd win;          // WIN only
 };
 
 // Unit k -> (batch, head, key tile); its query tiles are kt .. nkt-1.  Block
@@ -228,26 +189,6 @@ struct BwdParams {
 // block), key tile-major; HB = 1 is (batch, head)-major.
 struct BUnit {
   int b, h, kt, nq;
-  __device__ int q_tile(int i) const { return kt + i; }
-  __device__ int q_head(int) const { return h; }
-};
-
-// A unit under a window: nt query tiles from q0 on, for each query head.
-// (48 bytes: it is passed on through shared memory.)
-struct alignas(16) WinBUnit {
-  int b, h, kt, nq;
-  int q0, nt, head0;
-  int n;     // valid rows; 0 where the unit has none: everything is masked
-  int slot;  // partial sums go to this slot, or -1: straight to dK, dV
-  int valid; // 0: no unit is left
-  int pad[2];
-  __device__ int q_tile(int i) const { return q0 + i % nt; }
-  __device__ int q_head(int i) const { return head0 + i / nt; }
-  // key `key` sees queries [*from, *to) of the query tile at row0
-  __device__ void seen(const WinBwd& w, int key, int row0, int* from, int* to) const {
-    *from = key - row0;
-    *to = (key < w.sinks ? n : min(n, key + w.window)) - row0;
-  }
 };
 
 template <int HB>
@@ -270,52 +211,6 @@ __device__ __forceinline__ BUnit bwd_unit(const BwdParams& prm, int k) {
   return u;
 }
 
-template <int HB>
-__device__ __forceinline__ WinBUnit bwd_win_unit(const BwdParams& prm, int k) {
-  const WinBwd& w = prm.win;
-  WinBUnit u;
-  const bool far = k < w.nfar_units;
-  int c = 0;
-  if (far) {
-    const int bh = k % prm.nbh, r = k / prm.nbh;
-    u.b = bh / prm.NH;
-    u.h = bh % prm.NH;
-    u.kt = r % w.nsplit;
-    c = r / w.nsplit;
-  } else {
-    const BUnit p = bwd_unit<HB>(prm, k - w.nfar_units);
-    u.b = p.b;
-    u.h = p.h;
-    u.kt = p.kt;
-  }
-  u.head0 = u.h * w.G;
-  u.n = w.lens ? min(max(__ldg(w.lens + u.b), 0), prm.T) : prm.T;
-  const bool split = u.kt < w.nsplit;
-  u.slot = split ? ((u.b * prm.NH + u.h) * w.nsplit + u.kt) * (1 + w.nfar) + (far ? 1 + c : 0) : -1;
-  const int k0 = u.kt * BK;
-  const int last = (u.n - 1) / BQ;                     // the last query tile with a valid row
-  const int win_last = (k0 + BK - 1 + w.window - 1) / BQ;  // and the last in the window
-  u.q0 = far ? win_last + 1 + c * w.far_tiles : u.kt;
-  int end = last;
-  if (far) end = min(last, u.q0 + w.far_tiles - 1);
-  else if (split || k0 >= w.sinks) end = min(last, win_last);
-  u.nt = end - u.q0 + 1;
-  u.nq = u.nt * w.G;
-  if (u.nt <= 0 || u.n <= k0) {
-    u.n = 0;
-    u.q0 = u.kt;
-    u.nt = u.nq = 1;
-  }
-  return u;
-}
-
-// The descriptors' ring: unit 0 in slot kSchedSlots, unit g in the slot of the
-// response that named it, which the readers release together.
-struct UnitRing {
-  WinBUnit* desc;
-  uint32_t full;  // slot 0's barrier
-};
-
 // Static schedule: the unit of this CTA in round g, -1 when rounds are
 // exhausted, -2 when this CTA has none in round g (last, partial round).
 __device__ __forceinline__ int bwd_unit_of_round(const BwdParams& prm, int g) {
@@ -328,44 +223,18 @@ __device__ __forceinline__ int bwd_unit_of_round(const BwdParams& prm, int g) {
 
 // Walks this CTA's (unit, query tile) steps in order.  t counts steps over
 // all units, uc counts units.
-template <bool WIN>
 struct StepIter {
   int g;        // dynamic: units fetched; static: next round to look at
-  std::conditional_t<WIN, WinBUnit, BUnit> u;
-  int i;        // step within the unit
+  BUnit u;
+  int i;        // query tile index within the unit
   uint32_t t;   // global step
   uint32_t uc;  // unit counter
   bool valid;
 };
 
-// PUBLISH (WIN's producer): decodes the unit and passes it on; WIN's other
-// roles read it (the code of twenty decodings would not fit the instruction
-// cache).
-template <bool DYN, int HB, bool WIN, bool WARP, bool PUBLISH = false>
-__device__ __forceinline__ bool next_unit(const BwdParams& prm, StepIter<WIN>& s, const Sched& sc, const UnitRing& ur) {
-  if constexpr (WIN && PUBLISH) {
-    const uint32_t g = (uint32_t)s.g++;
-    const int k = sched_unit<WARP>(sc, g);
-    const bool some = k >= 0 && k < prm.nunits;
-    if (some) s.u = bwd_win_unit<HB>(prm, k);
-    s.u.valid = some;
-    const uint32_t slot = g == 0 ? kSchedSlots : (g - 1) % kSchedSlots;
-    ur.desc[slot] = s.u;
-    mbar_arrive(ur.full + 8u * slot);
-    return some;
-  } else if constexpr (WIN) {
-    const uint32_t g = (uint32_t)s.g++;
-    const uint32_t slot = g == 0 ? kSchedSlots : (g - 1) % kSchedSlots;
-    const uint32_t ph = g == 0 ? 0u : ((g - 1) / kSchedSlots) & 1u;
-    if (!(WARP ? mbar_wait_warp(ur.full + 8u * slot, ph, sc.abort) : mbar_wait(ur.full + 8u * slot, ph, sc.abort)))
-      return false;
-    s.u = ur.desc[slot];
-    if (g > 0) {
-      if (WARP) __syncwarp();
-      if (!WARP || (threadIdx.x & 31) == 0) mbar_arrive(sc.empty + 8u * slot);
-    }
-    return s.u.valid != 0;
-  } else if constexpr (DYN) {
+template <bool DYN, int HB, bool WARP>
+__device__ __forceinline__ bool next_unit(const BwdParams& prm, StepIter& s, const Sched& sc) {
+  if constexpr (DYN) {
     const int k = sched_unit<WARP>(sc, (uint32_t)s.g++);
     if (k < 0 || k >= prm.nunits) return false;
     s.u = bwd_unit<HB>(prm, k);
@@ -383,19 +252,19 @@ __device__ __forceinline__ bool next_unit(const BwdParams& prm, StepIter<WIN>& s
   }
 }
 
-template <bool DYN, int HB, bool WIN, bool WARP, bool PUBLISH = false>
-__device__ __forceinline__ StepIter<WIN> first_step(const BwdParams& prm, const Sched& sc, const UnitRing& ur) {
-  StepIter<WIN> s;
+template <bool DYN, int HB, bool WARP>
+__device__ __forceinline__ StepIter first_step(const BwdParams& prm, const Sched& sc) {
+  StepIter s;
   s.g = 0;
   s.i = 0;
   s.t = 0;
   s.uc = 0;
-  s.valid = next_unit<DYN, HB, WIN, WARP, PUBLISH>(prm, s, sc, ur);
+  s.valid = next_unit<DYN, HB, WARP>(prm, s, sc);
   return s;
 }
 
-template <bool DYN, int HB, bool WIN, bool WARP, bool PUBLISH = false>
-__device__ __forceinline__ void advance(const BwdParams& prm, StepIter<WIN>& s, const Sched& sc, const UnitRing& ur) {
+template <bool DYN, int HB, bool WARP>
+__device__ __forceinline__ void advance(const BwdParams& prm, StepIter& s, const Sched& sc) {
   ++s.t;
   if (s.i + 1 < s.u.nq) {
     ++s.i;
@@ -403,18 +272,15 @@ __device__ __forceinline__ void advance(const BwdParams& prm, StepIter<WIN>& s, 
   }
   s.i = 0;
   ++s.uc;
-  s.valid = next_unit<DYN, HB, WIN, WARP, PUBLISH>(prm, s, sc, ur);
+  s.valid = next_unit<DYN, HB, WARP>(prm, s, sc);
 }
 
 // P^T and dS^T for N query columns of one key row.  s[] holds S^T on entry
 // and P^T on exit; dp[] holds dP^T on entry and dS^T on exit.  nl = -l*log2e
 // and nd = -D/sqrt(D) per query column (shared memory, broadcast reads).
-// SEEN (a window's step): bit j of see[] says whether query column j is visible;
-// else P and with it dS are 0 (padding rows hold zeros, so dP is finite).
-template <bool DIAG, int N, bool SEEN = false>
+template <bool DIAG, int N>
 __device__ __forceinline__ void p_ds_row(float (&s)[N], float (&dp)[N], const float* nl,
-                                         const float* nd, float c, float sc, int krow, int qcol0,
-                                         const uint32_t* see = nullptr) {
+                                         const float* nd, float c, float sc, int krow, int qcol0) {
   const float2 c2 = make_float2(c, c), sc2 = make_float2(sc, sc);
 #pragma unroll
   for (int j = 0; j < N; j += 4) {
@@ -423,13 +289,6 @@ __device__ __forceinline__ void p_ds_row(float (&s)[N], float (&dp)[N], const fl
     const float2 t0 = __ffma2_rn(make_float2(s[j], s[j + 1]), c2, make_float2(L.x, L.y));
     const float2 t1 = __ffma2_rn(make_float2(s[j + 2], s[j + 3]), c2, make_float2(L.z, L.w));
     float p0 = ex2(t0.x), p1 = ex2(t0.y), p2 = ex2(t1.x), p3 = ex2(t1.y);
-    if constexpr (SEEN) {
-      const uint32_t m = see[j / 32] >> (j % 32);
-      if (!(m & 1u)) p0 = 0.0f;
-      if (!(m & 2u)) p1 = 0.0f;
-      if (!(m & 4u)) p2 = 0.0f;
-      if (!(m & 8u)) p3 = 0.0f;
-    }
     if (DIAG) {  // key after query: P = 0 (attention.metal:282)
       const int q = qcol0 + j;
       if (krow > q) p0 = 0.0f;
@@ -468,14 +327,14 @@ __device__ __forceinline__ void store_row_sw128(uint8_t* rowp, int row, const fl
   }
 }
 
-template <int HD, bool PERSIST, bool WIN>
-__global__ void __launch_bounds__(BwdCfg<HD, PERSIST, WIN>::NUM_THREADS, 1)
+template <int HD, bool PERSIST>
+__global__ void __launch_bounds__(BwdCfg<HD, PERSIST>::NUM_THREADS, 1)
     flash_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                      const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmdO,
                      const __grid_constant__ CUtensorMap tmdQ, __nv_bfloat16* __restrict__ dK,
                      __nv_bfloat16* __restrict__ dV, const BwdParams prm) {
-  if constexpr (!WIN) pdl_wait_and_release();  // WIN: after the set-up below
-  using C = BwdCfg<HD, PERSIST, WIN>;
+  pdl_wait_and_release();
+  using C = BwdCfg<HD, PERSIST>;
   extern __shared__ uint8_t smem_raw[];
   __shared__ int abort_flag;
   const uint32_t raw = smem_u32(smem_raw);
@@ -505,7 +364,6 @@ __global__ void __launch_bounds__(BwdCfg<HD, PERSIST, WIN>::NUM_THREADS, 1)
   const uint32_t BAR_FIN = BAR_SF + 88;   // the UMMA issuer's last commit (wind-down)
   const uint32_t BAR_UF = BAR_SF + 96 + 16u * (C::DQSB - 1);  // sched_full[NSCHED], then sched_empty
   const uint32_t BAR_UE = BAR_UF + 8u * C::NSCHED;
-  auto BAR_QZ = [&](int s) { return BAR_UE + 8u * (C::NSCHED + s); };  // WIN: padding rows of stage s zeroed
   const uint32_t tslot = sbase + C::OFF_TSLOT;
   float* stat_base = reinterpret_cast<float*>(gbase + C::OFF_STAT);
 
@@ -513,12 +371,11 @@ __global__ void __launch_bounds__(BwdCfg<HD, PERSIST, WIN>::NUM_THREADS, 1)
     abort_flag = 0;
     for (int s = 0; s < C::KVB; ++s) {
       mbar_init(BAR_KF(s), 1);
-      mbar_init(BAR_KE(s), WIN ? 2 : 1);  // WIN: the warp that zeroes rows, too
+      mbar_init(BAR_KE(s), 1);
     }
     for (int s = 0; s < C::STAGES; ++s) {
       mbar_init(BAR_QF(s), 1);
-      mbar_init(BAR_QE(s), WIN ? 2 : 1);
-      if constexpr (WIN) mbar_init(BAR_QZ(s), 1);
+      mbar_init(BAR_QE(s), 1);
     }
     for (int s = 0; s < C::SSTG; ++s) {
       mbar_init(BAR_TF(s), 32);
@@ -542,7 +399,6 @@ __global__ void __launch_bounds__(BwdCfg<HD, PERSIST, WIN>::NUM_THREADS, 1)
       mbar_init(BAR_UF + 8u * u, 1);
       mbar_init(BAR_UE + 8u * u, C::SCHED_READERS);
     }
-    for (int u = 0; u < C::NDESC; ++u) mbar_init(BAR_QZ(C::STAGES + u), 1);  // desc_full
     fence_mbar_init();
   }
   if (warp == 1) {
@@ -552,24 +408,9 @@ __global__ void __launch_bounds__(BwdCfg<HD, PERSIST, WIN>::NUM_THREADS, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  // nothing before here touches global memory, so the barriers and TMEM are set
-  // up while the kernel before is still draining
-  if constexpr (WIN) pdl_wait_and_release();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(gbase + C::OFF_TSLOT);
   volatile int* abort_p = &abort_flag;
   const Sched sch{sbase + C::OFF_SCHED, BAR_UF, BAR_UE, abort_p};  // the unit schedule
-  const UnitRing ring{reinterpret_cast<WinBUnit*>(gbase + C::OFF_DESC), BAR_QZ(C::STAGES)};
-
-  // WIN: whether step s brings tiles with padding rows (a unit's first step:
-  // its K tile too); past the tensor's end TMA has filled in zeros itself
-  auto fix_q = [&](const StepIter<WIN>& s) {
-    if constexpr (WIN) return s.u.n < prm.T && s.u.q_tile(s.i) * BQ + BQ > s.u.n;
-    else return false;
-  };
-  auto fix_k = [&](const StepIter<WIN>& s) {
-    if constexpr (WIN) return s.i == 0 && s.u.n < prm.T && s.u.kt * BK + BK > s.u.n;
-    else return false;
-  };
 
   if (warp < 4) {
     reg_dealloc<C::REGS_PRODUCER>();
@@ -580,8 +421,8 @@ __global__ void __launch_bounds__(BwdCfg<HD, PERSIST, WIN>::NUM_THREADS, 1)
         tma_prefetch_desc(&tmdO);
         uint32_t kv_armed = 0, q_armed = 0;  // loads issued into each ring
         uint32_t nreq = 0;                   // launch-control requests issued
-        for (StepIter<WIN> s = first_step<C::DYN, C::HB, WIN, false, true>(prm, sch, ring); s.valid; advance<C::DYN, C::HB, WIN, false, true>(prm, s, sch, ring)) {
-          const int kv0 = s.u.h * HD, col0 = s.u.q_head(s.i) * HD;
+        for (StepIter s = first_step<C::DYN, C::HB, false>(prm, sch); s.valid; advance<C::DYN, C::HB, false>(prm, s, sch)) {
+          const int col0 = s.u.h * HD;
           if (s.i == 0) {  // K/V of a new unit
             const int kvs = s.uc % C::KVB;
             if (s.uc >= C::KVB && !mbar_wait(BAR_KE(kvs), ((s.uc / C::KVB) - 1) & 1, abort_p)) break;
@@ -589,14 +430,14 @@ __global__ void __launch_bounds__(BwdCfg<HD, PERSIST, WIN>::NUM_THREADS, 1)
             ++kv_armed;
             for (int kb = 0; kb < C::KB; ++kb) {
               tma_load_3d(sbase + C::OFF_K + kvs * C::KV_BYTES + kb * BK * 128, &tmK, BAR_KF(kvs),
-                          kv0 + kb * 64, s.u.kt * BK, s.u.b);
+                          col0 + kb * 64, s.u.kt * BK, s.u.b);
               tma_load_3d(sbase + C::OFF_V + kvs * C::KV_BYTES + kb * BK * 128, &tmV, BAR_KF(kvs),
-                          kv0 + kb * 64, s.u.kt * BK, s.u.b);
+                          col0 + kb * 64, s.u.kt * BK, s.u.b);
             }
           }
           const int st = s.t % C::STAGES;
           if (s.t >= C::STAGES && !mbar_wait(BAR_QE(st), ((s.t / C::STAGES) - 1) & 1, abort_p)) break;
-          const int qt = s.u.q_tile(s.i);
+          const int qt = s.u.kt + s.i;
           mbar_arrive_expect_tx(BAR_QF(st), 2 * C::QD_BYTES);
           ++q_armed;
           for (int kb = 0; kb < C::KB; ++kb) {
@@ -625,19 +466,12 @@ __global__ void __launch_bounds__(BwdCfg<HD, PERSIST, WIN>::NUM_THREADS, 1)
         constexpr uint32_t IDESC_KV = idesc_bf16_f32(BK, HD, 0, 1);  // dV, dK
         constexpr uint32_t IDESC_Q = idesc_bf16_f32(BQ, HD, 1, 1);   // dQ
         const uint32_t spt = sbase + C::OFF_PT, sdst = sbase + C::OFF_DST;
-        uint32_t qzp = 0;  // WIN: bit s = parity of qd_fixed[s]'s next phase
         // S^T and dP^T of step s into their TMEM columns
-        auto issue_s = [&](const StepIter<WIN>& s) -> bool {
+        auto issue_s = [&](const StepIter& s) -> bool {
           const int st = s.t % C::STAGES;
           const int kvs = s.uc % C::KVB;
           if (s.i == 0 && !mbar_wait(BAR_KF(kvs), (s.uc / C::KVB) & 1, abort_p)) return false;
           if (!mbar_wait(BAR_QF(st), (s.t / C::STAGES) & 1, abort_p)) return false;
-          if constexpr (WIN) {
-            if (fix_q(s) || fix_k(s)) {  // warp 2 has zeroed the padding rows
-              if (!mbar_wait(BAR_QZ(st), (qzp >> st) & 1, abort_p)) return false;
-              qzp ^= 1u << st;
-            }
-          }
           if (s.t >= 1 && !mbar_wait(BAR_SE, (s.t - 1) & 1, abort_p)) return false;
           if (C::DQ_ALIAS && s.t >= 1 && !mbar_wait(BAR_DQE, (s.t - 1) & 1, abort_p)) return false;
           tc_fence_after();
@@ -645,39 +479,39 @@ __global__ void __launch_bounds__(BwdCfg<HD, PERSIST, WIN>::NUM_THREADS, 1)
           const uint32_t sv = sbase + C::OFF_V + kvs * C::KV_BYTES;
           const uint32_t sq = sbase + C::OFF_Q + st * C::QD_BYTES;
           const uint32_t sdo = sbase + C::OFF_DO + st * C::QD_BYTES;
-          const uint64_t dk = smem_desc_sw128(sk, 16, 1024), dv = smem_desc_sw128(sv, 16, 1024);
-          const uint64_t dq = smem_desc_sw128(sq, 16, 1024), ddo = smem_desc_sw128(sdo, 16, 1024);
-#pragma unroll C::UMMA_UNROLL
+#pragma unroll
           for (int kk = 0; kk < HD / 16; ++kk) {
             const uint32_t off = (kk >> 2) * (BK * 128) + (kk & 3) * 32;
-            umma_bf16_ss(tmem + C::TCOL_S, desc_at(dk, off), desc_at(dq, off), IDESC_S, kk > 0 ? 1u : 0u);
+            umma_bf16_ss(tmem + C::TCOL_S, smem_desc_sw128(sk + off, 16, 1024),
+                         smem_desc_sw128(sq + off, 16, 1024), IDESC_S, kk > 0 ? 1u : 0u);
           }
-#pragma unroll C::UMMA_UNROLL
+#pragma unroll
           for (int kk = 0; kk < HD / 16; ++kk) {
             const uint32_t off = (kk >> 2) * (BK * 128) + (kk & 3) * 32;
-            umma_bf16_ss(tmem + C::TCOL_DP, desc_at(dv, off), desc_at(ddo, off), IDESC_S, kk > 0 ? 1u : 0u);
+            umma_bf16_ss(tmem + C::TCOL_DP, smem_desc_sw128(sv + off, 16, 1024),
+                         smem_desc_sw128(sdo + off, 16, 1024), IDESC_S, kk > 0 ? 1u : 0u);
           }
           umma_commit(BAR_SF);
           return true;
         };
-        StepIter<WIN> cur = first_step<C::DYN, C::HB, WIN, false>(prm, sch, ring);
-        StepIter<WIN> la = cur;  // next step whose S^T/dP^T is to be issued
+        StepIter cur = first_step<C::DYN, C::HB, false>(prm, sch);
+        StepIter la = cur;  // next step whose S^T/dP^T is to be issued
         bool ok = true;
         if (la.valid) {
           ok = issue_s(la);
-          advance<C::DYN, C::HB, WIN, false>(prm, la, sch, ring);
+          advance<C::DYN, C::HB, false>(prm, la, sch);
         }
         // time-out test hook: with the first products in flight, wait on a
         // barrier nothing arrives at until the hook's limit runs out
         if (ok && prm.expire_ns) ok = mbar_wait(BAR_NEVER, 0, abort_p, prm.expire_ns);
-        for (; ok && cur.valid; advance<C::DYN, C::HB, WIN, false>(prm, cur, sch, ring)) {
+        for (; ok && cur.valid; advance<C::DYN, C::HB, false>(prm, cur, sch)) {
           // the next step's S^T/dP^T ahead of this step's products, except
           // where it starts a unit whose K/V can only be loaded into the
           // single K/V buffer once this step's products are done with it
           const bool early = C::EARLY_S && la.valid && (C::KVB > 1 || la.uc == cur.uc);
           if (early) {
             if (!issue_s(la)) break;
-            advance<C::DYN, C::HB, WIN, false>(prm, la, sch, ring);
+            advance<C::DYN, C::HB, false>(prm, la, sch);
           }
           const int st = cur.t % C::STAGES;
           const int kvs = cur.uc % C::KVB;
@@ -688,30 +522,33 @@ __global__ void __launch_bounds__(BwdCfg<HD, PERSIST, WIN>::NUM_THREADS, 1)
           // the previous unit's epilogue must have read dK/dV out of TMEM
           if (cur.i == 0 && cur.uc >= 1 && !mbar_wait(BAR_ACC, (cur.uc - 1) & 1, abort_p)) break;
           tc_fence_after();
-          const uint64_t bdo = smem_desc_sw128(sdo, BQ * 128, 1024), bq = smem_desc_sw128(sq, BQ * 128, 1024);
-          const uint64_t apt = smem_desc_sw128(spt, 16, 1024), adst = smem_desc_sw128(sdst, 16, 1024);
-#pragma unroll C::UMMA_UNROLL
+#pragma unroll
           for (int kk = 0; kk < BQ / 16; ++kk) {  // dV += P^T dO_i
-            const uint32_t acc = (cur.i > 0 || kk > 0) ? 1u : 0u;
-            if (C::P_IN_TMEM)
-              umma_bf16_ts(tmem + C::TCOL_DV, tmem + C::TCOL_PT + kk * 8, desc_at(bdo, kk * 2048), IDESC_KV, acc);
-            else
-              umma_bf16_ss(tmem + C::TCOL_DV, desc_at(apt, (kk >> 2) * (BK * 128) + (kk & 3) * 32),
-                           desc_at(bdo, kk * 2048), IDESC_KV, acc);
+            const uint64_t bd = smem_desc_sw128(sdo + kk * 2048, BQ * 128, 1024);
+            if (C::P_IN_TMEM) {
+              umma_bf16_ts(tmem + C::TCOL_DV, tmem + C::TCOL_PT + kk * 8, bd, IDESC_KV,
+                           (cur.i > 0 || kk > 0) ? 1u : 0u);
+            } else {
+              const uint64_t ad = smem_desc_sw128(spt + (kk >> 2) * (BK * 128) + (kk & 3) * 32, 16, 1024);
+              umma_bf16_ss(tmem + C::TCOL_DV, ad, bd, IDESC_KV, (cur.i > 0 || kk > 0) ? 1u : 0u);
+            }
           }
-#pragma unroll C::UMMA_UNROLL
+#pragma unroll
           for (int kk = 0; kk < BQ / 16; ++kk) {  // dK += dS^T Q_i
-            umma_bf16_ss(tmem + C::TCOL_DK, desc_at(adst, (kk >> 2) * (BK * 128) + (kk & 3) * 32),
-                         desc_at(bq, kk * 2048), IDESC_KV, (cur.i > 0 || kk > 0) ? 1u : 0u);
+            const uint64_t ad = smem_desc_sw128(sdst + (kk >> 2) * (BK * 128) + (kk & 3) * 32, 16, 1024);
+            const uint64_t bd = smem_desc_sw128(sq + kk * 2048, BQ * 128, 1024);
+            umma_bf16_ss(tmem + C::TCOL_DK, ad, bd, IDESC_KV, (cur.i > 0 || kk > 0) ? 1u : 0u);
           }
           umma_commit(BAR_QE(st));
           // the dQ columns must have been drained (previous step)
           if (cur.t >= 1 && !mbar_wait(BAR_DQE, (cur.t - 1) & 1, abort_p)) break;
           tc_fence_after();
-          const uint64_t aq = smem_desc_sw128(sdst, BK * 128, 1024), bk = smem_desc_sw128(sk, BK * 128, 1024);
-#pragma unroll C::UMMA_UNROLL
-          for (int kk = 0; kk < BK / 16; ++kk)  // dQ_i = dS K (A = dS^T as MN-major)
-            umma_bf16_ss(tmem + C::TCOL_DQ, desc_at(aq, kk * 2048), desc_at(bk, kk * 2048), IDESC_Q, kk > 0 ? 1u : 0u);
+#pragma unroll
+          for (int kk = 0; kk < BK / 16; ++kk) {  // dQ_i = dS K (A = dS^T as MN-major)
+            const uint64_t ad = smem_desc_sw128(sdst + kk * 2048, BK * 128, 1024);
+            const uint64_t bd = smem_desc_sw128(sk + kk * 2048, BK * 128, 1024);
+            umma_bf16_ss(tmem + C::TCOL_DQ, ad, bd, IDESC_Q, kk > 0 ? 1u : 0u);
+          }
           umma_commit(BAR_DQF);
           umma_commit(BAR_PE);
           if (cur.i + 1 == cur.u.nq) {  // the unit's last UMMA
@@ -721,7 +558,7 @@ __global__ void __launch_bounds__(BwdCfg<HD, PERSIST, WIN>::NUM_THREADS, 1)
           // (after them: D=128, or a unit start with a single K/V buffer)
           if ((!C::EARLY_S || C::KVB == 1) && !early && la.valid) {
             if (!issue_s(la)) break;
-            advance<C::DYN, C::HB, WIN, false>(prm, la, sch, ring);
+            advance<C::DYN, C::HB, false>(prm, la, sch);
           }
         }
         if (*abort_p) {  // wind-down: every UMMA issued must complete before TMEM is freed
@@ -735,72 +572,29 @@ __global__ void __launch_bounds__(BwdCfg<HD, PERSIST, WIN>::NUM_THREADS, 1)
       // are loaded into registers one step ahead, so the ring slot is filled
       // as soon as the compute warps free it, whatever the load latency.
       float nl[4], nd[4];
-      auto load_stats = [&](const StepIter<WIN>& s) {
-        const int qt = s.u.q_tile(s.i);
-        if constexpr (WIN) {  // prepared, padded to whole tiles
-          const int heads = prm.NH * prm.win.G;
-          const long long si = ((long long)s.u.b * heads + s.u.q_head(s.i)) * prm.win.rows + qt * BQ + lane * 4;
-          const float4 L = __ldg(reinterpret_cast<const float4*>(prm.win.neg_l + si));
-          const float4 D4 = __ldg(reinterpret_cast<const float4*>(prm.win.neg_d + si));
-          nl[0] = L.x, nl[1] = L.y, nl[2] = L.z, nl[3] = L.w;
-          nd[0] = D4.x, nd[1] = D4.y, nd[2] = D4.z, nd[3] = D4.w;
-        } else {
-          const long long rbase = (long long)s.u.b * prm.T;
+      auto load_stats = [&](const StepIter& s) {
+        const int qt = s.u.kt + s.i;
+        const long long rbase = (long long)s.u.b * prm.T;
 #pragma unroll
-          for (int v = 0; v < 4; ++v) {
-            const int q = qt * BQ + lane * 4 + v;
-            nl[v] = 0.0f;
-            nd[v] = 0.0f;
-            if (q < prm.T) {
-              const long long si = (rbase + q) * prm.NH + s.u.h;
-              nl[v] = -__ldg(prm.lse + si) * LOG2E;
-              nd[v] = -__bfloat162float(prm.Dv[si]) * prm.scale;
-            }
+        for (int v = 0; v < 4; ++v) {
+          const int q = qt * BQ + lane * 4 + v;
+          nl[v] = 0.0f;
+          nd[v] = 0.0f;
+          if (q < prm.T) {
+            const long long si = (rbase + q) * prm.NH + s.u.h;
+            nl[v] = -__ldg(prm.lse + si) * LOG2E;
+            nd[v] = -__bfloat162float(prm.Dv[si]) * prm.scale;
           }
         }
       };
-      // WIN: rows [a, 128) of a tile are contiguous in each 64-column block
-      // (the swizzle permutes the chunks of a row within its 128 bytes)
-      auto zero_rows = [&](uint32_t off, int a) {
-        for (int kb = 0; kb < C::KB; ++kb) {
-          uint4* blk = reinterpret_cast<uint4*>(gbase + off + kb * BQ * 128);
-          for (int i = a * 8 + lane; i < BQ * 8; i += 32) blk[i] = make_uint4(0u, 0u, 0u, 0u);
-        }
-      };
-      StepIter<WIN> s = first_step<C::DYN, C::HB, WIN, true>(prm, sch, ring);
+      StepIter s = first_step<C::DYN, C::HB, true>(prm, sch);
       if (s.valid) load_stats(s);
       while (s.valid) {
         const float cl[4] = {nl[0], nl[1], nl[2], nl[3]};
         const float cd[4] = {nd[0], nd[1], nd[2], nd[3]};
-        StepIter<WIN> nx = s;
-        advance<C::DYN, C::HB, WIN, true>(prm, nx, sch, ring);
+        StepIter nx = s;
+        advance<C::DYN, C::HB, true>(prm, nx, sch);
         if (nx.valid) load_stats(nx);  // the next step's, in flight while this one waits
-        if constexpr (WIN) {
-          // every stage (and a unit's K/V) is waited for and released, so that
-          // this warp stays within one phase of each slot's barriers
-          const int qs = s.t % C::STAGES, kvs = s.uc % C::KVB;
-          if (s.i == 0 && !mbar_wait_warp(BAR_KF(kvs), (s.uc / C::KVB) & 1, abort_p)) break;
-          if (!mbar_wait_warp(BAR_QF(qs), (s.t / C::STAGES) & 1, abort_p)) break;
-          const bool fq = fix_q(s), fk = fix_k(s);
-          if (fk) {
-            zero_rows(C::OFF_K + kvs * C::KV_BYTES, max(0, s.u.n - s.u.kt * BK));
-            zero_rows(C::OFF_V + kvs * C::KV_BYTES, max(0, s.u.n - s.u.kt * BK));
-          }
-          if (fq) {
-            const int a = max(0, s.u.n - s.u.q_tile(s.i) * BQ);
-            zero_rows(C::OFF_Q + qs * C::QD_BYTES, a);
-            zero_rows(C::OFF_DO + qs * C::QD_BYTES, a);
-          }
-          if (fq || fk) {
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(BAR_QZ(qs));
-          }
-          if (lane == 0) {
-            mbar_arrive(BAR_QE(qs));
-            if (s.i == 0) mbar_arrive(BAR_KE(kvs));
-          }
-        }
         const int st = s.t % C::SSTG;
         if (s.t >= C::SSTG && !mbar_wait_warp(BAR_TE(st), ((s.t / C::SSTG) - 1) & 1, abort_p)) break;
         float* stt = stat_base + st * (2 * BQ);
@@ -815,12 +609,12 @@ __global__ void __launch_bounds__(BwdCfg<HD, PERSIST, WIN>::NUM_THREADS, 1)
     } else {
       // ------------------------------------------------- dQ reduce issuer
       if (lane == 0) {
-        for (StepIter<WIN> s = first_step<C::DYN, C::HB, WIN, false>(prm, sch, ring); s.valid; advance<C::DYN, C::HB, WIN, false>(prm, s, sch, ring)) {
+        for (StepIter s = first_step<C::DYN, C::HB, false>(prm, sch); s.valid; advance<C::DYN, C::HB, false>(prm, s, sch)) {
           const int b = s.t % C::DQSB;
           if (!mbar_wait(BAR_DSF(b), (s.t / C::DQSB) & 1, abort_p)) break;
           for (int box = 0; box < HD / 32; ++box)
             tma_reduce_add_3d(&tmdQ, sbase + C::OFF_DQS + b * C::DQS_BYTES + box * (BQ * 128),
-                              s.u.q_head(s.i) * HD + box * 32, s.u.q_tile(s.i) * BQ, s.u.b);
+                              s.u.h * HD + box * 32, (s.u.kt + s.i) * BQ, s.u.b);
           bulk_commit();
           // the reduction DQSB-1 steps back has read its buffer, which may
           // now be rewritten (with one buffer: this step's)
@@ -877,7 +671,7 @@ __global__ void __launch_bounds__(BwdCfg<HD, PERSIST, WIN>::NUM_THREADS, 1)
     // registers; frees the accumulators (BAR_ACC) for the next unit, then
     // converts to bf16 and stores this thread's row slice straight to global
     // memory (rows past T are not stored)
-    auto epilogue = [&](const auto& v, uint32_t vuc) {
+    auto epilogue = [&](const BUnit& v, uint32_t vuc) {
       if (ok) ok = mbar_wait_warp(BAR_DONE, vuc & 1, abort_p);
       if (!ok) return;
       tc_fence_after();
@@ -898,20 +692,6 @@ __global__ void __launch_bounds__(BwdCfg<HD, PERSIST, WIN>::NUM_THREADS, 1)
       tc_fence_before();
       mbar_arrive(BAR_ACC);  // the next unit may overwrite dK/dV in TMEM
       const int key = v.kt * BK + krow;
-      if constexpr (WIN) {
-        if (v.slot >= 0) {  // partial sums, fp32
-#pragma unroll
-          for (int which = 0; which < 2; ++which) {
-            float4* dst = reinterpret_cast<float4*>(
-                prm.win.part + (((long long)v.slot * 2 + which) * BK + krow) * HD + part * CPH);
-#pragma unroll
-            for (int cc = 0; cc < CPH; cc += 4)
-              dst[cc / 4] = make_float4(__uint_as_float(acc[which][cc + 0]), __uint_as_float(acc[which][cc + 1]),
-                                        __uint_as_float(acc[which][cc + 2]), __uint_as_float(acc[which][cc + 3]));
-          }
-          return;
-        }
-      }
       if (key < prm.T) {
         const long long off = ((long long)v.b * prm.T + key) * prm.N + v.h * HD + part * CPH;
 #pragma unroll
@@ -933,16 +713,17 @@ __global__ void __launch_bounds__(BwdCfg<HD, PERSIST, WIN>::NUM_THREADS, 1)
     // A unit's last dQ drain and its dK/dV epilogue run after the first step
     // of the next unit has been handed to the tensor core (or after the last
     // step of the last unit), so they overlap the next unit's UMMAs.
-    decltype(StepIter<WIN>::u) prev{};
+    BUnit prev{};
+    uint32_t t = 0, uc = 0;
     bool have_prev = false;
-    // Step st: P^T and dS^T formed and handed to the UMMA issuer.
-    auto form = [&](const StepIter<WIN>& st_it) {
-      const auto& u = st_it.u;
+    for (StepIter st_it = first_step<C::DYN, C::HB, true>(prm, sch); ok && st_it.valid; advance<C::DYN, C::HB, true>(prm, st_it, sch)) {
+      const BUnit& u = st_it.u;
       const int i = st_it.i;
-      const uint32_t t = st_it.t;
+      t = st_it.t;
+      uc = st_it.uc;
       const int ss = t % C::SSTG;
       ok = mbar_wait_warp(BAR_SF, t & 1, abort_p);
-      if (!ok) return;
+      if (!ok) break;
       tc_fence_after();
       float s[CPP], dp[CPP];
       if constexpr (CPP == 64) {
@@ -978,29 +759,16 @@ __global__ void __launch_bounds__(BwdCfg<HD, PERSIST, WIN>::NUM_THREADS, 1)
       tc_fence_before();
       mbar_arrive(BAR_SE);
       ok = mbar_wait_warp(BAR_TF(ss), (t / C::SSTG) & 1, abort_p);
-      if (!ok) return;
+      if (!ok) break;
       const float* stt = stat_base + ss * (2 * BQ) + part * CPP;
-      if constexpr (WIN) {
-        const int row0 = u.q_tile(i) * BQ;
-        // one form for masked and whole steps (a second would cost more in
-        // instruction fetches than it saves)
-        int from, to;
-        u.seen(prm.win, u.kt * BK + krow, row0 + part * CPP, &from, &to);
-        uint32_t see[CPP / 32];
-#pragma unroll
-        for (int w = 0; w < CPP / 32; ++w) see[w] = bits_below(to - 32 * w) & ~bits_below(from - 32 * w);
-        p_ds_row<false, CPP, true>(s, dp, stt, stt + BQ, c, sc, krow, part * CPP, see);
-      } else if (i == 0) {
-        p_ds_row<true, CPP>(s, dp, stt, stt + BQ, c, sc, krow, part * CPP);
-      } else {
-        p_ds_row<false, CPP>(s, dp, stt, stt + BQ, c, sc, krow, part * CPP);
-      }
+      if (i == 0) p_ds_row<true, CPP>(s, dp, stt, stt + BQ, c, sc, krow, part * CPP);
+      else p_ds_row<false, CPP>(s, dp, stt, stt + BQ, c, sc, krow, part * CPP);
       mbar_arrive(BAR_TE(ss));
       // the previous step's UMMAs must be done with P^T/dS^T, and when the dQ
       // staging shares their smem its reduction must have read it
       if (t >= 1) ok = mbar_wait_warp(BAR_PE, (t - 1) & 1, abort_p);
       if (ok && C::DQS_ALIAS && t >= 1) ok = mbar_wait_warp(BAR_DSE(0), (t - 1) & 1, abort_p);
-      if (!ok) return;
+      if (!ok) break;
       // this part's columns of the key row: P^T (bf16 pairs in TMEM, or smem),
       // dS^T (smem); chunk (part*CPP % 64) / 8 of 64-column block part*CPP / 64
       const int blk = (part * CPP) / 64, ch0 = ((part * CPP) % 64) / 8;
@@ -1018,32 +786,25 @@ __global__ void __launch_bounds__(BwdCfg<HD, PERSIST, WIN>::NUM_THREADS, 1)
       fence_proxy_async_smem();
       tc_fence_before();
       mbar_arrive(BAR_PR);
-    };
-    for (StepIter<WIN> st_it = first_step<C::DYN, C::HB, WIN, true>(prm, sch, ring); ok;
-         advance<C::DYN, C::HB, WIN, true>(prm, st_it, sch, ring)) {
-      if (st_it.valid) form(st_it);
-      if (!ok) break;
       // on a unit's first step the previous unit's dK/dV epilogue comes
       // first: the UMMA issuer waits for it before this step's products,
-      // the dQ product that drain_dq(t) waits for among them.  The last
-      // unit's follows its last step.
+      // the dQ product that drain_dq(t) waits for among them
       if constexpr (C::EPI_COMPUTE) {
-        if (have_prev && (!st_it.valid || st_it.i == 0)) {
-          if constexpr (!C::DRAIN_WG && C::EARLY_S)
-            if (!st_it.valid) drain_dq(st_it.t - 1);
-          epilogue(prev, st_it.uc - 1);
-        }
-        if (!st_it.valid) break;
-        prev = st_it.u;
+        if (i == 0 && have_prev) epilogue(prev, uc - 1);
+        prev = u;
         have_prev = true;
       }
       if constexpr (!C::DRAIN_WG) {
         if (C::EARLY_S) {
-          if (st_it.t >= 1) drain_dq(st_it.t - 1);
+          if (t >= 1) drain_dq(t - 1);
         } else {
-          drain_dq(st_it.t);
+          drain_dq(t);
         }
       }
+    }
+    if (ok && have_prev) {  // the last unit of this CTA
+      if constexpr (!C::DRAIN_WG && C::EARLY_S) drain_dq(t);
+      if constexpr (C::EPI_COMPUTE) epilogue(prev, uc);
     }
   } else {
     reg_dealloc<C::REGS_DRAIN>();
@@ -1053,7 +814,7 @@ __global__ void __launch_bounds__(BwdCfg<HD, PERSIST, WIN>::NUM_THREADS, 1)
     const int row = quarter * 32 + lane;
     const uint32_t tl = tmem + ((uint32_t)(quarter * 32) << 16);
     bool ok = true;
-    for (StepIter<WIN> s = first_step<C::DYN, C::HB, WIN, true>(prm, sch, ring); ok && s.valid; advance<C::DYN, C::HB, WIN, true>(prm, s, sch, ring)) {
+    for (StepIter s = first_step<C::DYN, C::HB, true>(prm, sch); ok && s.valid; advance<C::DYN, C::HB, true>(prm, s, sch)) {
       const uint32_t t = s.t;
       const int b = t % C::DQSB;
       uint8_t* dqs = gbase + C::OFF_DQS + b * C::DQS_BYTES;
@@ -1108,18 +869,17 @@ __global__ void zero_dq_shard_kernel(float4* __restrict__ dQ, int T, int N, int 
   }
 }
 
-// T rows of queries and keys, nq and nkv columns.
-template <int HD, bool PERSIST, bool WIN = false>
+template <int HD, bool PERSIST>
 cudaError_t launch_bwd_kernel(const __nv_bfloat16* dO, const __nv_bfloat16* q,
                               const __nv_bfloat16* k, const __nv_bfloat16* v, float* dQ,
-                              __nv_bfloat16* dK, __nv_bfloat16* dV, int T, int B, uint64_t nq, uint64_t nkv,
+                              __nv_bfloat16* dK, __nv_bfloat16* dV, const AttnShape& s,
                               const BwdParams& prm, int grid, cudaStream_t st) {
-  using C = BwdCfg<HD, PERSIST, WIN>;
+  using C = BwdCfg<HD, PERSIST>;
   // The setmaxnreg split assumes the kernel was compiled to exactly
   // LAUNCH_REGS registers per thread; refuse to launch otherwise.
   static const cudaError_t reg_check = [] {
     cudaFuncAttributes a;
-    cudaError_t e = cudaFuncGetAttributes(&a, flash_bwd_kernel<HD, PERSIST, WIN>);
+    cudaError_t e = cudaFuncGetAttributes(&a, flash_bwd_kernel<HD, PERSIST>);
     if (e != cudaSuccess) return e;
     return a.numRegs == C::LAUNCH_REGS ? cudaSuccess : cudaErrorInvalidKernelImage;
   }();
@@ -1127,17 +887,17 @@ cudaError_t launch_bwd_kernel(const __nv_bfloat16* dO, const __nv_bfloat16* q,
   CUtensorMap tq, tk, tv, tdo, tdq;
   const CUtensorMapDataType bf = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   const CUtensorMapSwizzle sw = CU_TENSOR_MAP_SWIZZLE_128B;
-  if (!make_tmap_3d(&tq, q, bf, 2, nq, T, B, 64, BQ, sw) ||
-      !make_tmap_3d(&tk, k, bf, 2, nkv, T, B, 64, BK, sw) ||
-      !make_tmap_3d(&tv, v, bf, 2, nkv, T, B, 64, BK, sw) ||
-      !make_tmap_3d(&tdo, dO, bf, 2, nq, T, B, 64, BQ, sw) ||
-      !make_tmap_3d(&tdq, dQ, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, nq, T, B, 32, BQ, sw))
+  if (!make_tmap_3d(&tq, q, bf, 2, s.N, s.T, s.B, 64, BQ, sw) ||
+      !make_tmap_3d(&tk, k, bf, 2, s.N, s.T, s.B, 64, BK, sw) ||
+      !make_tmap_3d(&tv, v, bf, 2, s.N, s.T, s.B, 64, BK, sw) ||
+      !make_tmap_3d(&tdo, dO, bf, 2, s.N, s.T, s.B, 64, BQ, sw) ||
+      !make_tmap_3d(&tdq, dQ, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, s.N, s.T, s.B, 32, BQ, sw))
     return cudaErrorInvalidValue;
-  cudaError_t e = cudaFuncSetAttribute(flash_bwd_kernel<HD, PERSIST, WIN>,
+  cudaError_t e = cudaFuncSetAttribute(flash_bwd_kernel<HD, PERSIST>,
                                        cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES);
   if (e != cudaSuccess) return e;
-  launch_pdl(flash_bwd_kernel<HD, PERSIST, WIN>, grid, C::NUM_THREADS, C::SMEM_BYTES, st, tq, tk, tv, tdo, tdq, dK,
-             dV, prm);
+  launch_pdl(flash_bwd_kernel<HD, PERSIST>, grid, C::NUM_THREADS, C::SMEM_BYTES, st, tq, tk, tv, tdo, tdq, dK,
+                                                                        dV, prm);
   count_launches(1);
   return cudaGetLastError();
 }
@@ -1154,7 +914,7 @@ cudaError_t launch_bwd(const __nv_bfloat16* dO, const __nv_bfloat16* Dv, const f
     const cudaError_t e = launch_zero_dq(dQ, s, st);
     if (e != cudaSuccess) return e;
   }
-  BwdParams prm{};
+  BwdParams prm;
   prm.T = s.T;
   prm.N = s.N;
   prm.NH = s.NH;
@@ -1176,211 +936,12 @@ cudaError_t launch_bwd(const __nv_bfloat16* dO, const __nv_bfloat16* Dv, const f
     cudaGetDevice(&dev);
     cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
     const int grid = prm.nunits < sms ? prm.nunits : sms;
-    return launch_bwd_kernel<HD, true>(dO, q, k, v, dQ, dK, dV, s.T, s.B, s.N, s.N, prm, grid, st);
+    return launch_bwd_kernel<HD, true>(dO, q, k, v, dQ, dK, dV, s, prm, grid, st);
   }
-  return launch_bwd_kernel<HD, false>(dO, q, k, v, dQ, dK, dV, s.T, s.B, s.N, s.N, prm, prm.nunits, st);
-}
-
-// ------------------------------------------------------- windowed backward
-// How a call's workspace is laid out, and how its sink tiles are split.
-struct WinPlan {
-  int nqt, rows, nsplit, nfar, far_tiles;
-  size_t stat, part, dq;  // bytes: one statistic, the partial sums, dQ in fp32
-  size_t total() const { return 2 * stat + part + dq; }
-};
-
-WinPlan win_plan(const WindowArgs& a, bool dq_f32) {
-  WinPlan p{};
-  p.nqt = (a.M + BQ - 1) / BQ;
-  p.rows = p.nqt * BQ;
-  const int nbh = a.B * a.NKV;
-  const int ns = (int)std::min<long long>(((long long)a.sinks + BK - 1) / BK, p.nqt);
-  const int window = std::min(a.window, 1 << 25);
-  const int near = (BK - 1 + window - 1) / BQ + 1;  // query tiles of tile 0's window
-  const int far = p.nqt - near;
-  // A sink tile's far queries are a chain of `far` steps a head where other
-  // units have `near`.  Where the sink tiles alone would not keep the GPU busy
-  // twice over, the chain is cut into pieces of a window's length, of 8 tiles
-  // at least (a piece costs 2 x 128 x D fp32 written and read) and 16 at most.
-  if (far > near && far > 8 && (long long)ns * nbh < 2 * 148) {
-    p.nsplit = ns;
-    p.far_tiles = std::max({near, 8, (far + 15) / 16});
-    p.nfar = ns > 0 ? (far + p.far_tiles - 1) / p.far_tiles : 0;
-  }
-  auto up = [](size_t x) { return (x + 255) & ~(size_t)255; };
-  p.stat = up((size_t)a.B * a.NH * p.rows * sizeof(float));
-  p.part = up((size_t)nbh * p.nsplit * (1 + p.nfar) * 2 * BK * a.D * sizeof(float));
-  p.dq = dq_f32 ? 0 : up((size_t)a.B * a.M * a.NH * a.D * sizeof(float));
-  return p;
-}
-
-__device__ __forceinline__ float dot8(uint4 a, uint4 b) {
-  const __nv_bfloat162* x = reinterpret_cast<const __nv_bfloat162*>(&a);
-  const __nv_bfloat162* y = reinterpret_cast<const __nv_bfloat162*>(&b);
-  float s = 0.0f;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 u = __bfloat1622float2(x[i]), v = __bfloat1622float2(y[i]);
-    s = fmaf(u.x, v.x, s);
-    s = fmaf(u.y, v.y, s);
-  }
-  return s;
-}
-
-// The statistics -l*log2e and -(dO . O)/sqrt(D), [B][NH][rows] (0 for padding
-// and past the end), and zeros for dQ.  HBM-bound: dO, O read and dQ written
-// once.  A warp takes 32 rows of a head, D/8 lanes a row with 16-byte loads,
-// and writes 32 neighbouring statistics.
-template <int HD>
-__global__ void __launch_bounds__(256) window_stats_kernel(const WindowArgs a, const __nv_bfloat16* __restrict__ dO,
-                                                           float* __restrict__ neg_l, float* __restrict__ neg_d,
-                                                           float* __restrict__ dQ, int rows) {
-  pdl_wait_and_release();
-  constexpr int G = HD / 8, RPI = 32 / G;  // lanes a row, rows an instruction
-  const int lane = threadIdx.x % 32;
-  const int tiles = rows / 32;
-  const long long items = (long long)a.B * tiles * a.NH;
-  for (long long it = blockIdx.x * 8ll + threadIdx.x / 32; it < items; it += gridDim.x * 8ll) {
-    const int h = (int)(it % a.NH);
-    const long long r = it / a.NH;
-    const int b = (int)(r / tiles), row0 = (int)(r % tiles) * 32;
-    const int n = a.len(b);
-    float mine = 0.0f;  // of row row0 + lane
-    // loads before stores: 8 rows of a lane in flight at once
-#pragma unroll
-    for (int i0 = 0; i0 < 32; i0 += 8 * RPI < 32 ? 8 * RPI : 32) {
-      constexpr int N = 8 * RPI < 32 ? 8 : 32 / RPI;
-      uint4 x[N], y[N];
-#pragma unroll
-      for (int k = 0; k < N; ++k) {
-        const int row = row0 + i0 + k * RPI + lane / G;
-        const long long off = (((long long)b * a.M + row) * a.NH + h) * HD;
-        x[k] = y[k] = make_uint4(0u, 0u, 0u, 0u);
-        if (row < n) {
-          x[k] = __ldcs(reinterpret_cast<const uint4*>(dO + off) + lane % G);
-          y[k] = __ldcs(reinterpret_cast<const uint4*>(a.out + off) + lane % G);
-        }
-      }
-#pragma unroll
-      for (int k = 0; k < N; ++k) {
-        const int i = i0 + k * RPI;
-        float s = dot8(x[k], y[k]);
-#pragma unroll
-        for (int m = G / 2; m >= 1; m >>= 1) s += __shfl_xor_sync(0xffffffffu, s, m);
-        const float got = __shfl_sync(0xffffffffu, s, (lane - i) * G & 31);
-        if (lane >= i && lane < i + RPI) mine = got;
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < 32; i += RPI) {
-      const int row = row0 + i + lane / G;
-      if (row < a.M) {
-        float4* z = reinterpret_cast<float4*>(dQ + (((long long)b * a.M + row) * a.NH + h) * HD) + lane % G;
-        z[0] = z[G] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      }
-    }
-    const int row = row0 + lane;
-    const bool valid = row < n;
-    const long long at = ((long long)b * a.NH + h) * rows + row;
-    neg_l[at] = valid ? -a.l[((long long)b * a.M + row) * a.NH + h] * LOG2E : 0.0f;
-    neg_d[at] = valid ? -mine * a.scale : 0.0f;
-  }
-}
-
-// dQ rounded to bf16, and the split sink tiles' partial dV, dK added up in
-// slot order and rounded.
-__global__ void __launch_bounds__(256) window_finish_kernel(const float* __restrict__ dQ, __nv_bfloat16* __restrict__ dQ16,
-                                                            long long nq4, const float* __restrict__ part, int slots,
-                                                            int nsplit, int D, int NKV, int T, long long npart4,
-                                                            __nv_bfloat16* __restrict__ dK, __nv_bfloat16* __restrict__ dV) {
-  pdl_wait_and_release();
-  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < nq4 + npart4; i += gridDim.x * 256ll) {
-    if (i < npart4) {
-      const int d4 = D / 4;
-      const int c = (int)(i % d4);
-      long long r = i / d4;
-      const int row = (int)(r % BK);
-      r /= BK;
-      const int which = (int)(r % 2);
-      r /= 2;  // (batch, K/V head, sink tile)
-      const int tile = (int)(r % nsplit);
-      const long long bh = r / nsplit;
-      const int key = tile * BK + row;
-      if (key >= T) continue;
-      float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      for (int k = 0; k < slots; ++k) {
-        const float4 x = __ldg(reinterpret_cast<const float4*>(part) + (((r * slots + k) * 2 + which) * BK + row) * d4 + c);
-        s.x += x.x, s.y += x.y, s.z += x.z, s.w += x.w;
-      }
-      __nv_bfloat16* to = (which == 0 ? dV : dK) + ((bh / NKV * T + key) * NKV + bh % NKV) * D + c * 4;
-      *reinterpret_cast<uint2*>(to) = make_uint2(pack_bf16(s.x, s.y), pack_bf16(s.z, s.w));
-    } else {
-      const long long j = i - npart4;
-      const float4 x = __ldcs(reinterpret_cast<const float4*>(dQ) + j);
-      reinterpret_cast<uint2*>(dQ16)[j] = make_uint2(pack_bf16(x.x, x.y), pack_bf16(x.z, x.w));
-    }
-  }
-}
-
-template <int HD>
-cudaError_t launch_win_bwd(const WindowArgs& a, const WindowGrads& g, cudaStream_t st) {
-  const WinPlan p = win_plan(a, g.dq_f32);
-  char* ws = static_cast<char*>(g.workspace);
-  float* neg_l = reinterpret_cast<float*>(ws);
-  float* neg_d = reinterpret_cast<float*>(ws + p.stat);
-  float* part = reinterpret_cast<float*>(ws + 2 * p.stat);
-  float* dQ = g.dq_f32 ? static_cast<float*>(g.dQ) : reinterpret_cast<float*>(ws + 2 * p.stat + p.part);
-  int dev = 0, sms = 148;
-  cudaGetDevice(&dev);
-  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  auto blocks = [&](long long n, int per) { return (unsigned)std::min<long long>((n + per - 1) / per, sms * 16ll); };
-  launch_pdl(window_stats_kernel<HD>, blocks((long long)a.B * a.NH * (p.rows / 32), 8), 256, 0, st, a, g.dO, neg_l,
-             neg_d, dQ, p.rows);
-  count_launches(1);
-  cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return e;
-  BwdParams prm{};
-  prm.T = a.M;
-  prm.N = a.NKV * HD;
-  prm.NH = a.NKV;
-  prm.nbh = a.B * a.NKV;
-  prm.nkt = p.nqt;
-  prm.scale = 1.0f / sqrtf((float)HD);
-  prm.scale_log2 = LOG2E / sqrtf((float)HD);
-  prm.status = a.status;
-  WinBwd& w = prm.win;
-  w.lens = a.lens;
-  w.G = a.NH / a.NKV;
-  w.window = std::min(a.window, 1 << 25);  // M <= 2^24: the same mask, and sums of positions stay in range
-  w.sinks = a.sinks;
-  w.nsplit = p.nsplit;
-  w.nfar = p.nfar;
-  w.far_tiles = p.far_tiles;
-  w.nfar_units = p.nsplit * p.nfar * prm.nbh;
-  w.rows = p.rows;
-  w.neg_l = neg_l;
-  w.neg_d = neg_d;
-  w.part = part;
-  prm.nunits = w.nfar_units + prm.nkt * prm.nbh;
-  e = launch_bwd_kernel<HD, false, true>(g.dO, a.q, a.k, a.v, dQ, g.dK, g.dV, a.M, a.B, (uint64_t)a.NH * HD,
-                                         (uint64_t)a.NKV * HD, prm, prm.nunits, st);
-  if (e != cudaSuccess) return e;
-  const long long nq4 = g.dq_f32 ? 0 : (long long)a.B * a.M * a.NH * HD / 4;
-  const long long npart4 = (long long)prm.nbh * p.nsplit * 2 * BK * HD / 4;
-  if (nq4 + npart4 == 0) return cudaSuccess;
-  launch_pdl(window_finish_kernel, blocks(nq4 + npart4, 256), 256, 0, st, dQ,
-             static_cast<__nv_bfloat16*>(g.dQ), nq4, part, 1 + p.nfar, p.nsplit, HD, a.NKV, a.M, npart4, g.dK, g.dV);
-  count_launches(1);
-  return cudaGetLastError();
+  return launch_bwd_kernel<HD, false>(dO, q, k, v, dQ, dK, dV, s, prm, prm.nunits, st);
 }
 
 }  // namespace
-
-size_t window_bwd_workspace(const WindowArgs& a, bool dq_f32) { return win_plan(a, dq_f32).total(); }
-
-cudaError_t launch_window_bwd(const WindowArgs& a, const WindowGrads& g, cudaStream_t st) {
-  return a.D == 64 ? launch_win_bwd<64>(a, g, st) : launch_win_bwd<128>(a, g, st);
-}
 
 cudaError_t launch_zero_dq(float* dQ, const AttnShape& s, cudaStream_t st) {
   if (s.bh_begin == 0 && s.bh_end == s.B * s.NH)
