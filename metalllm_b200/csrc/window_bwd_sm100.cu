@@ -337,9 +337,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   const uint32_t BAR_PE = BAR(B_1 + 5);                     // a step's products completed
   const uint32_t BAR_U = BAR(B_1 + 6);                      // sched full, empty, desc_full
   float* stat_base = reinterpret_cast<float*>(gbase + C::OFF_STAT);
-  // readers of a unit: the producer, the issuer twice (its two positions), warp
-  // 2 and the 8 compute warps
-  constexpr uint32_t READERS = 4 + NCOMP / 32;
+  // readers of a unit: the producer, the issuer, warp 2 and the 8 compute warps
+  constexpr uint32_t READERS = 3 + NCOMP / 32;
 
   if (threadIdx.x == 0) {
     abort_flag = 0;
@@ -431,27 +430,27 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         auto x2 = [&](uint32_t t) { return sbase + C::OFF_X2 + t % C::X2ST * C::TILE; };
         // 128 x 128 scores: both operands K-major
         auto scores = [&](uint32_t d, uint32_t a, uint32_t b) {
-          const uint64_t da = smem_desc_sw128(a, 16, 1024), db = smem_desc_sw128(b, 16, 1024);
+          const uint32_t da = desc_lo(a, 16), db = desc_lo(b, 16);
 #pragma unroll
           for (int kk = 0; kk < HD / 16; ++kk) {
-            const uint32_t off = (kk >> 2) * (BT * 128) + (kk & 3) * 32;
-            umma_bf16_ss(d, desc_at(da, off), desc_at(db, off), IDESC_S, kk > 0 ? 1u : 0u);
+            const uint32_t off = ((kk >> 2) * (BT * 128) + (kk & 3) * 32) >> 4;
+            umma_bf16_ss_lo(d, da + off, db + off, IDESC_S, kk > 0 ? 1u : 0u);
           }
         };
         // sums: A = P or dS in TMEM (each half of the columns over its half of
         // dP), B = a streamed tile, MN-major
         auto product = [&](uint32_t d, uint32_t a, uint32_t b, bool start) {
-          const uint64_t db = smem_desc_sw128(b, BT * 128, 1024);
+          const uint32_t db = desc_lo(b, BT * 128);
 #pragma unroll
           for (int kk = 0; kk < BT / 16; ++kk)
-            umma_bf16_ts(d, a + (kk >> 2) * 64 + (kk & 3) * 8, desc_at(db, kk * 2048), IDESC_ACC,
-                         start && kk == 0 ? 0u : 1u);
+            umma_bf16_ts_lo(d, a + (kk >> 2) * 64 + (kk & 3) * 8, db + kk * (2048 >> 4), IDESC_ACC,
+                            start && kk == 0 ? 0u : 1u);
         };
-        auto issue_s = [&](const Step& s) -> bool {
+        auto issue_s = [&](const Step& s, bool pad) -> bool {
           const uint32_t rs = s.uc % C::RST, st = s.t % C::X1ST;
           if (s.i == 0 && !mbar_wait(BAR_RF(rs), (s.uc / C::RST) & 1, abort_p)) return false;
           if (!mbar_wait(BAR_X1F(st), (s.t / C::X1ST) & 1, abort_p)) return false;
-          if (padded(s)) {
+          if (pad) {
             if (!mbar_wait(BAR_X1Z(st), (z1 >> st) & 1, abort_p)) return false;
             z1 ^= 1u << st;
           }
@@ -462,10 +461,10 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
           return true;
         };
         // (the products that read P and dS out of its columns have completed)
-        auto issue_dp = [&](const Step& s) -> bool {
+        auto issue_dp = [&](const Step& s, bool pad) -> bool {
           const uint32_t rs = s.uc % C::RST, st = s.t % C::X2ST;
           if (!mbar_wait(BAR_X2F(st), (s.t / C::X2ST) & 1, abort_p)) return false;
-          if (padded(s)) {
+          if (pad) {
             if (!mbar_wait(BAR_X2Z(st), (z2 >> st) & 1, abort_p)) return false;
             z2 ^= 1u << st;
           }
@@ -476,38 +475,49 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
           if (s.i + 1 == s.u.nq) umma_commit(BAR_RE(rs));  // the resident tiles' last use
           return true;
         };
-        Step cur = first_step<DQ, false>(prm, ring);
-        Step la = cur;  // the next step whose S is to be issued
-        bool ok = true;
-        if (la.valid) {
-          ok = issue_s(la) && issue_dp(la);
+        // la: the next step whose S is to be issued; of the step before it,
+        // whose products come next, only its place in its unit is kept (this
+        // one thread's instructions are most of what a short unit waits for)
+        Step la = first_step<DQ, false>(prm, ring);
+        bool ok = true, have = la.valid, first = true, last = false;
+        uint32_t t = 0, uc = 0;
+        if (have) {
+          const bool pad = padded(la);
+          ok = issue_s(la, pad) && issue_dp(la, pad);
+          last = la.u.nq == 1;
           advance<DQ, false>(prm, la, ring);
         }
-        for (; ok && cur.valid; advance<DQ, false>(prm, cur, ring)) {
+        while (ok && have) {
           // ahead of this step's products, except where the next unit's
           // resident tiles are only now being loaded
           const bool early = la.valid && (C::RST > 1 || la.i > 0);
-          if (early && !issue_s(la)) break;
+          const bool pad = la.valid && padded(la);
+          if (early && !issue_s(la, pad)) break;
           if constexpr (C::DPB == 2) {
-            if (cur.t >= 1 && !mbar_wait(BAR_PE, (cur.t - 1) & 1, abort_p)) break;
-            if (early && !issue_dp(la)) break;
+            if (t >= 1 && !mbar_wait(BAR_PE, (t - 1) & 1, abort_p)) break;
+            if (early && !issue_dp(la, pad)) break;
           }
-          if (!mbar_wait(BAR_PR(cur.t % C::DPB), (cur.t / C::DPB) & 1, abort_p)) break;
-          if (cur.i == 0 && cur.uc >= 1 && !mbar_wait(BAR_ACC, (cur.uc - 1) & 1, abort_p)) break;
+          if (!mbar_wait(BAR_PR(t % C::DPB), (t / C::DPB) & 1, abort_p)) break;
+          if (first && uc >= 1 && !mbar_wait(BAR_ACC, (uc - 1) & 1, abort_p)) break;
           tc_fence_after();
-          const uint32_t p = tmem + C::TCOL_DP + cur.t % C::DPB * 128, ds = p + 32;
+          const uint32_t p = tmem + C::TCOL_DP + t % C::DPB * 128, ds = p + 32;
           if constexpr (!DQ) {
-            product(tmem + C::TCOL_ACC, p, x2(cur.t), cur.i == 0);  // dV += P dO
-            umma_commit(BAR_X2E(cur.t % C::X2ST));
+            product(tmem + C::TCOL_ACC, p, x2(t), first);  // dV += P dO
+            umma_commit(BAR_X2E(t % C::X2ST));
           }
-          product(tmem + C::TCOL_ACC + (DQ ? 0 : HD), ds, x1(cur.t), cur.i == 0);  // dK += dS Q, dQ += dS K
-          umma_commit(BAR_X1E(cur.t % C::X1ST));
+          product(tmem + C::TCOL_ACC + (DQ ? 0 : HD), ds, x1(t), first);  // dK += dS Q, dQ += dS K
+          umma_commit(BAR_X1E(t % C::X1ST));
           umma_commit(BAR_PE);
-          if (cur.i + 1 == cur.u.nq) umma_commit(BAR_DONE);
-          if (!early && la.valid && !issue_s(la)) break;
-          if (C::DPB == 1 && !mbar_wait(BAR_PE, cur.t & 1, abort_p)) break;
-          if (la.valid) {
-            if ((C::DPB == 1 || !early) && !issue_dp(la)) break;
+          if (last) umma_commit(BAR_DONE);
+          if (!early && la.valid && !issue_s(la, pad)) break;
+          if (C::DPB == 1 && !mbar_wait(BAR_PE, t & 1, abort_p)) break;
+          have = la.valid;
+          if (have) {
+            if ((C::DPB == 1 || !early) && !issue_dp(la, pad)) break;
+            first = la.i == 0;
+            last = la.i + 1 == la.u.nq;
+            t = la.t;
+            uc = la.uc;
             advance<DQ, false>(prm, la, ring);
           }
         }
