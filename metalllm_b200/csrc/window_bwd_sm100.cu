@@ -26,14 +26,17 @@
 // L2 and convert the sums: at B=2, 4096 tokens, 16 heads of 128, window 1000 it
 // took 384 us, at 64 x 1024, 12 heads of 64, window 250 605 us.)
 //
-// Pipeline: S of the next step is issued before this step's products, and with
-// two dP buffers (all but dK/dV at D=128) dP too, so the tensor core works on
-// the next step while the compute warps form this one's P and dS.
+// Pipeline: S of the next step is issued as soon as this step's has been read,
+// and with two dP buffers (all but dK/dV at D=128) dP ahead of this step's
+// products too, so the tensor core works on the next step while the compute
+// warps form this one's P and dS.
 //
 // Roles (384 threads): warpgroup 0 (120 registers): warp 0 TMA producer, which
 // also decodes the units and passes them on through shared memory (each role
 // decoding for itself is more code than the instruction cache holds); warp 1
-// UMMA issuer; warp 2 statistics of the dK/dV pass, and zeroes padding rows of
+// issues S and dP, warp 3 the products (one thread for both spent more on waits
+// and addresses than the tensor core on the work: a step 2.9 us); warp 2
+// statistics of the dK/dV pass, and zeroes padding rows of
 // streamed tiles (their P is 0, but 0 * NaN is not).  Warpgroups 1, 2 (192
 // registers) compute: thread = row = TMEM lane, 64 columns each, and store the
 // unit's sums.
@@ -87,9 +90,9 @@ struct Cfg {
   static constexpr uint32_t OFF_DESC = OFF_SCHED + kSchedSlots * 16;
   static constexpr uint32_t OFF_BAR = OFF_DESC + NDESC * DESC;
   // full and empty of R, X1, X2, stat; X1/X2 fixed; dp_full[DPB],
-  // p_ready[DPB]; s_full, s_free, done, acc_free, fin, p_free; sched
+  // p_ready[DPB], p_free[DPB]; s_full, s_free, done, acc_free, fin[2]; sched
   // full/empty, desc_full
-  static constexpr int NBAR = 2 * (RST + X1ST + X2ST + SSTG) + X1ST + X2ST + 2 * DPB + 6 + 2 * (int)kSchedSlots + NDESC;
+  static constexpr int NBAR = 2 * (RST + X1ST + X2ST + SSTG) + X1ST + X2ST + 3 * DPB + 6 + 2 * (int)kSchedSlots + NDESC;
   static constexpr uint32_t OFF_TSLOT = OFF_BAR + NBAR * 8;
   static constexpr uint32_t SMEM = OFF_TSLOT + 16 + 1024;  // + alignment slack
   static_assert(SMEM <= 232448, "shared memory");
@@ -315,7 +318,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   const uint32_t bar0 = sbase + C::OFF_BAR;
   auto BAR = [&](int n) { return bar0 + 8u * n; };
   constexpr int B_X1 = 2 * C::RST, B_X2 = B_X1 + 3 * C::X1ST, B_T = B_X2 + 3 * C::X2ST, B_DP = B_T + 2 * C::SSTG,
-                B_PR = B_DP + C::DPB, B_1 = B_PR + C::DPB;
+                B_PR = B_DP + C::DPB, B_PE = B_PR + C::DPB, B_1 = B_PE + C::DPB;
   auto BAR_RF = [&](int s) { return BAR(s); };
   auto BAR_RE = [&](int s) { return BAR(C::RST + s); };
   auto BAR_X1F = [&](int s) { return BAR(B_X1 + s); };
@@ -327,18 +330,18 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   auto BAR_TF = [&](int s) { return BAR(B_T + s); };
   auto BAR_TE = [&](int s) { return BAR(B_T + C::SSTG + s); };
   auto BAR_DPF = [&](int s) { return BAR(B_DP + s); };
-  // P and dS written, one barrier a dP buffer: with two buffers the compute
-  // warps may be done with step t + 1 before the issuer looks at step t's
+  // P and dS written, and read by the products: one barrier each a dP buffer,
+  // since with two buffers the next step's may come before a waiter has looked
   auto BAR_PR = [&](int s) { return BAR(B_PR + s); };
+  auto BAR_PE = [&](int s) { return BAR(B_PE + s); };
   const uint32_t BAR_SF = BAR(B_1), BAR_SE = BAR(B_1 + 1);  // S ready, S read
   const uint32_t BAR_DONE = BAR(B_1 + 2);                   // a unit's last product completed
   const uint32_t BAR_ACC = BAR(B_1 + 3);                    // its sums read
-  const uint32_t BAR_FIN = BAR(B_1 + 4);                    // wind-down
-  const uint32_t BAR_PE = BAR(B_1 + 5);                     // a step's products completed
+  const uint32_t BAR_FIN = BAR(B_1 + 4);                    // wind-down, one for each issuer
   const uint32_t BAR_U = BAR(B_1 + 6);                      // sched full, empty, desc_full
   float* stat_base = reinterpret_cast<float*>(gbase + C::OFF_STAT);
-  // readers of a unit: the producer, the issuer, warp 2 and the 8 compute warps
-  constexpr uint32_t READERS = 3 + NCOMP / 32;
+  // readers of a unit: the producer, the issuers, warp 2 and the 8 compute warps
+  constexpr uint32_t READERS = 4 + NCOMP / 32;
 
   if (threadIdx.x == 0) {
     abort_flag = 0;
@@ -348,7 +351,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       if (i >= B_X2 + C::X2ST && i < B_X2 + 2 * C::X2ST) n = 2;
       if (i >= B_T && i < B_T + C::SSTG) n = 32;
       if (i >= B_T + C::SSTG && i < B_DP) n = NCOMP;
-      if ((i >= B_PR && i < B_1) || i == B_1 + 1 || i == B_1 + 3) n = NCOMP;
+      if ((i >= B_PR && i < B_PE) || i == B_1 + 1 || i == B_1 + 3) n = NCOMP;
       if (i >= B_1 + 6 + (int)kSchedSlots && i < B_1 + 6 + 2 * (int)kSchedSlots) n = READERS;
       mbar_init(BAR(i), n);
     }
@@ -421,13 +424,10 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         }
       }
     } else if (warp == 1) {
-      // ------------------------------------------------------------- UMMA
+      // ---------------------------------------------------------- S and dP
       if (lane == 0) {
         constexpr uint32_t IDESC_S = idesc_bf16_f32(BT, BT, 0, 0);
-        constexpr uint32_t IDESC_ACC = idesc_bf16_f32(BT, HD, 0, 1);
         uint32_t z1 = 0, z2 = 0;  // bit s: parity of the next phase of X1Z(s), X2Z(s)
-        auto x1 = [&](uint32_t t) { return sbase + C::OFF_X1 + t % C::X1ST * C::TILE; };
-        auto x2 = [&](uint32_t t) { return sbase + C::OFF_X2 + t % C::X2ST * C::TILE; };
         // 128 x 128 scores: both operands K-major
         auto scores = [&](uint32_t d, uint32_t a, uint32_t b) {
           const uint32_t da = desc_lo(a, 16), db = desc_lo(b, 16);
@@ -437,8 +437,44 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
             umma_bf16_ss_lo(d, da + off, db + off, IDESC_S, kk > 0 ? 1u : 0u);
           }
         };
-        // sums: A = P or dS in TMEM (each half of the columns over its half of
-        // dP), B = a streamed tile, MN-major
+        for (Step s = first_step<DQ, false>(prm, ring); s.valid; advance<DQ, false>(prm, s, ring)) {
+          const uint32_t t = s.t, rs = s.uc % C::RST, s1 = t % C::X1ST, s2 = t % C::X2ST, b = t % C::DPB;
+          const bool pad = padded(s);
+          if (s.i == 0 && !mbar_wait(BAR_RF(rs), (s.uc / C::RST) & 1, abort_p)) break;
+          if (!mbar_wait(BAR_X1F(s1), (t / C::X1ST) & 1, abort_p)) break;
+          if (pad) {
+            if (!mbar_wait(BAR_X1Z(s1), (z1 >> s1) & 1, abort_p)) break;
+            z1 ^= 1u << s1;
+          }
+          if (t >= 1 && !mbar_wait(BAR_SE, (t - 1) & 1, abort_p)) break;
+          tc_fence_after();
+          scores(tmem + C::TCOL_S, sbase + C::OFF_R + rs * 2 * C::TILE, sbase + C::OFF_X1 + s1 * C::TILE);
+          umma_commit(BAR_SF);
+          if (!mbar_wait(BAR_X2F(s2), (t / C::X2ST) & 1, abort_p)) break;
+          if (pad) {
+            if (!mbar_wait(BAR_X2Z(s2), (z2 >> s2) & 1, abort_p)) break;
+            z2 ^= 1u << s2;
+          }
+          // the products that read P and dS out of its columns have completed
+          if (t >= C::DPB && !mbar_wait(BAR_PE(b), ((t / C::DPB) - 1) & 1, abort_p)) break;
+          tc_fence_after();
+          scores(tmem + C::TCOL_DP + b * 128, sbase + C::OFF_R + (rs * 2 + 1) * C::TILE,
+                 sbase + C::OFF_X2 + s2 * C::TILE);
+          umma_commit(BAR_DPF(b));
+          if (DQ) umma_commit(BAR_X2E(s2));
+          if (s.i + 1 == s.u.nq) umma_commit(BAR_RE(rs));  // the resident tiles' last use
+        }
+        if (*abort_p) {  // wind-down: every UMMA issued must complete before TMEM is freed
+          umma_commit(BAR_FIN);
+          mbar_wait_for(BAR_FIN, 0, kDrainLimitNs);
+        }
+      }
+    } else if (warp == 3) {
+      // ----------------------------------------------------------- products
+      if (lane == 0) {
+        constexpr uint32_t IDESC_ACC = idesc_bf16_f32(BT, HD, 0, 1);
+        // A = P or dS in TMEM (each half of the columns over its half of dP),
+        // B = a streamed tile, MN-major
         auto product = [&](uint32_t d, uint32_t a, uint32_t b, bool start) {
           const uint32_t db = desc_lo(b, BT * 128);
 #pragma unroll
@@ -446,84 +482,26 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
             umma_bf16_ts_lo(d, a + (kk >> 2) * 64 + (kk & 3) * 8, db + kk * (2048 >> 4), IDESC_ACC,
                             start && kk == 0 ? 0u : 1u);
         };
-        auto issue_s = [&](const Step& s, bool pad) -> bool {
-          const uint32_t rs = s.uc % C::RST, st = s.t % C::X1ST;
-          if (s.i == 0 && !mbar_wait(BAR_RF(rs), (s.uc / C::RST) & 1, abort_p)) return false;
-          if (!mbar_wait(BAR_X1F(st), (s.t / C::X1ST) & 1, abort_p)) return false;
-          if (pad) {
-            if (!mbar_wait(BAR_X1Z(st), (z1 >> st) & 1, abort_p)) return false;
-            z1 ^= 1u << st;
-          }
-          if (s.t >= 1 && !mbar_wait(BAR_SE, (s.t - 1) & 1, abort_p)) return false;
+        for (Step s = first_step<DQ, false>(prm, ring); s.valid; advance<DQ, false>(prm, s, ring)) {
+          const uint32_t t = s.t, s1 = t % C::X1ST, s2 = t % C::X2ST, b = t % C::DPB;
+          const uint32_t p = tmem + C::TCOL_DP + b * 128, ds = p + 32;
+          if (!mbar_wait(BAR_PR(b), (t / C::DPB) & 1, abort_p)) break;
+          // the unit before has been read out of the sums' columns
+          if (s.i == 0 && s.uc >= 1 && !mbar_wait(BAR_ACC, (s.uc - 1) & 1, abort_p)) break;
           tc_fence_after();
-          scores(tmem + C::TCOL_S, sbase + C::OFF_R + rs * 2 * C::TILE, x1(s.t));
-          umma_commit(BAR_SF);
-          return true;
-        };
-        // (the products that read P and dS out of its columns have completed)
-        auto issue_dp = [&](const Step& s, bool pad) -> bool {
-          const uint32_t rs = s.uc % C::RST, st = s.t % C::X2ST;
-          if (!mbar_wait(BAR_X2F(st), (s.t / C::X2ST) & 1, abort_p)) return false;
-          if (pad) {
-            if (!mbar_wait(BAR_X2Z(st), (z2 >> st) & 1, abort_p)) return false;
-            z2 ^= 1u << st;
-          }
-          tc_fence_after();
-          scores(tmem + C::TCOL_DP + s.t % C::DPB * 128, sbase + C::OFF_R + (rs * 2 + 1) * C::TILE, x2(s.t));
-          umma_commit(BAR_DPF(s.t % C::DPB));
-          if (DQ) umma_commit(BAR_X2E(st));
-          if (s.i + 1 == s.u.nq) umma_commit(BAR_RE(rs));  // the resident tiles' last use
-          return true;
-        };
-        // la: the next step whose S is to be issued; of the step before it,
-        // whose products come next, only its place in its unit is kept (this
-        // one thread's instructions are most of what a short unit waits for)
-        Step la = first_step<DQ, false>(prm, ring);
-        bool ok = true, have = la.valid, first = true, last = false;
-        uint32_t t = 0, uc = 0;
-        if (have) {
-          const bool pad = padded(la);
-          ok = issue_s(la, pad) && issue_dp(la, pad);
-          last = la.u.nq == 1;
-          advance<DQ, false>(prm, la, ring);
-        }
-        while (ok && have) {
-          // ahead of this step's products, except where the next unit's
-          // resident tiles are only now being loaded
-          const bool early = la.valid && (C::RST > 1 || la.i > 0);
-          const bool pad = la.valid && padded(la);
-          if (early && !issue_s(la, pad)) break;
-          if constexpr (C::DPB == 2) {
-            if (t >= 1 && !mbar_wait(BAR_PE, (t - 1) & 1, abort_p)) break;
-            if (early && !issue_dp(la, pad)) break;
-          }
-          if (!mbar_wait(BAR_PR(t % C::DPB), (t / C::DPB) & 1, abort_p)) break;
-          if (first && uc >= 1 && !mbar_wait(BAR_ACC, (uc - 1) & 1, abort_p)) break;
-          tc_fence_after();
-          const uint32_t p = tmem + C::TCOL_DP + t % C::DPB * 128, ds = p + 32;
           if constexpr (!DQ) {
-            product(tmem + C::TCOL_ACC, p, x2(t), first);  // dV += P dO
-            umma_commit(BAR_X2E(t % C::X2ST));
+            product(tmem + C::TCOL_ACC, p, sbase + C::OFF_X2 + s2 * C::TILE, s.i == 0);  // dV += P dO
+            umma_commit(BAR_X2E(s2));
           }
-          product(tmem + C::TCOL_ACC + (DQ ? 0 : HD), ds, x1(t), first);  // dK += dS Q, dQ += dS K
-          umma_commit(BAR_X1E(t % C::X1ST));
-          umma_commit(BAR_PE);
-          if (last) umma_commit(BAR_DONE);
-          if (!early && la.valid && !issue_s(la, pad)) break;
-          if (C::DPB == 1 && !mbar_wait(BAR_PE, t & 1, abort_p)) break;
-          have = la.valid;
-          if (have) {
-            if ((C::DPB == 1 || !early) && !issue_dp(la, pad)) break;
-            first = la.i == 0;
-            last = la.i + 1 == la.u.nq;
-            t = la.t;
-            uc = la.uc;
-            advance<DQ, false>(prm, la, ring);
-          }
+          // dK += dS Q, dQ += dS K
+          product(tmem + C::TCOL_ACC + (DQ ? 0 : HD), ds, sbase + C::OFF_X1 + s1 * C::TILE, s.i == 0);
+          umma_commit(BAR_PE(b));
+          umma_commit(BAR_X1E(s1));
+          if (s.i + 1 == s.u.nq) umma_commit(BAR_DONE);
         }
-        if (*abort_p) {  // wind-down: every UMMA issued must complete before TMEM is freed
-          umma_commit(BAR_FIN);
-          mbar_wait_for(BAR_FIN, 0, kDrainLimitNs);
+        if (*abort_p) {
+          umma_commit(BAR_FIN + 8);
+          mbar_wait_for(BAR_FIN + 8, 0, kDrainLimitNs);
         }
       }
     } else if (warp == 2) {
