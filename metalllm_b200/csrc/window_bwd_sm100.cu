@@ -31,15 +31,15 @@
 // products too, so the tensor core works on the next step while the compute
 // warps form this one's P and dS.
 //
-// Roles (384 threads): warpgroup 0 (120 registers): warp 0 TMA producer, which
+// Roles (512 threads): warpgroup 0 (72 registers): warp 0 TMA producer, which
 // also decodes the units and passes them on through shared memory (each role
 // decoding for itself is more code than the instruction cache holds); warp 1
 // issues S and dP, warp 3 the products (one thread for both spent more on waits
 // and addresses than the tensor core on the work: a step 2.9 us); warp 2
 // statistics of the dK/dV pass, and zeroes padding rows of
-// streamed tiles (their P is 0, but 0 * NaN is not).  Warpgroups 1, 2 (192
-// registers) compute: thread = row = TMEM lane, 64 columns each, and store the
-// unit's sums.
+// streamed tiles (their P is 0, but 0 * NaN is not).  Warpgroups 1, 2 (184
+// registers) compute: thread = row = TMEM lane, 64 columns each.  Warpgroup 3
+// (72 registers) stores a unit's sums while the next unit is under way.
 //
 // A sink tile is seen by every later query, a chain of steps far longer than
 // any other unit's; what lies past its window is cut into units of their own
@@ -59,12 +59,13 @@ namespace {
 using namespace sm100;
 
 constexpr int BT = 128;  // rows of every tile
-constexpr int NUM_THREADS = 384;
-constexpr int LAUNCH_REGS = 168;
-constexpr int REGS_PRODUCER = 120;
-constexpr int REGS_COMPUTE = 192;
+constexpr int NUM_THREADS = 512;
+constexpr int LAUNCH_REGS = 128;
+constexpr int REGS_PRODUCER = 72;
+constexpr int REGS_COMPUTE = 184;
+constexpr int REGS_STORE = 72;
 constexpr int NCOMP = 256;
-static_assert(128 * REGS_PRODUCER + NCOMP * REGS_COMPUTE == NUM_THREADS * LAUNCH_REGS,
+static_assert(128 * (REGS_PRODUCER + REGS_STORE) + NCOMP * REGS_COMPUTE == NUM_THREADS * LAUNCH_REGS,
               "register split must equal the launch allocation");
 constexpr float LOG2E = 1.4426950408889634f;
 
@@ -340,8 +341,9 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   const uint32_t BAR_FIN = BAR(B_1 + 4);                    // wind-down, one for each issuer
   const uint32_t BAR_U = BAR(B_1 + 6);                      // sched full, empty, desc_full
   float* stat_base = reinterpret_cast<float*>(gbase + C::OFF_STAT);
-  // readers of a unit: the producer, the issuers, warp 2 and the 8 compute warps
-  constexpr uint32_t READERS = 4 + NCOMP / 32;
+  // readers of a unit: the producer, the issuers, warp 2, the 8 compute and the
+  // 4 storing warps
+  constexpr uint32_t READERS = 4 + NCOMP / 32 + 4;
 
   if (threadIdx.x == 0) {
     abort_flag = 0;
@@ -351,7 +353,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       if (i >= B_X2 + C::X2ST && i < B_X2 + 2 * C::X2ST) n = 2;
       if (i >= B_T && i < B_T + C::SSTG) n = 32;
       if (i >= B_T + C::SSTG && i < B_DP) n = NCOMP;
-      if ((i >= B_PR && i < B_PE) || i == B_1 + 1 || i == B_1 + 3) n = NCOMP;
+      if ((i >= B_PR && i < B_PE) || i == B_1 + 1) n = NCOMP;
+      if (i == B_1 + 3) n = 128;
       if (i >= B_1 + 6 + (int)kSchedSlots && i < B_1 + 6 + 2 * (int)kSchedSlots) n = READERS;
       mbar_init(BAR(i), n);
     }
@@ -551,7 +554,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         }
       }
     }
-  } else {
+  } else if (warp < 12) {
     reg_alloc<REGS_COMPUTE>();
     // ------------------------------------------------------------ compute
     const int quarter = warp & 3, part = (warp - 4) >> 2;  // columns part*64 .. +63
@@ -560,62 +563,6 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     const float2 c2 = make_float2(prm.scale_log2, prm.scale_log2), sc2 = make_float2(prm.scale, prm.scale);
     bool ok = true;
     float nl = 0.0f, nd = 0.0f;  // dQ: the row's statistics
-
-    // a unit's sums (all its products complete): TMEM -> registers, which frees
-    // the columns for the next unit, then straight to global memory
-    auto store_sums = [&](const Unit& v, uint32_t vuc) {
-      ok = mbar_wait_warp(BAR_DONE, vuc & 1, abort_p);
-      if (!ok) return;
-      tc_fence_after();
-      constexpr int CPH = HD / 2;  // columns of a sum per part
-      constexpr int NS = DQ ? 1 : 2;
-      uint32_t acc[NS][CPH];
-#pragma unroll
-      for (int w = 0; w < NS; ++w)
-#pragma unroll
-        for (int cc = 0; cc < CPH; cc += 32) {
-          uint32_t r[32];
-          tmem_ld32(tl + C::TCOL_ACC + w * HD + part * CPH + cc, r);
-          tmem_wait_ld_dep(r);
-#pragma unroll
-          for (int j = 0; j < 32; ++j) acc[w][cc + j] = r[j];
-        }
-      tc_fence_before();
-      mbar_arrive(BAR_ACC);
-      const int at = v.tile * BT + row;
-      // a padding row's sums are 0, whatever its own tile held
-      if (at >= v.n) {
-#pragma unroll
-        for (int w = 0; w < NS; ++w)
-#pragma unroll
-          for (int j = 0; j < CPH; ++j) acc[w][j] = 0u;
-      }
-      auto store_f32 = [&](float* to, const uint32_t (&x)[CPH]) {
-#pragma unroll
-        for (int j = 0; j < CPH; j += 4)
-          *reinterpret_cast<uint4*>(to + j) = make_uint4(x[j], x[j + 1], x[j + 2], x[j + 3]);
-      };
-      auto store_bf16 = [&](__nv_bfloat16* to, const uint32_t (&x)[CPH]) {
-        auto pair = [&](int j) { return pack_bf16(__uint_as_float(x[j]), __uint_as_float(x[j + 1])); };
-#pragma unroll
-        for (int j = 0; j < CPH; j += 8)
-          *reinterpret_cast<uint4*>(to + j) = make_uint4(pair(j), pair(j + 2), pair(j + 4), pair(j + 6));
-      };
-      if constexpr (DQ) {
-        if (at >= prm.T) return;
-        const long long off = (((long long)v.b * prm.T + at) * prm.NH + v.head) * HD + part * CPH;
-        if (prm.dq_f32) store_f32(static_cast<float*>(prm.dQ) + off, acc[0]);
-        else store_bf16(static_cast<__nv_bfloat16*>(prm.dQ) + off, acc[0]);
-      } else if (v.slot >= 0) {
-#pragma unroll
-        for (int w = 0; w < 2; ++w)
-          store_f32(prm.part + (((long long)v.slot * 2 + w) * BT + row) * HD + part * CPH, acc[w]);
-      } else if (at < prm.T) {
-        const long long off = (((long long)v.b * prm.T + at) * prm.NKV + v.head) * HD + part * CPH;
-        store_bf16(prm.dV + off, acc[0]);
-        store_bf16(prm.dK + off, acc[1]);
-      }
-    };
 
     // P and dS of step s, handed to the UMMA issuer
     auto form = [&](const Step& s) {
@@ -695,16 +642,59 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       mbar_arrive(BAR_PR(t % C::DPB));
     };
 
-    // A unit's sums are stored after the next unit's first step has been handed
-    // to the tensor core (or after the last step of the last unit).
-    Unit prev{};
-    bool have_prev = false;
-    for (Step s = first_step<DQ, true>(prm, ring); ok; advance<DQ, true>(prm, s, ring)) {
-      if (s.valid) form(s);
-      if (ok && have_prev && (!s.valid || s.i == 0)) store_sums(prev, s.uc - 1);
-      if (!ok || !s.valid) break;
-      prev = s.u;
-      have_prev = true;
+    for (Step s = first_step<DQ, true>(prm, ring); ok && s.valid; advance<DQ, true>(prm, s, ring)) form(s);
+  } else {
+    reg_dealloc<REGS_STORE>();
+    // ------------------------------------------------------- a unit's sums
+    // thread = row = TMEM lane; 32 columns at a time, TMEM -> registers ->
+    // global memory
+    const int row = (warp & 3) * 32 + lane;
+    const uint32_t tl = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    Step s = first_step<DQ, true>(prm, ring);
+    while (s.valid) {
+      if (!mbar_wait_warp(BAR_DONE, s.uc & 1, abort_p)) break;
+      tc_fence_after();
+      const Unit& v = s.u;
+      const int at = v.tile * BT + row;
+      const bool valid = at < v.n;  // a padding row's sums are 0, whatever its own tile held
+      constexpr int COLS = (DQ ? 1 : 2) * HD;
+#pragma unroll 1
+      for (int cc = 0; cc < COLS; cc += 32) {
+        uint32_t r[32];
+        tmem_ld32(tl + C::TCOL_ACC + cc, r);
+        tmem_wait_ld_dep(r);
+        if (cc + 32 == COLS) {  // all read: the next unit may overwrite them
+          tc_fence_before();
+          mbar_arrive(BAR_ACC);
+        }
+#pragma unroll
+        for (int j = 0; j < 32; ++j) r[j] = valid ? r[j] : 0u;
+        const int which = cc / HD, col = cc % HD;
+        float* f32 = nullptr;
+        __nv_bfloat16* b16 = nullptr;
+        if constexpr (DQ) {
+          const long long off = (((long long)v.b * prm.T + at) * prm.NH + v.head) * HD + col;
+          if (prm.dq_f32) f32 = static_cast<float*>(prm.dQ) + off;
+          else b16 = static_cast<__nv_bfloat16*>(prm.dQ) + off;
+        } else if (v.slot >= 0) {
+          f32 = prm.part + (((long long)v.slot * 2 + which) * BT + row) * HD + col;
+        } else {
+          b16 = (which == 0 ? prm.dV : prm.dK) + (((long long)v.b * prm.T + at) * prm.NKV + v.head) * HD + col;
+        }
+        if (at >= prm.T && (DQ || v.slot < 0)) continue;
+        if (f32) {
+#pragma unroll
+          for (int j = 0; j < 32; j += 4)
+            *reinterpret_cast<uint4*>(f32 + j) = make_uint4(r[j], r[j + 1], r[j + 2], r[j + 3]);
+        } else {
+          auto pair = [&](int j) { return pack_bf16(__uint_as_float(r[j]), __uint_as_float(r[j + 1])); };
+#pragma unroll
+          for (int j = 0; j < 32; j += 8)
+            *reinterpret_cast<uint4*>(b16 + j) = make_uint4(pair(j), pair(j + 2), pair(j + 4), pair(j + 6));
+        }
+      }
+      ++s.uc;
+      s.valid = next_unit<DQ, true, false>(prm, s, ring);
     }
   }
 
