@@ -132,6 +132,28 @@ __device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, vo
   return __all_sync(0xffffffffu, ok);
 }
 
+// mbar_wait in a third of the code, for kernels whose many waits would crowd the
+// instruction cache: at most 2^21 polls, each suspended for at most about a
+// microsecond, bound the wait (by 0.05 to some 3 s).
+__device__ __forceinline__ bool mbar_poll(uint32_t bar, uint32_t parity, volatile int* abort) {
+  for (uint32_t i = 0;; ++i) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.b32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity), "r"(1000u)
+        : "memory");
+    if (ok) return true;
+    if (i >> 21) *abort = 1;
+    if (*abort) return false;
+  }
+}
+__device__ __forceinline__ bool mbar_poll_warp(uint32_t bar, uint32_t parity, volatile int* abort) {
+  return __all_sync(0xffffffffu, mbar_poll(bar, parity, abort));
+}
+
 // Named barrier `id` over `nthreads` threads that also returns the AND of
 // every participant's `v` (bar.red.and.pred), so a group can agree on a flag.
 __device__ __forceinline__ bool bar_red_and(uint32_t id, uint32_t nthreads, bool v) {

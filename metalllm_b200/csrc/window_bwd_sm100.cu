@@ -45,7 +45,7 @@
 // any other unit's; what lies past its window is cut into units of their own
 // whose partial dV, dK a last kernel adds up in slot order (win_plan).
 //
-// All mbarrier waits are bounded (about 2 s); on time-out the CTA winds down,
+// All mbarrier waits are bounded (mbar_poll); on time-out the CTA winds down,
 // frees its TMEM and sets STATUS_BWD_TIMEOUT.
 #include <algorithm>
 
@@ -250,7 +250,7 @@ __device__ __forceinline__ bool next_unit(const Params& p, Step& s, const Ring& 
   } else {
     const uint32_t ph = g == 0 ? 0u : ((g - 1) / kSchedSlots) & 1u;
     volatile int* abort = ring.sched.abort;
-    if (!(WARP ? mbar_wait_warp(ring.full + 8u * slot, ph, abort) : mbar_wait(ring.full + 8u * slot, ph, abort)))
+    if (!(WARP ? mbar_poll_warp(ring.full + 8u * slot, ph, abort) : mbar_poll(ring.full + 8u * slot, ph, abort)))
       return false;
     s.u = ring.desc[slot];
     if (g > 0) {
@@ -391,7 +391,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         for (Step s = first_step<DQ, false, true>(prm, ring); s.valid; advance<DQ, false, true>(prm, s, ring)) {
           if (s.i == 0) {
             const int rs = s.uc % C::RST, col = s.u.head * HD;
-            if (s.uc >= C::RST && !mbar_wait(BAR_RE(rs), ((s.uc / C::RST) - 1) & 1, abort_p)) break;
+            if (s.uc >= C::RST && !mbar_poll(BAR_RE(rs), ((s.uc / C::RST) - 1) & 1, abort_p)) break;
             mbar_arrive_expect_tx(BAR_RF(rs), 2 * C::TILE);
             ++r_armed;
             for (int kb = 0; kb < C::KB; ++kb) {
@@ -402,12 +402,12 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
           }
           const int s1 = s.t % C::X1ST, s2 = s.t % C::X2ST;
           const int col = s.u.x_head<DQ>(s.i) * HD, row = s.u.x_tile<DQ>(s.i) * BT;
-          if (s.t >= C::X1ST && !mbar_wait(BAR_X1E(s1), ((s.t / C::X1ST) - 1) & 1, abort_p)) break;
+          if (s.t >= C::X1ST && !mbar_poll(BAR_X1E(s1), ((s.t / C::X1ST) - 1) & 1, abort_p)) break;
           mbar_arrive_expect_tx(BAR_X1F(s1), C::TILE);
           ++x1_armed;
           for (int kb = 0; kb < C::KB; ++kb)
             tma_load_3d(sbase + C::OFF_X1 + s1 * C::TILE + kb * BT * 128, &tmX1, BAR_X1F(s1), col + kb * 64, row, s.u.b);
-          if (s.t >= C::X2ST && !mbar_wait(BAR_X2E(s2), ((s.t / C::X2ST) - 1) & 1, abort_p)) break;
+          if (s.t >= C::X2ST && !mbar_poll(BAR_X2E(s2), ((s.t / C::X2ST) - 1) & 1, abort_p)) break;
           mbar_arrive_expect_tx(BAR_X2F(s2), C::TILE);
           ++x2_armed;
           for (int kb = 0; kb < C::KB; ++kb)
@@ -443,23 +443,23 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         for (Step s = first_step<DQ, false>(prm, ring); s.valid; advance<DQ, false>(prm, s, ring)) {
           const uint32_t t = s.t, rs = s.uc % C::RST, s1 = t % C::X1ST, s2 = t % C::X2ST, b = t % C::DPB;
           const bool pad = padded(s);
-          if (s.i == 0 && !mbar_wait(BAR_RF(rs), (s.uc / C::RST) & 1, abort_p)) break;
-          if (!mbar_wait(BAR_X1F(s1), (t / C::X1ST) & 1, abort_p)) break;
+          if (s.i == 0 && !mbar_poll(BAR_RF(rs), (s.uc / C::RST) & 1, abort_p)) break;
+          if (!mbar_poll(BAR_X1F(s1), (t / C::X1ST) & 1, abort_p)) break;
           if (pad) {
-            if (!mbar_wait(BAR_X1Z(s1), (z1 >> s1) & 1, abort_p)) break;
+            if (!mbar_poll(BAR_X1Z(s1), (z1 >> s1) & 1, abort_p)) break;
             z1 ^= 1u << s1;
           }
-          if (t >= 1 && !mbar_wait(BAR_SE, (t - 1) & 1, abort_p)) break;
+          if (t >= 1 && !mbar_poll(BAR_SE, (t - 1) & 1, abort_p)) break;
           tc_fence_after();
           scores(tmem + C::TCOL_S, sbase + C::OFF_R + rs * 2 * C::TILE, sbase + C::OFF_X1 + s1 * C::TILE);
           umma_commit(BAR_SF);
-          if (!mbar_wait(BAR_X2F(s2), (t / C::X2ST) & 1, abort_p)) break;
+          if (!mbar_poll(BAR_X2F(s2), (t / C::X2ST) & 1, abort_p)) break;
           if (pad) {
-            if (!mbar_wait(BAR_X2Z(s2), (z2 >> s2) & 1, abort_p)) break;
+            if (!mbar_poll(BAR_X2Z(s2), (z2 >> s2) & 1, abort_p)) break;
             z2 ^= 1u << s2;
           }
           // the products that read P and dS out of its columns have completed
-          if (t >= C::DPB && !mbar_wait(BAR_PE(b), ((t / C::DPB) - 1) & 1, abort_p)) break;
+          if (t >= C::DPB && !mbar_poll(BAR_PE(b), ((t / C::DPB) - 1) & 1, abort_p)) break;
           tc_fence_after();
           scores(tmem + C::TCOL_DP + b * 128, sbase + C::OFF_R + (rs * 2 + 1) * C::TILE,
                  sbase + C::OFF_X2 + s2 * C::TILE);
@@ -488,9 +488,9 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         for (Step s = first_step<DQ, false>(prm, ring); s.valid; advance<DQ, false>(prm, s, ring)) {
           const uint32_t t = s.t, s1 = t % C::X1ST, s2 = t % C::X2ST, b = t % C::DPB;
           const uint32_t p = tmem + C::TCOL_DP + b * 128, ds = p + 32;
-          if (!mbar_wait(BAR_PR(b), (t / C::DPB) & 1, abort_p)) break;
+          if (!mbar_poll(BAR_PR(b), (t / C::DPB) & 1, abort_p)) break;
           // the unit before has been read out of the sums' columns
-          if (s.i == 0 && s.uc >= 1 && !mbar_wait(BAR_ACC, (s.uc - 1) & 1, abort_p)) break;
+          if (s.i == 0 && s.uc >= 1 && !mbar_poll(BAR_ACC, (s.uc - 1) & 1, abort_p)) break;
           tc_fence_after();
           if constexpr (!DQ) {
             product(tmem + C::TCOL_ACC, p, sbase + C::OFF_X2 + s2 * C::TILE, s.i == 0);  // dV += P dO
@@ -532,7 +532,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
           L = __ldg(reinterpret_cast<const float4*>(prm.neg_l + at));
           D4 = __ldg(reinterpret_cast<const float4*>(prm.neg_d + at));
         }
-        if (!mbar_wait_warp(BAR_X1F(s1), (s.t / C::X1ST) & 1, abort_p)) break;
+        if (!mbar_poll_warp(BAR_X1F(s1), (s.t / C::X1ST) & 1, abort_p)) break;
         if (pad) zero_rows(C::OFF_X1 + s1 * C::TILE, a);
         if (lane == 0) {
           if (pad) mbar_arrive(BAR_X1Z(s1));
@@ -540,13 +540,13 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         }
         if constexpr (!DQ) {
           const int st = s.t % C::SSTG;
-          if (s.t >= C::SSTG && !mbar_wait_warp(BAR_TE(st), ((s.t / C::SSTG) - 1) & 1, abort_p)) break;
+          if (s.t >= C::SSTG && !mbar_poll_warp(BAR_TE(st), ((s.t / C::SSTG) - 1) & 1, abort_p)) break;
           float* stt = stat_base + st * (2 * BT);
           reinterpret_cast<float4*>(stt)[lane] = L;
           reinterpret_cast<float4*>(stt + BT)[lane] = D4;
           mbar_arrive(BAR_TF(st));
         }
-        if (!mbar_wait_warp(BAR_X2F(s2), (s.t / C::X2ST) & 1, abort_p)) break;
+        if (!mbar_poll_warp(BAR_X2F(s2), (s.t / C::X2ST) & 1, abort_p)) break;
         if (pad) zero_rows(C::OFF_X2 + s2 * C::TILE, a);
         if (lane == 0) {
           if (pad) mbar_arrive(BAR_X2Z(s2));
@@ -589,7 +589,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
 #pragma unroll
         for (int w = 0; w < 2; ++w) see[w] = bits_below(to - 32 * w) & ~bits_below(from - 32 * w);
       }
-      ok = mbar_wait_warp(BAR_SF, t & 1, abort_p);
+      ok = mbar_poll_warp(BAR_SF, t & 1, abort_p);
       if (!ok) return;
       tc_fence_after();
       float p[64];
@@ -599,7 +599,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       const float* stt = stat_base;
       if constexpr (!DQ) {
         const int st = t % C::SSTG;
-        ok = mbar_wait_warp(BAR_TF(st), (t / C::SSTG) & 1, abort_p);
+        ok = mbar_poll_warp(BAR_TF(st), (t / C::SSTG) & 1, abort_p);
         if (!ok) return;
         stt += st * (2 * BT) + part * 64;
       }
@@ -615,7 +615,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         p[j + 2] = m & 4u ? ex2(t1.x) : 0.0f;
         p[j + 3] = m & 8u ? ex2(t1.y) : 0.0f;
       }
-      ok = mbar_wait_warp(BAR_DPF(t % C::DPB), (t / C::DPB) & 1, abort_p);
+      ok = mbar_poll_warp(BAR_DPF(t % C::DPB), (t / C::DPB) & 1, abort_p);
       if (!ok) return;
       tc_fence_after();
       const uint32_t tdp = tl + C::TCOL_DP + t % C::DPB * 128 + part * 64;
@@ -652,7 +652,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     const uint32_t tl = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     Step s = first_step<DQ, true>(prm, ring);
     while (s.valid) {
-      if (!mbar_wait_warp(BAR_DONE, s.uc & 1, abort_p)) break;
+      if (!mbar_poll_warp(BAR_DONE, s.uc & 1, abort_p)) break;
       tc_fence_after();
       const Unit& v = s.u;
       const int at = v.tile * BT + row;
