@@ -261,25 +261,28 @@ __device__ __forceinline__ bool next_unit(const Params& p, Step& s, const Ring& 
   }
 }
 
-template <bool DQ, bool WARP, bool PUBLISH = false>
-__device__ __forceinline__ Step first_step(const Params& p, const Ring& ring) {
+// A role's loop is `for (Step s = before_first(); advance<...>(prm, s, ring);)`:
+// one copy of the code that goes on to the next unit.
+__device__ __forceinline__ Step before_first() {
   Step s;
   s.g = s.i = 0;
-  s.t = s.uc = 0;
-  s.valid = next_unit<DQ, WARP, PUBLISH>(p, s, ring);
+  s.u.nq = 1;
+  s.t = s.uc = ~0u;
+  s.valid = false;
   return s;
 }
 
 template <bool DQ, bool WARP, bool PUBLISH = false>
-__device__ __forceinline__ void advance(const Params& p, Step& s, const Ring& ring) {
+__device__ __forceinline__ bool advance(const Params& p, Step& s, const Ring& ring) {
   ++s.t;
   if (s.i + 1 < s.u.nq) {
     ++s.i;
-    return;
+    return true;
   }
   s.i = 0;
   ++s.uc;
   s.valid = next_unit<DQ, WARP, PUBLISH>(p, s, ring);
+  return s.valid;
 }
 
 // 64 fp32 columns of this lane's TMEM row
@@ -388,7 +391,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         tma_prefetch_desc(&tmX1);
         tma_prefetch_desc(&tmX2);
         uint32_t r_armed = 0, x1_armed = 0, x2_armed = 0, nreq = 0;
-        for (Step s = first_step<DQ, false, true>(prm, ring); s.valid; advance<DQ, false, true>(prm, s, ring)) {
+        for (Step s = before_first(); advance<DQ, false, true>(prm, s, ring);) {
           if (s.i == 0) {
             const int rs = s.uc % C::RST, col = s.u.head * HD;
             if (s.uc >= C::RST && !mbar_poll(BAR_RE(rs), ((s.uc / C::RST) - 1) & 1, abort_p)) break;
@@ -440,7 +443,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
             umma_bf16_ss_lo(d, da + off, db + off, IDESC_S, kk > 0 ? 1u : 0u);
           }
         };
-        for (Step s = first_step<DQ, false>(prm, ring); s.valid; advance<DQ, false>(prm, s, ring)) {
+        for (Step s = before_first(); advance<DQ, false>(prm, s, ring);) {
           const uint32_t t = s.t, rs = s.uc % C::RST, s1 = t % C::X1ST, s2 = t % C::X2ST, b = t % C::DPB;
           const bool pad = padded(s);
           if (s.i == 0 && !mbar_poll(BAR_RF(rs), (s.uc / C::RST) & 1, abort_p)) break;
@@ -485,7 +488,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
             umma_bf16_ts_lo(d, a + (kk >> 2) * 64 + (kk & 3) * 8, db + kk * (2048 >> 4), IDESC_ACC,
                             start && kk == 0 ? 0u : 1u);
         };
-        for (Step s = first_step<DQ, false>(prm, ring); s.valid; advance<DQ, false>(prm, s, ring)) {
+        for (Step s = before_first(); advance<DQ, false>(prm, s, ring);) {
           const uint32_t t = s.t, s1 = t % C::X1ST, s2 = t % C::X2ST, b = t % C::DPB;
           const uint32_t p = tmem + C::TCOL_DP + b * 128, ds = p + 32;
           if (!mbar_poll(BAR_PR(b), (t / C::DPB) & 1, abort_p)) break;
@@ -521,7 +524,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       };
       // every stage is waited for and released, so that this warp stays within
       // one phase of each slot's barriers
-      for (Step s = first_step<DQ, true>(prm, ring); s.valid; advance<DQ, true>(prm, s, ring)) {
+      for (Step s = before_first(); advance<DQ, true>(prm, s, ring);) {
         const int s1 = s.t % C::X1ST, s2 = s.t % C::X2ST;
         const bool pad = padded(s);
         const int a = max(0, s.u.n - s.u.x_tile<DQ>(s.i) * BT);
@@ -642,7 +645,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       mbar_arrive(BAR_PR(t % C::DPB));
     };
 
-    for (Step s = first_step<DQ, true>(prm, ring); ok && s.valid; advance<DQ, true>(prm, s, ring)) form(s);
+    for (Step s = before_first(); ok && advance<DQ, true>(prm, s, ring);) form(s);
   } else {
     reg_dealloc<REGS_STORE>();
     // ------------------------------------------------------- a unit's sums
@@ -650,8 +653,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     // global memory
     const int row = (warp & 3) * 32 + lane;
     const uint32_t tl = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-    Step s = first_step<DQ, true>(prm, ring);
-    while (s.valid) {
+    Step s = before_first();
+    while (++s.uc, next_unit<DQ, true, false>(prm, s, ring)) {
       if (!mbar_poll_warp(BAR_DONE, s.uc & 1, abort_p)) break;
       tc_fence_after();
       const Unit& v = s.u;
@@ -693,8 +696,6 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
             *reinterpret_cast<uint4*>(b16 + j) = make_uint4(pair(j), pair(j + 2), pair(j + 4), pair(j + 6));
         }
       }
-      ++s.uc;
-      s.valid = next_unit<DQ, true, false>(prm, s, ring);
     }
   }
 
