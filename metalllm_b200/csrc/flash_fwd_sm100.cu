@@ -106,8 +106,8 @@ struct FwdCfg {
   // q_full/empty[QST], k_full/empty[KST], v_full/empty[VST], per tile X:
   // s_full, s_free, p_full, pv_done, o_free, do_full; then never (nothing
   // arrives: the time-out test hook), fin (the UMMA issuer's wind-down),
-  // sched_full/empty[NSCHED] and, for WIN, v_fixed[VST]
-  static constexpr int NBAR = 2 * QST + 2 * KST + 2 * VST + 2 * 6 + 2 + 2 * NSCHED + (WIN ? VST : 0);
+  // sched_full/empty[NSCHED] and, for WIN, v_fixed[VST] and a second fin
+  static constexpr int NBAR = 2 * QST + 2 * KST + 2 * VST + 2 * 6 + 2 + 2 * NSCHED + (WIN ? VST + 1 : 0);
   static constexpr uint32_t OFF_TSLOT = OFF_BAR + NBAR * 8;
   static constexpr uint32_t SMEM_BYTES = OFF_TSLOT + 16 + 1024;  // + alignment slack
   static constexpr uint32_t TCOL_S = 0;     // S_A, S_B at columns 0, 128
@@ -305,11 +305,12 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   auto BAR_UF = [&](int s) { return barX + 8u * (14 + s); };              // response s landed
   auto BAR_UE = [&](int s) { return barX + 8u * (14 + C::NSCHED + s); };  // response s read by all
   auto BAR_VZ = [&](int s) { return barX + 8u * (14 + 2 * C::NSCHED + s); };  // WIN: V slot s zeroed where it must be
+  const uint32_t BAR_FIN2 = barX + 8u * (14 + 2 * C::NSCHED + C::VST);  // WIN: the PV issuer's wind-down
   // dynamic schedule: unit g >= 1 of this CTA is the one launch-control
   // response g-1 names (requested by the TMA producer when it starts unit
-  // g-1); readers: the producer, the UMMA issuer, the 8 softmax warps and,
-  // for WIN, the warp that zeroes V rows
-  constexpr uint32_t SCHED_READERS = WIN ? 11 : 10;
+  // g-1); readers: the producer, the UMMA issuer (WIN: both), the 8 softmax
+  // warps and, for WIN, the warp that zeroes V rows
+  constexpr uint32_t SCHED_READERS = WIN ? 12 : 10;
   auto unit = [&](int k) {
     if constexpr (WIN) return decode_win_unit<C::HB>(prm, k);
     else return decode_unit<C::HB>(prm, k);
@@ -345,7 +346,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       mbar_init(BAR_UE(u), SCHED_READERS);
     }
     if constexpr (WIN)
-      for (int s = 0; s < C::VST; ++s) mbar_init(BAR_VZ(s), 1);
+      for (int s = 0; s <= C::VST; ++s) mbar_init(BAR_VZ(s), 1);  // and BAR_FIN2
     fence_mbar_init();
   }
   if (warp == 1) {
@@ -394,7 +395,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         int tile0 = 2 * un.pair;
         if constexpr (WIN) tile0 = un.tile0;
         const int qs = qc % C::QST;
-        if (qc >= C::QST && !mbar_wait(BAR_QE(qs), ((qc / C::QST) - 1) & 1, abort_p)) break;
+        if (qc >= C::QST && !wait_on<WIN>(BAR_QE(qs), ((qc / C::QST) - 1) & 1, abort_p)) break;
         const int ntile = un.nB > 0 ? 2 : 1;
         mbar_arrive_expect_tx(BAR_QF(qs), ntile * C::QT_BYTES);
         for (int x = 0; x < ntile; ++x)
@@ -406,14 +407,14 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
           int kt = j;
           if constexpr (WIN) kt = un.key_tile(j);
           const int ks = kc % C::KST;
-          if (kc >= C::KST && !mbar_wait(BAR_KE(ks), ((kc / C::KST) - 1) & 1, abort_p)) { ok = false; break; }
+          if (kc >= C::KST && !wait_on<WIN>(BAR_KE(ks), ((kc / C::KST) - 1) & 1, abort_p)) { ok = false; break; }
           mbar_arrive_expect_tx(BAR_KF(ks), C::KV_BYTES);
           for (int kb = 0; kb < C::KB; ++kb)
             tma_load_3d(sbase + C::OFF_K + ks * C::KV_BYTES + kb * BN * 128, &tmK, BAR_KF(ks),
                         kv0 + kb * 64, kt * BN, un.b);
           ++kc;
           const int vs = vc % C::VST;
-          if (vc >= C::VST && !mbar_wait(BAR_VE(vs), ((vc / C::VST) - 1) & 1, abort_p)) { ok = false; break; }
+          if (vc >= C::VST && !wait_on<WIN>(BAR_VE(vs), ((vc / C::VST) - 1) & 1, abort_p)) { ok = false; break; }
           mbar_arrive_expect_tx(BAR_VF(vs), C::KV_BYTES);
           for (int kb = 0; kb < C::KB; ++kb)
             tma_load_3d(sbase + C::OFF_V + vs * C::KV_BYTES + kb * BN * 128, &tmV, BAR_VF(vs),
@@ -427,16 +428,14 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         drain_ring(BAR_KF, C::KST, kc);
         drain_ring(BAR_VF, C::VST, vc);
       }
-    } else if (warp == 1 && lane == 0) {
+    } else if (!WIN && warp == 1 && lane == 0) {
       // ----------------------------------------------------------- MMA
       constexpr uint32_t IDESC_S = idesc_bf16_f32(BM, BN, 0, 0);
-      constexpr uint32_t IDESC_SN = idesc_bf16_f32(BM, NARROW, 0, 0);
       constexpr uint32_t IDESC_O = idesc_bf16_f32(BM, HD, 0, 1);
       uint32_t qc = 0, kc = 0, vc = 0;
       uint32_t sc[2] = {0, 0};   // S_X issued so far
       uint32_t pvc[2] = {0, 0};  // PV_X issued so far
       uint32_t uc[2] = {0, 0};   // units in which tile X was active
-      uint32_t vzp = 0;          // WIN: bit s = parity of v_fixed[s]'s next phase
       bool ok = true;
       for (int g = 0; ok; ++g) {
         int k;
@@ -445,14 +444,6 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         if (k < 0) break;
         const auto un = unit(k);
         const int n[2] = {un.nA, un.nB};
-        if (WIN && un.nkv == 0) continue;  // only padding
-        // tile x works on list index j; f[x] is the first it works on
-        auto act = [&](int x, int j) {
-          if constexpr (WIN) return un.active(x, j);
-          else return j < n[x];
-        };
-        int f[2] = {0, 0};
-        if constexpr (WIN) f[1] = un.first(1);
         const int qs = qc % C::QST;
         if (!mbar_wait(BAR_QF(qs), (qc / C::QST) & 1, abort_p)) break;
         // S_X(j) = Q_X K_j^T
@@ -461,14 +452,11 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
           tc_fence_after();
           const uint32_t sq = sbase + C::OFF_Q + (qs * 2 + x) * C::QT_BYTES;
           const uint32_t sk = sbase + C::OFF_K + ((kc + j) % C::KST) * C::KV_BYTES;
-          uint32_t idesc = IDESC_S;
-          if constexpr (WIN)
-            if (un.narrow(prm.win, j)) idesc = IDESC_SN;
           const uint64_t dq = smem_desc_sw128(sq, 16, 1024), dk = smem_desc_sw128(sk, 16, 1024);
 #pragma unroll
           for (int kk = 0; kk < HD / 16; ++kk) {
             const uint32_t off = (kk >> 2) * (BM * 128) + (kk & 3) * 32;
-            umma_bf16_ss(tmem + C::TCOL_S + x * BN, desc_at(dq, off), desc_at(dk, off), idesc, kk > 0 ? 1u : 0u);
+            umma_bf16_ss(tmem + C::TCOL_S + x * BN, desc_at(dq, off), desc_at(dk, off), IDESC_S, kk > 0 ? 1u : 0u);
           }
           umma_commit(BAR_SF(x));
           ++sc[x];
@@ -477,24 +465,20 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         // O_X += P_X V_j
         auto issue_pv = [&](int x, int j) -> bool {
           if (!mbar_wait(BAR_PF(x), pvc[x] & 1, abort_p)) return false;
-          if (j == f[x] && uc[x] >= 1 && !mbar_wait(BAR_OE(x), (uc[x] - 1) & 1, abort_p)) return false;
+          if (j == 0 && uc[x] >= 1 && !mbar_wait(BAR_OE(x), (uc[x] - 1) & 1, abort_p)) return false;
           tc_fence_after();
           const uint32_t sp = sbase + C::OFF_P + x * C::STG_BYTES;
           const uint32_t sv = sbase + C::OFF_V + ((vc + j) % C::VST) * C::KV_BYTES;
           const uint64_t dv = smem_desc_sw128(sv, BN * 128, 1024), dp = smem_desc_sw128(sp, 16, 1024);
-          int steps = BN / 16;
-          if constexpr (WIN)
-            if (un.narrow(prm.win, j)) steps = NARROW / 16;
 #pragma unroll
           for (int kk = 0; kk < BN / 16; ++kk) {
-            if (WIN && kk >= steps) break;
             const uint64_t bd = desc_at(dv, kk * 2048);
             if (C::P_TMEM) {  // A = P_X from TMEM: 8 columns per 16 keys
               umma_bf16_ts(tmem + C::TCOL_O + x * HD, tmem + C::TCOL_P + x * (BN / 2) + kk * 8, bd,
-                           IDESC_O, (j > f[x] || kk > 0) ? 1u : 0u);
+                           IDESC_O, (j > 0 || kk > 0) ? 1u : 0u);
             } else {
               const uint64_t ad = desc_at(dp, (kk >> 2) * (BM * 128) + (kk & 3) * 32);
-              umma_bf16_ss(tmem + C::TCOL_O + x * HD, ad, bd, IDESC_O, (j > f[x] || kk > 0) ? 1u : 0u);
+              umma_bf16_ss(tmem + C::TCOL_O + x * HD, ad, bd, IDESC_O, (j > 0 || kk > 0) ? 1u : 0u);
             }
           }
           umma_commit(BAR_PV(x));
@@ -507,18 +491,10 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         };
         auto wait_v = [&](int j) {
           const uint32_t v = vc + j;
-          if (!mbar_wait(BAR_VF(v % C::VST), (v / C::VST) & 1, abort_p)) return false;
-          if constexpr (WIN) {
-            if (un.fix(prm.win, un.key_tile(j) * BN)) {  // warp 2 has zeroed its unseen rows
-              const uint32_t vs = v % C::VST;
-              if (!mbar_wait(BAR_VZ(vs), (vzp >> vs) & 1, abort_p)) return false;
-              vzp ^= 1u << vs;
-            }
-          }
-          return true;
+          return mbar_wait(BAR_VF(v % C::VST), (v / C::VST) & 1, abort_p);
         };
         // prologue: S_A(0), S_B(0); K_0 is consumed once both are done
-        ok = wait_k(0) && issue_s(0, 0) && (!act(1, 0) || issue_s(1, 0));
+        ok = wait_k(0) && issue_s(0, 0) && (n[1] == 0 || issue_s(1, 0));
         if (ok) umma_commit(BAR_KE(kc % C::KST));
         // time-out test hook: with the first products in flight, wait on a
         // barrier nothing arrives at until the hook's limit runs out
@@ -529,13 +505,13 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
             // that), so the next scores are ready before this tile's softmax ends
             if (j + 1 < un.nkv) {
               if (!wait_k(j + 1)) { ok = false; break; }
-              if (act(0, j + 1) && !issue_s(0, j + 1)) { ok = false; break; }
-              if (act(1, j + 1) && !issue_s(1, j + 1)) { ok = false; break; }
+              if (j + 1 < n[0] && !issue_s(0, j + 1)) { ok = false; break; }
+              if (j + 1 < n[1] && !issue_s(1, j + 1)) { ok = false; break; }
               umma_commit(BAR_KE((kc + j + 1) % C::KST));  // K_{j+1} consumed
             }
             if (!wait_v(j)) { ok = false; break; }
-            if (act(0, j) && !issue_pv(0, j)) { ok = false; break; }
-            if (act(1, j) && !issue_pv(1, j)) { ok = false; break; }
+            if (j < n[0] && !issue_pv(0, j)) { ok = false; break; }
+            if (j < n[1] && !issue_pv(1, j)) { ok = false; break; }
           } else {
             // PV_A(j) S_A(j+1) | PV_B(j) S_B(j+1)
             if (!wait_v(j)) { ok = false; break; }
@@ -544,11 +520,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
               if (!issue_pv(0, j)) { ok = false; break; }
               if (!lastA && (!wait_k(j + 1) || !issue_s(0, j + 1))) { ok = false; break; }
             }
-            if constexpr (WIN) {
-              // B may start one tile after A (skip), so its next S does not hang on its PV
-              if (act(1, j) && !issue_pv(1, j)) { ok = false; break; }
-              if (act(1, j + 1) && ((lastA && !wait_k(j + 1)) || !issue_s(1, j + 1))) { ok = false; break; }
-            } else if (j < n[1]) {
+            if (j < n[1]) {
               if (!issue_pv(1, j)) { ok = false; break; }
               if (j + 1 < n[1] && ((lastA && !wait_k(j + 1)) || !issue_s(1, j + 1))) { ok = false; break; }
             }
@@ -567,6 +539,109 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         umma_commit(BAR_FIN);
         mbar_wait_for(BAR_FIN, 0, kDrainLimitNs);
       }
+    } else if (WIN && warp == 1 && lane == 0) {
+      // ---------------------------------------------------- S, under a window
+      // S_X(j) = Q_X K_j^T, as soon as softmax X has read S_X(j-1).  Another
+      // warp issues the products with V, so neither waits for the other's tile.
+      if constexpr (WIN) {
+        constexpr uint32_t IDESC_S = idesc_bf16_f32(BM, BN, 0, 0);
+        constexpr uint32_t IDESC_SN = idesc_bf16_f32(BM, NARROW, 0, 0);
+        uint32_t qc = 0, kc = 0, sc[2] = {0, 0};
+        bool ok = true;
+        for (int g = 0; ok; ++g) {
+          const int k = sched_unit<false>(sch, g);
+          if (k < 0) break;
+          const auto un = unit(k);
+          if (un.nkv == 0) continue;  // only padding
+          const int qs = qc % C::QST;
+          if (!mbar_poll(BAR_QF(qs), (qc / C::QST) & 1, abort_p)) break;
+          for (int j = 0; ok && j < un.nkv; ++j, ++kc) {
+            const int ks = kc % C::KST;
+            ok = mbar_poll(BAR_KF(ks), (kc / C::KST) & 1, abort_p);
+            const uint32_t idesc = un.narrow(prm.win, j) ? IDESC_SN : IDESC_S;
+            const uint32_t dk = desc_lo(sbase + C::OFF_K + ks * C::KV_BYTES, 16);
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              if (!ok || !un.active(x, j)) continue;
+              if (sc[x] >= 1 && !mbar_poll(BAR_SE(x), (sc[x] - 1) & 1, abort_p)) {
+                ok = false;
+                continue;
+              }
+              tc_fence_after();
+              const uint32_t dq = desc_lo(sbase + C::OFF_Q + (qs * 2 + x) * C::QT_BYTES, 16);
+#pragma unroll
+              for (int kk = 0; kk < HD / 16; ++kk) {
+                const uint32_t off = ((kk >> 2) * (BM * 128) + (kk & 3) * 32) >> 4;
+                umma_bf16_ss_lo(tmem + C::TCOL_S + x * BN, dq + off, dk + off, idesc, kk > 0 ? 1u : 0u);
+              }
+              umma_commit(BAR_SF(x));
+              ++sc[x];
+            }
+            if (ok) umma_commit(BAR_KE(ks));
+          }
+          if (ok) umma_commit(BAR_QE(qs));
+          ++qc;
+        }
+        if (*abort_p) {  // wind-down: every UMMA issued must complete before TMEM is freed
+          umma_commit(BAR_FIN);
+          mbar_wait_for(BAR_FIN, 0, kDrainLimitNs);
+        }
+      }
+    } else if (WIN && warp == 3 && lane == 0) {
+      // --------------------------------------------------- PV, under a window
+      // O_X += P_X V_j, once softmax X has written P_X(j)
+      if constexpr (WIN) {
+        constexpr uint32_t IDESC_O = idesc_bf16_f32(BM, HD, 0, 1);
+        uint32_t vc = 0, pvc[2] = {0, 0}, uc[2] = {0, 0};
+        uint32_t vzp = 0;  // bit s = parity of v_fixed[s]'s next phase
+        bool ok = true;
+        for (int g = 0; ok; ++g) {
+          const int k = sched_unit<false>(sch, g);
+          if (k < 0) break;
+          const auto un = unit(k);
+          for (int j = 0; ok && j < un.nkv; ++j, ++vc) {
+            const int vs = vc % C::VST;
+            ok = mbar_poll(BAR_VF(vs), (vc / C::VST) & 1, abort_p);
+            if (ok && un.fix(prm.win, un.key_tile(j) * BN)) {  // warp 2 has zeroed its unseen rows
+              ok = mbar_poll(BAR_VZ(vs), (vzp >> vs) & 1, abort_p);
+              vzp ^= 1u << vs;
+            }
+            const bool narrow = un.narrow(prm.win, j);
+            const uint32_t dv = desc_lo(sbase + C::OFF_V + vs * C::KV_BYTES, BN * 128);
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              if (!ok || !un.active(x, j)) continue;
+              const bool first = j == un.first(x);
+              ok = mbar_poll(BAR_PF(x), pvc[x] & 1, abort_p);
+              // the tile's previous unit has been read out of O_X
+              if (ok && first && uc[x] >= 1) ok = mbar_poll(BAR_OE(x), (uc[x] - 1) & 1, abort_p);
+              if (!ok) continue;
+              tc_fence_after();
+              const uint32_t dp = desc_lo(sbase + C::OFF_P + x * C::STG_BYTES, 16);
+#pragma unroll
+              for (int kk = 0; kk < BN / 16; ++kk) {
+                if (narrow && kk >= NARROW / 16) break;
+                const uint32_t acc = !first || kk > 0 ? 1u : 0u;
+                if (C::P_TMEM)  // A = P_X from TMEM: 8 columns per 16 keys
+                  umma_bf16_ts_lo(tmem + C::TCOL_O + x * HD, tmem + C::TCOL_P + x * (BN / 2) + kk * 8,
+                                  dv + kk * (2048 >> 4), IDESC_O, acc);
+                else
+                  umma_bf16_ss_lo(tmem + C::TCOL_O + x * HD, dp + (((kk >> 2) * (BM * 128) + (kk & 3) * 32) >> 4),
+                                  dv + kk * (2048 >> 4), IDESC_O, acc);
+              }
+              umma_commit(BAR_PV(x));
+              ++pvc[x];
+            }
+            if (ok) umma_commit(BAR_VE(vs));
+          }
+          if (un.nA > 0) ++uc[0];
+          if (un.nB > 0) ++uc[1];
+        }
+        if (*abort_p) {
+          umma_commit(BAR_FIN2);
+          mbar_wait_for(BAR_FIN2, 0, kDrainLimitNs);
+        }
+      }
     } else if (WIN && warp == 2) {
       // ------------------------------------------------ unseen rows of V
       if constexpr (WIN) {
@@ -581,7 +656,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
             // within one phase of each slot's barriers
             const int k0 = un.key_tile(j) * BN;
             const uint32_t v = vc + j, vs = v % C::VST;
-            ok = mbar_wait_warp(BAR_VF(vs), (v / C::VST) & 1, abort_p);
+            ok = wait_on_warp<WIN>(BAR_VF(vs), (v / C::VST) & 1, abort_p);
             if (!ok) break;
             if (!un.fix(prm.win, k0)) {
               if (lane == 0) mbar_arrive(BAR_VE(vs));
@@ -694,7 +769,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
                           un.b);
           }
         }
-        if (!mbar_wait_warp(BAR_SF(x), sc & 1, abort_p)) return false;
+        if (!wait_on_warp<WIN>(BAR_SF(x), sc & 1, abort_p)) return false;
         tc_fence_after();
         float s[NC];
         if constexpr (NC == 32) {
@@ -787,7 +862,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         // PV_X(j-1) must be complete before O_X is rescaled and before P_X(j)
         // overwrites P_X (waited for only now, so the exponentials overlap it)
         if (!first) {
-          if (!mbar_wait_warp(BAR_PV(x), (sc - 1) & 1, abort_p)) return false;
+          if (!wait_on_warp<WIN>(BAR_PV(x), (sc - 1) & 1, abort_p)) return false;
           tc_fence_after();
         }
         if (rescale) {
@@ -841,7 +916,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         }
       }
       // --------------------------------------------- epilogue of tile X
-      const bool epi = ok && mbar_wait_warp(BAR_PV(x), (sc - 1) & 1, abort_p);
+      const bool epi = ok && wait_on_warp<WIN>(BAR_PV(x), (sc - 1) & 1, abort_p);
       if constexpr (C::P_TMEM) {
         // without dO the epilogue is the staging's first writer in this unit
         // (with dO the warpgroup waits for the dO load, issued after the wait)
@@ -858,7 +933,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         if constexpr (WIN) valid = grow < un.n;
         const bool fuse_d = C::P_TMEM && !WIN && prm.dO;
         bool dok = true;
-        if (fuse_d) dok = mbar_wait_warp(BAR_DO(x), nd & 1, abort_p);
+        if (fuse_d) dok = wait_on_warp<WIN>(BAR_DO(x), nd & 1, abort_p);
         float dsum = 0.0f;
         // stage O (bf16) in this tile's P buffer (free: its last PV is done);
         // O is read from TMEM 64 columns (two loads, one wait) at a time

@@ -154,6 +154,15 @@ __device__ __forceinline__ bool mbar_poll_warp(uint32_t bar, uint32_t parity, vo
   return __all_sync(0xffffffffu, mbar_poll(bar, parity, abort));
 }
 
+template <bool SHORT>
+__device__ __forceinline__ bool wait_on(uint32_t bar, uint32_t parity, volatile int* abort) {
+  return SHORT ? mbar_poll(bar, parity, abort) : mbar_wait(bar, parity, abort);
+}
+template <bool SHORT>
+__device__ __forceinline__ bool wait_on_warp(uint32_t bar, uint32_t parity, volatile int* abort) {
+  return SHORT ? mbar_poll_warp(bar, parity, abort) : mbar_wait_warp(bar, parity, abort);
+}
+
 // Named barrier `id` over `nthreads` threads that also returns the AND of
 // every participant's `v` (bar.red.and.pred), so a group can agree on a flag.
 __device__ __forceinline__ bool bar_red_and(uint32_t id, uint32_t nthreads, bool v) {
