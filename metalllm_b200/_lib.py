@@ -101,6 +101,7 @@ SIGNATURES = {
 }
 
 _lib = None
+_fns: dict = {}  # entry points called so far
 
 
 def load() -> ctypes.CDLL:
@@ -127,8 +128,10 @@ def load() -> ctypes.CDLL:
 
 def call(name: str, *args) -> None:
     """Calls an entry point and raises MetalAttnError on a non-zero status."""
-    lib = load()
-    rc = getattr(lib, name)(*args)
+    fn = _fns.get(name)
+    if fn is None:
+        fn = _fns[name] = getattr(load(), name)
+    rc = fn(*args)
     if rc != MA_OK:
-        msg = lib.ma_last_error_string().decode(errors="replace")
+        msg = load().ma_last_error_string().decode(errors="replace")
         raise MetalAttnError(rc, msg, name)

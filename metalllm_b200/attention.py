@@ -24,6 +24,7 @@ batches (lens, int32 [B]: rows from lens[b] on are padding).
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 from typing import Optional
 
@@ -333,13 +334,16 @@ def _groups(p: AttentionParams, NKV: Optional[int]) -> int:
 
 
 def _check_all(*specs) -> None:
-    """_check for each (tensor, name, dtype, shape), and for each (tensor,
-    name, dtype, shape, True) that is not None."""
+    """_check for each (tensor, name, dtype, shape)."""
     cur = torch.cuda.current_device() if torch.cuda.is_initialized() else -1
-    for t, name, dtype, shape, *optional in specs:
-        if type(t) is torch.Tensor and t.dtype is dtype and t.shape == shape and t.is_contiguous() and t.is_cuda and \
-                t.get_device() == cur or (t is None and optional):
-            continue
+    for t, name, dtype, shape in specs:
+        if not (type(t) is torch.Tensor and t.dtype is dtype and t.shape == shape and t.is_contiguous()
+                and t.get_device() == cur and t.is_cuda):
+            _check(t, name, dtype, shape)
+
+
+def _check_optional(t: Optional[torch.Tensor], name: str, dtype: torch.dtype, shape: tuple) -> None:
+    if t is not None:
         _check(t, name, dtype, shape)
 
 
@@ -347,7 +351,7 @@ def _rotary(inv_freq: torch.Tensor, NKV: int, interleaved: bool, amplitude: floa
     if not isinstance(inv_freq, torch.Tensor) or inv_freq.dim() != 1:
         raise TypeError("inv_freq must be a one-dimensional tensor (rotaryFrequencies)")
     _check(inv_freq, "inv_freq", torch.float64, inv_freq.shape)
-    return _lib.Rotary(inv_freq.data_ptr(), 2 * inv_freq.numel(), bool(interleaved), NKV, amplitude)
+    return _lib.Rotary(inv_freq.data_ptr(), 2 * inv_freq.shape[0], bool(interleaved), NKV, amplitude)
 
 
 def _u32(x: int, name: str) -> int:
@@ -360,11 +364,26 @@ def _window(window: int, sinks: int, NKV: int) -> _lib.Window:
     return _lib.Window(NKV, _u32(window, "window"), _u32(sinks, "sinks"))
 
 
-def _workspace(like: torch.Tensor, stream: Optional[torch.cuda.Stream], name: str, *args):
-    """Device memory of the size that entry point `name` gives, for a call on `stream`."""
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(M: int, D: int, NH: int, NKV: int, window: int, sinks: int, B: int, dq_f32: int,
+                     cap: Optional[int]) -> int:
+    """Bytes of workspace of a backward (cap None) or of a call over a cache."""
     need = ctypes.c_uint64()
-    _lib.call(name, *args, ctypes.byref(need))
-    ws = torch.empty(need.value, dtype=torch.uint8, device=like.device)
+    w, p = ctypes.byref(_lib.Window(NKV, window, sinks)), ctypes.byref(make_params(M, NH, D))
+    if cap is None:
+        _lib.call("ma_windowAttentionBackward_workspace", dq_f32, w, p, B, ctypes.byref(need))
+    else:
+        _lib.call("ma_windowAttentionCached_workspace", w, p, B, cap, ctypes.byref(need))
+    return need.value
+
+
+def _workspace(like: torch.Tensor, stream: Optional[torch.cuda.Stream], p: AttentionParams, w: _lib.Window, B: int,
+               dq_f32: int = 0, cap: Optional[int] = None) -> Optional[torch.Tensor]:
+    """Device memory for a call on `stream`, or None where it needs none."""
+    need = _workspace_bytes(p.M, p.D, p.NH, w.NKV, w.window, w.sinks, B, dq_f32, cap)
+    if need == 0:
+        return None
+    ws = torch.empty(need, dtype=torch.uint8, device=like.device)
     if stream is not None and stream != torch.cuda.current_stream():
         ws.record_stream(stream)  # freed on return, while `stream` may still be using it
     return ws
@@ -382,8 +401,8 @@ def rotaryForward(q: torch.Tensor, k: torch.Tensor, inv_freq: torch.Tensor, p: A
     NKV = _groups(p, NKV)
     r = _rotary(inv_freq, NKV, interleaved, amplitude)
     qs, ks = (B, p.M, p.N), (B, p.M, NKV * p.D)
-    _check_all((q, "q", torch.bfloat16, qs), (k, "k", torch.bfloat16, ks),
-               (positions, "positions", torch.int32, (B, p.M), True))
+    _check_all((q, "q", torch.bfloat16, qs), (k, "k", torch.bfloat16, ks))
+    _check_optional(positions, "positions", torch.int32, (B, p.M))
     q_out = _out(q_out, q, qs, torch.bfloat16, "q_out")
     k_out = _out(k_out, k, ks, torch.bfloat16, "k_out")
     _lib.call("ma_rotaryForward", _ptr(q), _ptr(k), _ptr(q_out), _ptr(k_out), ctypes.byref(r), _ptr(positions),
@@ -402,7 +421,8 @@ def rotaryBackward(dQ: torch.Tensor, dK: torch.Tensor, inv_freq: torch.Tensor, p
     r = _rotary(inv_freq, NKV, interleaved, amplitude)
     qs, ks = (B, p.M, p.N), (B, p.M, NKV * p.D)
     t = torch.float32 if isinstance(dQ, torch.Tensor) and dQ.dtype == torch.float32 else torch.bfloat16
-    _check_all((dQ, "dQ", t, qs), (dK, "dK", torch.bfloat16, ks), (positions, "positions", torch.int32, (B, p.M), True))
+    _check_all((dQ, "dQ", t, qs), (dK, "dK", torch.bfloat16, ks))
+    _check_optional(positions, "positions", torch.int32, (B, p.M))
     dQ_out = _out(dQ_out, dQ, qs, t, "dQ_out")
     dK_out = _out(dK_out, dK, ks, torch.bfloat16, "dK_out")
     _lib.call("ma_rotaryBackward", _ptr(dQ), _ptr(dK), _ptr(dQ_out), _ptr(dK_out), int(t == torch.float32),
@@ -432,7 +452,8 @@ def rotaryCacheAppend(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache
     cs = (B, cap, NKV * p.D)
     _check_all((q, "q", torch.bfloat16, qs), (k, "k", torch.bfloat16, ks), (v, "v", torch.bfloat16, ks),
                (k_cache, "k_cache", torch.bfloat16, cs), (v_cache, "v_cache", torch.bfloat16, cs),
-               (start, "start", torch.int32, (B,)), (lens, "lens", torch.int32, (B,), True))
+               (start, "start", torch.int32, (B,)))
+    _check_optional(lens, "lens", torch.int32, (B,))
     q_out = _out(q_out, q, qs, torch.bfloat16, "q_out")
     _lib.call("ma_rotaryCacheAppend", _ptr(q), _ptr(k), _ptr(v), _ptr(q_out), _ptr(k_cache), _ptr(v_cache),
               _ptr(start), _ptr(lens), ctypes.byref(r), ctypes.byref(p), B, cap, _stream(stream))
@@ -449,8 +470,8 @@ def windowAttentionForward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, p:
     NKV = _groups(p, NKV)
     w = _window(window, sinks, NKV)
     qs, ks = (B, p.M, p.N), (B, p.M, NKV * p.D)
-    _check_all((q, "q", torch.bfloat16, qs), (k, "k", torch.bfloat16, ks), (v, "v", torch.bfloat16, ks),
-               (lens, "lens", torch.int32, (B,), True))
+    _check_all((q, "q", torch.bfloat16, qs), (k, "k", torch.bfloat16, ks), (v, "v", torch.bfloat16, ks))
+    _check_optional(lens, "lens", torch.int32, (B,))
     out = _out(out, q, qs, torch.bfloat16, "out")
     l = _out(l, q, (B, p.M, p.NH), torch.float32, "l")
     _lib.call("ma_windowAttentionForward", _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(l), _ptr(lens),
@@ -472,8 +493,8 @@ def windowAttentionBackward(dO: torch.Tensor, out: torch.Tensor, l: torch.Tensor
     w = _window(window, sinks, NKV)
     qs, ks = (B, p.M, p.N), (B, p.M, NKV * p.D)
     _check_all((dO, "dO", torch.bfloat16, qs), (out, "out", torch.bfloat16, qs), (q, "q", torch.bfloat16, qs),
-               (l, "l", torch.float32, (B, p.M, p.NH)), (k, "k", torch.bfloat16, ks), (v, "v", torch.bfloat16, ks),
-               (lens, "lens", torch.int32, (B,), True))
+               (l, "l", torch.float32, (B, p.M, p.NH)), (k, "k", torch.bfloat16, ks), (v, "v", torch.bfloat16, ks))
+    _check_optional(lens, "lens", torch.int32, (B,))
     if dQ_dtype is None:
         dQ_dtype = dQ.dtype if isinstance(dQ, torch.Tensor) else torch.float32
     if dQ_dtype not in (torch.float32, torch.bfloat16):
@@ -482,7 +503,7 @@ def windowAttentionBackward(dO: torch.Tensor, out: torch.Tensor, l: torch.Tensor
     dQ = _out(dQ, q, qs, dQ_dtype, "dQ")
     dK = _out(dK, k, ks, torch.bfloat16, "dK")
     dV = _out(dV, k, ks, torch.bfloat16, "dV")
-    ws = _workspace(q, stream, "ma_windowAttentionBackward_workspace", f32, ctypes.byref(w), ctypes.byref(p), B)
+    ws = _workspace(q, stream, p, w, B, dq_f32=f32)
     _lib.call("ma_windowAttentionBackward", _ptr(dO), _ptr(out), _ptr(l), _ptr(q), _ptr(k), _ptr(v), _ptr(dQ),
               _ptr(dK), _ptr(dV), f32, _ptr(lens), ctypes.byref(w), ctypes.byref(p), B, _ptr(ws), ws.numel(),
               _stream(stream))
@@ -503,13 +524,14 @@ def windowAttentionCached(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch
     qs, cap = (B, p.M, p.N), _cap(k_cache, "k_cache")
     cs = (B, cap, NKV * p.D)
     _check_all((q, "q", torch.bfloat16, qs), (k_cache, "k_cache", torch.bfloat16, cs),
-               (v_cache, "v_cache", torch.bfloat16, cs), (start, "start", torch.int32, (B,)),
-               (lens, "lens", torch.int32, (B,), True))
+               (v_cache, "v_cache", torch.bfloat16, cs), (start, "start", torch.int32, (B,)))
+    _check_optional(lens, "lens", torch.int32, (B,))
     out = _out(out, q, qs, torch.bfloat16, "out")
     l = _out(l, q, (B, p.M, p.NH), torch.float32, "l")
-    ws = _workspace(q, stream, "ma_windowAttentionCached_workspace", ctypes.byref(w), ctypes.byref(p), B, cap)
+    ws = _workspace(q, stream, p, w, B, cap=cap)
     _lib.call("ma_windowAttentionCached", _ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(out), _ptr(l), _ptr(start),
-              _ptr(lens), ctypes.byref(w), ctypes.byref(p), B, cap, _ptr(ws), ws.numel(), _stream(stream))
+              _ptr(lens), ctypes.byref(w), ctypes.byref(p), B, cap, _ptr(ws), 0 if ws is None else ws.numel(),
+              _stream(stream))
     return out, l
 
 

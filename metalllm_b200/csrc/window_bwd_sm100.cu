@@ -371,8 +371,12 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   __syncthreads();
   tc_fence_after();
   // nothing before here touches global memory, so the barriers and TMEM are set
-  // up while the kernel before is still draining
-  pdl_wait_and_release();
+  // up while the kernel before is still draining.  The dQ pass does not wait
+  // for the dK/dV pass before it at all, which shares nothing with it but
+  // inputs: it may start once that pass's last blocks have, each of which has
+  // waited for the statistics, and fills the SMs that they leave idle.
+  if constexpr (DQ) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  else pdl_wait_and_release();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(gbase + C::OFF_TSLOT);
   volatile int* abort_p = &abort_flag;
   const Ring ring{Sched{sbase + C::OFF_SCHED, BAR_U, BAR_U + 8u * kSchedSlots, abort_p},
@@ -705,6 +709,9 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
+  // what follows the dQ pass waits for it, and so must not find the dK/dV pass
+  // still running
+  if constexpr (DQ) asm volatile("griddepcontrol.wait;" ::: "memory");
   if (threadIdx.x == 0 && abort_flag) atomicOr(prm.status, STATUS_BWD_TIMEOUT);
 }
 
@@ -754,14 +761,14 @@ __device__ __forceinline__ float dot8(uint4 a, uint4 b) {
 
 // The statistics -l*log2e and -(dO . O)/sqrt(D), [B][NH][rows] (0 for padding
 // and past the end).  HBM-bound: dO and O read once.  A warp takes 32 rows of a
-// head, D/8 lanes a row with 16-byte loads, 8 rows of a lane in flight, and
-// writes 32 neighbouring statistics.
+// head, D/8 lanes a row with 16-byte loads, all of them in flight, and writes
+// 32 neighbouring statistics.
 template <int HD>
 __global__ void __launch_bounds__(256) window_stats_kernel(const WindowArgs a, const __nv_bfloat16* __restrict__ dO,
                                                            float* __restrict__ neg_l, float* __restrict__ neg_d,
                                                            int rows) {
   pdl_wait_and_release();
-  constexpr int G = HD / 8, RPI = 32 / G, N = 8;  // lanes a row, rows an instruction, loads in flight
+  constexpr int G = HD / 8, RPI = 32 / G, N = 32 / RPI;  // lanes a row, rows an instruction, loads in flight
   const int lane = threadIdx.x % 32;
   const int tiles = rows / 32;
   const long long items = (long long)a.B * tiles * a.NH;
