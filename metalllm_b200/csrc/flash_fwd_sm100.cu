@@ -452,11 +452,11 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
           tc_fence_after();
           const uint32_t sq = sbase + C::OFF_Q + (qs * 2 + x) * C::QT_BYTES;
           const uint32_t sk = sbase + C::OFF_K + ((kc + j) % C::KST) * C::KV_BYTES;
-          const uint64_t dq = smem_desc_sw128(sq, 16, 1024), dk = smem_desc_sw128(sk, 16, 1024);
 #pragma unroll
           for (int kk = 0; kk < HD / 16; ++kk) {
             const uint32_t off = (kk >> 2) * (BM * 128) + (kk & 3) * 32;
-            umma_bf16_ss(tmem + C::TCOL_S + x * BN, desc_at(dq, off), desc_at(dk, off), IDESC_S, kk > 0 ? 1u : 0u);
+            umma_bf16_ss(tmem + C::TCOL_S + x * BN, smem_desc_sw128(sq + off, 16, 1024),
+                         smem_desc_sw128(sk + off, 16, 1024), IDESC_S, kk > 0 ? 1u : 0u);
           }
           umma_commit(BAR_SF(x));
           ++sc[x];
@@ -469,15 +469,14 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
           tc_fence_after();
           const uint32_t sp = sbase + C::OFF_P + x * C::STG_BYTES;
           const uint32_t sv = sbase + C::OFF_V + ((vc + j) % C::VST) * C::KV_BYTES;
-          const uint64_t dv = smem_desc_sw128(sv, BN * 128, 1024), dp = smem_desc_sw128(sp, 16, 1024);
 #pragma unroll
           for (int kk = 0; kk < BN / 16; ++kk) {
-            const uint64_t bd = desc_at(dv, kk * 2048);
+            const uint64_t bd = smem_desc_sw128(sv + kk * 2048, BN * 128, 1024);
             if (C::P_TMEM) {  // A = P_X from TMEM: 8 columns per 16 keys
               umma_bf16_ts(tmem + C::TCOL_O + x * HD, tmem + C::TCOL_P + x * (BN / 2) + kk * 8, bd,
                            IDESC_O, (j > 0 || kk > 0) ? 1u : 0u);
             } else {
-              const uint64_t ad = desc_at(dp, (kk >> 2) * (BM * 128) + (kk & 3) * 32);
+              const uint64_t ad = smem_desc_sw128(sp + (kk >> 2) * (BM * 128) + (kk & 3) * 32, 16, 1024);
               umma_bf16_ss(tmem + C::TCOL_O + x * HD, ad, bd, IDESC_O, (j > 0 || kk > 0) ? 1u : 0u);
             }
           }

@@ -414,11 +414,6 @@ __device__ __forceinline__ uint64_t smem_desc_sw128(uint32_t addr, uint32_t lbo,
   return d;
 }
 
-// The descriptor of an operand `bytes` further on (a multiple of 16; shared
-// memory's addresses do not reach the field's end, so it is one addition
-// where encoding anew takes a dozen instructions of the one issuing thread).
-__device__ __forceinline__ uint64_t desc_at(uint64_t desc, uint32_t bytes) { return desc + (bytes >> 4); }
-
 // The same operands by the low word of their descriptors: the high word of a
 // 128-byte-swizzled operand with 1024 bytes between its 8-row groups is a
 // constant, so one 32-bit addition and no second register moves an operand on.
