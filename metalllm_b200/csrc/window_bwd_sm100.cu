@@ -126,8 +126,8 @@ struct Params {
 // What one unit does.  (48 bytes: passed on through shared memory.)
 struct alignas(16) Unit {
   int b, tile, head;  // the resident tiles: rows tile*128.., head `head`
-  int nq;             // steps
-  int n;              // valid rows of the sequence; 0: everything is masked
+  int nq;             // steps; 0: no valid row, zeros are stored
+  int n;              // valid rows of the sequence
   int first, count;   // dK/dV: query tiles first .. first+count-1, for each head
                       // dQ: list index j < count is sink tile j, else tile first + j - count
   int head0;          // head of the streamed tiles at step 0
@@ -186,11 +186,7 @@ __device__ __forceinline__ Unit decode_dkv(const Params& p, int k) {
   else if (split || k0 >= p.sinks) end = min(last, win_last);
   u.count = end - u.first + 1;
   u.nq = u.count * p.G;
-  if (u.count <= 0 || u.n <= k0) {  // no valid row: one step, in which all is masked
-    u.n = 0;
-    u.first = u.tile;
-    u.count = u.nq = 1;
-  }
+  if (u.count <= 0 || u.n <= k0) u.n = u.nq = 0;  // no valid row
   return u;
 }
 
@@ -209,10 +205,7 @@ __device__ __forceinline__ Unit decode_dq(const Params& p, int k) {
   u.first = max(0, q0 - p.window + 1) / BT;
   u.count = min(p.sinks / BT + (p.sinks % BT != 0), u.first);
   u.nq = u.count + u.tile - u.first + 1;
-  if (q0 >= u.n) {  // only padding
-    u.n = 0;
-    u.nq = 1;
-  }
+  if (q0 >= u.n) u.n = u.nq = 0;  // only padding
   return u;
 }
 
@@ -221,8 +214,9 @@ struct Step {
   Unit u;
   int i;       // step within the unit
   uint32_t t;  // step over all units
-  uint32_t uc; // unit counter
+  uint32_t uc; // unit with steps
   bool valid;
+  uint32_t nreq;  // the producer: launch-control requests issued (request r names unit r + 1)
 };
 
 // The units of a CTA as its producer passes them on: unit 0 in descriptor slot
@@ -269,6 +263,7 @@ __device__ __forceinline__ Step before_first() {
   s.u.nq = 1;
   s.t = s.uc = ~0u;
   s.valid = false;
+  s.nreq = 0;
   return s;
 }
 
@@ -281,8 +276,11 @@ __device__ __forceinline__ bool advance(const Params& p, Step& s, const Ring& ri
   }
   s.i = 0;
   ++s.uc;
-  s.valid = next_unit<DQ, WARP, PUBLISH>(p, s, ring);
-  return s.valid;
+  for (;;) {  // past units that only store zeros
+    s.valid = next_unit<DQ, WARP, PUBLISH>(p, s, ring);
+    if (!s.valid || s.u.nq > 0) return s.valid;
+    if (PUBLISH && !sched_request(ring.sched, s.nreq++)) return false;
+  }
 }
 
 // 64 fp32 columns of this lane's TMEM row
@@ -394,8 +392,9 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         tma_prefetch_desc(&tmR2);
         tma_prefetch_desc(&tmX1);
         tma_prefetch_desc(&tmX2);
-        uint32_t r_armed = 0, x1_armed = 0, x2_armed = 0, nreq = 0;
-        for (Step s = before_first(); advance<DQ, false, true>(prm, s, ring);) {
+        uint32_t r_armed = 0, x1_armed = 0, x2_armed = 0;
+        Step s = before_first();
+        while (advance<DQ, false, true>(prm, s, ring)) {
           if (s.i == 0) {
             const int rs = s.uc % C::RST, col = s.u.head * HD;
             if (s.uc >= C::RST && !mbar_poll(BAR_RE(rs), ((s.uc / C::RST) - 1) & 1, abort_p)) break;
@@ -421,13 +420,10 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
             tma_load_3d(sbase + C::OFF_X2 + s2 * C::TILE + kb * BT * 128, &tmX2, BAR_X2F(s2), col + kb * 64, row, s.u.b);
           // three steps before the unit's end (or at its start), ask for the
           // next unit
-          if (s.i == max(0, s.u.nq - 3)) {
-            if (!sched_request(ring.sched, nreq)) break;
-            ++nreq;
-          }
+          if (s.i == max(0, s.u.nq - 3) && !sched_request(ring.sched, s.nreq++)) break;
         }
         if (*abort_p) {  // wind-down: let the loads and the request still in flight land
-          sched_drain(ring.sched, nreq);
+          sched_drain(ring.sched, s.nreq);
           drain_ring(BAR_RF, C::RST, r_armed);
           drain_ring(BAR_X1F, C::X1ST, x1_armed);
           drain_ring(BAR_X2F, C::X2ST, x2_armed);
@@ -658,24 +654,29 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     const int row = (warp & 3) * 32 + lane;
     const uint32_t tl = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     Step s = before_first();
-    while (++s.uc, next_unit<DQ, true, false>(prm, s, ring)) {
-      if (!mbar_poll_warp(BAR_DONE, s.uc & 1, abort_p)) break;
-      tc_fence_after();
+    while (next_unit<DQ, true, false>(prm, s, ring)) {
+      const bool some = s.u.nq > 0;
+      if (some) {
+        if (!mbar_poll_warp(BAR_DONE, ++s.uc & 1, abort_p)) break;
+        tc_fence_after();
+      }
       const Unit& v = s.u;
       const int at = v.tile * BT + row;
       const bool valid = at < v.n;  // a padding row's sums are 0, whatever its own tile held
       constexpr int COLS = (DQ ? 1 : 2) * HD;
 #pragma unroll 1
       for (int cc = 0; cc < COLS; cc += 32) {
-        uint32_t r[32];
-        tmem_ld32(tl + C::TCOL_ACC + cc, r);
-        tmem_wait_ld_dep(r);
-        if (cc + 32 == COLS) {  // all read: the next unit may overwrite them
-          tc_fence_before();
-          mbar_arrive(BAR_ACC);
-        }
+        uint32_t r[32] = {};
+        if (some) {
+          tmem_ld32(tl + C::TCOL_ACC + cc, r);
+          tmem_wait_ld_dep(r);
+          if (cc + 32 == COLS) {  // all read: the next unit may overwrite them
+            tc_fence_before();
+            mbar_arrive(BAR_ACC);
+          }
 #pragma unroll
-        for (int j = 0; j < 32; ++j) r[j] = valid ? r[j] : 0u;
+          for (int j = 0; j < 32; ++j) r[j] = valid ? r[j] : 0u;
+        }
         const int which = cc / HD, col = cc % HD;
         float* f32 = nullptr;
         __nv_bfloat16* b16 = nullptr;
