@@ -38,7 +38,9 @@
 // the first row's window on, the tiles that every row sees whole carry no
 // masking code, and a tile in which some row sees nothing is allowed.  Warp 2
 // zeroes the rows of a V tile that no query may see (padding, a cache's rows
-// past the end or out of the window): P is 0 there, but 0 * NaN is not.
+// past the end or out of the window): P is 0 there, but 0 * NaN is not.  Warp 1
+// issues S and warp 3 PV.  SINGLE: a unit is one query tile, not a pair, and the
+// two softmax warpgroups share its key tiles (few units, long windows).
 //
 // Every mbarrier wait is bounded (about 2 s); on time-out the CTA sets an
 // abort flag that all roles poll, winds down, frees its TMEM and sets
@@ -101,13 +103,16 @@ struct FwdCfg {
   // (their query pairs share K/V in L2: C3 forward -4.6 %), one block at D=64
   // (C4: blocks of 8-32 heads measured 1-2 % slower)
   static constexpr int HB = (DYN && HD == 128) ? 16 : 0;
-  static constexpr uint32_t OFF_SCHED = OFF_ZT + ZT_BYTES;
+  // WIN: B's maximum and sum of each row, for A to join
+  static constexpr uint32_t OFF_ML = OFF_ZT + ZT_BYTES;
+  static constexpr uint32_t ML_BYTES = WIN ? BM * 8 : 0;
+  static constexpr uint32_t OFF_SCHED = OFF_ML + ML_BYTES;
   static constexpr uint32_t OFF_BAR = OFF_SCHED + NSCHED * 16;
   // q_full/empty[QST], k_full/empty[KST], v_full/empty[VST], per tile X:
   // s_full, s_free, p_full, pv_done, o_free, do_full; then never (nothing
   // arrives: the time-out test hook), fin (the UMMA issuer's wind-down),
-  // sched_full/empty[NSCHED] and, for WIN, v_fixed[VST] and a second fin
-  static constexpr int NBAR = 2 * QST + 2 * KST + 2 * VST + 2 * 6 + 2 + 2 * NSCHED + (WIN ? VST + 1 : 0);
+  // sched_full/empty[NSCHED] and, for WIN, v_fixed[VST], a second fin and b_done
+  static constexpr int NBAR = 2 * QST + 2 * KST + 2 * VST + 2 * 6 + 2 + 2 * NSCHED + (WIN ? VST + 2 : 0);
   static constexpr uint32_t OFF_TSLOT = OFF_BAR + NBAR * 8;
   static constexpr uint32_t SMEM_BYTES = OFF_TSLOT + 16 + 1024;  // + alignment slack
   static constexpr uint32_t TCOL_S = 0;     // S_A, S_B at columns 0, 128
@@ -133,7 +138,6 @@ struct FwdParams {
   float* dQz;
   uint32_t expire_ns;  // time-out test hook (ma_debug_expire_next_wait), 0 = off
   WindowArgs win;      // WIN only
-  bool single;         // WIN: a unit is one query tile (A), not a pair
 };
 
 // sum over 8 bf16 pairs of a[i] * b[i], fp32 (products of bf16 values are
@@ -193,8 +197,10 @@ __device__ __forceinline__ Unit decode_unit(const FwdParams& prm, int k) {
 // A unit under a window.  The key tiles it visits, by list index j: the sink
 // tiles 0 .. ns-1 before the window, then lo, lo+1, ...; tile A is active for
 // j < nA, tile B for j < nB except j == skip (the one tile that A's window
-// reaches and B's does not).
+// reaches and B's does not).  A unit of one query tile (single) works on it
+// with both: A takes the even list indices, B the odd ones, and A joins them.
 struct WinUnit : Unit {
+  bool single;
   int tile0; // query tile of A; B's is the next
   int n;     // valid rows of the sequence
   int ns, lo, skip;
@@ -203,9 +209,12 @@ struct WinUnit : Unit {
   bool cached;
 
   __device__ int key_tile(int j) const { return j < ns ? j : lo + (j - ns); }
-  __device__ bool active(int x, int j) const { return x == 0 ? j < nA : j < nB && j != skip; }
+  __device__ bool active(int x, int j) const {
+    if (single) return (j & 1) == x && j < nkv;
+    return x == 0 ? j < nA : j < nB && j != skip;
+  }
   // the first list index of a tile: its PV starts the sum
-  __device__ int first(int x) const { return x == 1 && skip == 0 ? 1 : 0; }
+  __device__ int first(int x) const { return x == 1 && (single || skip == 0) ? 1 : 0; }
   // only the sinks of this tile are visible, and they fill a quarter at most:
   // its products and exponentials stop there
   __device__ bool narrow(const WindowArgs& w, int j) const { return j < ns && w.sinks - j * BN <= NARROW; }
@@ -231,12 +240,13 @@ struct WinUnit : Unit {
   }
 };
 
-template <int HB>
+template <int HB, bool SINGLE>
 __device__ __forceinline__ WinUnit decode_win_unit(const FwdParams& prm, int k) {
   const WindowArgs& w = prm.win;
   WinUnit x;
   static_cast<Unit&>(x) = decode_unit<HB>(prm, k);
-  x.tile0 = prm.single ? x.pair : 2 * x.pair;
+  x.single = SINGLE;
+  x.tile0 = SINGLE ? x.pair : 2 * x.pair;
   x.n = w.len(x.b);
   x.cached = w.start != nullptr;
   x.nA = x.nB = x.nkv = x.ns = x.lo = 0;
@@ -246,8 +256,8 @@ __device__ __forceinline__ WinUnit decode_win_unit(const FwdParams& prm, int k) 
   const int r0 = x.tile0 * BM;
   if (r0 >= x.n) return x;
   const int nS = w.sinks / BN + (w.sinks % BN != 0);
-  const bool b = !prm.single && r0 + BM < x.n;
-  const int rB = min(r0 + BM, x.n - 1);
+  const bool b = !SINGLE && r0 + BM < x.n;
+  const int rB = SINGLE ? r0 : min(r0 + BM, x.n - 1);  // one tile: B's rows are A's
   x.t0A = w.pos(x.b, r0);
   x.t1A = w.pos(x.b, min(r0 + BM - 1, x.n - 1));
   x.t0B = w.pos(x.b, rB);
@@ -259,6 +269,7 @@ __device__ __forceinline__ WinUnit decode_win_unit(const FwdParams& prm, int k) 
   x.nB = b ? x.ns + x.t1B / BN - x.lo + 1 : 0;
   x.skip = b && loB > x.lo && x.lo >= nS ? x.ns : -1;
   x.nkv = b ? x.nB : x.nA;
+  if (SINGLE && x.nkv > 1) x.nB = x.nkv;
   return x;
 }
 
@@ -270,7 +281,7 @@ __device__ __forceinline__ int unit_of_round(const FwdParams& prm, int g) {
   return k < prm.nunits ? (int)k : -1;
 }
 
-template <int HD, bool DYN, bool WIN>
+template <int HD, bool DYN, bool WIN, bool SINGLE>
 __global__ void __launch_bounds__(NUM_THREADS, 1)
     flash_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                      const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmO,
@@ -306,13 +317,14 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   auto BAR_UE = [&](int s) { return barX + 8u * (14 + C::NSCHED + s); };  // response s read by all
   auto BAR_VZ = [&](int s) { return barX + 8u * (14 + 2 * C::NSCHED + s); };  // WIN: V slot s zeroed where it must be
   const uint32_t BAR_FIN2 = barX + 8u * (14 + 2 * C::NSCHED + C::VST);  // WIN: the PV issuer's wind-down
+  const uint32_t BAR_MG = BAR_FIN2 + 8;  // WIN: B's part of a shared tile is complete
   // dynamic schedule: unit g >= 1 of this CTA is the one launch-control
   // response g-1 names (requested by the TMA producer when it starts unit
   // g-1); readers: the producer, the UMMA issuer (WIN: both), the 8 softmax
   // warps and, for WIN, the warp that zeroes V rows
   constexpr uint32_t SCHED_READERS = WIN ? 12 : 10;
   auto unit = [&](int k) {
-    if constexpr (WIN) return decode_win_unit<C::HB>(prm, k);
+    if constexpr (WIN) return decode_win_unit<C::HB, SINGLE>(prm, k);
     else return decode_unit<C::HB>(prm, k);
   };
   const uint32_t tslot = sbase + C::OFF_TSLOT;
@@ -346,7 +358,10 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       mbar_init(BAR_UE(u), SCHED_READERS);
     }
     if constexpr (WIN)
+    {
       for (int s = 0; s <= C::VST; ++s) mbar_init(BAR_VZ(s), 1);  // and BAR_FIN2
+      mbar_init(BAR_MG, 128);
+    }
     fence_mbar_init();
   }
   if (warp == 1) {
@@ -396,7 +411,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         if constexpr (WIN) tile0 = un.tile0;
         const int qs = qc % C::QST;
         if (qc >= C::QST && !wait_on<WIN>(BAR_QE(qs), ((qc / C::QST) - 1) & 1, abort_p)) break;
-        const int ntile = un.nB > 0 ? 2 : 1;
+        int ntile = un.nB > 0 ? 2 : 1;
+        if (WIN && SINGLE) ntile = 1;
         mbar_arrive_expect_tx(BAR_QF(qs), ntile * C::QT_BYTES);
         for (int x = 0; x < ntile; ++x)
           for (int kb = 0; kb < C::KB; ++kb)
@@ -567,7 +583,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
                 continue;
               }
               tc_fence_after();
-              const uint32_t dq = desc_lo(sbase + C::OFF_Q + (qs * 2 + x) * C::QT_BYTES, 16);
+              const uint32_t dq = desc_lo(sbase + C::OFF_Q + (qs * 2 + (SINGLE ? 0 : x)) * C::QT_BYTES, 16);
 #pragma unroll
               for (int kk = 0; kk < HD / 16; ++kk) {
                 const uint32_t off = ((kk >> 2) * (BM * 128) + (kk & 3) * 32) >> 4;
@@ -698,6 +714,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     uint32_t sc = 0;  // S_X consumed so far (== P_X produced)
     uint32_t nd = 0;  // dO tiles of X consumed so far (fused computeD)
     uint32_t nd_armed = 0;  // dO tile loads issued (leader)
+    uint32_t nmg = 0;       // WIN, A: shared tiles joined so far
+    uint32_t scb = 0;       // WIN, A: key tiles B has worked on in them
     bool ok = true;
     for (int g = 0; ok; ++g) {
       int k;
@@ -708,9 +726,9 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       const int nt = x == 0 ? un.nA : un.nB;
       int qtile = 2 * un.pair + x;
       if constexpr (WIN) {
-        qtile = un.tile0 + x;
+        qtile = un.tile0 + (SINGLE ? 0 : x);
         if (nt == 0) {  // only padding: O = 0, l = -inf (rows past T are clipped)
-          if ((prm.single && x == 1) || qtile * BM >= prm.T) continue;
+          if ((SINGLE && x == 1) || qtile * BM >= prm.T) continue;
           if (wg_leader) bulk_wait_read<0>();
           bar_sync_named(wg_bar, 128);
           for (int kb = 0; kb < C::KB; ++kb)
@@ -915,13 +933,39 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         }
       }
       // --------------------------------------------- epilogue of tile X
-      const bool epi = ok && wait_on_warp<WIN>(BAR_PV(x), (sc - 1) & 1, abort_p);
+      bool epi = ok && wait_on_warp<WIN>(BAR_PV(x), (sc - 1) & 1, abort_p);
       if constexpr (C::P_TMEM) {
         // without dO the epilogue is the staging's first writer in this unit
         // (with dO the warpgroup waits for the dO load, issued after the wait)
         if (WIN || !prm.dO) {
           if (wg_leader) bulk_wait_read<0>();
           bar_sync_named(wg_bar, 128);
+        }
+      }
+      bool joined = false;
+      if constexpr (WIN) joined = SINGLE && un.nB > 0;
+      if (joined && x == 1) {
+        // this half's maximum and sum; O_B stays in TMEM, where A reads it
+        if (epi) {
+          reinterpret_cast<float2*>(gbase + C::OFF_ML)[row] = make_float2(m_used, l_sum);
+          tc_fence_before();
+          mbar_arrive(BAR_MG);
+        }
+        ok = bar_red_and(wg_bar, 128, epi);
+        continue;
+      }
+      float fa = 1.0f, fb = 0.0f;  // factors of O_A and O_B
+      if (joined) {
+        scb += un.nkv / 2;
+        epi = epi && wait_on_warp<WIN>(BAR_MG, nmg++ & 1, abort_p) &&
+              wait_on_warp<WIN>(BAR_PV(1), (scb - 1) & 1, abort_p);
+        if (epi) {
+          const float2 ml = reinterpret_cast<const float2*>(gbase + C::OFF_ML)[row];
+          const float top = fmaxf(m_used, ml.x), base = top == -INFINITY ? 0.0f : top;
+          fa = ex2(m_used - base);
+          fb = ex2(ml.x - base);
+          l_sum = l_sum * fa + ml.y * fb;
+          m_used = top;
         }
       }
       if (epi) {
@@ -942,6 +986,19 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
           tmem_ld32(trow + tcol_o + c64, ra);
           tmem_ld32(trow + tcol_o + c64 + 32, rb);
           tmem_wait_ld_dep(ra, rb);
+          if constexpr (WIN) {
+            if (joined) {
+              uint32_t rc[32], rd[32];
+              tmem_ld32(trow + C::TCOL_O + HD + c64, rc);
+              tmem_ld32(trow + C::TCOL_O + HD + c64 + 32, rd);
+              tmem_wait_ld_dep(rc, rd);
+              auto join = [&](uint32_t a, uint32_t b) {
+                return __float_as_uint(__uint_as_float(a) * fa + __uint_as_float(b) * fb);
+              };
+#pragma unroll
+              for (int i = 0; i < 32; ++i) ra[i] = join(ra[i], rc[i]), rb[i] = join(rb[i], rd[i]);
+            }
+          }
 #pragma unroll
           for (int c16 = 0; c16 < 64; c16 += 16) {
             const uint32_t* r = c16 < 32 ? ra + c16 : rb + (c16 - 32);
@@ -967,6 +1024,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         }
         tc_fence_before();
         mbar_arrive(BAR_OE(x));  // O_X may be overwritten by the next unit
+        if (joined) mbar_arrive(BAR_OE(1));
         fence_proxy_async_smem();
         if (grow < prm.T) {
           const long long ri = ((long long)un.b * prm.T + grow) * prm.NH + un.h;
@@ -1003,7 +1061,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
 
 // Launches the instantiation DYN (dynamic schedule: one CTA per unit, else
 // one per SM).
-template <int HD, bool DYN, bool WIN = false>
+template <int HD, bool DYN, bool WIN = false, bool SINGLE = false>
 cudaError_t launch_fwd_kernel(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
                               const CUtensorMap& to, const CUtensorMap& tdo, const CUtensorMap& tdqz,
                               const FwdParams& prm, cudaStream_t st) {
@@ -1012,12 +1070,12 @@ cudaError_t launch_fwd_kernel(const CUtensorMap& tq, const CUtensorMap& tk, cons
   // LAUNCH_REGS registers per thread; refuse to launch otherwise.
   static const cudaError_t reg_check = [] {
     cudaFuncAttributes a;
-    cudaError_t e = cudaFuncGetAttributes(&a, flash_fwd_kernel<HD, DYN, WIN>);
+    cudaError_t e = cudaFuncGetAttributes(&a, flash_fwd_kernel<HD, DYN, WIN, SINGLE>);
     if (e != cudaSuccess) return e;
     return a.numRegs == LAUNCH_REGS ? cudaSuccess : cudaErrorInvalidKernelImage;
   }();
   if (reg_check != cudaSuccess) return reg_check;
-  cudaError_t e = cudaFuncSetAttribute(flash_fwd_kernel<HD, DYN, WIN>,
+  cudaError_t e = cudaFuncSetAttribute(flash_fwd_kernel<HD, DYN, WIN, SINGLE>,
                                        cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES);
   if (e != cudaSuccess) return e;
   int grid = prm.nunits;  // dynamic: one CTA per unit (see decode_unit)
@@ -1027,7 +1085,7 @@ cudaError_t launch_fwd_kernel(const CUtensorMap& tq, const CUtensorMap& tk, cons
     cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
     grid = prm.nunits < sms ? prm.nunits : sms;
   }
-  launch_pdl(flash_fwd_kernel<HD, DYN, WIN>, grid, NUM_THREADS, C::SMEM_BYTES, st, tq, tk, tv, to, tdo, tdqz, prm);
+  launch_pdl(flash_fwd_kernel<HD, DYN, WIN, SINGLE>, grid, NUM_THREADS, C::SMEM_BYTES, st, tq, tk, tv, to, tdo, tdqz, prm);
   count_launches(1);
   return cudaGetLastError();
 }
@@ -1094,19 +1152,20 @@ cudaError_t launch_win(const WindowArgs& a, cudaStream_t st) {
   prm.nbh = a.B * a.NH;
   prm.nqt = (a.M + BM - 1) / BM;
   // pairs share their K/V tiles, but a few of them leave most SMs idle: then a
-  // unit is one tile (2 x 500 queries of 16 heads over a cache, 64 pairs or 128
-  // tiles for 148 SMs)
+  // unit is one tile, its keys shared by the two softmax warpgroups (2 x 500
+  // queries of 16 heads over a cache: 64 pairs or 128 tiles for 148 SMs)
   int dev = 0, sms = 148;
   cudaGetDevice(&dev);
   cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  prm.single = (long long)prm.nqt * prm.nbh <= sms;
-  prm.npairs = prm.single ? prm.nqt : (prm.nqt + 1) / 2;
+  const bool single = (long long)prm.nqt * prm.nbh <= sms;
+  prm.npairs = single ? prm.nqt : (prm.nqt + 1) / 2;
   prm.nunits = prm.npairs * prm.nbh;
   prm.scale_log2 = LOG2E / sqrtf((float)HD);
   prm.lse = a.l;
   prm.status = a.status;
   prm.win = a;
-  return launch_fwd_kernel<HD, true, true>(tq, tk, tv, to, tq, tq, prm, st);
+  return single ? launch_fwd_kernel<HD, true, true, true>(tq, tk, tv, to, tq, tq, prm, st)
+                : launch_fwd_kernel<HD, true, true>(tq, tk, tv, to, tq, tq, prm, st);
 }
 
 }  // namespace
