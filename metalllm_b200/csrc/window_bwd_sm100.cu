@@ -761,52 +761,51 @@ __device__ __forceinline__ float dot8(uint4 a, uint4 b) {
 }
 
 // The statistics -l*log2e and -(dO . O)/sqrt(D), [B][NH][rows] (0 for padding
-// and past the end).  HBM-bound: dO and O read once.  A warp takes 32 rows of a
-// head, D/8 lanes a row with 16-byte loads, all of them in flight, and writes
-// 32 neighbouring statistics.
+// and past the end).  HBM-bound: dO and O read once.  A warp takes 8 * 32 / (D/8)
+// rows of a head, D/8 lanes a row with 16-byte loads, all of them in flight, and
+// writes neighbouring statistics.
 template <int HD>
-__global__ void __launch_bounds__(256) window_stats_kernel(const WindowArgs a, const __nv_bfloat16* __restrict__ dO,
-                                                           float* __restrict__ neg_l, float* __restrict__ neg_d,
-                                                           int rows) {
+__global__ void __launch_bounds__(256, 2) window_stats_kernel(const WindowArgs a, const __nv_bfloat16* __restrict__ dO,
+                                                              float* __restrict__ neg_l, float* __restrict__ neg_d,
+                                                              int rows) {
   pdl_wait_and_release();
-  constexpr int G = HD / 8, RPI = 32 / G, N = 32 / RPI;  // lanes a row, rows an instruction, loads in flight
+  constexpr int G = HD / 8, RPI = 32 / G, N = 8, ROWS = N * RPI;  // lanes a row, rows an instruction, loads in flight
   const int lane = threadIdx.x % 32;
-  const int tiles = rows / 32;
+  const int tiles = rows / ROWS;
   const long long items = (long long)a.B * tiles * a.NH;
   for (long long it = blockIdx.x * 8ll + threadIdx.x / 32; it < items; it += gridDim.x * 8ll) {
     const int h = (int)(it % a.NH);
     const long long r = it / a.NH;
-    const int b = (int)(r / tiles), row0 = (int)(r % tiles) * 32;
+    const int b = (int)(r / tiles), row0 = (int)(r % tiles) * ROWS;
     const int n = a.len(b);
-    float mine = 0.0f;  // of row row0 + lane
-#pragma unroll 1
-    for (int i0 = 0; i0 < 32; i0 += N * RPI) {
-      uint4 x[N], y[N];
+    uint4 x[N], y[N];
 #pragma unroll
-      for (int k = 0; k < N; ++k) {
-        const int row = row0 + i0 + k * RPI + lane / G;
-        const long long off = (((long long)b * a.M + row) * a.NH + h) * HD;
-        x[k] = y[k] = make_uint4(0u, 0u, 0u, 0u);
-        if (row < n) {
-          x[k] = __ldcs(reinterpret_cast<const uint4*>(dO + off) + lane % G);
-          y[k] = __ldcs(reinterpret_cast<const uint4*>(a.out + off) + lane % G);
-        }
-      }
-#pragma unroll
-      for (int k = 0; k < N; ++k) {
-        const int i = i0 + k * RPI;
-        float s = dot8(x[k], y[k]);
-#pragma unroll
-        for (int m = G / 2; m >= 1; m >>= 1) s += __shfl_xor_sync(0xffffffffu, s, m);
-        const float got = __shfl_sync(0xffffffffu, s, (lane - i) * G & 31);
-        if (lane >= i && lane < i + RPI) mine = got;
+    for (int k = 0; k < N; ++k) {
+      const int row = row0 + k * RPI + lane / G;
+      const long long off = (((long long)b * a.M + row) * a.NH + h) * HD;
+      x[k] = y[k] = make_uint4(0u, 0u, 0u, 0u);
+      if (row < n) {
+        x[k] = __ldcs(reinterpret_cast<const uint4*>(dO + off) + lane % G);
+        y[k] = __ldcs(reinterpret_cast<const uint4*>(a.out + off) + lane % G);
       }
     }
-    const int row = row0 + lane;
-    const bool valid = row < n;
-    const long long at = ((long long)b * a.NH + h) * rows + row;
-    neg_l[at] = valid ? -a.l[((long long)b * a.M + row) * a.NH + h] * LOG2E : 0.0f;
-    neg_d[at] = valid ? -mine * a.scale : 0.0f;
+    float mine = 0.0f;  // of row row0 + lane
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const int i = k * RPI;
+      float s = dot8(x[k], y[k]);
+#pragma unroll
+      for (int m = G / 2; m >= 1; m >>= 1) s += __shfl_xor_sync(0xffffffffu, s, m);
+      const float got = __shfl_sync(0xffffffffu, s, (lane - i) * G & 31);
+      if (lane >= i && lane < i + RPI) mine = got;
+    }
+    if (lane < ROWS) {
+      const int row = row0 + lane;
+      const bool valid = row < n;
+      const long long at = ((long long)b * a.NH + h) * rows + row;
+      neg_l[at] = valid ? -a.l[((long long)b * a.M + row) * a.NH + h] * LOG2E : 0.0f;
+      neg_d[at] = valid ? -mine * a.scale : 0.0f;
+    }
   }
 }
 
@@ -869,7 +868,7 @@ cudaError_t launch_all(const WindowArgs& a, const WindowGrads& g, cudaStream_t s
   cudaGetDevice(&dev);
   cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
   auto blocks = [&](long long n, int per) { return (unsigned)std::min<long long>((n + per - 1) / per, sms * 16ll); };
-  launch_pdl(window_stats_kernel<HD>, blocks((long long)a.B * a.NH * (p.rows / 32), 8), 256, 0, st, a, g.dO, neg_l,
+  launch_pdl(window_stats_kernel<HD>, blocks((long long)a.B * a.NH * p.rows / (2048 / HD), 8), 256, 0, st, a, g.dO, neg_l,
              neg_d, p.rows);
   count_launches(1);
   cudaError_t e = cudaGetLastError();
