@@ -305,8 +305,8 @@ MA_API const char* ma_last_error_string(void);
 
 /* Bits of the status word read by ma_device_status: the kernels whose bounded
  * waits ran out. */
-#define MA_STATUS_FWD_TIMEOUT (1u << 0)  /* flashAttentionForward */
-#define MA_STATUS_BWD_TIMEOUT (1u << 1)  /* flashAttentionBackward */
+#define MA_STATUS_FWD_TIMEOUT (1u << 0)  /* flashAttentionForward, windowAttentionForward, windowAttentionCached */
+#define MA_STATUS_BWD_TIMEOUT (1u << 1)  /* flashAttentionBackward, windowAttentionBackward */
 #define MA_STATUS_QKV_TIMEOUT (1u << 2)  /* computeQKV */
 #define MA_STATUS_GEMM_TIMEOUT (1u << 3) /* the GEMMs around attention */
 
@@ -318,7 +318,8 @@ MA_API const char* ma_last_error_string(void);
 MA_API int ma_device_status(uint32_t* status, ma_stream_t stream);
 
 /* Test hook of the kernels' time-out path.  The next launch of each kernel
- * named in `kernels` (MA_STATUS_FWD_TIMEOUT and/or MA_STATUS_BWD_TIMEOUT) lets
+ * named in `kernels` (MA_STATUS_FWD_TIMEOUT and/or MA_STATUS_BWD_TIMEOUT, of
+ * the flashAttention* entry points) lets
  * one wait run out on purpose: once its first tensor-core products are in
  * flight, its UMMA-issuing thread waits on an mbarrier that nothing arrives
  * at, for `wait_ns` nanoseconds (1 .. 10^9).  The kernel then winds down as
@@ -385,7 +386,8 @@ MA_API int ma_attentionForwardBackward_host(ma_host_pipeline* pl, const ma_bf16*
  *   start            : int32 [B], rows a sequence's cache holds already, which
  *                      is the position of its first new row
  * lens and start are device arrays, whose values the host cannot check: lens
- * is clamped to [0, M] and start to [0, cap]. */
+ * is clamped to [0, M]; a row whose position lies outside the cache is not
+ * stored, and attention takes the position clamped to [0, cap). */
 
 /* Rotary positions: columns 0 .. rot-1 of each head turn in pairs, pair i of a
  * row at position t by the angle t * inv_freq[i], and are multiplied by
@@ -444,8 +446,8 @@ MA_API int ma_windowAttentionBackward(const ma_bf16* dO, const ma_bf16* out, con
                                       uint32_t dq_f32, const int32_t* lens, const MaWindow* w,
                                       const AttentionParams* p, uint32_t B, void* workspace,
                                       uint64_t workspace_bytes, ma_stream_t stream);
-MA_API int ma_windowAttentionBackward_workspace(uint32_t dq_f32, const MaWindow* w, const AttentionParams* p,
-                                                uint32_t B, uint64_t* bytes);
+MA_API int ma_windowAttentionBackward_workspace(const MaWindow* w, const AttentionParams* p, uint32_t B,
+                                                uint64_t* bytes);
 /* The forward for p->M >= 1 new tokens per sequence over a cache that already
  * holds their keys and values (ma_rotaryCacheAppend): row i is the query at
  * position start[b] + i and sees the cache's rows under the mask above.

@@ -92,7 +92,7 @@ SIGNATURES = {
     "ma_rotaryCacheAppend": [_P, _P, _P, _P, _P, _P, _P, _P, _PR, _PP, _U32, _U32, _P],
     "ma_windowAttentionForward": [_P, _P, _P, _P, _P, _P, _PW, _PP, _U32, _P],
     "ma_windowAttentionBackward": [_P, _P, _P, _P, _P, _P, _P, _P, _P, _U32, _P, _PW, _PP, _U32, _P, _U64, _P],
-    "ma_windowAttentionBackward_workspace": [_U32, _PW, _PP, _U32, ctypes.POINTER(_U64)],
+    "ma_windowAttentionBackward_workspace": [_PW, _PP, _U32, ctypes.POINTER(_U64)],
     "ma_windowAttentionCached": [_P, _P, _P, _P, _P, _P, _P, _PW, _PP, _U32, _U32, _P, _U64, _P],
     "ma_windowAttentionCached_workspace": [_PW, _PP, _U32, _U32, ctypes.POINTER(_U64)],
     "ma_device_status": [ctypes.POINTER(ctypes.c_uint32), _P],

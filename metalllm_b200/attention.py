@@ -365,28 +365,28 @@ def _window(window: int, sinks: int, NKV: int) -> _lib.Window:
 
 
 @functools.lru_cache(maxsize=256)
-def _workspace_bytes(M: int, D: int, NH: int, NKV: int, window: int, sinks: int, B: int, dq_f32: int,
+def _workspace_bytes(M: int, D: int, NH: int, NKV: int, window: int, sinks: int, B: int,
                      cap: Optional[int]) -> int:
     """Bytes of workspace of a backward (cap None) or of a call over a cache."""
     need = ctypes.c_uint64()
     w, p = ctypes.byref(_lib.Window(NKV, window, sinks)), ctypes.byref(make_params(M, NH, D))
     if cap is None:
-        _lib.call("ma_windowAttentionBackward_workspace", dq_f32, w, p, B, ctypes.byref(need))
+        _lib.call("ma_windowAttentionBackward_workspace", w, p, B, ctypes.byref(need))
     else:
         _lib.call("ma_windowAttentionCached_workspace", w, p, B, cap, ctypes.byref(need))
     return need.value
 
 
 def _workspace(like: torch.Tensor, stream: Optional[torch.cuda.Stream], p: AttentionParams, w: _lib.Window, B: int,
-               dq_f32: int = 0, cap: Optional[int] = None) -> Optional[torch.Tensor]:
+               cap: Optional[int] = None) -> Optional[torch.Tensor]:
     """Device memory for a call on `stream`, or None where it needs none."""
-    need = _workspace_bytes(p.M, p.D, p.NH, w.NKV, w.window, w.sinks, B, dq_f32, cap)
+    need = _workspace_bytes(p.M, p.D, p.NH, w.NKV, w.window, w.sinks, B, cap)
     if need == 0:
         return None
-    ws = torch.empty(need, dtype=torch.uint8, device=like.device)
-    if stream is not None and stream != torch.cuda.current_stream():
-        ws.record_stream(stream)  # freed on return, while `stream` may still be using it
-    return ws
+    if stream is None:
+        return torch.empty(need, dtype=torch.uint8, device=like.device)
+    with torch.cuda.stream(stream):  # the allocator then reuses it in that stream's order
+        return torch.empty(need, dtype=torch.uint8, device=like.device)
 
 
 def rotaryForward(q: torch.Tensor, k: torch.Tensor, inv_freq: torch.Tensor, p: AttentionParams, B: int,
@@ -503,7 +503,7 @@ def windowAttentionBackward(dO: torch.Tensor, out: torch.Tensor, l: torch.Tensor
     dQ = _out(dQ, q, qs, dQ_dtype, "dQ")
     dK = _out(dK, k, ks, torch.bfloat16, "dK")
     dV = _out(dV, k, ks, torch.bfloat16, "dV")
-    ws = _workspace(q, stream, p, w, B, dq_f32=f32)
+    ws = _workspace(q, stream, p, w, B)
     _lib.call("ma_windowAttentionBackward", _ptr(dO), _ptr(out), _ptr(l), _ptr(q), _ptr(k), _ptr(v), _ptr(dQ),
               _ptr(dK), _ptr(dV), f32, _ptr(lens), ctypes.byref(w), ctypes.byref(p), B, _ptr(ws), ws.numel(),
               _stream(stream))

@@ -967,7 +967,7 @@ int window_args(const MaWindow* w, const AttentionParams* p, uint32_t B, uint32_
   a->NH = s.NH;
   a->NKV = (int)w->NKV;
   a->D = s.D;
-  const uint32_t most = 0x7fffffffu;
+  const uint32_t most = 1u << 30;  // no sequence or cache has more keys: the same mask, and positions stay in range
   a->window = (int)(w->window < most ? w->window : most);
   a->sinks = (int)(w->sinks < most ? w->sinks : most);
   a->scale = s.D == 64 ? 0.125f : 0.08838834764831845f;  // 1/sqrt(D)
@@ -1072,13 +1072,13 @@ extern "C" int ma_windowAttentionForward(const ma_bf16* q, const ma_bf16* k, con
   return ok();
 }
 
-extern "C" int ma_windowAttentionBackward_workspace(uint32_t dq_f32, const MaWindow* w, const AttentionParams* p,
-                                                    uint32_t B, uint64_t* bytes) {
+extern "C" int ma_windowAttentionBackward_workspace(const MaWindow* w, const AttentionParams* p, uint32_t B,
+                                                    uint64_t* bytes) {
   ma::WindowArgs a;
   int rc = window_args(w, p, B, 0, &a);
   if (rc) return rc;
   if (!bytes) return fail(MA_ERR_NULL, "pointer 'bytes' is NULL");
-  *bytes = ma::window_bwd_workspace(a, dq_f32 != 0);
+  *bytes = ma::window_bwd_workspace(a);
   return ok();
 }
 
@@ -1100,7 +1100,7 @@ extern "C" int ma_windowAttentionBackward(const ma_bf16* dO, const ma_bf16* out,
   MA_REQUIRE_PTR(dK);
   MA_REQUIRE_PTR(dV);
   MA_REQUIRE_I32(lens);
-  const uint64_t need = ma::window_bwd_workspace(a, dq_f32 != 0);
+  const uint64_t need = ma::window_bwd_workspace(a);
   rc = check_workspace(workspace, workspace_bytes, need);
   if (rc) return rc;
   const WindowBytes n(a);

@@ -202,6 +202,6 @@ struct WindowGrads {
 cudaError_t launch_window_fwd(const WindowArgs& a, cudaStream_t st);
 size_t window_cached_workspace(const WindowArgs& a);
 cudaError_t launch_window_cached(const WindowArgs& a, void* workspace, cudaStream_t st);
-size_t window_bwd_workspace(const WindowArgs& a, bool dq_f32);
+size_t window_bwd_workspace(const WindowArgs& a);
 cudaError_t launch_window_bwd(const WindowArgs& a, const WindowGrads& g, cudaStream_t st);
 }  // namespace ma

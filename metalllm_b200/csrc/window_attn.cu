@@ -163,7 +163,8 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM)
     }
   } else {
     // ---------------------------------------------------------- consumers
-    // Q as MMA fragments: rows g and g + 8 of the group (padding: zeros)
+    // Q as MMA fragments: rows g and g + 8 of the group (padding: zeros).  Not
+    // __ldg: this grid may be on the GPU before the one that writes q has ended.
     uint32_t q[HD / 16][4];
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
@@ -173,8 +174,8 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM)
           a.q + (((long long)b * a.M + r / G) * a.NH + kh * G + r % G) * HD);
 #pragma unroll
       for (int kk = 0; kk < HD / 16; ++kk) {
-        q[kk][half] = in ? __ldg(p + kk * 8 + c) : 0u;
-        q[kk][half + 2] = in ? __ldg(p + kk * 8 + 4 + c) : 0u;
+        q[kk][half] = in ? __ldcg(p + kk * 8 + c) : 0u;
+        q[kk][half + 2] = in ? __ldcg(p + kk * 8 + 4 + c) : 0u;
       }
     }
     // position of each of the two rows (of the last valid one, for padding)
@@ -353,8 +354,8 @@ __global__ void __launch_bounds__(JOIN) window_join_kernel(const DecodeParams pr
 #pragma unroll 4
   for (int s = slice; s < prm.nsplit; s += SLICES) {
     const long long at = at0 + (long long)s * ROWS;
-    add(__ldg(reinterpret_cast<const float2*>(prm.part_ml) + at),
-        __ldg(reinterpret_cast<const float4*>(prm.part_o + at * HD) + lane));
+    add(__ldcg(reinterpret_cast<const float2*>(prm.part_ml) + at),
+        __ldcg(reinterpret_cast<const float4*>(prm.part_o + at * HD) + lane));
   }
   so[slice][lane] = x;
   if (lane == 0) sml[slice] = make_float2(top, sum);

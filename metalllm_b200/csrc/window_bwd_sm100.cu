@@ -532,8 +532,9 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         if constexpr (!DQ) {  // in flight while the tiles land
           const long long at =
               ((long long)s.u.b * prm.NH + s.u.x_head<DQ>(s.i)) * prm.rows + s.u.x_tile<DQ>(s.i) * BT + lane * 4;
-          L = __ldg(reinterpret_cast<const float4*>(prm.neg_l + at));
-          D4 = __ldg(reinterpret_cast<const float4*>(prm.neg_d + at));
+          // (not __ldg: this grid was on the GPU before they were written)
+          L = __ldcg(reinterpret_cast<const float4*>(prm.neg_l + at));
+          D4 = __ldcg(reinterpret_cast<const float4*>(prm.neg_d + at));
         }
         if (!mbar_poll_warp(BAR_X1F(s1), (s.t / C::X1ST) & 1, abort_p)) break;
         if (pad) zero_rows(C::OFF_X1 + s1 * C::TILE, a);
@@ -575,8 +576,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       if constexpr (DQ) {
         if (s.i == 0) {
           const long long at = ((long long)s.u.b * prm.NH + s.u.head) * prm.rows + r;
-          nl = __ldg(prm.neg_l + at);
-          nd = __ldg(prm.neg_d + at);
+          nl = __ldcg(prm.neg_l + at);
+          nd = __ldcg(prm.neg_d + at);
         }
       }
       uint32_t see[2];
@@ -830,7 +831,7 @@ __global__ void __launch_bounds__(256) window_join_sinks_kernel(const float* __r
     float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 4
     for (int k = 0; k < slots; ++k) {
-      const float4 x = __ldg(reinterpret_cast<const float4*>(part) + (((r * slots + k) * 2 + which) * BT + row) * d4 + c);
+      const float4 x = __ldcg(reinterpret_cast<const float4*>(part) + (((r * slots + k) * 2 + which) * BT + row) * d4 + c);
       s.x += x.x, s.y += x.y, s.z += x.z, s.w += x.w;
     }
     __nv_bfloat16* to = (which == 0 ? dV : dK) + ((bh / NKV * T + key) * NKV + bh % NKV) * D + c * 4;
@@ -922,7 +923,7 @@ cudaError_t launch_all(const WindowArgs& a, const WindowGrads& g, cudaStream_t s
 
 }  // namespace
 
-size_t window_bwd_workspace(const WindowArgs& a, bool) { return win_plan(a).total(); }
+size_t window_bwd_workspace(const WindowArgs& a) { return win_plan(a).total(); }
 
 cudaError_t launch_window_bwd(const WindowArgs& a, const WindowGrads& g, cudaStream_t st) {
   return a.D == 64 ? launch_all<64>(a, g, st) : launch_all<128>(a, g, st);

@@ -354,6 +354,8 @@ CACHED = [
     (1, 17, 16, 1, 64, 2000, 513, 3, [1900], None),
     (2, 40, 4, 2, 64, 1000, 90, 3, [960, 130], [40, 11]), (2, 200, 4, 1, 128, 3000, 500, 140, [2800, 77], [200, 130]),
     (1, 300, 2, 2, 64, 4096, 4096, 0, [3796], None), (2, 260, 2, 1, 64, 700, 100, 4, [0, 440], None),
+    # a window without end, from a position inside a tile
+    (1, 200, 2, 1, 64, 700, 2 ** 32 - 1, 0, [77], None), (2, 3, 4, 1, 128, 700, 2 ** 32 - 1, 2 ** 32 - 1, [77, 690], None),
     # more query tiles than SMs: units are pairs of tiles, which start inside the cache
     (3, 700, 12, 2, 64, 3000, 400, 70, [2300, 129, 0], [700, 500, 257]),
     (2, 1100, 10, 5, 128, 2000, 300, 3, [900, 13], None),

@@ -98,7 +98,7 @@ def test_window_refuses(cuda_lib, kw, code):
     x = [at(i) for i in range(5)]
     n = ctypes.c_uint64()
     assert name(lib.ma_windowAttentionForward(*x, None, ctypes.byref(w), ctypes.byref(p), 1, None)) == code
-    assert name(lib.ma_windowAttentionBackward_workspace(1, ctypes.byref(w), ctypes.byref(p), 1, ctypes.byref(n))) == code
+    assert name(lib.ma_windowAttentionBackward_workspace(ctypes.byref(w), ctypes.byref(p), 1, ctypes.byref(n))) == code
     assert name(lib.ma_windowAttentionCached_workspace(ctypes.byref(w), ctypes.byref(p), 1, 64, ctypes.byref(n))) == code
 
 
@@ -126,8 +126,8 @@ def test_window_forward_refuses_pointers(cuda_lib):
 def test_window_backward_refuses(cuda_lib):
     lib, p, w = cuda_lib, params(), window()
     n = ctypes.c_uint64()
-    assert lib.ma_windowAttentionBackward_workspace(0, ctypes.byref(w), ctypes.byref(p), 1, ctypes.byref(n)) == 0
-    assert name(lib.ma_windowAttentionBackward_workspace(0, ctypes.byref(w), ctypes.byref(p), 1, None)) == "MA_ERR_NULL"
+    assert lib.ma_windowAttentionBackward_workspace(ctypes.byref(w), ctypes.byref(p), 1, ctypes.byref(n)) == 0
+    assert name(lib.ma_windowAttentionBackward_workspace(ctypes.byref(w), ctypes.byref(p), 1, None)) == "MA_ERR_NULL"
     need = n.value
 
     def call(x, ws=at(12), have=need):
