@@ -309,6 +309,65 @@ def test_window_far_offsets(A, D):
     torch.cuda.empty_cache()
 
 
+def test_many_short_sequences(A):
+    """70000 sequences of two rows: each as it would be alone, in every operator."""
+    B, T, NH, NKV, D, W = 70000, 2, 2, 1, 64, 2
+    p, f = A.make_params(T, NH, D), A.rotaryFrequencies(D)
+    q, dO = (randn(B, T, NH * D, seed=s) for s in (1, 4))
+    k, v = (randn(B, T, NKV * D, seed=s) for s in (2, 3))
+    ln = (torch.arange(B, device="cuda") % 3).to(torch.int32)
+
+    def calls(i):
+        n, x = len(i), [t[i].contiguous() for t in (q, k, v, dO, ln)]
+        out, l = A.windowAttentionForward(*x[:3], p, n, W, 0, NKV, lens=x[4])
+        g = A.windowAttentionBackward(x[3], out, l, *x[:3], p, n, W, 0, NKV, lens=x[4])
+        kc, vc = torch.zeros_like(x[1]), torch.zeros_like(x[2])
+        st = torch.zeros(n, dtype=torch.int32, device="cuda")
+        qr = A.rotaryCacheAppend(*x[:3], kc, vc, st, f, p, n, NKV, lens=x[4])
+        return (out, l) + g + (qr, kc, vc) + A.windowAttentionCached(qr, kc, vc, st, p, n, W, 0, NKV, lens=x[4])
+
+    some = torch.tensor([0, 1, 2, 65535, 65536, B - 2, B - 1], device="cuda")
+    for a, b in zip(calls(torch.arange(B, device="cuda")), calls(some)):
+        assert torch.equal(a[some], b)
+
+
+def test_refuses_layouts(A):
+    """Strided, misaligned, mistyped and misplaced tensors are refused before anything runs."""
+    B, T, NH, NKV, D = 2, 8, 2, 1, 64
+    p, f = A.make_params(T, NH, D), A.rotaryFrequencies(D)
+    q, k, v = randn(B, T, NH * D), randn(B, T, NKV * D), randn(B, T, NKV * D)
+    qkv = randn(B, T, (NH + 2 * NKV) * D)
+    st = i32([0, 0])
+    shifted = randn(B * T * NH * D + 1).view(-1)[1:].view(B, T, NH * D)  # 2 bytes off a 16-byte boundary
+    fwd = lambda x, **kw: A.windowAttentionForward(x, k, v, p, B, 4, 0, NKV, **kw)
+    step = lambda x, **kw: A.windowAttentionCached(x, k, v, kw.pop("start", st), p, B, 4, 0, NKV, **kw)
+    rot = lambda x, **kw: A.rotaryForward(x, k, kw.pop("f", f), p, B, NKV, **kw)
+    for call in (fwd, step, rot):
+        with pytest.raises(ValueError, match="contiguous"):
+            call(qkv[..., :NH * D])
+        with pytest.raises(A.MetalAttnError, match="aligned"):
+            call(shifted)
+        with pytest.raises(TypeError, match="bfloat16"):
+            call(q.float())
+        with pytest.raises(ValueError, match="CUDA"):
+            call(q.cpu())
+        with pytest.raises(ValueError, match="shape"):
+            call(q[:1].contiguous())
+    with pytest.raises(TypeError, match="int32"):
+        fwd(q, lens=torch.tensor([3, 8], device="cuda"))
+    with pytest.raises(ValueError, match="CUDA"):
+        step(q, start=torch.zeros(2, dtype=torch.int32))
+    with pytest.raises(TypeError, match="float64"):
+        rot(q, f=f.float())
+    with pytest.raises(A.MetalAttnError, match="overlaps"):
+        fwd(q, out=q)
+    with pytest.raises(A.MetalAttnError, match="window"):
+        A.windowAttentionForward(q, k, v, p, B, 0, 0, NKV)
+    with pytest.raises(A.MetalAttnError, match="cap=0"):
+        A.windowAttentionCached(q, k[:, :0], v[:, :0], st, p, B, 4, 0, NKV)
+    assert A.device_status() == 0
+
+
 def test_window_results_repeat(A):
     """The same call gives the same bits: no sum's order is left to chance."""
     B, T, NH, NKV, D, W, S = 2, 2500, 8, 2, 128, 300, 70
@@ -354,6 +413,8 @@ CACHED = [
     (1, 17, 16, 1, 64, 2000, 513, 3, [1900], None),
     (2, 40, 4, 2, 64, 1000, 90, 3, [960, 130], [40, 11]), (2, 200, 4, 1, 128, 3000, 500, 140, [2800, 77], [200, 130]),
     (1, 300, 2, 2, 64, 4096, 4096, 0, [3796], None), (2, 260, 2, 1, 64, 700, 100, 4, [0, 440], None),
+    # 128 query heads of one K/V head; padding rows of a split call
+    (2, 1, 128, 1, 128, 900, 200, 5, [899, 3], None), (3, 3, 4, 2, 64, 9000, 9000, 0, [8000, 20, 8990], [3, 1, 0]),
     # a window without end, from a position inside a tile
     (1, 200, 2, 1, 64, 700, 2 ** 32 - 1, 0, [77], None), (2, 3, 4, 1, 128, 700, 2 ** 32 - 1, 2 ** 32 - 1, [77, 690], None),
     # more query tiles than SMs: units are pairs of tiles, which start inside the cache
