@@ -268,6 +268,10 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM)
           mma16816(o[2 * d + 1], p4, v4[2], v4[3]);
         }
       }
+      // V has been read.  (Without the fence the last ldmatrix can be scheduled
+      // after the arrival, which the compiler orders before them only for plain
+      // loads: a warp held up in between then reads the next block's rows.)
+      __threadfence_block();
       __syncwarp();
       if (lane == 0) mbar_arrive(BAR_E(st));
     }

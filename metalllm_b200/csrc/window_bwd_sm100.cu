@@ -248,6 +248,7 @@ __device__ __forceinline__ bool next_unit(const Params& p, Step& s, const Ring& 
       return false;
     s.u = ring.desc[slot];
     if (g > 0) {
+      __threadfence_block();  // read, before the slot is released
       if (WARP) __syncwarp();
       if (!WARP || (threadIdx.x & 31) == 0) mbar_arrive(ring.sched.empty + 8u * slot);
     }
@@ -639,9 +640,9 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         d[j + 2] = r1.x;
         d[j + 3] = r1.y;
       }
-      if constexpr (!DQ) mbar_arrive(BAR_TE(t % C::SSTG));
       store_row64(tdp + 32, d);
       tmem_wait_st();
+      if constexpr (!DQ) mbar_arrive(BAR_TE(t % C::SSTG));  // all read: dS is stored
       tc_fence_before();
       mbar_arrive(BAR_PR(t % C::DPB));
     };

@@ -435,6 +435,24 @@ def test_cached(A, B, M, NH, NKV, D, cap, window, sinks, start, lens):
     check_cached(A, q, kc, vc, start, NH, NKV, D, window, sinks, lens)
 
 
+@pytest.mark.parametrize("B,M,NH,NKV,D,cap,window,sinks", [(64, 1, 32, 8, 128, 4300, 4096, 4), (64, 4, 16, 4, 64, 4300, 4096, 0),
+                                                            (2, 1, 32, 8, 128, 60000, 60000, 0), (4, 100, 16, 4, 128, 5000, 2000, 4)])
+def test_cached_results_repeat(A, B, M, NH, NKV, D, cap, window, sinks):
+    """Many blocks through the ring of every SM: each of ten calls gives the same bits, and the right ones."""
+    q = randn(B, M, NH * D, seed=1)
+    kc, vc = randn(B, cap, NKV * D, seed=2), randn(B, cap, NKV * D, seed=3)
+    start = [cap - M - 17 * (b % 8) for b in range(B)]
+    p, st = A.make_params(M, NH, D), i32(start)
+    runs = [A.windowAttentionCached(q, kc, vc, st, p, B, window, sinks, NKV) for _ in range(10)]
+    for o, l in runs[1:]:
+        assert torch.equal(o, runs[0][0]) and torch.equal(l, runs[0][1])
+    o, l = runs[0]
+    for b in range(0, B, 9):
+        o64, l64, to, tl = ref.forward(q[b], kc[b], vc[b], NH, NKV, D, window, sinks, start[b], M)
+        near("out", o[b], o64, to)
+        near("l", l[b], l64, tl)
+
+
 def test_cached_far_rows(A):
     """A cache of more than 2^32 bytes and more than 2^31 elements: the last sequence's rows."""
     B, M, NH, NKV, D, cap, W, S = 3, 1, 8, 8, 128, 1 << 20, 200, 4
