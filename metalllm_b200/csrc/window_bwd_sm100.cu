@@ -190,12 +190,15 @@ __device__ __forceinline__ Unit decode_dkv(const Params& p, int k) {
   return u;
 }
 
-// dQ pass: unit k, the longest windows first.
+// dQ pass: unit k, in blocks of (batch, head)s as above, the longest windows
+// of a block first.
 __device__ __forceinline__ Unit decode_dq(const Params& p, int k) {
+  constexpr int HB = 16;
   Unit u;
-  const int nbh = p.B * p.NH;
-  const int bh = k % nbh;
-  u.tile = p.ntiles - 1 - k / nbh;
+  const int nbh = p.B * p.NH, per = HB * p.ntiles;
+  const int blk = k / per, r = k % per, hb = min(HB, nbh - blk * HB);
+  const int bh = blk * HB + r % hb;
+  u.tile = p.ntiles - 1 - r / hb;
   u.b = bh / p.NH;
   u.head = bh % p.NH;
   u.head0 = u.head / p.G;
