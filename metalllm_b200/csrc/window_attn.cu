@@ -17,7 +17,9 @@
 // 16 keys of every block with its own m, l and O in registers, joined at the
 // end.  Few rows on a long axis leave most SMs idle, so the blocks are split
 // over CTAs until the GPU is full, and a second kernel joins the splits'
-// (m, l, O) in a fixed order.
+// (m, l, O) in a fixed order.  Measured: 64 requests, 32 / 8 heads of 128, window
+// 4096: 165 us, 6.5 TB/s; one request over 131072 keys: 92 us, 83 of them the
+// splits at 6.5 TB/s.
 //
 // Cache rows that no query sees may hold anything: their scores are replaced
 // by -inf and their V rows zeroed in shared memory, since 0 * NaN is NaN.
@@ -231,7 +233,7 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM)
       }
       // P as two bf16 operands, hi + lo: 16 bits of it, so that the output's own
       // rounding is all that is lost (one operand: 1.4 times that).  The tensor
-      // cores have the time: a step of 64 requests takes 164 us, with one 161.
+      // cores have the time: a step of 64 requests takes 165 us, with one 162.
       uint32_t p4[4], r4[4];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {

@@ -23,8 +23,11 @@
 // write, its reads and the room for the rings).  (The form that computes all
 // three gradients in one pass and adds dQ up in global memory spends 5 products
 // a step where these spend 4 + 3, but it had to zero dQ, add 64 KB a step into
-// L2 and convert the sums: at B=2, 4096 tokens, 16 heads of 128, window 1000 it
-// took 384 us, at 64 x 1024, 12 heads of 64, window 250 605 us.)
+// L2 and convert the sums: at B=2, 4096 tokens, 16 / 4 heads of 128, window 1000
+// it took 384 us, at up to 64 x 1024, 12 heads of 64, window 250 605 us; these
+// passes take 279 (557 TFLOP/s; the tensor pipe is busy 54 % of the time) and 443
+// (units of three steps).  The chain from a step's scores over the row math to
+// its products bounds them.)
 //
 // Pipeline: S of the next step is issued as soon as this step's has been read,
 // and with two dP buffers (all but dK/dV at D=128) dP ahead of this step's
