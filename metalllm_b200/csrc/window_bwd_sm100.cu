@@ -82,8 +82,11 @@ struct Cfg {
   static constexpr int X1ST = HD == 64 ? 4 : 3;
   static constexpr int X2ST = HD == 64 ? 4 : 2;
   static constexpr int DPB = !DQ && HD == 128 ? 1 : 2;
-  static constexpr int SSTG = DQ ? 0 : HD == 64 ? 4 : 1;  // statistics ring
-  static constexpr uint32_t STAT = 2 * BT * 4;
+  // the dK/dV pass's statistics: at D=64 added by the tensor core (see EXT in
+  // the kernel), else a ring of fp32 rows
+  static constexpr bool EXT = !DQ && HD == 64;
+  static constexpr int SSTG = DQ ? 0 : EXT ? 2 : 1;
+  static constexpr uint32_t STAT = EXT ? BT * 128 / 2 : 2 * BT * 4;  // EXT: one tile in all
   static constexpr int NDESC = (int)kSchedSlots + 1;
   static constexpr uint32_t DESC = 48;
   static constexpr uint32_t OFF_R = 0;                              // [RST][2]
@@ -114,6 +117,7 @@ struct Params {
   float scale, scale_log2;
   int rows;                    // rows of a (batch, head) in the statistics
   const float *neg_l, *neg_d;  // -l*log2e, -delta/sqrt(D), [B][NH][rows]
+  const uint4* ext;            // D=64: -l*sqrt(D) and -delta as three bf16 each, and two zeros
   uint32_t* status;
   // dK/dV pass: sink tiles 0 .. nsplit-1 are split: their query tiles past the
   // window go, far_tiles at a time, to nfar units each, dealt first; unit
@@ -360,13 +364,28 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       if (i >= B_X1 + C::X1ST && i < B_X1 + 2 * C::X1ST) n = 2;  // the products, and warp 2
       if (i >= B_X2 + C::X2ST && i < B_X2 + 2 * C::X2ST) n = 2;
       if (i >= B_T && i < B_T + C::SSTG) n = 32;
-      if (i >= B_T + C::SSTG && i < B_DP) n = NCOMP;
+      if (i >= B_T + C::SSTG && i < B_DP) n = C::EXT ? 1 : NCOMP;
       if ((i >= B_PR && i < B_PE) || i == B_1 + 1) n = NCOMP;
       if (i == B_1 + 3) n = 128;
       if (i >= B_1 + 6 + (int)kSchedSlots && i < B_1 + 6 + 2 * (int)kSchedSlots) n = READERS;
       mbar_init(BAR(i), n);
     }
     fence_mbar_init();
+  }
+  // EXT: S - l sqrt(D) and dP - delta come from one more product of 16 columns.  A
+  // tile's rows of 128 bytes hold four operands of 16: ones in columns 0-2, ones
+  // in 3-5, and two stages of statistics, each value as three bf16 (24 bits).
+  // (As fp32 in shared memory they cost the compute warps a broadcast load for
+  // every two scores.)
+  if constexpr (C::EXT) {
+    for (int i = threadIdx.x; i < BT * 8; i += NUM_THREADS) {
+      const int r = i / 8, ch = i % 8;
+      uint4 v = make_uint4(0u, 0u, 0u, 0u);
+      if (ch == 0) v.x = 0x3f803f80u, v.y = 0x3f80u;
+      if (ch == 2) v.y = 0x3f800000u, v.z = 0x3f803f80u;
+      *reinterpret_cast<uint4*>(gbase + C::OFF_STAT + r * 128 + ((ch ^ (r & 7)) * 16)) = v;
+    }
+    fence_proxy_async_smem();
   }
   if (warp == 1) {
     tmem_alloc(sbase + C::OFF_TSLOT, 512);
@@ -459,9 +478,13 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
             if (!mbar_poll(BAR_X1Z(s1), (z1 >> s1) & 1, abort_p)) break;
             z1 ^= 1u << s1;
           }
+          const uint32_t st = C::EXT ? t % C::SSTG : 0;
+          if (C::EXT && !mbar_poll(BAR_TF(st), (t / C::SSTG) & 1, abort_p)) break;
           if (t >= 1 && !mbar_poll(BAR_SE, (t - 1) & 1, abort_p)) break;
           tc_fence_after();
+          const uint32_t de = desc_lo(sbase + C::OFF_STAT, 16);  // 32 bytes an operand
           scores(tmem + C::TCOL_S, sbase + C::OFF_R + rs * 2 * C::TILE, sbase + C::OFF_X1 + s1 * C::TILE);
+          if (C::EXT) umma_bf16_ss_lo(tmem + C::TCOL_S, de, de + 4 + 2 * st, IDESC_S, 1u);
           umma_commit(BAR_SF);
           if (!mbar_poll(BAR_X2F(s2), (t / C::X2ST) & 1, abort_p)) break;
           if (pad) {
@@ -473,7 +496,9 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
           tc_fence_after();
           scores(tmem + C::TCOL_DP + b * 128, sbase + C::OFF_R + (rs * 2 + 1) * C::TILE,
                  sbase + C::OFF_X2 + s2 * C::TILE);
+          if (C::EXT) umma_bf16_ss_lo(tmem + C::TCOL_DP + b * 128, de + 2, de + 4 + 2 * st, IDESC_S, 1u);
           umma_commit(BAR_DPF(b));
+          if (C::EXT) umma_commit(BAR_TE(st));
           if (DQ) umma_commit(BAR_X2E(s2));
           if (s.i + 1 == s.u.nq) umma_commit(BAR_RE(rs));  // the resident tiles' last use
         }
@@ -536,12 +561,17 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         const bool pad = padded(s);
         const int a = max(0, s.u.n - s.u.x_tile<DQ>(s.i) * BT);
         float4 L, D4;
+        uint4 x4[4];
         if constexpr (!DQ) {  // in flight while the tiles land
-          const long long at =
-              ((long long)s.u.b * prm.NH + s.u.x_head<DQ>(s.i)) * prm.rows + s.u.x_tile<DQ>(s.i) * BT + lane * 4;
+          const long long at = ((long long)s.u.b * prm.NH + s.u.x_head<DQ>(s.i)) * prm.rows + s.u.x_tile<DQ>(s.i) * BT;
           // (not __ldg: this grid was on the GPU before they were written)
-          L = __ldcg(reinterpret_cast<const float4*>(prm.neg_l + at));
-          D4 = __ldcg(reinterpret_cast<const float4*>(prm.neg_d + at));
+          if constexpr (C::EXT) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x4[j] = __ldcg(prm.ext + at + lane + 32 * j);
+          } else {
+            L = __ldcg(reinterpret_cast<const float4*>(prm.neg_l + at) + lane);
+            D4 = __ldcg(reinterpret_cast<const float4*>(prm.neg_d + at) + lane);
+          }
         }
         if (!mbar_poll_warp(BAR_X1F(s1), (s.t / C::X1ST) & 1, abort_p)) break;
         if (pad) zero_rows(C::OFF_X1 + s1 * C::TILE, a);
@@ -552,9 +582,18 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         if constexpr (!DQ) {
           const int st = s.t % C::SSTG;
           if (s.t >= C::SSTG && !mbar_poll_warp(BAR_TE(st), ((s.t / C::SSTG) - 1) & 1, abort_p)) break;
-          float* stt = stat_base + st * (2 * BT);
-          reinterpret_cast<float4*>(stt)[lane] = L;
-          reinterpret_cast<float4*>(stt + BT)[lane] = D4;
+          if constexpr (C::EXT) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {  // lane + 32 j: its 16 bytes of the stage
+              const int r = lane + 32 * j;
+              *reinterpret_cast<uint4*>(gbase + C::OFF_STAT + r * 128 + (((4 + 2 * st) ^ (r & 7)) * 16)) = x4[j];
+            }
+            fence_proxy_async_smem();
+          } else {
+            float* stt = stat_base + st * (2 * BT);
+            reinterpret_cast<float4*>(stt)[lane] = L;
+            reinterpret_cast<float4*>(stt + BT)[lane] = D4;
+          }
           mbar_arrive(BAR_TF(st));
         }
         if (!mbar_poll_warp(BAR_X2F(s2), (s.t / C::X2ST) & 1, abort_p)) break;
@@ -608,7 +647,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       tc_fence_before();
       mbar_arrive(BAR_SE);
       const float* stt = stat_base;
-      if constexpr (!DQ) {
+      if constexpr (!DQ && !C::EXT) {
         const int st = t % C::SSTG;
         ok = mbar_poll_warp(BAR_TF(st), (t / C::SSTG) & 1, abort_p);
         if (!ok) return;
@@ -617,7 +656,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
 #pragma unroll
       for (int j = 0; j < 64; j += 4) {
         float4 L = make_float4(nl, nl, nl, nl);
-        if constexpr (!DQ) L = *reinterpret_cast<const float4*>(stt + j);
+        if constexpr (!DQ && !C::EXT) L = *reinterpret_cast<const float4*>(stt + j);
         const float2 t0 = __ffma2_rn(make_float2(p[j], p[j + 1]), c2, make_float2(L.x, L.y));
         const float2 t1 = __ffma2_rn(make_float2(p[j + 2], p[j + 3]), c2, make_float2(L.z, L.w));
         const uint32_t m = see[j / 32] >> (j % 32);
@@ -636,9 +675,12 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
 #pragma unroll
       for (int j = 0; j < 64; j += 4) {
         float4 Dn = make_float4(nd, nd, nd, nd);
-        if constexpr (!DQ) Dn = *reinterpret_cast<const float4*>(stt + BT + j);
-        const float2 d0 = __ffma2_rn(make_float2(d[j], d[j + 1]), sc2, make_float2(Dn.x, Dn.y));
-        const float2 d1 = __ffma2_rn(make_float2(d[j + 2], d[j + 3]), sc2, make_float2(Dn.z, Dn.w));
+        if constexpr (!DQ && !C::EXT) Dn = *reinterpret_cast<const float4*>(stt + BT + j);
+        float2 d0 = make_float2(d[j], d[j + 1]), d1 = make_float2(d[j + 2], d[j + 3]);
+        if constexpr (!C::EXT) {  // EXT: dK is multiplied by 1/sqrt(D) as it is stored
+          d0 = __ffma2_rn(d0, sc2, make_float2(Dn.x, Dn.y));
+          d1 = __ffma2_rn(d1, sc2, make_float2(Dn.z, Dn.w));
+        }
         const float2 r0 = __fmul2_rn(make_float2(p[j], p[j + 1]), d0);
         const float2 r1 = __fmul2_rn(make_float2(p[j + 2], p[j + 3]), d1);
         d[j] = r0.x;
@@ -648,7 +690,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       }
       store_row64(tdp + 32, d);
       tmem_wait_st();
-      if constexpr (!DQ) mbar_arrive(BAR_TE(t % C::SSTG));  // all read: dS is stored
+      if constexpr (!DQ && !C::EXT) mbar_arrive(BAR_TE(t % C::SSTG));  // all read: dS is stored
       tc_fence_before();
       mbar_arrive(BAR_PR(t % C::DPB));
     };
@@ -686,6 +728,10 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
           for (int j = 0; j < 32; ++j) r[j] = valid ? r[j] : 0u;
         }
         const int which = cc / HD, col = cc % HD;
+        if (C::EXT && which == 1) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) * prm.scale);
+        }
         float* f32 = nullptr;
         __nv_bfloat16* b16 = nullptr;
         if constexpr (DQ) {
@@ -727,8 +773,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
 // How a call's workspace is laid out, and how its sink tiles are split.
 struct Plan {
   int ntiles, rows, nsplit, nfar, far_tiles;
-  size_t stat, part;  // bytes: one statistic, the partial sums
-  size_t total() const { return 2 * stat + part; }
+  size_t stat, ext, part;  // bytes: one statistic, both as bf16, the partial sums
+  size_t total() const { return 2 * stat + ext + part; }
 };
 
 Plan win_plan(const WindowArgs& a) {
@@ -751,6 +797,7 @@ Plan win_plan(const WindowArgs& a) {
   }
   auto up = [](size_t x) { return (x + 255) & ~(size_t)255; };
   p.stat = up((size_t)a.B * a.NH * p.rows * sizeof(float));
+  p.ext = a.D == 64 ? 4 * p.stat : 0;
   p.part = up((size_t)nbh * p.nsplit * (1 + p.nfar) * 2 * BT * a.D * sizeof(float));
   return p;
 }
@@ -775,7 +822,7 @@ __device__ __forceinline__ float dot8(uint4 a, uint4 b) {
 template <int HD>
 __global__ void __launch_bounds__(256, 2) window_stats_kernel(const WindowArgs a, const __nv_bfloat16* __restrict__ dO,
                                                               float* __restrict__ neg_l, float* __restrict__ neg_d,
-                                                              int rows) {
+                                                              uint4* __restrict__ ext, int rows) {
   pdl_wait_and_release();
   constexpr int G = HD / 8, RPI = 32 / G, N = 8, ROWS = N * RPI;  // lanes a row, rows an instruction, loads in flight
   const int lane = threadIdx.x % 32;
@@ -811,8 +858,22 @@ __global__ void __launch_bounds__(256, 2) window_stats_kernel(const WindowArgs a
       const int row = row0 + lane;
       const bool valid = row < n;
       const long long at = ((long long)b * a.NH + h) * rows + row;
-      neg_l[at] = valid ? -a.l[((long long)b * a.M + row) * a.NH + h] * LOG2E : 0.0f;
-      neg_d[at] = valid ? -mine * a.scale : 0.0f;
+      const float l = valid ? -a.l[((long long)b * a.M + row) * a.NH + h] : 0.0f, d = valid ? -mine : 0.0f;
+      neg_l[at] = l * LOG2E;
+      neg_d[at] = d * a.scale;
+      if constexpr (HD == 64) {  // 24 bits each, as three operands of the tensor core
+        uint32_t x[6];
+        auto three = [&](float v, uint32_t* to) {
+#pragma unroll
+          for (int i = 0; i < 3; ++i) {
+            to[i] = sm100::pack_bf16(v, 0.0f) & 0xffffu;
+            v -= __uint_as_float(to[i] << 16);
+          }
+        };
+        three(l * 8.0f, x);  // sqrt(D) = 8
+        three(d, x + 3);
+        ext[at] = make_uint4(x[0] | x[1] << 16, x[2] | x[3] << 16, x[4] | x[5] << 16, 0u);
+      }
     }
   }
 }
@@ -872,12 +933,13 @@ cudaError_t launch_all(const WindowArgs& a, const WindowGrads& g, cudaStream_t s
   char* ws = static_cast<char*>(g.workspace);
   float* neg_l = reinterpret_cast<float*>(ws);
   float* neg_d = reinterpret_cast<float*>(ws + p.stat);
+  uint4* ext = reinterpret_cast<uint4*>(ws + 2 * p.stat);
   int dev = 0, sms = 148;
   cudaGetDevice(&dev);
   cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
   auto blocks = [&](long long n, int per) { return (unsigned)std::min<long long>((n + per - 1) / per, sms * 16ll); };
   launch_pdl(window_stats_kernel<HD>, blocks((long long)a.B * a.NH * p.rows / (2048 / HD), 8), 256, 0, st, a, g.dO, neg_l,
-             neg_d, p.rows);
+             neg_d, ext, p.rows);
   count_launches(1);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return e;
@@ -910,7 +972,8 @@ cudaError_t launch_all(const WindowArgs& a, const WindowGrads& g, cudaStream_t s
   prm.nfar = p.nfar;
   prm.far_tiles = p.far_tiles;
   prm.nfar_units = p.nsplit * p.nfar * a.B * a.NKV;
-  prm.part = reinterpret_cast<float*>(ws + 2 * p.stat);
+  prm.ext = ext;
+  prm.part = reinterpret_cast<float*>(ws + 2 * p.stat + p.ext);
   prm.dK = g.dK;
   prm.dV = g.dV;
   prm.dQ = g.dQ;
