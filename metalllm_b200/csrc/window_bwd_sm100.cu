@@ -85,6 +85,10 @@ struct Cfg {
   // the dK/dV pass's statistics: at D=64 added by the tensor core (see EXT in
   // the kernel), else a ring of fp32 rows
   static constexpr bool EXT = !DQ && HD == 64;
+  // warp 2 passes a step on to the issuer of S and dP when all of it is ready
+  // (tiles, zeroed rows, statistics): one wait for five.  Not where S must not
+  // wait for X2, whose two stages are held until the products.
+  static constexpr bool ONE = DPB == 2;
   static constexpr int SSTG = DQ ? 0 : EXT ? 2 : 1;
   static constexpr uint32_t STAT = EXT ? BT * 128 / 2 : 2 * BT * 4;  // EXT: one tile in all
   static constexpr int NDESC = (int)kSchedSlots + 1;
@@ -473,23 +477,28 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
           const uint32_t t = s.t, rs = s.uc % C::RST, s1 = t % C::X1ST, s2 = t % C::X2ST, b = t % C::DPB;
           const bool pad = padded(s);
           if (s.i == 0 && !mbar_poll(BAR_RF(rs), (s.uc / C::RST) & 1, abort_p)) break;
-          if (!mbar_poll(BAR_X1F(s1), (t / C::X1ST) & 1, abort_p)) break;
-          if (pad) {
-            if (!mbar_poll(BAR_X1Z(s1), (z1 >> s1) & 1, abort_p)) break;
-            z1 ^= 1u << s1;
-          }
           const uint32_t st = C::EXT ? t % C::SSTG : 0;
-          if (C::EXT && !mbar_poll(BAR_TF(st), (t / C::SSTG) & 1, abort_p)) break;
+          if constexpr (C::ONE) {
+            if (!mbar_poll(BAR_X2Z(s2), (t / C::X2ST) & 1, abort_p)) break;
+          } else {
+            if (!mbar_poll(BAR_X1F(s1), (t / C::X1ST) & 1, abort_p)) break;
+            if (pad) {
+              if (!mbar_poll(BAR_X1Z(s1), (z1 >> s1) & 1, abort_p)) break;
+              z1 ^= 1u << s1;
+            }
+          }
           if (t >= 1 && !mbar_poll(BAR_SE, (t - 1) & 1, abort_p)) break;
           tc_fence_after();
           const uint32_t de = desc_lo(sbase + C::OFF_STAT, 16);  // 32 bytes an operand
           scores(tmem + C::TCOL_S, sbase + C::OFF_R + rs * 2 * C::TILE, sbase + C::OFF_X1 + s1 * C::TILE);
           if (C::EXT) umma_bf16_ss_lo(tmem + C::TCOL_S, de, de + 4 + 2 * st, IDESC_S, 1u);
           umma_commit(BAR_SF);
-          if (!mbar_poll(BAR_X2F(s2), (t / C::X2ST) & 1, abort_p)) break;
-          if (pad) {
-            if (!mbar_poll(BAR_X2Z(s2), (z2 >> s2) & 1, abort_p)) break;
-            z2 ^= 1u << s2;
+          if constexpr (!C::ONE) {
+            if (!mbar_poll(BAR_X2F(s2), (t / C::X2ST) & 1, abort_p)) break;
+            if (pad) {
+              if (!mbar_poll(BAR_X2Z(s2), (z2 >> s2) & 1, abort_p)) break;
+              z2 ^= 1u << s2;
+            }
           }
           // the products that read P and dS out of its columns have completed
           if (t >= C::DPB && !mbar_poll(BAR_PE(b), ((t / C::DPB) - 1) & 1, abort_p)) break;
@@ -576,7 +585,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         if (!mbar_poll_warp(BAR_X1F(s1), (s.t / C::X1ST) & 1, abort_p)) break;
         if (pad) zero_rows(C::OFF_X1 + s1 * C::TILE, a);
         if (lane == 0) {
-          if (pad) mbar_arrive(BAR_X1Z(s1));
+          if (pad && !C::ONE) mbar_arrive(BAR_X1Z(s1));
           mbar_arrive(BAR_X1E(s1));
         }
         if constexpr (!DQ) {
@@ -588,18 +597,21 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
               const int r = lane + 32 * j;
               *reinterpret_cast<uint4*>(gbase + C::OFF_STAT + r * 128 + (((4 + 2 * st) ^ (r & 7)) * 16)) = x4[j];
             }
-            fence_proxy_async_smem();
           } else {
             float* stt = stat_base + st * (2 * BT);
             reinterpret_cast<float4*>(stt)[lane] = L;
             reinterpret_cast<float4*>(stt + BT)[lane] = D4;
           }
-          mbar_arrive(BAR_TF(st));
+          if constexpr (!C::EXT) mbar_arrive(BAR_TF(st));
         }
         if (!mbar_poll_warp(BAR_X2F(s2), (s.t / C::X2ST) & 1, abort_p)) break;
         if (pad) zero_rows(C::OFF_X2 + s2 * C::TILE, a);
+        if constexpr (C::ONE) {
+          fence_proxy_async_smem();
+          __syncwarp();
+        }
         if (lane == 0) {
-          if (pad) mbar_arrive(BAR_X2Z(s2));
+          if (pad || C::ONE) mbar_arrive(BAR_X2Z(s2));
           mbar_arrive(BAR_X2E(s2));
         }
       }
