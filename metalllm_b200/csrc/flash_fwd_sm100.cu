@@ -44,7 +44,7 @@
 // Measured: 8192 tokens, 32 / 8 heads of 128, window 1024, 16 sinks 202 us, 647
 // TFLOP/s, bound like the causal form by the chain of a tile's scores,
 // exponentials and product; 500 tokens over a cache, 16 heads of 64, window 2048
-// 27 us (SINGLE; in pairs 33).
+// 26 us (SINGLE; in pairs 33).
 //
 // Every mbarrier wait is bounded (about 2 s); on time-out the CTA sets an
 // abort flag that all roles poll, winds down, frees its TMEM and sets

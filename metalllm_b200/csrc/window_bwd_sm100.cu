@@ -25,9 +25,9 @@
 // a step where these spend 4 + 3, but it had to zero dQ, add 64 KB a step into
 // L2 and convert the sums: at B=2, 4096 tokens, 16 / 4 heads of 128, window 1000
 // it took 384 us, at up to 64 x 1024, 12 heads of 64, window 250 605 us; these
-// passes take 279 (557 TFLOP/s; the tensor pipe is busy 54 % of the time) and 443
+// passes take 274 (567 TFLOP/s; the tensor pipe is busy 55 % of the time) and 418
 // (units of three steps).  The chain from a step's scores over the row math to
-// its products bounds them.)
+// its products bounds them, at D=64 the row math's instructions.)
 //
 // Pipeline: S of the next step is issued as soon as this step's has been read,
 // and with two dP buffers (all but dK/dV at D=128) dP ahead of this step's
@@ -39,8 +39,8 @@
 // decoding for itself is more code than the instruction cache holds); warp 1
 // issues S and dP, warp 3 the products (one thread for both spent more on waits
 // and addresses than the tensor core on the work: a step 2.9 us); warp 2
-// statistics of the dK/dV pass, and zeroes padding rows of
-// streamed tiles (their P is 0, but 0 * NaN is not).  Warpgroups 1, 2 (184
+// brings the statistics of the dK/dV pass and zeroes padding rows of streamed
+// tiles (their P is 0, but 0 * NaN is not), and passes the step on (Cfg::ONE).  Warpgroups 1, 2 (184
 // registers) compute: thread = row = TMEM lane, 64 columns each.  Warpgroup 3
 // (72 registers) stores a unit's sums while the next unit is under way.
 //
