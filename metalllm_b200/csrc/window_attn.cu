@@ -279,9 +279,9 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM)
           mma16816(o[2 * d + 1], r4, v4[2], v4[3]);
         }
       }
-      // V has been read.  (Without the fence the last ldmatrix can be scheduled
-      // after the arrival, which the compiler orders before them only for plain
-      // loads: a warp held up in between then reads the next block's rows.)
+      // V has been read.  (Without the fence the last ldmatrix of a block could
+      // still be to come at the arrival, and a warp held up there read the next
+      // block's rows: one unit in a few hundred.)
       __threadfence_block();
       __syncwarp();
       if (lane == 0) mbar_arrive(BAR_E(st));
