@@ -16,8 +16,8 @@
 //
 // HBM-bound: each element is read and written once.  A thread owns one unit
 // of a row's rotation (8 pairs of the half layout = two 16-byte vectors, 4
-// pairs of the interleaved one = one vector, or a single pair where `rot`
-// does not allow vectors) and walks heads with it, so a sine is computed once
+// pairs of the interleaved one = one vector, or fewer where `rot` does not
+// allow that) and walks heads with it, so a sine is computed once
 // for the heads of a thread and not once for each head.  Neighbouring lanes
 // take the units of one head and then the next head, so a warp reads whole
 // rows.  A thread loads BATCH heads before it turns the first.  Heads are dealt
@@ -50,7 +50,8 @@ struct RotArgs {
   int hq, hk, D, rot;
   int hsplit;     // threads a row's heads are dealt to
   int units;      // rotation units of one head
-  int cunits;     // copied units of one head: q's and k's columns from rot on
+  int cunits;     // copied units of one head: q's and k's columns from rot on,
+  int edge;       // `edge` pairs up to a multiple of 8, then vectors of 8
   int vunits;     // append: copied units of one head of v
   bool copy_q, copy_k;  // out of place, so the columns from rot on move too
   float amp, sign;      // sign -1: the backward's negative angle
@@ -183,8 +184,20 @@ __device__ __forceinline__ long long cache_row(const RotArgs& a, int b, int t, b
   return valid && pos >= 0 && pos < a.cap ? (long long)b * a.cap + pos : -1;
 }
 
-// P pairs a unit, C elements a copied unit.
-template <typename TQ, bool INTER, int P, int C, bool APPEND>
+// N columns from `in` to `out`, or zeros.
+template <int N, typename T>
+__device__ __forceinline__ void copy(const T* in, T* out, bool zero) {
+  Piece<T, N> x;
+  x.load(in);
+  if (zero) {
+#pragma unroll
+    for (int i = 0; i < N; i += 2) x.set2(i, 0.0f, 0.0f);
+  }
+  x.store(out);
+}
+
+// P pairs a unit.
+template <typename TQ, bool INTER, int P, bool APPEND>
 __global__ void __launch_bounds__(THREADS) rotary_kernel(const RotArgs a) {
   pdl_wait_and_release();
   const int heads = a.hq + a.hk, D = a.D, half = a.rot / 2;
@@ -228,24 +241,24 @@ __global__ void __launch_bounds__(THREADS) rotary_kernel(const RotArgs a) {
     const int b = (int)(row / a.T), t = (int)(row % a.T);
     const bool valid = !APPEND || !a.lens || t < a.lens[b];
     if (u < heads * a.cunits) {
-      const int h = u / a.cunits, at = a.rot + (u % a.cunits) * C;
+      const int h = u / a.cunits, c = u % a.cunits;
+      const bool pair = c < a.edge;
+      const int at = pair ? a.rot + 2 * c : a.rot + 2 * a.edge + 8 * (c - a.edge);
       if (h < a.hq) {
         if (!a.copy_q && valid) continue;
         const long long off = (row * a.hq + h) * D + at;
-        Piece<TQ, C> x;
-        x.load(static_cast<const TQ*>(a.q) + off);
-        if (!valid) {
-#pragma unroll
-          for (int i = 0; i < C; i += 2) x.set2(i, 0.0f, 0.0f);
-        }
-        x.store(static_cast<TQ*>(a.q_out) + off);
+        const TQ* in = static_cast<const TQ*>(a.q) + off;
+        TQ* out = static_cast<TQ*>(a.q_out) + off;
+        if (pair) copy<2>(in, out, !valid);
+        else copy<8>(in, out, !valid);
       } else if (a.copy_k) {
         const long long krow = APPEND ? cache_row(a, b, t, valid) : row;
         if (krow < 0) continue;
         const int kh = h - a.hq;
-        Piece<__nv_bfloat16, C> x;
-        x.load(a.k + (row * a.hk + kh) * D + at);
-        x.store(a.k_out + (krow * a.hk + kh) * D + at);
+        const __nv_bfloat16* in = a.k + (row * a.hk + kh) * D + at;
+        __nv_bfloat16* out = a.k_out + (krow * a.hk + kh) * D + at;
+        if (pair) copy<2>(in, out, false);
+        else copy<8>(in, out, false);
       }
     } else if constexpr (APPEND) {  // v, always in 16-byte pieces
       u -= heads * a.cunits;
@@ -259,7 +272,7 @@ __global__ void __launch_bounds__(THREADS) rotary_kernel(const RotArgs a) {
   }
 }
 
-template <typename TQ, bool INTER, int P, int C, bool APPEND>
+template <typename TQ, bool INTER, int P, bool APPEND>
 cudaError_t launch_as(RotArgs a, cudaStream_t st) {
   int dev = 0, sms = 148;
   cudaGetDevice(&dev);
@@ -267,7 +280,8 @@ cudaError_t launch_as(RotArgs a, cudaStream_t st) {
   const int heads = a.hq + a.hk;
   a.units = a.rot / 2 / P;
   const bool copied = APPEND || a.copy_q || a.copy_k;
-  a.cunits = copied ? (a.D - a.rot) / C : 0;
+  a.edge = copied ? (8 - a.rot % 8) % 8 / 2 : 0;
+  a.cunits = copied ? a.edge + (a.D - a.rot) / 8 : 0;
   a.vunits = APPEND ? a.D / 8 : 0;
   // threads enough for half of what a SM holds, each at least one head (at
   // 16384 rows of 40 heads 57.5 us against 58.5 for all it holds and 63 for a
@@ -279,17 +293,21 @@ cudaError_t launch_as(RotArgs a, cudaStream_t st) {
                           a.rows * ((long long)heads * a.cunits + (APPEND ? a.hk * a.vunits : 0));
   const long long blocks = (total + THREADS - 1) / THREADS;
   const long long most = 1ll << 30;
-  launch_pdl(rotary_kernel<TQ, INTER, P, C, APPEND>, (unsigned)(blocks < most ? blocks : most), THREADS, 0, st, a);
+  launch_pdl(rotary_kernel<TQ, INTER, P, APPEND>, (unsigned)(blocks < most ? blocks : most), THREADS, 0, st, a);
   count_launches(1);
   return cudaGetLastError();
 }
 
-// Vectors where `rot` is a whole number of them, else single pairs.
+// The widest vectors that `rot` is a whole number of.
 template <typename TQ, bool APPEND>
 cudaError_t launch_type(const RotArgs& a, bool inter, cudaStream_t st) {
-  if (inter)
-    return a.rot % 8 == 0 ? launch_as<TQ, true, 4, 8, APPEND>(a, st) : launch_as<TQ, true, 1, 2, APPEND>(a, st);
-  return a.rot % 16 == 0 ? launch_as<TQ, false, 8, 8, APPEND>(a, st) : launch_as<TQ, false, 1, 2, APPEND>(a, st);
+  if (inter) {
+    if (a.rot % 8 == 0) return launch_as<TQ, true, 4, APPEND>(a, st);
+    return a.rot % 4 == 0 ? launch_as<TQ, true, 2, APPEND>(a, st) : launch_as<TQ, true, 1, APPEND>(a, st);
+  }
+  if (a.rot % 16 == 0) return launch_as<TQ, false, 8, APPEND>(a, st);
+  if (a.rot % 8 == 0) return launch_as<TQ, false, 4, APPEND>(a, st);
+  return a.rot % 4 == 0 ? launch_as<TQ, false, 2, APPEND>(a, st) : launch_as<TQ, false, 1, APPEND>(a, st);
 }
 
 RotArgs rot_args(const AttnShape& s, int NKV, const MaRotary& r, bool back) {

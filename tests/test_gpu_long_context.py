@@ -497,6 +497,8 @@ ROTARY = [
     (1, 257, 6, 6, 64, 32, True, None), (1, 50, 2, 1, 128, 64, False, 4000000), (1, 33, 2, 2, 64, 2, False, None),
     (1, 33, 2, 2, 64, 6, True, 12), (2, 65, 3, 3, 128, 126, False, -30), (1, 40, 5, 1, 64, 48, False, None),
     (1, 40, 5, 1, 128, 72, True, 2 ** 31 - 100), (3, 1, 32, 8, 128, 128, True, 7),
+    (2, 37, 3, 1, 64, 24, False, None), (2, 37, 3, 1, 64, 20, False, None), (1, 37, 4, 2, 128, 100, True, 5),
+    (1, 37, 4, 2, 128, 118, True, None), (1, 300, 4, 2, 64, 18, False, None),
 ]
 
 
@@ -543,6 +545,8 @@ def test_rotary_frequencies(A):
 APPEND = [
     (1, 1, 1, 1, 64, 1, 64, False, [0], None), (4, 1, 8, 2, 128, 50, 128, False, [49, 0, 7, 33], [1, 1, 0, 1]),
     (2, 70, 4, 1, 64, 200, 32, True, [0, 130], [70, 33]), (1, 9, 2, 2, 128, 40, 6, False, [31], None),
+    (3, 33, 4, 2, 64, 90, 18, False, [3, 0, 57], [33, 1, 30]), (2, 12, 4, 2, 128, 90, 100, True, [3, 0], [0, 12]),
+    (2, 12, 3, 1, 64, 90, 24, False, [3, 70], [5, 12]), (1, 12, 3, 1, 64, 90, 28, False, [3], [5]),
     (2, 5, 3, 3, 64, 8, 64, True, [6, -2], None),     # rows past the end and before the start are not stored
 ]
 
