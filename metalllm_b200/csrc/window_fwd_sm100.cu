@@ -5,14 +5,14 @@
 // 128-row query tile each, S, P and O in TMEM, lazy rescaling of O), a kernel of
 // its own so that neither carries the other's code.
 //
-// A unit then visits the sink tiles and the tiles from
-// the first row's window on, the tiles that every row sees whole carry no
-// masking code, and a tile in which some row sees nothing is allowed.  Warp 2
+// A unit visits the sink tiles and the tiles from the first row's window on, the
+// tiles that every row sees whole carry no masking code, and a tile in which
+// some row sees nothing is allowed.  Warp 2
 // zeroes the rows of a V tile that no query may see (padding, a cache's rows
 // past the end or out of the window): P is 0 there, but 0 * NaN is not.  Warp 1
 // issues S and warp 3 PV.  SINGLE: a unit is one query tile, not a pair, and the
 // two softmax warpgroups share its key tiles (few units, long windows).
-// Measured: 8192 tokens, 32 / 8 heads of 128, window 1024, 16 sinks 202 us, 647
+// Measured: 8192 tokens, 32 / 8 heads of 128, window 1024, 16 sinks 198 us, 660
 // TFLOP/s, bound like the causal form by the chain of a tile's scores,
 // exponentials and product; 500 tokens over a cache, 16 heads of 64, window 2048
 // 26 us (SINGLE; in pairs 33).
@@ -44,16 +44,12 @@ constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LN2 = 0.6931471805599453f;
 constexpr float RESCALE_THRESHOLD = 8.0f;  // log2 units
 
-template <int HD, bool DYN = false, bool WIN = false>
+template <int HD>
 struct FwdCfg {
   static constexpr int KB = HD / 64;  // 64-column blocks per row
   static constexpr int QST = HD == 64 ? 2 : 1;  // Q-pair stages
   static constexpr int KST = HD == 64 ? 3 : 2;  // K tile stages
   static constexpr int VST = HD == 64 ? 3 : 1;  // V tile stages
-  // UMMA issue order: D=64 issues S_X(j+1) before PV_X(j) (softmax-bound: the
-  // next scores should be ready early); D=128 interleaves PV_X(j), S_X(j+1)
-  // (tensor-bound: keeps PV close to its P)
-  static constexpr bool EARLY_S = HD == 64;
   // D=64: P_X lives in TMEM (bf16 pairs) and PV_X reads it from there, which
   // halves the shared-memory traffic of the tensor core; D=128 has no TMEM
   // columns left and stages P in shared memory
@@ -68,26 +64,21 @@ struct FwdCfg {
   static constexpr uint32_t OFF_K = OFF_Q + QST * 2 * QT_BYTES;  // [KST]
   static constexpr uint32_t OFF_V = OFF_K + KST * KV_BYTES;      // [VST]
   static constexpr uint32_t OFF_P = OFF_V + VST * KV_BYTES;      // [2 tiles] P / O staging
-  // D=64: an all-zero fp32 tile (128 rows x 32 columns) that TMA stores copy
-  // into dQ when the forward zeroes it for an accumulating backward
-  static constexpr uint32_t ZT_BYTES = P_TMEM && !WIN ? BM * 32 * 4 : 0;
-  static constexpr uint32_t OFF_ZT = OFF_P + 2 * STG_BYTES;
   // the unit schedule: NSCHED 16-byte launch-control responses
-  static constexpr int NSCHED = DYN ? (int)kSchedSlots : 0;  // dynamic schedule only
-  // dynamic schedule's unit order: blocks of HB (batch, head) pairs at D=128
-  // (their query pairs share K/V in L2: C3 forward -4.6 %), one block at D=64
-  // (C4: blocks of 8-32 heads measured 1-2 % slower)
-  static constexpr int HB = (DYN && HD == 128) ? 16 : 0;
-  // WIN: B's maximum and sum of each row, for A to join
-  static constexpr uint32_t OFF_ML = OFF_ZT + ZT_BYTES;
-  static constexpr uint32_t ML_BYTES = WIN ? BM * 8 : 0;
+  static constexpr int NSCHED = (int)kSchedSlots;
+  // unit order: blocks of HB (batch, head) pairs at D=128, whose query tiles share
+  // K/V in L2, one block at D=64 (blocks of 16 at 64 x 1024, 12 heads of 64, window
+  // 250: 258 us against 216)
+  static constexpr int HB = HD == 128 ? 16 : 0;
+  // SINGLE: B's maximum and sum of each row, for A to join
+  static constexpr uint32_t OFF_ML = OFF_P + 2 * STG_BYTES;
+  static constexpr uint32_t ML_BYTES = BM * 8;
   static constexpr uint32_t OFF_SCHED = OFF_ML + ML_BYTES;
   static constexpr uint32_t OFF_BAR = OFF_SCHED + NSCHED * 16;
   // q_full/empty[QST], k_full/empty[KST], v_full/empty[VST], per tile X:
-  // s_full, s_free, p_full, pv_done, o_free, do_full; then never (nothing
-  // arrives: the time-out test hook), fin (the UMMA issuer's wind-down),
-  // sched_full/empty[NSCHED] and, for WIN, v_fixed[VST], a second fin and b_done
-  static constexpr int NBAR = 2 * QST + 2 * KST + 2 * VST + 2 * 6 + 2 + 2 * NSCHED + (WIN ? VST + 2 : 0);
+  // s_full, s_free, p_full, pv_done, o_free; then fin (the S issuer's wind-down),
+  // sched_full/empty[NSCHED], v_fixed[VST], fin of the PV issuer and b_done
+  static constexpr int NBAR = 2 * QST + 2 * KST + 2 * VST + 2 * 5 + 1 + 2 * NSCHED + VST + 2;
   static constexpr uint32_t OFF_TSLOT = OFF_BAR + NBAR * 8;
   static constexpr uint32_t SMEM_BYTES = OFF_TSLOT + 16 + 1024;  // + alignment slack
   static constexpr uint32_t TCOL_S = 0;     // S_A, S_B at columns 0, 128
@@ -98,51 +89,20 @@ struct FwdCfg {
 };
 
 struct FwdParams {
-  int T, NH, bh_begin, nbh, npairs, nqt;
+  int T, NH, nbh, npairs, nqt;
   int nunits;
   float scale_log2;
   float* lse;
   uint32_t* status;
-  // fused computeD (D = 64 only, both or neither set): D[row][h] =
-  // bf16(sum_c O[row][h*64+c] * dO[row][h*64+c]) from the bf16-rounded O
-  const __nv_bfloat16* dO;
-  __nv_bfloat16* D;
-  // optional (D=64): zeros are written to dQ's slab of every query tile the
-  // kernel computes (by TMA stores, tensor map tmdQz), for a backward that
-  // then accumulates into dQ
-  float* dQz;
-  uint32_t expire_ns;  // time-out test hook (ma_debug_expire_next_wait), 0 = off
-  WindowArgs win;      // WIN only
+  WindowArgs win;
 };
 
-// sum over 8 bf16 pairs of a[i] * b[i], fp32 (products of bf16 values are
-// exact in fp32)
-__device__ __forceinline__ float dot_bf16x8(uint4 a, uint4 b) {
-  const __nv_bfloat162* x = reinterpret_cast<const __nv_bfloat162*>(&a);
-  const __nv_bfloat162* y = reinterpret_cast<const __nv_bfloat162*>(&b);
-  float s = 0.0f;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 fx = __bfloat1622float2(x[i]), fy = __bfloat1622float2(y[i]);
-    s = fmaf(fx.x, fy.x, s);
-    s = fmaf(fx.y, fy.y, s);
-  }
-  return s;
-}
-
-// Work units, heaviest first (causal work grows with the pair index):
-// k -> (pair = npairs-1 - k / nbh, bh = bh_begin + k % nbh), dealt in one of
-// two ways.  Static (up to 16 query tiles): one CTA per SM, units in rounds of
-// G = gridDim.x in alternating direction (round g gives CTA c unit g*G + c
-// for even g and g*G + G-1-c for odd g), which balances the decreasing unit
-// sizes across CTAs.  Dynamic (longer sequences, whose units differ more in
-// size): one CTA per unit; a running CTA takes its own unit (k = blockIdx.x)
-// and then, by cluster launch control, the units of CTAs that have not
-// started yet, in launch order, so units go greedily to whichever SM is free.
-// With HB > 0 (the dynamic schedule at D=128) the order is blocked instead:
-// block k / (HB*npairs) holds HB (batch, head) pairs (fewer in the last
-// block), heaviest pair first within it, so the units in flight share their
-// heads' K/V tiles in L2 and the grid still ends on light units.
+// Work units, one CTA each, later queries first: k -> (pair = npairs-1 - k / nbh,
+// bh = k % nbh).  A running CTA takes its own unit (k = blockIdx.x) and then, by
+// cluster launch control, the units of CTAs that have not started yet, in launch
+// order, so units go greedily to whichever SM is free.  With HB > 0 the order is
+// blocked: block k / (HB*npairs) holds HB (batch, head) pairs (fewer in the last
+// block), whose units in flight share their heads' K/V tiles in L2.
 struct Unit {
   int pair, b, h, nA, nB, nkv;
 };
@@ -156,16 +116,13 @@ __device__ __forceinline__ Unit decode_unit(const FwdParams& prm, int k) {
     const int blk = k / per, r = k % per;
     const int hb = min(HB, prm.nbh - blk * HB);
     x.pair = prm.npairs - 1 - r / hb;
-    bh = prm.bh_begin + blk * HB + r % hb;
+    bh = blk * HB + r % hb;
   } else {
     x.pair = prm.npairs - 1 - k / prm.nbh;
-    bh = prm.bh_begin + k % prm.nbh;
+    bh = k % prm.nbh;
   }
   x.b = bh / prm.NH;
   x.h = bh % prm.NH;
-  x.nA = 2 * x.pair + 1;                                   // key tiles 0..2p
-  x.nB = (2 * x.pair + 1 < prm.nqt) ? 2 * x.pair + 2 : 0;  // tile B inside T?
-  x.nkv = x.nB > 0 ? x.nB : x.nA;
   return x;
 }
 
@@ -248,22 +205,12 @@ __device__ __forceinline__ WinUnit decode_win_unit(const FwdParams& prm, int k) 
   return x;
 }
 
-// Static schedule: the g-th unit of this CTA, or -1 when it has none left.
-__device__ __forceinline__ int unit_of_round(const FwdParams& prm, int g) {
-  const int G = gridDim.x;
-  const long long k = (long long)g * G + ((g & 1) ? G - 1 - (int)blockIdx.x : (int)blockIdx.x);
-  // past the end only in the last (partial) round: nothing follows it
-  return k < prm.nunits ? (int)k : -1;
-}
-
-template <int HD, bool DYN, bool WIN, bool SINGLE>
+template <int HD, bool SINGLE>
 __global__ void __launch_bounds__(NUM_THREADS, 1)
-    flash_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+    window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                      const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmO,
-                     const __grid_constant__ CUtensorMap tmdO, const __grid_constant__ CUtensorMap tmdQz,
                      const FwdParams prm) {
-  if constexpr (!WIN) pdl_wait_and_release();  // WIN: after the set-up below
-  using C = FwdCfg<HD, DYN, WIN>;
+  using C = FwdCfg<HD>;
   extern __shared__ uint8_t smem_raw[];
   __shared__ int abort_flag;
   const uint32_t raw = smem_u32(smem_raw);
@@ -285,23 +232,17 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   auto BAR_PF = [&](int x) { return barX + 8u * (2 * 2 + x); };
   auto BAR_PV = [&](int x) { return barX + 8u * (3 * 2 + x); };
   auto BAR_OE = [&](int x) { return barX + 8u * (4 * 2 + x); };
-  auto BAR_DO = [&](int x) { return barX + 8u * (5 * 2 + x); };  // dO tile of X landed (fused computeD)
-  const uint32_t BAR_NEVER = barX + 8u * 12;  // nothing arrives (time-out test hook)
-  const uint32_t BAR_FIN = barX + 8u * 13;    // the UMMA issuer's last commit (wind-down)
-  auto BAR_UF = [&](int s) { return barX + 8u * (14 + s); };              // response s landed
-  auto BAR_UE = [&](int s) { return barX + 8u * (14 + C::NSCHED + s); };  // response s read by all
-  auto BAR_VZ = [&](int s) { return barX + 8u * (14 + 2 * C::NSCHED + s); };  // WIN: V slot s zeroed where it must be
-  const uint32_t BAR_FIN2 = barX + 8u * (14 + 2 * C::NSCHED + C::VST);  // WIN: the PV issuer's wind-down
-  const uint32_t BAR_MG = BAR_FIN2 + 8;  // WIN: B's part of a shared tile is complete
-  // dynamic schedule: unit g >= 1 of this CTA is the one launch-control
-  // response g-1 names (requested by the TMA producer when it starts unit
-  // g-1); readers: the producer, the UMMA issuer (WIN: both), the 8 softmax
-  // warps and, for WIN, the warp that zeroes V rows
-  constexpr uint32_t SCHED_READERS = WIN ? 12 : 10;
-  auto unit = [&](int k) {
-    if constexpr (WIN) return decode_win_unit<C::HB, SINGLE>(prm, k);
-    else return decode_unit<C::HB>(prm, k);
-  };
+  const uint32_t BAR_FIN = barX + 8u * 10;    // the S issuer's last commit (wind-down)
+  auto BAR_UF = [&](int s) { return barX + 8u * (11 + s); };              // response s landed
+  auto BAR_UE = [&](int s) { return barX + 8u * (11 + C::NSCHED + s); };  // response s read by all
+  auto BAR_VZ = [&](int s) { return barX + 8u * (11 + 2 * C::NSCHED + s); };  // V slot s zeroed where it must be
+  const uint32_t BAR_FIN2 = barX + 8u * (11 + 2 * C::NSCHED + C::VST);  // the PV issuer's wind-down
+  const uint32_t BAR_MG = BAR_FIN2 + 8;  // B's part of a shared tile is complete
+  // unit g >= 1 of this CTA is the one launch-control response g-1 names
+  // (requested by the TMA producer when it starts unit g-1); readers: the
+  // producer, both issuers, the warp that zeroes V rows and the 8 softmax warps
+  constexpr uint32_t SCHED_READERS = 12;
+  auto unit = [&](int k) { return decode_win_unit<C::HB, SINGLE>(prm, k); };
   const uint32_t tslot = sbase + C::OFF_TSLOT;
 
   if (threadIdx.x == 0) {
@@ -316,7 +257,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     }
     for (int s = 0; s < C::VST; ++s) {
       mbar_init(BAR_VF(s), 1);
-      mbar_init(BAR_VE(s), WIN ? 2 : 1);  // WIN: the warp that zeroes rows, too
+      mbar_init(BAR_VE(s), 2);  // PV, and the warp that zeroes rows
     }
     for (int x = 0; x < 2; ++x) {
       mbar_init(BAR_SF(x), 1);
@@ -324,36 +265,26 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       mbar_init(BAR_PF(x), 128);
       mbar_init(BAR_PV(x), 1);
       mbar_init(BAR_OE(x), 128);
-      mbar_init(BAR_DO(x), 1);
     }
-    mbar_init(BAR_NEVER, 1);
     mbar_init(BAR_FIN, 1);
     for (int u = 0; u < C::NSCHED; ++u) {
       mbar_init(BAR_UF(u), 1);
       mbar_init(BAR_UE(u), SCHED_READERS);
     }
-    if constexpr (WIN)
-    {
-      for (int s = 0; s <= C::VST; ++s) mbar_init(BAR_VZ(s), 1);  // and BAR_FIN2
-      mbar_init(BAR_MG, 128);
-    }
+    for (int s = 0; s <= C::VST; ++s) mbar_init(BAR_VZ(s), 1);  // and BAR_FIN2
+    mbar_init(BAR_MG, 128);
     fence_mbar_init();
   }
   if (warp == 1) {
     tmem_alloc(tslot, 512);
     tmem_relinquish();
   }
-  if (C::ZT_BYTES && prm.dQz) {  // the zero tile the dQ stores copy from
-    for (uint32_t i = threadIdx.x; i < C::ZT_BYTES / 16; i += NUM_THREADS)
-      reinterpret_cast<uint4*>(gbase + C::OFF_ZT)[i] = make_uint4(0u, 0u, 0u, 0u);
-    fence_proxy_async_smem();
-  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   // nothing before here touches global memory, so the barriers and TMEM are set
   // up while the kernel before is still draining
-  if constexpr (WIN) pdl_wait_and_release();
+  pdl_wait_and_release();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(gbase + C::OFF_TSLOT);
   volatile int* abort_p = &abort_flag;
   const Sched sch{sbase + C::OFF_SCHED, BAR_UF(0), BAR_UE(0), abort_p};
@@ -369,43 +300,35 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       uint32_t nreq = 0;  // launch-control requests issued (request r names unit r+1)
       bool ok = true;
       for (int g = 0; ok; ++g) {
-        int k;
-        if constexpr (DYN) k = sched_unit<false>(sch, g);
-        else k = unit_of_round(prm, g);
+        const int k = sched_unit<false>(sch, g);
         if (k < 0) break;
-        // dynamic: request unit g+1 now, a unit ahead of every reader
-        if constexpr (DYN) {
-          if (!sched_request(sch, nreq)) break;
-          ++nreq;
-        }
+        // request unit g+1 now, a unit ahead of every reader
+        if (!sched_request(sch, nreq)) break;
+        ++nreq;
         const auto un = unit(k);
         const int col0 = un.h * HD;
-        const int kv0 = WIN ? un.h / (prm.win.NH / prm.win.NKV) * HD : col0;  // columns of the K/V head
-        if (WIN && un.nkv == 0) continue;  // only padding
-        int tile0 = 2 * un.pair;
-        if constexpr (WIN) tile0 = un.tile0;
+        const int kv0 = un.h / (prm.win.NH / prm.win.NKV) * HD;  // columns of the K/V head
+        if (un.nkv == 0) continue;  // only padding
         const int qs = qc % C::QST;
-        if (qc >= C::QST && !wait_on<WIN>(BAR_QE(qs), ((qc / C::QST) - 1) & 1, abort_p)) break;
-        int ntile = un.nB > 0 ? 2 : 1;
-        if (WIN && SINGLE) ntile = 1;
+        if (qc >= C::QST && !mbar_poll(BAR_QE(qs), ((qc / C::QST) - 1) & 1, abort_p)) break;
+        const int ntile = !SINGLE && un.nB > 0 ? 2 : 1;
         mbar_arrive_expect_tx(BAR_QF(qs), ntile * C::QT_BYTES);
         for (int x = 0; x < ntile; ++x)
           for (int kb = 0; kb < C::KB; ++kb)
             tma_load_3d(sbase + C::OFF_Q + (qs * 2 + x) * C::QT_BYTES + kb * BM * 128, &tmQ,
-                        BAR_QF(qs), col0 + kb * 64, (tile0 + x) * BM, un.b);
+                        BAR_QF(qs), col0 + kb * 64, (un.tile0 + x) * BM, un.b);
         ++qc;
         for (int j = 0; j < un.nkv; ++j) {
-          int kt = j;
-          if constexpr (WIN) kt = un.key_tile(j);
+          const int kt = un.key_tile(j);
           const int ks = kc % C::KST;
-          if (kc >= C::KST && !wait_on<WIN>(BAR_KE(ks), ((kc / C::KST) - 1) & 1, abort_p)) { ok = false; break; }
+          if (kc >= C::KST && !mbar_poll(BAR_KE(ks), ((kc / C::KST) - 1) & 1, abort_p)) { ok = false; break; }
           mbar_arrive_expect_tx(BAR_KF(ks), C::KV_BYTES);
           for (int kb = 0; kb < C::KB; ++kb)
             tma_load_3d(sbase + C::OFF_K + ks * C::KV_BYTES + kb * BN * 128, &tmK, BAR_KF(ks),
                         kv0 + kb * 64, kt * BN, un.b);
           ++kc;
           const int vs = vc % C::VST;
-          if (vc >= C::VST && !wait_on<WIN>(BAR_VE(vs), ((vc / C::VST) - 1) & 1, abort_p)) { ok = false; break; }
+          if (vc >= C::VST && !mbar_poll(BAR_VE(vs), ((vc / C::VST) - 1) & 1, abort_p)) { ok = false; break; }
           mbar_arrive_expect_tx(BAR_VF(vs), C::KV_BYTES);
           for (int kb = 0; kb < C::KB; ++kb)
             tma_load_3d(sbase + C::OFF_V + vs * C::KV_BYTES + kb * BN * 128, &tmV, BAR_VF(vs),
@@ -414,126 +337,16 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         }
       }
       if (*abort_p) {  // wind-down: let the loads and the request still in flight land
-        if (DYN) sched_drain(sch, nreq);
+        sched_drain(sch, nreq);
         drain_ring(BAR_QF, C::QST, qc);
         drain_ring(BAR_KF, C::KST, kc);
         drain_ring(BAR_VF, C::VST, vc);
       }
-    } else if (!WIN && warp == 1 && lane == 0) {
-      // ----------------------------------------------------------- MMA
-      constexpr uint32_t IDESC_S = idesc_bf16_f32(BM, BN, 0, 0);
-      constexpr uint32_t IDESC_O = idesc_bf16_f32(BM, HD, 0, 1);
-      uint32_t qc = 0, kc = 0, vc = 0;
-      uint32_t sc[2] = {0, 0};   // S_X issued so far
-      uint32_t pvc[2] = {0, 0};  // PV_X issued so far
-      uint32_t uc[2] = {0, 0};   // units in which tile X was active
-      bool ok = true;
-      for (int g = 0; ok; ++g) {
-        int k;
-        if constexpr (DYN) k = sched_unit<false>(sch, g);
-        else k = unit_of_round(prm, g);
-        if (k < 0) break;
-        const auto un = unit(k);
-        const int n[2] = {un.nA, un.nB};
-        const int qs = qc % C::QST;
-        if (!mbar_wait(BAR_QF(qs), (qc / C::QST) & 1, abort_p)) break;
-        // S_X(j) = Q_X K_j^T
-        auto issue_s = [&](int x, int j) -> bool {
-          if (sc[x] >= 1 && !mbar_wait(BAR_SE(x), (sc[x] - 1) & 1, abort_p)) return false;
-          tc_fence_after();
-          const uint32_t sq = sbase + C::OFF_Q + (qs * 2 + x) * C::QT_BYTES;
-          const uint32_t sk = sbase + C::OFF_K + ((kc + j) % C::KST) * C::KV_BYTES;
-#pragma unroll
-          for (int kk = 0; kk < HD / 16; ++kk) {
-            const uint32_t off = (kk >> 2) * (BM * 128) + (kk & 3) * 32;
-            umma_bf16_ss(tmem + C::TCOL_S + x * BN, smem_desc_sw128(sq + off, 16, 1024),
-                         smem_desc_sw128(sk + off, 16, 1024), IDESC_S, kk > 0 ? 1u : 0u);
-          }
-          umma_commit(BAR_SF(x));
-          ++sc[x];
-          return true;
-        };
-        // O_X += P_X V_j
-        auto issue_pv = [&](int x, int j) -> bool {
-          if (!mbar_wait(BAR_PF(x), pvc[x] & 1, abort_p)) return false;
-          if (j == 0 && uc[x] >= 1 && !mbar_wait(BAR_OE(x), (uc[x] - 1) & 1, abort_p)) return false;
-          tc_fence_after();
-          const uint32_t sp = sbase + C::OFF_P + x * C::STG_BYTES;
-          const uint32_t sv = sbase + C::OFF_V + ((vc + j) % C::VST) * C::KV_BYTES;
-#pragma unroll
-          for (int kk = 0; kk < BN / 16; ++kk) {
-            const uint64_t bd = smem_desc_sw128(sv + kk * 2048, BN * 128, 1024);
-            if (C::P_TMEM) {  // A = P_X from TMEM: 8 columns per 16 keys
-              umma_bf16_ts(tmem + C::TCOL_O + x * HD, tmem + C::TCOL_P + x * (BN / 2) + kk * 8, bd,
-                           IDESC_O, (j > 0 || kk > 0) ? 1u : 0u);
-            } else {
-              const uint64_t ad = smem_desc_sw128(sp + (kk >> 2) * (BM * 128) + (kk & 3) * 32, 16, 1024);
-              umma_bf16_ss(tmem + C::TCOL_O + x * HD, ad, bd, IDESC_O, (j > 0 || kk > 0) ? 1u : 0u);
-            }
-          }
-          umma_commit(BAR_PV(x));
-          ++pvc[x];
-          return true;
-        };
-        auto wait_k = [&](int j) {
-          const uint32_t k = kc + j;
-          return mbar_wait(BAR_KF(k % C::KST), (k / C::KST) & 1, abort_p);
-        };
-        auto wait_v = [&](int j) {
-          const uint32_t v = vc + j;
-          return mbar_wait(BAR_VF(v % C::VST), (v / C::VST) & 1, abort_p);
-        };
-        // prologue: S_A(0), S_B(0); K_0 is consumed once both are done
-        ok = wait_k(0) && issue_s(0, 0) && (n[1] == 0 || issue_s(1, 0));
-        if (ok) umma_commit(BAR_KE(kc % C::KST));
-        // time-out test hook: with the first products in flight, wait on a
-        // barrier nothing arrives at until the hook's limit runs out
-        if (ok && g == 0 && prm.expire_ns) ok = mbar_wait(BAR_NEVER, 0, abort_p, prm.expire_ns);
-        for (int j = 0; ok && j < un.nkv; ++j) {
-          if (C::EARLY_S) {
-            // S_X(j+1) as soon as softmax X has read S_X(j) (issue_s waits for
-            // that), so the next scores are ready before this tile's softmax ends
-            if (j + 1 < un.nkv) {
-              if (!wait_k(j + 1)) { ok = false; break; }
-              if (j + 1 < n[0] && !issue_s(0, j + 1)) { ok = false; break; }
-              if (j + 1 < n[1] && !issue_s(1, j + 1)) { ok = false; break; }
-              umma_commit(BAR_KE((kc + j + 1) % C::KST));  // K_{j+1} consumed
-            }
-            if (!wait_v(j)) { ok = false; break; }
-            if (j < n[0] && !issue_pv(0, j)) { ok = false; break; }
-            if (j < n[1] && !issue_pv(1, j)) { ok = false; break; }
-          } else {
-            // PV_A(j) S_A(j+1) | PV_B(j) S_B(j+1)
-            if (!wait_v(j)) { ok = false; break; }
-            const bool lastA = (j + 1 >= n[0]);
-            if (j < n[0]) {
-              if (!issue_pv(0, j)) { ok = false; break; }
-              if (!lastA && (!wait_k(j + 1) || !issue_s(0, j + 1))) { ok = false; break; }
-            }
-            if (j < n[1]) {
-              if (!issue_pv(1, j)) { ok = false; break; }
-              if (j + 1 < n[1] && ((lastA && !wait_k(j + 1)) || !issue_s(1, j + 1))) { ok = false; break; }
-            }
-            if (j + 1 < un.nkv) umma_commit(BAR_KE((kc + j + 1) % C::KST));  // K_{j+1} consumed
-          }
-          umma_commit(BAR_VE((vc + j) % C::VST));           // V_j consumed
-          if (j + 1 == un.nkv) umma_commit(BAR_QE(qs));     // every S of the unit issued
-        }
-        kc += un.nkv;
-        vc += un.nkv;
-        ++qc;
-        for (int x = 0; x < 2; ++x)
-          if (n[x] > 0) ++uc[x];
-      }
-      if (*abort_p) {  // wind-down: every UMMA issued must complete before TMEM is freed
-        umma_commit(BAR_FIN);
-        mbar_wait_for(BAR_FIN, 0, kDrainLimitNs);
-      }
-    } else if (WIN && warp == 1 && lane == 0) {
+    } else if (warp == 1 && lane == 0) {
       // ---------------------------------------------------- S, under a window
       // S_X(j) = Q_X K_j^T, as soon as softmax X has read S_X(j-1).  Another
       // warp issues the products with V, so neither waits for the other's tile.
-      if constexpr (WIN) {
+      {
         constexpr uint32_t IDESC_S = idesc_bf16_f32(BM, BN, 0, 0);
         constexpr uint32_t IDESC_SN = idesc_bf16_f32(BM, NARROW, 0, 0);
         uint32_t qc = 0, kc = 0, sc[2] = {0, 0};
@@ -577,10 +390,10 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
           mbar_wait_for(BAR_FIN, 0, kDrainLimitNs);
         }
       }
-    } else if (WIN && warp == 3 && lane == 0) {
+    } else if (warp == 3 && lane == 0) {
       // --------------------------------------------------- PV, under a window
       // O_X += P_X V_j, once softmax X has written P_X(j)
-      if constexpr (WIN) {
+      {
         constexpr uint32_t IDESC_O = idesc_bf16_f32(BM, HD, 0, 1);
         uint32_t vc = 0, pvc[2] = {0, 0}, uc[2] = {0, 0};
         uint32_t vzp = 0;  // bit s = parity of v_fixed[s]'s next phase
@@ -632,9 +445,9 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
           mbar_wait_for(BAR_FIN2, 0, kDrainLimitNs);
         }
       }
-    } else if (WIN && warp == 2) {
+    } else if (warp == 2) {
       // ------------------------------------------------ unseen rows of V
-      if constexpr (WIN) {
+      {
         uint32_t vc = 0;
         bool ok = true;
         for (int g = 0; ok; ++g) {
@@ -646,7 +459,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
             // within one phase of each slot's barriers
             const int k0 = un.key_tile(j) * BN;
             const uint32_t v = vc + j, vs = v % C::VST;
-            ok = wait_on_warp<WIN>(BAR_VF(vs), (v / C::VST) & 1, abort_p);
+            ok = mbar_poll_warp(BAR_VF(vs), (v / C::VST) & 1, abort_p);
             if (!ok) break;
             if (!un.fix(prm.win, k0)) {
               if (lane == 0) mbar_arrive(BAR_VE(vs));
@@ -687,21 +500,16 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     const bool wg_leader = (warp == 4 + 4 * x) && lane == 0;
     uint8_t* pbuf = gbase + C::OFF_P + x * C::STG_BYTES;
     uint32_t sc = 0;  // S_X consumed so far (== P_X produced)
-    uint32_t nd = 0;  // dO tiles of X consumed so far (fused computeD)
-    uint32_t nd_armed = 0;  // dO tile loads issued (leader)
-    uint32_t nmg = 0;       // WIN, A: shared tiles joined so far
-    uint32_t scb = 0;       // WIN, A: key tiles B has worked on in them
+    uint32_t nmg = 0;       // A: shared tiles joined so far
+    uint32_t scb = 0;       // A: key tiles B has worked on in them
     bool ok = true;
     for (int g = 0; ok; ++g) {
-      int k;
-      if constexpr (DYN) k = sched_unit<true>(sch, g);
-      else k = unit_of_round(prm, g);
+      const int k = sched_unit<true>(sch, g);
       if (k < 0) break;
       const auto un = unit(k);
       const int nt = x == 0 ? un.nA : un.nB;
-      int qtile = 2 * un.pair + x;
-      if constexpr (WIN) {
-        qtile = un.tile0 + (SINGLE ? 0 : x);
+      const int qtile = un.tile0 + (SINGLE ? 0 : x);
+      {
         if (nt == 0) {  // only padding: O = 0, l = -inf (rows past T are clipped)
           if ((SINGLE && x == 1) || qtile * BM >= prm.T) continue;
           if (wg_leader) bulk_wait_read<0>();
@@ -722,20 +530,10 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
           }
           continue;
         }
-      } else {
-        if (nt == 0) continue;
-      }
-      if (C::ZT_BYTES && prm.dQz && wg_leader) {
-        // this query tile's dQ slab (128 rows x HD fp32; rows past T are
-        // clipped) from the zero tile, by TMA stores that need no waiting for
-        for (int box = 0; box < HD / 32; ++box)
-          tma_store_3d(&tmdQz, sbase + C::OFF_ZT, un.h * HD + box * 32, qtile * BM, un.b);
-        bulk_commit();
       }
       // the previous unit's O store must have read the staging before it is
       // written again: at D=128 it holds P from this unit's first tile on, so
-      // wait here; at D=64 (P in TMEM) it is next written by this unit's dO
-      // load or epilogue, which wait there instead, so this unit's first
+      // wait here; at D=64 (P in TMEM) the epilogue waits, so this unit's first
       // tiles overlap the store
       if constexpr (!C::P_TMEM) {
         if (sc >= 1 && wg_leader) bulk_wait_read<0>();
@@ -748,20 +546,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       auto tile = [&](auto diag_tag, auto nc_tag, int j) -> bool {
         constexpr bool DIAG = decltype(diag_tag)::value;
         constexpr int NC = decltype(nc_tag)::value;
-        if constexpr (DIAG && C::P_TMEM && !WIN) {
-          // the unit's last key tile: the dO tile of X goes by TMA into the O
-          // staging (idle until the epilogue; rows past T read as zero); the
-          // epilogue reads each chunk back before writing O over it
-          if (prm.dO && wg_leader) {
-            bulk_wait_read<0>();  // the previous unit's O store has read the staging
-            mbar_arrive_expect_tx(BAR_DO(x), BM * HD * 2);
-            ++nd_armed;
-            for (int kb = 0; kb < C::KB; ++kb)
-              tma_load_3d(smem_u32(pbuf) + kb * BM * 128, &tmdO, BAR_DO(x), un.h * HD + kb * 64, qtile * BM,
-                          un.b);
-          }
-        }
-        if (!wait_on_warp<WIN>(BAR_SF(x), sc & 1, abort_p)) return false;
+        if (!mbar_poll_warp(BAR_SF(x), sc & 1, abort_p)) return false;
         tc_fence_after();
         float s[NC];
         if constexpr (NC == 32) {
@@ -786,7 +571,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         }
         tc_fence_before();
         mbar_arrive(BAR_SE(x));
-        if constexpr (WIN) {
+        {
           if constexpr (DIAG) {
             // key k0 + i is visible up to the row's own position, and from its
             // window's first key on or among the sinks; 32 keys to a word of
@@ -802,10 +587,6 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
                 if (!(see & (1u << i))) s[w + i] = -INFINITY;
             }
           }
-        } else if constexpr (DIAG) {
-#pragma unroll
-          for (int i = 0; i < BN; ++i)
-            if (i > row) s[i] = -INFINITY;
         }
         // row maximum: 8 independent partial maxima, 3-input max (short chains)
         float pm[8];
@@ -822,8 +603,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         // m_used; O_X is rescaled below, once PV_X(j-1) has completed
         bool rescale = false;
         float alpha = 1.0f;
-        bool first = j == 0;
-        if constexpr (WIN) first = j == un.first(x);
+        const bool first = j == un.first(x);
         if (first) {
           m_used = m_new;
         } else {
@@ -836,8 +616,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
           }
         }
         // P = 2^(S*c - m) with packed fp32x2 FMAs; row sum in 4 packed partials
-        // (WIN: a row that has seen no key yet has m = -inf and P = 2^-inf = 0)
-        const float base = WIN && m_used == -INFINITY ? 0.0f : m_used;
+        // (a row that has seen no key yet has m = -inf and P = 2^-inf = 0)
+        const float base = m_used == -INFINITY ? 0.0f : m_used;
         const float2 c2 = make_float2(c, c), nm2 = make_float2(-base, -base);
         float2 ps[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f),
                         make_float2(0.f, 0.f)};
@@ -854,7 +634,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         // PV_X(j-1) must be complete before O_X is rescaled and before P_X(j)
         // overwrites P_X (waited for only now, so the exponentials overlap it)
         if (!first) {
-          if (!wait_on_warp<WIN>(BAR_PV(x), (sc - 1) & 1, abort_p)) return false;
+          if (!mbar_poll_warp(BAR_PV(x), (sc - 1) & 1, abort_p)) return false;
           tc_fence_after();
         }
         if (rescale) {
@@ -898,27 +678,19 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       };
       using All = std::integral_constant<int, BN>;
       for (int j = 0; ok && j < nt; ++j) {
-        if constexpr (WIN) {
-          if (!un.active(x, j)) continue;
-          if (un.narrow(prm.win, j)) ok = tile(std::true_type{}, std::integral_constant<int, NARROW>{}, j);
-          else if (un.whole(prm.win, x, un.key_tile(j) * BN)) ok = tile(std::false_type{}, All{}, j);
-          else ok = tile(std::true_type{}, All{}, j);
-        } else {
-          ok = (j == qtile) ? tile(std::true_type{}, All{}, j) : tile(std::false_type{}, All{}, j);
-        }
+        if (!un.active(x, j)) continue;
+        if (un.narrow(prm.win, j)) ok = tile(std::true_type{}, std::integral_constant<int, NARROW>{}, j);
+        else if (un.whole(prm.win, x, un.key_tile(j) * BN)) ok = tile(std::false_type{}, All{}, j);
+        else ok = tile(std::true_type{}, All{}, j);
       }
       // --------------------------------------------- epilogue of tile X
-      bool epi = ok && wait_on_warp<WIN>(BAR_PV(x), (sc - 1) & 1, abort_p);
+      bool epi = ok && mbar_poll_warp(BAR_PV(x), (sc - 1) & 1, abort_p);
       if constexpr (C::P_TMEM) {
-        // without dO the epilogue is the staging's first writer in this unit
-        // (with dO the warpgroup waits for the dO load, issued after the wait)
-        if (WIN || !prm.dO) {
-          if (wg_leader) bulk_wait_read<0>();
-          bar_sync_named(wg_bar, 128);
-        }
+        // the epilogue is the staging's first writer in this unit
+        if (wg_leader) bulk_wait_read<0>();
+        bar_sync_named(wg_bar, 128);
       }
-      bool joined = false;
-      if constexpr (WIN) joined = SINGLE && un.nB > 0;
+      const bool joined = SINGLE && un.nB > 0;
       if (joined && x == 1) {
         // this half's maximum and sum; O_B stays in TMEM, where A reads it
         if (epi) {
@@ -932,8 +704,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       float fa = 1.0f, fb = 0.0f;  // factors of O_A and O_B
       if (joined) {
         scb += un.nkv / 2;
-        epi = epi && wait_on_warp<WIN>(BAR_MG, nmg++ & 1, abort_p) &&
-              wait_on_warp<WIN>(BAR_PV(1), (scb - 1) & 1, abort_p);
+        epi = epi && mbar_poll_warp(BAR_MG, nmg++ & 1, abort_p) &&
+              mbar_poll_warp(BAR_PV(1), (scb - 1) & 1, abort_p);
         if (epi) {
           const float2 ml = reinterpret_cast<const float2*>(gbase + C::OFF_ML)[row];
           const float top = fmaxf(m_used, ml.x), base = top == -INFINITY ? 0.0f : top;
@@ -947,12 +719,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         tc_fence_after();
         const float inv = 1.0f / l_sum;
         const int grow = qtile * BM + row;
-        bool valid = true;
-        if constexpr (WIN) valid = grow < un.n;
-        const bool fuse_d = C::P_TMEM && !WIN && prm.dO;
-        bool dok = true;
-        if (fuse_d) dok = wait_on_warp<WIN>(BAR_DO(x), nd & 1, abort_p);
-        float dsum = 0.0f;
+        const bool valid = grow < un.n;
         // stage O (bf16) in this tile's P buffer (free: its last PV is done);
         // O is read from TMEM 64 columns (two loads, one wait) at a time
 #pragma unroll
@@ -961,7 +728,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
           tmem_ld32(trow + tcol_o + c64, ra);
           tmem_ld32(trow + tcol_o + c64 + 32, rb);
           tmem_wait_ld_dep(ra, rb);
-          if constexpr (WIN) {
+          {
             if (joined) {
               uint32_t rc[32], rd[32];
               tmem_ld32(trow + C::TCOL_O + HD + c64, rc);
@@ -987,12 +754,11 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
             v1.y = pack_bf16(__uint_as_float(r[10]) * inv, __uint_as_float(r[11]) * inv);
             v1.z = pack_bf16(__uint_as_float(r[12]) * inv, __uint_as_float(r[13]) * inv);
             v1.w = pack_bf16(__uint_as_float(r[14]) * inv, __uint_as_float(r[15]) * inv);
-            if (WIN && !valid) v0 = v1 = make_uint4(0u, 0u, 0u, 0u);  // a padding row, whatever it computed
+            if (!valid) v0 = v1 = make_uint4(0u, 0u, 0u, 0u);  // a padding row, whatever it computed
             const int kb = cc / 64, ch = (cc % 64) / 8;
             uint8_t* blk = pbuf + kb * (BM * 128) + row * 128;
             uint4* p0 = reinterpret_cast<uint4*>(blk + ((ch ^ (row & 7)) * 16));
             uint4* p1 = reinterpret_cast<uint4*>(blk + (((ch + 1) ^ (row & 7)) * 16));
-            if (fuse_d) dsum += dot_bf16x8(v0, *p0) + dot_bf16x8(v1, *p1);  // dO, then O over it
             *p0 = v0;
             *p1 = v1;
           }
@@ -1003,10 +769,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         fence_proxy_async_smem();
         if (grow < prm.T) {
           const long long ri = ((long long)un.b * prm.T + grow) * prm.NH + un.h;
-          prm.lse[ri] = WIN && !valid ? -INFINITY : (m_used + log2f(l_sum)) * LN2;
-          if (fuse_d && dok) prm.D[ri] = __float2bfloat16_rn(dsum);
+          prm.lse[ri] = !valid ? -INFINITY : (m_used + log2f(l_sum)) * LN2;
         }
-        if (fuse_d) ++nd;
       }
       // every thread of the warpgroup takes this barrier and leaves it with the
       // same verdict, so the warpgroup stays in step after a failed wait
@@ -1018,11 +782,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         bulk_commit();
       }
     }
-    if (wg_leader) {
-      bulk_wait<0>();
-      // wind-down: a dO tile load whose epilogue never ran must land first
-      if (*abort_p && nd_armed > 0) mbar_wait_for(BAR_DO(x), (nd_armed - 1) & 1, kDrainLimitNs);
-    }
+    if (wg_leader) bulk_wait<0>();
   }
 
   tc_fence_before();
@@ -1034,33 +794,23 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   if (threadIdx.x == 0 && abort_flag) atomicOr(prm.status, STATUS_FWD_TIMEOUT);
 }
 
-// Launches the instantiation DYN (dynamic schedule: one CTA per unit, else
-// one per SM).
-template <int HD, bool DYN, bool WIN = false, bool SINGLE = false>
+template <int HD, bool SINGLE>
 cudaError_t launch_fwd_kernel(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
-                              const CUtensorMap& to, const CUtensorMap& tdo, const CUtensorMap& tdqz,
-                              const FwdParams& prm, cudaStream_t st) {
-  using C = FwdCfg<HD, DYN, WIN>;
+                              const CUtensorMap& to, const FwdParams& prm, cudaStream_t st) {
+  using C = FwdCfg<HD>;
   // The setmaxnreg split assumes the kernel was compiled to exactly
   // LAUNCH_REGS registers per thread; refuse to launch otherwise.
   static const cudaError_t reg_check = [] {
     cudaFuncAttributes a;
-    cudaError_t e = cudaFuncGetAttributes(&a, flash_fwd_kernel<HD, DYN, WIN, SINGLE>);
+    cudaError_t e = cudaFuncGetAttributes(&a, window_fwd_kernel<HD, SINGLE>);
     if (e != cudaSuccess) return e;
     return a.numRegs == LAUNCH_REGS ? cudaSuccess : cudaErrorInvalidKernelImage;
   }();
   if (reg_check != cudaSuccess) return reg_check;
-  cudaError_t e = cudaFuncSetAttribute(flash_fwd_kernel<HD, DYN, WIN, SINGLE>,
+  cudaError_t e = cudaFuncSetAttribute(window_fwd_kernel<HD, SINGLE>,
                                        cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES);
   if (e != cudaSuccess) return e;
-  int grid = prm.nunits;  // dynamic: one CTA per unit (see decode_unit)
-  if (!DYN) {
-    int dev = 0, sms = 148;
-    cudaGetDevice(&dev);
-    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-    grid = prm.nunits < sms ? prm.nunits : sms;
-  }
-  launch_pdl(flash_fwd_kernel<HD, DYN, WIN, SINGLE>, grid, NUM_THREADS, C::SMEM_BYTES, st, tq, tk, tv, to, tdo, tdqz, prm);
+  launch_pdl(window_fwd_kernel<HD, SINGLE>, prm.nunits, NUM_THREADS, C::SMEM_BYTES, st, tq, tk, tv, to, prm);
   count_launches(1);
   return cudaGetLastError();
 }
@@ -1094,8 +844,8 @@ cudaError_t launch_win(const WindowArgs& a, cudaStream_t st) {
   prm.lse = a.l;
   prm.status = a.status;
   prm.win = a;
-  return single ? launch_fwd_kernel<HD, true, true, true>(tq, tk, tv, to, tq, tq, prm, st)
-                : launch_fwd_kernel<HD, true, true>(tq, tk, tv, to, tq, tq, prm, st);
+  return single ? launch_fwd_kernel<HD, true>(tq, tk, tv, to, prm, st)
+                : launch_fwd_kernel<HD, false>(tq, tk, tv, to, prm, st);
 }
 
 }  // namespace
