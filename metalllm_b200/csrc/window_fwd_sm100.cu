@@ -535,8 +535,10 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       // written again: at D=128 it holds P from this unit's first tile on, so
       // wait here; at D=64 (P in TMEM) the epilogue waits, so this unit's first
       // tiles overlap the store
+      // (not only after a unit with key tiles: one of padding stores zeros from the
+      // staging too)
       if constexpr (!C::P_TMEM) {
-        if (sc >= 1 && wg_leader) bulk_wait_read<0>();
+        if (wg_leader) bulk_wait_read<0>();
         bar_sync_named(wg_bar, 128);
       }
       float m_used = -INFINITY, l_sum = 0.0f;

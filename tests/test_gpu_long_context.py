@@ -157,6 +157,29 @@ def test_window_padding_holds_anything(A, D, fill):
     assert torch.equal(got[1], want[1]) and torch.equal(got[2], want[2])
 
 
+@pytest.mark.parametrize("D", [64, 128])
+def test_window_units_of_padding_come_first(A, D):
+    """Sequences cut in their first or second tile, more units than the GPU holds at once: a SM's first units
+    store zeros only, and the units with keys that follow leave the padding rows zero, run after run."""
+    B, T, NH, NKV, W, S = 24, 2048, 16, 4, 300, 4
+    q = randn(B, T, NH * D, seed=1)
+    k, v = (randn(B, T, NKV * D, seed=s) for s in (2, 3))
+    lens = [1 + (37 * b) % 250 for b in range(B)]
+    p, ln = A.make_params(T, NH, D), i32(lens)
+    pad = torch.arange(T, device="cuda")[None, :] >= ln[:, None]
+    first = None
+    for _ in range(10):
+        out = torch.full_like(q, NAN)
+        out, l = A.windowAttentionForward(q, k, v, p, B, W, S, NKV, lens=ln, out=out)
+        assert not out[pad].any() and torch.isneginf(l[pad]).all()
+        first = first or (out, l)
+        assert torch.equal(out, first[0]) and torch.equal(l, first[1])
+    for b in (0, 11, 23):
+        o64, l64, to, tl = ref.forward(q[b], k[b], v[b], NH, NKV, D, W, S, 0, lens[b])
+        near(f"out[{b}]", first[0][b], o64, to)
+        near(f"l[{b}]", first[1][b], l64, tl)
+
+
 def test_window_outputs_written_whole(A):
     """Outputs given, full of NaN, come back written, and the bytes around them stay."""
     B, T, NH, NKV, D, W, S = 2, 200, 2, 1, 64, 50, 2
