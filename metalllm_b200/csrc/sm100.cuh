@@ -242,6 +242,12 @@ __device__ __forceinline__ int sched_unit(const Sched& sc, uint32_t g) {
   if (!(WARP ? mbar_wait_warp(sc.full + 8u * u, ph, sc.abort) : mbar_wait(sc.full + 8u * u, ph, sc.abort)))
     return -1;
   const int k = clc_cancelled_x(sc.resp + 16u * u);
+  // The response has been read, before its slot is released to the asynchronous
+  // proxy's next write.  (Without the fences a reader's load could still be to come
+  // at its arrival: a warp then took the unit four further on, and where units are
+  // short, padding that only stores zeros, a tile stayed unwritten.)
+  __threadfence_block();
+  fence_proxy_async_smem();
   if (WARP) {
     __syncwarp();
     if ((threadIdx.x & 31) == 0) mbar_arrive(sc.empty + 8u * u);

@@ -180,6 +180,39 @@ def test_window_units_of_padding_come_first(A, D):
         near(f"l[{b}]", first[1][b], l64, tl)
 
 
+@pytest.mark.parametrize("D", [64, 128])
+def test_window_thousands_of_padding_units(A, D):
+    """Units that take a microsecond each, 27 and more a SM: every one is taken once and its rows are written, in
+    the forward, the backward and over a cache, run after run."""
+    B, T, NH, NKV, W, S = 32, 4096, 8, 4, 300, 4
+    q, dO = (randn(B, T, NH * D, seed=s) for s in (1, 4))
+    k, v = (randn(B, T, NKV * D, seed=s) for s in (2, 3))
+    lens = [(37 * b) % 250 for b in range(B)]
+    p, ln, st = A.make_params(T, NH, D), i32(lens), i32([0] * B)
+    pad = torch.arange(T, device="cuda")[None, :] >= ln[:, None]
+
+    def run():
+        out, dQ = torch.full_like(q, NAN), torch.full_like(q, NAN)
+        l = torch.full((B, T, NH), NAN, device="cuda")
+        dK, dV = torch.full_like(k, NAN), torch.full_like(v, NAN)
+        o2, l2 = torch.full_like(q, NAN), torch.full_like(l, NAN)
+        A.windowAttentionForward(q, k, v, p, B, W, S, NKV, lens=ln, out=out, l=l)
+        A.windowAttentionBackward(dO, out, l, q, k, v, p, B, W, S, NKV, lens=ln, dQ=dQ, dK=dK, dV=dV)
+        A.windowAttentionCached(q, k, v, st, p, B, W, S, NKV, lens=ln, out=o2, l=l2)
+        return out, l, dQ, dK, dV, o2, l2
+
+    first = run()
+    for _ in range(15):
+        got = run()
+        for name, x, y in zip(("out", "l", "dQ", "dK", "dV", "out over a cache", "l over a cache"), got, first):
+            assert torch.isneginf(x[pad]).all() if name[0] == "l" else not x[pad].any(), name
+            assert torch.equal(x, y), name
+    for b in (1, 20):
+        o64, l64, to, tl = ref.forward(q[b], k[b], v[b], NH, NKV, D, W, S, 0, lens[b])
+        near(f"out[{b}]", first[0][b], o64, to)
+        near(f"l[{b}]", first[1][b], l64, tl)
+
+
 def test_window_outputs_written_whole(A):
     """Outputs given, full of NaN, come back written, and the bytes around them stay."""
     B, T, NH, NKV, D, W, S = 2, 200, 2, 1, 64, 50, 2
