@@ -94,6 +94,7 @@ struct FwdParams {
   float scale_log2;
   float* lse;
   uint32_t* status;
+  uint32_t expire_ns;  // time-out test hook (ma_debug_expire_next_wait), 0 = off
   WindowArgs win;
 };
 
@@ -380,6 +381,9 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
               umma_commit(BAR_SF(x));
               ++sc[x];
             }
+            // time-out test hook: with the first products in flight, wait until its
+            // limit runs out on the barrier that nothing arrives at before the wind-down
+            if (ok && kc == 0 && prm.expire_ns) ok = mbar_wait(BAR_FIN, 0, abort_p, prm.expire_ns);
             if (ok) umma_commit(BAR_KE(ks));
           }
           if (ok) umma_commit(BAR_QE(qs));
@@ -505,41 +509,39 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     bool ok = true;
     for (int g = 0; ok; ++g) {
       const int k = sched_unit<true>(sch, g);
-      if (k < 0) break;
+      // At D=128 the staging holds P from a unit's first tile on, so the last store
+      // (of O, or of a padding unit's zeros) must have read it; at D=64 (P in TMEM)
+      // the epilogue waits, so a unit's first tiles overlap the store.
+      if (!C::P_TMEM && wg_leader) bulk_wait_read<0>();
+      // One verdict for the warpgroup: after a time-out one warp's wait may have
+      // given up where another's found the response, and the barriers below wait
+      // for all four.
+      __syncwarp();
+      if (!bar_red_and(wg_bar, 128, k >= 0)) break;
       const auto un = unit(k);
       const int nt = x == 0 ? un.nA : un.nB;
       const int qtile = un.tile0 + (SINGLE ? 0 : x);
-      {
-        if (nt == 0) {  // only padding: O = 0, l = -inf (rows past T are clipped)
-          if ((SINGLE && x == 1) || qtile * BM >= prm.T) continue;
+      if (nt == 0) {  // only padding: O = 0, l = -inf (rows past T are clipped)
+        if ((SINGLE && x == 1) || qtile * BM >= prm.T) continue;
+        if constexpr (C::P_TMEM) {
           if (wg_leader) bulk_wait_read<0>();
           bar_sync_named(wg_bar, 128);
-          for (int kb = 0; kb < C::KB; ++kb)
-#pragma unroll
-            for (int ch = 0; ch < 8; ++ch)
-              *reinterpret_cast<uint4*>(pbuf + kb * (BM * 128) + row * 128 + ch * 16) = make_uint4(0u, 0u, 0u, 0u);
-          fence_proxy_async_smem();
-          const int grow = qtile * BM + row;
-          if (grow < prm.T) prm.lse[((long long)un.b * prm.T + grow) * prm.NH + un.h] = -INFINITY;
-          bar_sync_named(wg_bar, 128);
-          if (wg_leader) {
-            for (int kb = 0; kb < C::KB; ++kb)
-              tma_store_3d(&tmO, sbase + C::OFF_P + x * C::STG_BYTES + kb * BM * 128, un.h * HD + kb * 64,
-                           qtile * BM, un.b);
-            bulk_commit();
-          }
-          continue;
         }
-      }
-      // the previous unit's O store must have read the staging before it is
-      // written again: at D=128 it holds P from this unit's first tile on, so
-      // wait here; at D=64 (P in TMEM) the epilogue waits, so this unit's first
-      // tiles overlap the store
-      // (not only after a unit with key tiles: one of padding stores zeros from the
-      // staging too)
-      if constexpr (!C::P_TMEM) {
-        if (wg_leader) bulk_wait_read<0>();
+        for (int kb = 0; kb < C::KB; ++kb)
+#pragma unroll
+          for (int ch = 0; ch < 8; ++ch)
+            *reinterpret_cast<uint4*>(pbuf + kb * (BM * 128) + row * 128 + ch * 16) = make_uint4(0u, 0u, 0u, 0u);
+        fence_proxy_async_smem();
+        const int grow = qtile * BM + row;
+        if (grow < prm.T) prm.lse[((long long)un.b * prm.T + grow) * prm.NH + un.h] = -INFINITY;
         bar_sync_named(wg_bar, 128);
+        if (wg_leader) {
+          for (int kb = 0; kb < C::KB; ++kb)
+            tma_store_3d(&tmO, sbase + C::OFF_P + x * C::STG_BYTES + kb * BM * 128, un.h * HD + kb * 64,
+                         qtile * BM, un.b);
+          bulk_commit();
+        }
+        continue;
       }
       float m_used = -INFINITY, l_sum = 0.0f;
       // one key tile; DIAG: the diagonal tile (keys after the query masked).
@@ -845,6 +847,7 @@ cudaError_t launch_win(const WindowArgs& a, cudaStream_t st) {
   prm.scale_log2 = LOG2E / sqrtf((float)HD);
   prm.lse = a.l;
   prm.status = a.status;
+  prm.expire_ns = take_expire_request(STATUS_FWD_TIMEOUT);
   prm.win = a;
   return single ? launch_fwd_kernel<HD, true>(tq, tk, tv, to, prm, st)
                 : launch_fwd_kernel<HD, false>(tq, tk, tv, to, prm, st);
