@@ -456,9 +456,19 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     bool ok = true;
     for (int g = 0; ok; ++g) {
       int k;
-      if constexpr (DYN) k = sched_unit<true>(sch, g);
-      else k = unit_of_round(prm, g);
-      if (k < 0) break;
+      if constexpr (DYN) {
+        k = sched_unit<true>(sch, g);
+        // at D=128 the staging's last store must have read it (see below)
+        if (!C::P_TMEM && sc >= 1 && wg_leader) bulk_wait_read<0>();
+        // one verdict for the warpgroup: after a time-out one warp's wait may have
+        // given up where another's found the response, and the barriers below wait
+        // for all four
+        __syncwarp();
+        if (!bar_red_and(wg_bar, 128, k >= 0)) break;
+      } else {
+        k = unit_of_round(prm, g);
+        if (k < 0) break;
+      }
       const Unit un = decode_unit<C::HB>(prm, k);
       const int nt = x == 0 ? un.nA : un.nB;
       if (nt == 0) continue;
@@ -475,7 +485,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       // wait here; at D=64 (P in TMEM) it is next written by this unit's dO
       // load or epilogue, which wait there instead, so this unit's first
       // tiles overlap the store
-      if constexpr (!C::P_TMEM) {
+      if constexpr (!C::P_TMEM && !DYN) {
         if (sc >= 1 && wg_leader) bulk_wait_read<0>();
         bar_sync_named(wg_bar, 128);
       }

@@ -103,3 +103,20 @@ def test_expire_request_is_validated(A):
     A.flashAttentionForward(q, k, v, p, B)
     torch.cuda.synchronize()
     assert A.device_status() == 0
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_forward_with_more_units_than_sms(A, D):
+    """Launch control with units taken over from blocks that never start: warps that wait for their next unit when
+    the wait runs out leave together."""
+    B, T, H = 2, 2304, 24
+    q, k, v, do = _inputs(B, T, H, D, seed=D)
+    p = A.make_params(T, H, D)
+    ref = A.flashAttentionForward(q, k, v, p, B)
+    A.debug_expire_next_wait(_lib.STATUS_FWD_TIMEOUT, LIMIT_NS)
+    A.flashAttentionForward(q, k, v, p, B)
+    torch.cuda.synchronize()
+    assert A.device_status() == _lib.STATUS_FWD_TIMEOUT
+    for _ in range(3):
+        assert all(torch.equal(a, b) for a, b in zip(A.flashAttentionForward(q, k, v, p, B), ref))
+    assert A.device_status() == 0
