@@ -232,15 +232,15 @@ struct Sched {
   volatile int* abort;
 };
 
-// Unit g of the sequence, or -1 when there is none (or a wait timed out:
-// the abort flag is then set).  Every reader calls it once per g, in order;
+// Unit g of the sequence, or -1 when there is none, or -2 when the wait gave up
+// (the abort flag is then set).  Every reader calls it once per g, in order;
 // WARP: a whole warp reads (lane 0 releases the slot), else one thread.
 template <bool WARP>
 __device__ __forceinline__ int sched_unit(const Sched& sc, uint32_t g) {
   if (g == 0) return (int)blockIdx.x;
   const uint32_t u = (g - 1) % kSchedSlots, ph = ((g - 1) / kSchedSlots) & 1u;
   if (!(WARP ? mbar_wait_warp(sc.full + 8u * u, ph, sc.abort) : mbar_wait(sc.full + 8u * u, ph, sc.abort)))
-    return -1;
+    return -2;
   const int k = clc_cancelled_x(sc.resp + 16u * u);
   // The response has been read, before its slot is released to the asynchronous
   // proxy's next write.  (Without the fences a reader's load could still be to come

@@ -381,9 +381,6 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
               umma_commit(BAR_SF(x));
               ++sc[x];
             }
-            // time-out test hook: with the first products in flight, wait until its
-            // limit runs out on the barrier that nothing arrives at before the wind-down
-            if (ok && kc == 0 && prm.expire_ns) ok = mbar_wait(BAR_FIN, 0, abort_p, prm.expire_ns);
             if (ok) umma_commit(BAR_KE(ks));
           }
           if (ok) umma_commit(BAR_QE(qs));
@@ -401,6 +398,9 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         constexpr uint32_t IDESC_O = idesc_bf16_f32(BM, HD, 0, 1);
         uint32_t vc = 0, pvc[2] = {0, 0}, uc[2] = {0, 0};
         uint32_t vzp = 0;  // bit s = parity of v_fixed[s]'s next phase
+        // time-out test hook: while the first scores are formed, wait until its limit
+        // runs out on the barrier that nothing arrives at before the wind-down
+        if (prm.expire_ns) mbar_wait(BAR_FIN2, 0, abort_p, prm.expire_ns);
         bool ok = true;
         for (int g = 0; ok; ++g) {
           const int k = sched_unit<false>(sch, g);
@@ -506,280 +506,269 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     uint32_t sc = 0;  // S_X consumed so far (== P_X produced)
     uint32_t nmg = 0;       // A: shared tiles joined so far
     uint32_t scb = 0;       // A: key tiles B has worked on in them
-    bool ok = true;
-    for (int g = 0; ok; ++g) {
-      const int k = sched_unit<true>(sch, g);
-      // At D=128 the staging holds P from a unit's first tile on, so the last store
-      // (of O, or of a padding unit's zeros) must have read it; at D=64 (P in TMEM)
-      // the epilogue waits, so a unit's first tiles overlap the store.
-      if (!C::P_TMEM && wg_leader) bulk_wait_read<0>();
-      // One verdict for the warpgroup: after a time-out one warp's wait may have
-      // given up where another's found the response, and the barriers below wait
-      // for all four.
-      __syncwarp();
-      if (!bar_red_and(wg_bar, 128, k >= 0)) break;
+    int k = sched_unit<true>(sch, 0);
+    for (uint32_t g = 1; k >= 0; ++g) {
       const auto un = unit(k);
       const int nt = x == 0 ? un.nA : un.nB;
       const int qtile = un.tile0 + (SINGLE ? 0 : x);
+      const int grow = qtile * BM + row;
+      bool ok = true, store = true;
+      // The last store (of O, or of a padding unit's zeros) must have read the
+      // staging before it is written again: at D=128 it holds P from a unit's first
+      // tile on, so wait here; at D=64 (P in TMEM) only the epilogue writes it and
+      // waits, so a unit's first tiles overlap the store.
+      if (!C::P_TMEM || nt == 0) {
+        if (wg_leader) bulk_wait_read<0>();
+        bar_sync_named(wg_bar, 128);
+      }
       if (nt == 0) {  // only padding: O = 0, l = -inf (rows past T are clipped)
-        if ((SINGLE && x == 1) || qtile * BM >= prm.T) continue;
-        if constexpr (C::P_TMEM) {
-          if (wg_leader) bulk_wait_read<0>();
-          bar_sync_named(wg_bar, 128);
-        }
+        store = !(SINGLE && x == 1) && qtile * BM < prm.T;
         for (int kb = 0; kb < C::KB; ++kb)
 #pragma unroll
           for (int ch = 0; ch < 8; ++ch)
             *reinterpret_cast<uint4*>(pbuf + kb * (BM * 128) + row * 128 + ch * 16) = make_uint4(0u, 0u, 0u, 0u);
         fence_proxy_async_smem();
-        const int grow = qtile * BM + row;
-        if (grow < prm.T) prm.lse[((long long)un.b * prm.T + grow) * prm.NH + un.h] = -INFINITY;
-        bar_sync_named(wg_bar, 128);
-        if (wg_leader) {
-          for (int kb = 0; kb < C::KB; ++kb)
-            tma_store_3d(&tmO, sbase + C::OFF_P + x * C::STG_BYTES + kb * BM * 128, un.h * HD + kb * 64,
-                         qtile * BM, un.b);
-          bulk_commit();
-        }
-        continue;
-      }
-      float m_used = -INFINITY, l_sum = 0.0f;
-      // one key tile; DIAG: the diagonal tile (keys after the query masked).
-      // Instantiated twice so that the other tiles carry no masking code.
-      // NC: the tile's first columns that matter (all 128, or a sink tile's 32).
-      auto tile = [&](auto diag_tag, auto nc_tag, int j) -> bool {
-        constexpr bool DIAG = decltype(diag_tag)::value;
-        constexpr int NC = decltype(nc_tag)::value;
-        if (!mbar_poll_warp(BAR_SF(x), sc & 1, abort_p)) return false;
-        tc_fence_after();
-        float s[NC];
-        if constexpr (NC == 32) {
-          uint32_t ra[32];
-          tmem_ld32(trow + tcol_s, ra);
-          tmem_wait_ld_dep(ra);
-#pragma unroll
-          for (int i = 0; i < 32; ++i) s[i] = __uint_as_float(ra[i]);
-        } else {
-#pragma unroll
-          for (int cc = 0; cc < NC; cc += 64) {
-            uint32_t ra[32], rb[32];
-            tmem_ld32(trow + tcol_s + cc, ra);
-            tmem_ld32(trow + tcol_s + cc + 32, rb);
-            tmem_wait_ld_dep(ra, rb);
-#pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              s[cc + i] = __uint_as_float(ra[i]);
-              s[cc + 32 + i] = __uint_as_float(rb[i]);
-            }
-          }
-        }
-        tc_fence_before();
-        mbar_arrive(BAR_SE(x));
-        {
-          if constexpr (DIAG) {
-            // key k0 + i is visible up to the row's own position, and from its
-            // window's first key on or among the sinks; 32 keys to a word of
-            // bits, one test and one select a key
-            const int k0 = un.key_tile(j) * BN;
-            const int t = prm.win.pos(un.b, qtile * BM + row);
-            const int up = t - k0, from = t - prm.win.window + 1 - k0, sink = prm.win.sinks - k0;
-#pragma unroll
-            for (int w = 0; w < NC; w += 32) {
-              const uint32_t see = bits_below(up + 1 - w) & (~bits_below(from - w) | bits_below(sink - w));
-#pragma unroll
-              for (int i = 0; i < 32; ++i)
-                if (!(see & (1u << i))) s[w + i] = -INFINITY;
-            }
-          }
-        }
-        // row maximum: 8 independent partial maxima, 3-input max (short chains)
-        float pm[8];
-#pragma unroll
-        for (int q = 0; q < 8; ++q) pm[q] = fmaxf(s[q], s[8 + q]);
-#pragma unroll
-        for (int i = 16; i < NC; i += 16)
-#pragma unroll
-          for (int q = 0; q < 8; ++q) pm[q] = fmax3(pm[q], s[i + q], s[i + 8 + q]);
-        const float mx = fmax3(fmax3(pm[0], pm[1], pm[2]), fmax3(pm[3], pm[4], pm[5]),
-                               fmaxf(pm[6], pm[7]));
-        const float m_new = fmaxf(m_used, mx * c);
-        // lazy rescaling: only rows whose maximum grew by more than 2^8 move
-        // m_used; O_X is rescaled below, once PV_X(j-1) has completed
-        bool rescale = false;
-        float alpha = 1.0f;
-        const bool first = j == un.first(x);
-        if (first) {
-          m_used = m_new;
-        } else {
-          const bool need = m_new > m_used + RESCALE_THRESHOLD;
-          rescale = __any_sync(0xffffffffu, need);
-          if (need) {
-            alpha = ex2(m_used - m_new);
-            l_sum *= alpha;
-            m_used = m_new;
-          }
-        }
-        // P = 2^(S*c - m) with packed fp32x2 FMAs; row sum in 4 packed partials
-        // (a row that has seen no key yet has m = -inf and P = 2^-inf = 0)
-        const float base = m_used == -INFINITY ? 0.0f : m_used;
-        const float2 c2 = make_float2(c, c), nm2 = make_float2(-base, -base);
-        float2 ps[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f),
-                        make_float2(0.f, 0.f)};
-        uint32_t pk[NC / 2];  // P as bf16 pairs, even key in the low half
-#pragma unroll
-        for (int i = 0; i < NC; i += 2) {
-          const float2 t = __ffma2_rn(make_float2(s[i], s[i + 1]), c2, nm2);
-          const float e0 = ex2(t.x), e1 = ex2(t.y);
-          ps[(i >> 1) & 3] = __fadd2_rn(ps[(i >> 1) & 3], make_float2(e0, e1));
-          pk[i / 2] = pack_bf16(e0, e1);
-        }
-        l_sum += (ps[0].x + ps[0].y) + (ps[1].x + ps[1].y) + (ps[2].x + ps[2].y) +
-                 (ps[3].x + ps[3].y);
-        // PV_X(j-1) must be complete before O_X is rescaled and before P_X(j)
-        // overwrites P_X (waited for only now, so the exponentials overlap it)
-        if (!first) {
-          if (!mbar_poll_warp(BAR_PV(x), (sc - 1) & 1, abort_p)) return false;
+        if (store && grow < prm.T) prm.lse[((long long)un.b * prm.T + grow) * prm.NH + un.h] = -INFINITY;
+      } else {
+        float m_used = -INFINITY, l_sum = 0.0f;
+        // one key tile; DIAG: the diagonal tile (keys after the query masked).
+        // Instantiated twice so that the other tiles carry no masking code.
+        // NC: the tile's first columns that matter (all 128, or a sink tile's 32).
+        auto tile = [&](auto diag_tag, auto nc_tag, int j) -> bool {
+          constexpr bool DIAG = decltype(diag_tag)::value;
+          constexpr int NC = decltype(nc_tag)::value;
+          if (!mbar_poll_warp(BAR_SF(x), sc & 1, abort_p)) return false;
           tc_fence_after();
-        }
-        if (rescale) {
+          float s[NC];
+          if constexpr (NC == 32) {
+            uint32_t ra[32];
+            tmem_ld32(trow + tcol_s, ra);
+            tmem_wait_ld_dep(ra);
 #pragma unroll
-          for (int cc = 0; cc < HD; cc += 16) {
-            uint32_t r[16];
-            tmem_ld16(trow + tcol_o + cc, r);
-            tmem_wait_ld_dep(r);
+            for (int i = 0; i < 32; ++i) s[i] = __uint_as_float(ra[i]);
+          } else {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * alpha);
-            tmem_st16(trow + tcol_o + cc, r);
-          }
-          tmem_wait_st();
-        }
-        if constexpr (C::P_TMEM) {
-          // this lane's P row into P_X
+            for (int cc = 0; cc < NC; cc += 64) {
+              uint32_t ra[32], rb[32];
+              tmem_ld32(trow + tcol_s + cc, ra);
+              tmem_ld32(trow + tcol_s + cc + 32, rb);
+              tmem_wait_ld_dep(ra, rb);
 #pragma unroll
-          for (int q = 0; q < NC / 32; ++q) {
-            uint32_t r[16];
-#pragma unroll
-            for (int i = 0; i < 16; ++i) r[i] = pk[q * 16 + i];
-            tmem_st16(trow + C::TCOL_P + x * (BN / 2) + q * 16, r);
-          }
-          tmem_wait_st();
-        } else {
-#pragma unroll
-          for (int kb = 0; kb < (NC + 63) / 64; ++kb) {
-#pragma unroll
-            for (int ch = 0; ch < (NC < 64 ? NC / 8 : 8); ++ch) {
-              const int c0 = (kb * 64 + ch * 8) / 2;
-              const uint4 v = make_uint4(pk[c0], pk[c0 + 1], pk[c0 + 2], pk[c0 + 3]);
-              *reinterpret_cast<uint4*>(pbuf + kb * (BM * 128) + row * 128 + ((ch ^ (row & 7)) * 16)) = v;
+              for (int i = 0; i < 32; ++i) {
+                s[cc + i] = __uint_as_float(ra[i]);
+                s[cc + 32 + i] = __uint_as_float(rb[i]);
+              }
             }
           }
-          fence_proxy_async_smem();
-        }
-        tc_fence_before();
-        mbar_arrive(BAR_PF(x));
-        ++sc;
-        return true;
-      };
-      using All = std::integral_constant<int, BN>;
-      for (int j = 0; ok && j < nt; ++j) {
-        if (!un.active(x, j)) continue;
-        if (un.narrow(prm.win, j)) ok = tile(std::true_type{}, std::integral_constant<int, NARROW>{}, j);
-        else if (un.whole(prm.win, x, un.key_tile(j) * BN)) ok = tile(std::false_type{}, All{}, j);
-        else ok = tile(std::true_type{}, All{}, j);
-      }
-      // --------------------------------------------- epilogue of tile X
-      bool epi = ok && mbar_poll_warp(BAR_PV(x), (sc - 1) & 1, abort_p);
-      if constexpr (C::P_TMEM) {
-        // the epilogue is the staging's first writer in this unit
-        if (wg_leader) bulk_wait_read<0>();
-        bar_sync_named(wg_bar, 128);
-      }
-      const bool joined = SINGLE && un.nB > 0;
-      if (joined && x == 1) {
-        // this half's maximum and sum; O_B stays in TMEM, where A reads it
-        if (epi) {
-          reinterpret_cast<float2*>(gbase + C::OFF_ML)[row] = make_float2(m_used, l_sum);
           tc_fence_before();
-          mbar_arrive(BAR_MG);
-        }
-        ok = bar_red_and(wg_bar, 128, epi);
-        continue;
-      }
-      float fa = 1.0f, fb = 0.0f;  // factors of O_A and O_B
-      if (joined) {
-        scb += un.nkv / 2;
-        epi = epi && mbar_poll_warp(BAR_MG, nmg++ & 1, abort_p) &&
-              mbar_poll_warp(BAR_PV(1), (scb - 1) & 1, abort_p);
-        if (epi) {
-          const float2 ml = reinterpret_cast<const float2*>(gbase + C::OFF_ML)[row];
-          const float top = fmaxf(m_used, ml.x), base = top == -INFINITY ? 0.0f : top;
-          fa = ex2(m_used - base);
-          fb = ex2(ml.x - base);
-          l_sum = l_sum * fa + ml.y * fb;
-          m_used = top;
-        }
-      }
-      if (epi) {
-        tc_fence_after();
-        const float inv = 1.0f / l_sum;
-        const int grow = qtile * BM + row;
-        const bool valid = grow < un.n;
-        // stage O (bf16) in this tile's P buffer (free: its last PV is done);
-        // O is read from TMEM 64 columns (two loads, one wait) at a time
-#pragma unroll
-        for (int c64 = 0; c64 < HD; c64 += 64) {
-          uint32_t ra[32], rb[32];
-          tmem_ld32(trow + tcol_o + c64, ra);
-          tmem_ld32(trow + tcol_o + c64 + 32, rb);
-          tmem_wait_ld_dep(ra, rb);
+          mbar_arrive(BAR_SE(x));
           {
-            if (joined) {
-              uint32_t rc[32], rd[32];
-              tmem_ld32(trow + C::TCOL_O + HD + c64, rc);
-              tmem_ld32(trow + C::TCOL_O + HD + c64 + 32, rd);
-              tmem_wait_ld_dep(rc, rd);
-              auto join = [&](uint32_t a, uint32_t b) {
-                return __float_as_uint(__uint_as_float(a) * fa + __uint_as_float(b) * fb);
-              };
+            if constexpr (DIAG) {
+              // key k0 + i is visible up to the row's own position, and from its
+              // window's first key on or among the sinks; 32 keys to a word of
+              // bits, one test and one select a key
+              const int k0 = un.key_tile(j) * BN;
+              const int t = prm.win.pos(un.b, qtile * BM + row);
+              const int up = t - k0, from = t - prm.win.window + 1 - k0, sink = prm.win.sinks - k0;
 #pragma unroll
-              for (int i = 0; i < 32; ++i) ra[i] = join(ra[i], rc[i]), rb[i] = join(rb[i], rd[i]);
+              for (int w = 0; w < NC; w += 32) {
+                const uint32_t see = bits_below(up + 1 - w) & (~bits_below(from - w) | bits_below(sink - w));
+#pragma unroll
+                for (int i = 0; i < 32; ++i)
+                  if (!(see & (1u << i))) s[w + i] = -INFINITY;
+              }
             }
           }
+          // row maximum: 8 independent partial maxima, 3-input max (short chains)
+          float pm[8];
 #pragma unroll
-          for (int c16 = 0; c16 < 64; c16 += 16) {
-            const uint32_t* r = c16 < 32 ? ra + c16 : rb + (c16 - 32);
-            const int cc = c64 + c16;
-            uint4 v0, v1;
-            v0.x = pack_bf16(__uint_as_float(r[0]) * inv, __uint_as_float(r[1]) * inv);
-            v0.y = pack_bf16(__uint_as_float(r[2]) * inv, __uint_as_float(r[3]) * inv);
-            v0.z = pack_bf16(__uint_as_float(r[4]) * inv, __uint_as_float(r[5]) * inv);
-            v0.w = pack_bf16(__uint_as_float(r[6]) * inv, __uint_as_float(r[7]) * inv);
-            v1.x = pack_bf16(__uint_as_float(r[8]) * inv, __uint_as_float(r[9]) * inv);
-            v1.y = pack_bf16(__uint_as_float(r[10]) * inv, __uint_as_float(r[11]) * inv);
-            v1.z = pack_bf16(__uint_as_float(r[12]) * inv, __uint_as_float(r[13]) * inv);
-            v1.w = pack_bf16(__uint_as_float(r[14]) * inv, __uint_as_float(r[15]) * inv);
-            if (!valid) v0 = v1 = make_uint4(0u, 0u, 0u, 0u);  // a padding row, whatever it computed
-            const int kb = cc / 64, ch = (cc % 64) / 8;
-            uint8_t* blk = pbuf + kb * (BM * 128) + row * 128;
-            uint4* p0 = reinterpret_cast<uint4*>(blk + ((ch ^ (row & 7)) * 16));
-            uint4* p1 = reinterpret_cast<uint4*>(blk + (((ch + 1) ^ (row & 7)) * 16));
-            *p0 = v0;
-            *p1 = v1;
+          for (int q = 0; q < 8; ++q) pm[q] = fmaxf(s[q], s[8 + q]);
+#pragma unroll
+          for (int i = 16; i < NC; i += 16)
+#pragma unroll
+            for (int q = 0; q < 8; ++q) pm[q] = fmax3(pm[q], s[i + q], s[i + 8 + q]);
+          const float mx = fmax3(fmax3(pm[0], pm[1], pm[2]), fmax3(pm[3], pm[4], pm[5]),
+                                 fmaxf(pm[6], pm[7]));
+          const float m_new = fmaxf(m_used, mx * c);
+          // lazy rescaling: only rows whose maximum grew by more than 2^8 move
+          // m_used; O_X is rescaled below, once PV_X(j-1) has completed
+          bool rescale = false;
+          float alpha = 1.0f;
+          const bool first = j == un.first(x);
+          if (first) {
+            m_used = m_new;
+          } else {
+            const bool need = m_new > m_used + RESCALE_THRESHOLD;
+            rescale = __any_sync(0xffffffffu, need);
+            if (need) {
+              alpha = ex2(m_used - m_new);
+              l_sum *= alpha;
+              m_used = m_new;
+            }
+          }
+          // P = 2^(S*c - m) with packed fp32x2 FMAs; row sum in 4 packed partials
+          // (a row that has seen no key yet has m = -inf and P = 2^-inf = 0)
+          const float base = m_used == -INFINITY ? 0.0f : m_used;
+          const float2 c2 = make_float2(c, c), nm2 = make_float2(-base, -base);
+          float2 ps[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f),
+                          make_float2(0.f, 0.f)};
+          uint32_t pk[NC / 2];  // P as bf16 pairs, even key in the low half
+#pragma unroll
+          for (int i = 0; i < NC; i += 2) {
+            const float2 t = __ffma2_rn(make_float2(s[i], s[i + 1]), c2, nm2);
+            const float e0 = ex2(t.x), e1 = ex2(t.y);
+            ps[(i >> 1) & 3] = __fadd2_rn(ps[(i >> 1) & 3], make_float2(e0, e1));
+            pk[i / 2] = pack_bf16(e0, e1);
+          }
+          l_sum += (ps[0].x + ps[0].y) + (ps[1].x + ps[1].y) + (ps[2].x + ps[2].y) +
+                   (ps[3].x + ps[3].y);
+          // PV_X(j-1) must be complete before O_X is rescaled and before P_X(j)
+          // overwrites P_X (waited for only now, so the exponentials overlap it)
+          if (!first) {
+            if (!mbar_poll_warp(BAR_PV(x), (sc - 1) & 1, abort_p)) return false;
+            tc_fence_after();
+          }
+          if (rescale) {
+#pragma unroll
+            for (int cc = 0; cc < HD; cc += 16) {
+              uint32_t r[16];
+              tmem_ld16(trow + tcol_o + cc, r);
+              tmem_wait_ld_dep(r);
+#pragma unroll
+              for (int i = 0; i < 16; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * alpha);
+              tmem_st16(trow + tcol_o + cc, r);
+            }
+            tmem_wait_st();
+          }
+          if constexpr (C::P_TMEM) {
+            // this lane's P row into P_X
+#pragma unroll
+            for (int q = 0; q < NC / 32; ++q) {
+              uint32_t r[16];
+#pragma unroll
+              for (int i = 0; i < 16; ++i) r[i] = pk[q * 16 + i];
+              tmem_st16(trow + C::TCOL_P + x * (BN / 2) + q * 16, r);
+            }
+            tmem_wait_st();
+          } else {
+#pragma unroll
+            for (int kb = 0; kb < (NC + 63) / 64; ++kb) {
+#pragma unroll
+              for (int ch = 0; ch < (NC < 64 ? NC / 8 : 8); ++ch) {
+                const int c0 = (kb * 64 + ch * 8) / 2;
+                const uint4 v = make_uint4(pk[c0], pk[c0 + 1], pk[c0 + 2], pk[c0 + 3]);
+                *reinterpret_cast<uint4*>(pbuf + kb * (BM * 128) + row * 128 + ((ch ^ (row & 7)) * 16)) = v;
+              }
+            }
+            fence_proxy_async_smem();
+          }
+          tc_fence_before();
+          mbar_arrive(BAR_PF(x));
+          ++sc;
+          return true;
+        };
+        using All = std::integral_constant<int, BN>;
+        for (int j = 0; ok && j < nt; ++j) {
+          if (!un.active(x, j)) continue;
+          if (un.narrow(prm.win, j)) ok = tile(std::true_type{}, std::integral_constant<int, NARROW>{}, j);
+          else if (un.whole(prm.win, x, un.key_tile(j) * BN)) ok = tile(std::false_type{}, All{}, j);
+          else ok = tile(std::true_type{}, All{}, j);
+        }
+        // --------------------------------------------- epilogue of tile X
+        ok = ok && mbar_poll_warp(BAR_PV(x), (sc - 1) & 1, abort_p);
+        if constexpr (C::P_TMEM) {
+          // the epilogue is the staging's first writer in this unit
+          if (wg_leader) bulk_wait_read<0>();
+          bar_sync_named(wg_bar, 128);
+        }
+        const bool joined = SINGLE && un.nB > 0;
+        if (joined && x == 1) {
+          // this half's maximum and sum; O_B stays in TMEM, where A reads it
+          if (ok) {
+            reinterpret_cast<float2*>(gbase + C::OFF_ML)[row] = make_float2(m_used, l_sum);
+            tc_fence_before();
+            mbar_arrive(BAR_MG);
+          }
+          store = false;
+        }
+        float fa = 1.0f, fb = 0.0f;  // factors of O_A and O_B
+        if (joined && x == 0) {
+          scb += un.nkv / 2;
+          ok = ok && mbar_poll_warp(BAR_MG, nmg++ & 1, abort_p) &&
+                mbar_poll_warp(BAR_PV(1), (scb - 1) & 1, abort_p);
+          if (ok) {
+            const float2 ml = reinterpret_cast<const float2*>(gbase + C::OFF_ML)[row];
+            const float top = fmaxf(m_used, ml.x), base = top == -INFINITY ? 0.0f : top;
+            fa = ex2(m_used - base);
+            fb = ex2(ml.x - base);
+            l_sum = l_sum * fa + ml.y * fb;
+            m_used = top;
           }
         }
-        tc_fence_before();
-        mbar_arrive(BAR_OE(x));  // O_X may be overwritten by the next unit
-        if (joined) mbar_arrive(BAR_OE(1));
-        fence_proxy_async_smem();
-        if (grow < prm.T) {
-          const long long ri = ((long long)un.b * prm.T + grow) * prm.NH + un.h;
-          prm.lse[ri] = !valid ? -INFINITY : (m_used + log2f(l_sum)) * LN2;
+        if (ok && store) {
+          tc_fence_after();
+          const float inv = 1.0f / l_sum;
+          const bool valid = grow < un.n;
+          // stage O (bf16) in this tile's P buffer (free: its last PV is done);
+          // O is read from TMEM 64 columns (two loads, one wait) at a time
+#pragma unroll
+          for (int c64 = 0; c64 < HD; c64 += 64) {
+            uint32_t ra[32], rb[32];
+            tmem_ld32(trow + tcol_o + c64, ra);
+            tmem_ld32(trow + tcol_o + c64 + 32, rb);
+            tmem_wait_ld_dep(ra, rb);
+            {
+              if (joined) {
+                uint32_t rc[32], rd[32];
+                tmem_ld32(trow + C::TCOL_O + HD + c64, rc);
+                tmem_ld32(trow + C::TCOL_O + HD + c64 + 32, rd);
+                tmem_wait_ld_dep(rc, rd);
+                auto join = [&](uint32_t a, uint32_t b) {
+                  return __float_as_uint(__uint_as_float(a) * fa + __uint_as_float(b) * fb);
+                };
+#pragma unroll
+                for (int i = 0; i < 32; ++i) ra[i] = join(ra[i], rc[i]), rb[i] = join(rb[i], rd[i]);
+              }
+            }
+#pragma unroll
+            for (int c16 = 0; c16 < 64; c16 += 16) {
+              const uint32_t* r = c16 < 32 ? ra + c16 : rb + (c16 - 32);
+              const int cc = c64 + c16;
+              uint4 v0, v1;
+              v0.x = pack_bf16(__uint_as_float(r[0]) * inv, __uint_as_float(r[1]) * inv);
+              v0.y = pack_bf16(__uint_as_float(r[2]) * inv, __uint_as_float(r[3]) * inv);
+              v0.z = pack_bf16(__uint_as_float(r[4]) * inv, __uint_as_float(r[5]) * inv);
+              v0.w = pack_bf16(__uint_as_float(r[6]) * inv, __uint_as_float(r[7]) * inv);
+              v1.x = pack_bf16(__uint_as_float(r[8]) * inv, __uint_as_float(r[9]) * inv);
+              v1.y = pack_bf16(__uint_as_float(r[10]) * inv, __uint_as_float(r[11]) * inv);
+              v1.z = pack_bf16(__uint_as_float(r[12]) * inv, __uint_as_float(r[13]) * inv);
+              v1.w = pack_bf16(__uint_as_float(r[14]) * inv, __uint_as_float(r[15]) * inv);
+              if (!valid) v0 = v1 = make_uint4(0u, 0u, 0u, 0u);  // a padding row, whatever it computed
+              const int kb = cc / 64, ch = (cc % 64) / 8;
+              uint8_t* blk = pbuf + kb * (BM * 128) + row * 128;
+              uint4* p0 = reinterpret_cast<uint4*>(blk + ((ch ^ (row & 7)) * 16));
+              uint4* p1 = reinterpret_cast<uint4*>(blk + (((ch + 1) ^ (row & 7)) * 16));
+              *p0 = v0;
+              *p1 = v1;
+            }
+          }
+          tc_fence_before();
+          mbar_arrive(BAR_OE(x));  // O_X may be overwritten by the next unit
+          if (joined) mbar_arrive(BAR_OE(1));
+          fence_proxy_async_smem();
+          if (grow < prm.T) {
+            const long long ri = ((long long)un.b * prm.T + grow) * prm.NH + un.h;
+            prm.lse[ri] = !valid ? -INFINITY : (m_used + log2f(l_sum)) * LN2;
+          }
         }
       }
-      // every thread of the warpgroup takes this barrier and leaves it with the
-      // same verdict, so the warpgroup stays in step after a failed wait
-      ok = bar_red_and(wg_bar, 128, epi);
-      if (ok && wg_leader) {
+      // One verdict for the warpgroup, on this unit and on the wait for the next (after
+      // a time-out one warp's wait may have given up where another's found the
+      // response): the barriers above wait for all four warps.
+      k = sched_unit<true>(sch, g);
+      __syncwarp();
+      if (!bar_red_and(wg_bar, 128, ok && k != -2)) break;
+      if (store && wg_leader) {
         for (int kb = 0; kb < C::KB; ++kb)
           tma_store_3d(&tmO, sbase + C::OFF_P + x * C::STG_BYTES + kb * BM * 128, un.h * HD + kb * 64,
                        qtile * BM, un.b);
