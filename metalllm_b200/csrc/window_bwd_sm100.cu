@@ -123,6 +123,7 @@ struct Params {
   const float *neg_l, *neg_d;  // -l*log2e, -delta/sqrt(D), [B][NH][rows]
   const uint4* ext;            // D=64: -l*sqrt(D) and -delta as three bf16 each, and two zeros
   uint32_t* status;
+  uint32_t expire_ns;          // time-out test hook (ma_debug_expire_next_wait), 0 = off
   // dK/dV pass: sink tiles 0 .. nsplit-1 are split: their query tiles past the
   // window go, far_tiles at a time, to nfar units each, dealt first; unit
   // `slot`s of part hold 2 x 128 x D fp32 partial sums (dV, dK), slot 0 of a
@@ -529,6 +530,9 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
             umma_bf16_ts_lo(d, a + (kk >> 2) * 64 + (kk & 3) * 8, db + kk * (2048 >> 4), IDESC_ACC,
                             start && kk == 0 ? 0u : 1u);
         };
+        // time-out test hook: while the first scores are formed, wait until its limit
+        // runs out on the barrier that nothing arrives at before the wind-down
+        if (prm.expire_ns) mbar_wait(BAR_FIN + 8, 0, abort_p, prm.expire_ns);
         for (Step s = before_first(); advance<DQ, false>(prm, s, ring);) {
           const uint32_t t = s.t, s1 = t % C::X1ST, s2 = t % C::X2ST, b = t % C::DPB;
           const uint32_t p = tmem + C::TCOL_DP + b * 128, ds = p + 32;
@@ -980,6 +984,7 @@ cudaError_t launch_all(const WindowArgs& a, const WindowGrads& g, cudaStream_t s
   prm.neg_l = neg_l;
   prm.neg_d = neg_d;
   prm.status = a.status;
+  prm.expire_ns = take_expire_request(STATUS_BWD_TIMEOUT);  // of both passes
   prm.nsplit = p.nsplit;
   prm.nfar = p.nfar;
   prm.far_tiles = p.far_tiles;

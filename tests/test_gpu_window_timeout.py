@@ -72,3 +72,19 @@ def test_cached_many_rows(A, D, M, NH):
     q, kc, vc = randn(B, M, NH * D, seed=1), randn(B, cap, NKV * D, seed=2), randn(B, cap, NKV * D, seed=3)
     p, start = A.make_params(M, NH, D), i32([2000, 77])
     expire(A, _lib.STATUS_FWD_TIMEOUT, lambda: A.windowAttentionCached(q, kc, vc, start, p, B, 900, 4, NKV))
+
+
+# B, T, NH, NKV, window, lens: few units; more of them than SMs in each pass; sink tiles cut into units of their own,
+# whose partial sums a last kernel adds up; padded batches
+BACKWARD = [(1, 100, 2, 1, 300, None), (2, 1024, 24, 24, 300, None), (1, 4200, 3, 1, 70, None),
+            (8, 1500, 16, 16, 300, [1500, 3, 0, 129, 700, 1500, 1, 256])]
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("B,T,NH,NKV,window,lens", BACKWARD)
+def test_backward(A, D, B, T, NH, NKV, window, lens):
+    q, k, v, dO = (randn(B, T, h * D, seed=s) for h, s in ((NH, 1), (NKV, 2), (NKV, 3), (NH, 4)))
+    p, ln = A.make_params(T, NH, D), None if lens is None else i32(lens)
+    out, l = A.windowAttentionForward(q, k, v, p, B, window, 4, NKV, lens=ln)
+    expire(A, _lib.STATUS_BWD_TIMEOUT,
+           lambda: A.windowAttentionBackward(dO, out, l, q, k, v, p, B, window, 4, NKV, lens=ln))
