@@ -318,12 +318,12 @@ MA_API const char* ma_last_error_string(void);
 MA_API int ma_device_status(uint32_t* status, ma_stream_t stream);
 
 /* Test hook of the kernels' time-out path.  The next launch of each kernel
- * named in `kernels` (MA_STATUS_FWD_TIMEOUT: flashAttentionForward's and
- * windowAttentionForward's; MA_STATUS_BWD_TIMEOUT: flashAttentionBackward's
- * and both passes of windowAttentionBackward) lets one wait run out on
- * purpose: once its first tensor-core products are in flight, its
- * UMMA-issuing thread waits on an mbarrier that nothing arrives at, for
- * `wait_ns` nanoseconds (1 .. 10^9).  The kernel then winds down as
+ * named in `kernels` (MA_STATUS_FWD_TIMEOUT: flashAttentionForward's,
+ * windowAttentionForward's and windowAttentionCached's; MA_STATUS_BWD_TIMEOUT:
+ * flashAttentionBackward's and both passes of windowAttentionBackward) lets
+ * one wait run out on purpose: with its first copies or tensor-core products
+ * in flight, a thread that issues them waits on an mbarrier that nothing
+ * arrives at, for `wait_ns` nanoseconds (1 .. 10^9).  The kernel then winds down as
  * after a real time-out: every role stops at its next wait, the copies and
  * products already in flight are waited for, TMEM is freed and the kernel's
  * bit is set in the status word ma_device_status reads.  That launch's

@@ -51,7 +51,8 @@ struct DecodeCfg {
   static constexpr uint32_t TILE = KEYS * HD * 2;          // K or V of a block
   static constexpr int STAGES = 96 * 1024 / (2 * (int)TILE);
   static constexpr uint32_t OFF_BAR = STAGES * 2 * TILE;
-  static constexpr uint32_t SMEM = OFF_BAR + 2 * STAGES * 8 + 1024;  // + alignment slack
+  // full and empty of each stage, and one that nothing arrives at (the time-out hook's)
+  static constexpr uint32_t SMEM = OFF_BAR + (2 * STAGES + 1) * 8 + 1024;  // + alignment slack
   static_assert(WARPS * ROWS * HD * 4 + WARPS * ROWS * 8 <= OFF_BAR, "the join reuses the ring");
 };
 
@@ -59,6 +60,7 @@ struct DecodeParams {
   WindowArgs a;
   int groups, nsplit;  // 16-row groups a K/V head, splits of the key axis
   float scale_log2;
+  uint32_t expire_ns;  // time-out test hook (ma_debug_expire_next_wait), 0 = off
   float *part_o, *part_ml;  // nsplit > 1: [unit][split][16][D], [unit][split][16][2]
 };
 
@@ -122,6 +124,7 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM)
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   auto BAR_F = [&](int s) { return sbase + C::OFF_BAR + 8u * s; };
   auto BAR_E = [&](int s) { return sbase + C::OFF_BAR + 8u * (C::STAGES + s); };
+  const uint32_t BAR_NEVER = sbase + C::OFF_BAR + 16u * C::STAGES;
 
   const int split = blockIdx.x % prm.nsplit;
   const int unit = blockIdx.x / prm.nsplit;  // (batch, K/V head, row group)
@@ -137,6 +140,7 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM)
       mbar_init(BAR_F(s), 1);
       mbar_init(BAR_E(s), WARPS);
     }
+    mbar_init(BAR_NEVER, 1);
     fence_mbar_init();
   }
   __syncthreads();
@@ -152,6 +156,9 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM)
       uint32_t n = 0;
       for (int blk = blk0; blk < blk1; ++blk, ++n) {
         const int st = n % C::STAGES;
+        // time-out test hook: with the first block's loads in flight, wait until its
+        // limit runs out
+        if (n == 1 && prm.expire_ns && !mbar_wait(BAR_NEVER, 0, abort_p, prm.expire_ns)) break;
         if (n >= C::STAGES && !mbar_wait(BAR_E(st), ((n / C::STAGES) - 1) & 1, abort_p)) break;
         mbar_arrive_expect_tx(BAR_F(st), 2 * C::TILE);
         const int k0 = sp.first_key(blk);
@@ -421,6 +428,7 @@ cudaError_t launch_decode(const WindowArgs& a, void* workspace, cudaStream_t st)
   prm.groups = p.groups;
   prm.nsplit = p.nsplit;
   prm.scale_log2 = a.scale * LOG2E;
+  prm.expire_ns = take_expire_request(STATUS_FWD_TIMEOUT);
   prm.part_o = static_cast<float*>(workspace);
   prm.part_ml = prm.part_o + p.units * p.nsplit * ROWS * HD;
   cudaError_t e = cudaFuncSetAttribute(window_decode_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);

@@ -88,3 +88,13 @@ def test_backward(A, D, B, T, NH, NKV, window, lens):
     out, l = A.windowAttentionForward(q, k, v, p, B, window, 4, NKV, lens=ln)
     expire(A, _lib.STATUS_BWD_TIMEOUT,
            lambda: A.windowAttentionBackward(dO, out, l, q, k, v, p, B, window, 4, NKV, lens=ln))
+
+
+# B, M, NH, NKV, cap: one split, the key axis split and joined, some requests of padding
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("B,M,NH,NKV,cap,lens", [(64, 1, 32, 8, 1500, None), (1, 1, 8, 2, 20000, None),
+                                                 (3, 5, 8, 2, 3000, [5, 0, 2])])
+def test_cached_few_rows(A, D, B, M, NH, NKV, cap, lens):
+    q, kc, vc = randn(B, M, NH * D, seed=1), randn(B, cap, NKV * D, seed=2), randn(B, cap, NKV * D, seed=3)
+    p, start, ln = A.make_params(M, NH, D), i32([cap - M] * B), None if lens is None else i32(lens)
+    expire(A, _lib.STATUS_FWD_TIMEOUT, lambda: A.windowAttentionCached(q, kc, vc, start, p, B, cap, 0, NKV, lens=ln))
