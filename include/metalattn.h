@@ -386,6 +386,8 @@ MA_API int ma_attentionForwardBackward_host(ma_host_pipeline* pl, const ma_bf16*
  *                      before them count, the rest is padding), or NULL: all
  *   start            : int32 [B], rows a sequence's cache holds already, which
  *                      is the position of its first new row
+ * An output (a cache or a workspace too) that overlaps an input, index arrays
+ * included, or another output is refused with MA_ERR_RANGE.
  * lens and start are device arrays, whose values the host cannot check: lens
  * is clamped to [0, M]; a row whose position lies outside the cache is not
  * stored, and attention takes the position clamped to [0, cap). */

@@ -875,8 +875,9 @@ struct Range {
   int may_equal;  // index of the input an output may be in place of, or -1
 };
 
-// Refuses an output that shares memory with an input or another output
-// (in place, the same range as its input, where may_equal allows it).
+// Refuses an output that shares memory with an input (index arrays count; an
+// absent one has no bytes) or another output (in place, the same range as its
+// input, where may_equal allows it).
 template <int NI, int NO>
 int check_overlaps(const Range (&in)[NI], const Range (&out)[NO]) {
   auto share = [](const Range& a, const Range& b) {
@@ -937,7 +938,8 @@ int rotary_impl(const void* q, const ma_bf16* k, void* q_out, ma_bf16* k_out, bo
   MA_REQUIRE_I32(positions);
   const uint64_t rows = (uint64_t)B * p->M;
   const uint64_t nq = rows * p->N * (q_f32 ? 4 : 2), nk = rows * r->NKV * p->D * 2;
-  const Range in[] = {{"q", q, nq, -1}, {"k", k, nk, -1}};
+  const Range in[] = {{"q", q, nq, -1}, {"k", k, nk, -1}, {"positions", positions, positions ? rows * 4 : 0, -1},
+                      {"inv_freq", r->inv_freq, r->rot / 2 * 8, -1}};
   const Range out[] = {{"q_out", q_out, nq, 0}, {"k_out", k_out, nk, 1}};
   rc = check_overlaps(in, out);
   if (rc) return rc;
@@ -1027,7 +1029,8 @@ extern "C" int ma_rotaryCacheAppend(const ma_bf16* q, const ma_bf16* k, const ma
   MA_REQUIRE_I32(lens);
   const uint64_t rows = (uint64_t)B * p->M, nq = rows * p->N * 2, nk = rows * r->NKV * p->D * 2;
   const uint64_t nc = (uint64_t)B * cap * r->NKV * p->D * 2;
-  const Range in[] = {{"q", q, nq, -1}, {"k", k, nk, -1}, {"v", v, nk, -1}};
+  const Range in[] = {{"q", q, nq, -1}, {"k", k, nk, -1}, {"v", v, nk, -1}, {"start", start, 4ull * B, -1},
+                      {"lens", lens, lens ? 4ull * B : 0, -1}, {"inv_freq", r->inv_freq, r->rot / 2 * 8, -1}};
   const Range out[] = {{"q_out", q_out, nq, 0}, {"k_cache", k_cache, nc, -1}, {"v_cache", v_cache, nc, -1}};
   rc = check_overlaps(in, out);
   if (rc) return rc;
@@ -1055,7 +1058,7 @@ extern "C" int ma_windowAttentionForward(const ma_bf16* q, const ma_bf16* k, con
   MA_REQUIRE_PTR(l);
   MA_REQUIRE_I32(lens);
   const WindowBytes n(a);
-  const Range ins[] = {{"q", q, n.q, -1}, {"k", k, n.k, -1}, {"v", v, n.k, -1}};
+  const Range ins[] = {{"q", q, n.q, -1}, {"k", k, n.k, -1}, {"v", v, n.k, -1}, {"lens", lens, lens ? 4ull * B : 0, -1}};
   const Range outs[] = {{"out", out, n.q, -1}, {"l", l, n.l, -1}};
   rc = check_overlaps(ins, outs);
   if (rc) return rc;
@@ -1105,7 +1108,8 @@ extern "C" int ma_windowAttentionBackward(const ma_bf16* dO, const ma_bf16* out,
   if (rc) return rc;
   const WindowBytes n(a);
   const Range ins[] = {{"dO", dO, n.q, -1}, {"out", out, n.q, -1}, {"l", l, n.l, -1},
-                       {"q", q, n.q, -1},   {"k", k, n.k, -1},     {"v", v, n.k, -1}};
+                       {"q", q, n.q, -1},   {"k", k, n.k, -1},     {"v", v, n.k, -1},
+                       {"lens", lens, lens ? 4ull * B : 0, -1}};
   const Range outs[] = {{"dQ", dQ, dq_f32 ? 2 * n.q : n.q, -1}, {"dK", dK, n.k, -1}, {"dV", dV, n.k, -1},
                         {"workspace", workspace, need, -1}};
   rc = check_overlaps(ins, outs);
@@ -1163,7 +1167,8 @@ extern "C" int ma_windowAttentionCached(const ma_bf16* q, const ma_bf16* k_cache
   rc = check_workspace(workspace, workspace_bytes, need);
   if (rc) return rc;
   const WindowBytes n(a);
-  const Range ins[] = {{"q", q, n.q, -1}, {"k_cache", k_cache, n.k, -1}, {"v_cache", v_cache, n.k, -1}};
+  const Range ins[] = {{"q", q, n.q, -1}, {"k_cache", k_cache, n.k, -1}, {"v_cache", v_cache, n.k, -1},
+                       {"start", start, 4ull * B, -1}, {"lens", lens, lens ? 4ull * B : 0, -1}};
   const Range outs[] = {{"out", out, n.q, -1}, {"l", l, n.l, -1}, {"workspace", workspace, need, -1}};
   rc = check_overlaps(ins, outs);
   if (rc) return rc;

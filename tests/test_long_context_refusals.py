@@ -168,6 +168,57 @@ def test_cached_refuses(cuda_lib):
         assert call(y) == "MA_ERR_RANGE", (i, j)
 
 
+def test_outputs_over_index_arrays_are_refused(cuda_lib):
+    """positions, inv_freq, lens and start are inputs too: an output, a cache or a workspace over one of them is
+    refused."""
+    lib, p, w = cuda_lib, params(M=4), window()
+    r, B, i = rotary(), 3, at(20)
+    n = ctypes.c_uint64()
+
+    def fwd(x, pos):
+        return name(lib.ma_rotaryForward(*x, ctypes.byref(rotary(freq=at(21))), pos, ctypes.byref(p), B, None))
+
+    def append(x, start=at(22), lens=None, freq=at(21)):
+        return name(lib.ma_rotaryCacheAppend(*x, start, lens, ctypes.byref(rotary(freq=freq)), ctypes.byref(p), B, 8, None))
+
+    def cached(x, start, lens=None, ws=at(12)):
+        return name(lib.ma_windowAttentionCached(*x, start, lens, ctypes.byref(w), ctypes.byref(p), B, 512, ws, n.value, None))
+
+    assert lib.ma_windowAttentionCached_workspace(ctypes.byref(w), ctypes.byref(p), B, 512, ctypes.byref(n)) == 0
+    ends = 2 * B * 4 * 6 * 64  # bytes of q
+    x = [at(j) for j in range(9)]
+    assert fwd([x[0], x[1], i, x[3]], i + 64) == "MA_ERR_RANGE"
+    assert "positions" in lib.ma_last_error_string().decode()
+    assert fwd([x[0], x[1], i - ends + 16, x[3]], i) == "MA_ERR_RANGE"
+    assert name(forward(lib, p=p, r=rotary(freq=i), ptrs=[x[0], x[1], x[2], i + 240])) == "MA_ERR_RANGE"
+    assert "inv_freq" in lib.ma_last_error_string().decode()
+    rc = lib.ma_rotaryBackward(x[0], x[1], i, x[3], 1, ctypes.byref(r), i + 2 * ends - 4, ctypes.byref(p), B, None)
+    assert name(rc) == "MA_ERR_RANGE"  # fp32: twice the bytes
+    for kw, word in ((dict(start=i + 4), "start"), (dict(lens=i + 8), "lens"), (dict(freq=i + 8), "inv_freq")):
+        for j in (3, 4, 5):
+            y = x[:6]
+            y[j] = i
+            assert append(y, **kw) == "MA_ERR_RANGE"
+            assert word in lib.ma_last_error_string().decode()
+    for j in (3, 4):
+        y = x[:5]
+        y[j] = i
+        assert name(lib.ma_windowAttentionForward(*y, i + 4, ctypes.byref(w), ctypes.byref(p), B, None)) == "MA_ERR_RANGE"
+        assert cached(y, i + 4) == "MA_ERR_RANGE"
+        assert cached(y, at(22), i + 4) == "MA_ERR_RANGE"
+    assert n.value == 0 or cached(x[:5], i + 4, ws=i) == "MA_ERR_RANGE"
+    assert lib.ma_windowAttentionBackward_workspace(ctypes.byref(w), ctypes.byref(p), B, ctypes.byref(n)) == 0
+    for j in (6, 7, 8, None):
+        y, ws = list(x), at(12)
+        if j is None:
+            ws = i
+        else:
+            y[j] = i
+        rc = lib.ma_windowAttentionBackward(*y, 0, i + 4, ctypes.byref(w), ctypes.byref(p), B, ws, n.value, None)
+        assert name(rc) == "MA_ERR_RANGE"
+        assert "lens" in lib.ma_last_error_string().decode()
+
+
 def test_python_layer_refuses():
     """The Python layer's own checks: types, devices, groups, signs."""
     from metalllm_b200 import attention as A
