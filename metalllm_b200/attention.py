@@ -5,7 +5,9 @@ with the same buffer roles, order and dtypes, as its host code binds them
 (model.h:446-473 forward, model.h:639-665 backward).  Each call goes through the
 C ABI of libmetalattn (include/metalattn.h); PyTorch only provides the device
 memory and the stream.  Outputs may be passed in (as the reference's
-preallocated buffers) or are allocated here.
+preallocated buffers) or are allocated here, for a call with stream= in that
+stream's order.  The inputs of such a call have to be ready on that stream and
+kept (or recorded for it, Tensor.record_stream) until its work is done.
 
 Shapes (B sequences of length T = params.M, N = params.N = NH*D):
     X, q, k, v, out, dO, dK, dV : bf16 [B, T, N]
@@ -85,8 +87,17 @@ def _numel(shape: tuple) -> int:
 
 
 def _out(t: Optional[torch.Tensor], like: torch.Tensor, shape: tuple, dtype: torch.dtype,
-         name: str) -> torch.Tensor:
+         name: str, stream: Optional[torch.cuda.Stream] = None) -> torch.Tensor:
+    """The output given, checked, or a new one for a call on `stream`."""
     if t is None:
+        if stream is not None and stream.cuda_stream != _stream(None):
+            # Allocated in that stream's order: memory that work queued on the current
+            # stream may still use is not handed out.  Recorded for the current stream,
+            # where the caller will read it: dropped, it waits for that work.
+            with torch.cuda.stream(stream):
+                t = torch.empty(shape, dtype=dtype, device=like.device)
+            t.record_stream(torch.cuda.current_stream())
+            return t
         if like.dtype is dtype and like.shape == shape and like.is_contiguous():
             return torch.empty_like(like)  # half the host time of torch.empty
         return torch.empty(shape, dtype=dtype, device=like.device)
@@ -103,9 +114,9 @@ def computeQKV(X: torch.Tensor, q_w: torch.Tensor, k_w: torch.Tensor, v_w: torch
     _check(X, "X", torch.bfloat16, act)
     for w, n in ((q_w, "q_w"), (k_w, "k_w"), (v_w, "v_w")):
         _check(w, n, torch.bfloat16, (p.N, p.N))
-    q = _out(q, X, act, torch.bfloat16, "q")
-    k = _out(k, X, act, torch.bfloat16, "k")
-    v = _out(v, X, act, torch.bfloat16, "v")
+    q = _out(q, X, act, torch.bfloat16, "q", stream)
+    k = _out(k, X, act, torch.bfloat16, "k", stream)
+    v = _out(v, X, act, torch.bfloat16, "v", stream)
     _lib.call("ma_computeQKV", _ptr(X), _ptr(q), _ptr(k), _ptr(v), _ptr(q_w), _ptr(k_w),
               _ptr(v_w), ctypes.byref(p), B, _stream(stream))
     return q, k, v
@@ -117,7 +128,7 @@ def projForward(attn_out: torch.Tensor, proj_w: torch.Tensor, p: AttentionParams
     act = (B, p.M, p.N)
     _check(attn_out, "attn_out", torch.bfloat16, act)
     _check(proj_w, "proj_w", torch.bfloat16, (p.N, p.N))
-    out = _out(out, attn_out, act, torch.bfloat16, "out")
+    out = _out(out, attn_out, act, torch.bfloat16, "out", stream)
     _lib.call("ma_projForward", _ptr(attn_out), _ptr(proj_w), _ptr(out), ctypes.byref(p), B,
               _stream(stream))
     return out
@@ -130,7 +141,7 @@ def projBackwarddW(attn_out: torch.Tensor, dZ: torch.Tensor, p: AttentionParams,
     act = (B, p.M, p.N)
     _check(attn_out, "attn_out", torch.bfloat16, act)
     _check(dZ, "dZ", torch.bfloat16, act)
-    dProjw = _out(dProjw, attn_out, (p.N, p.N), torch.bfloat16, "dProjw")
+    dProjw = _out(dProjw, attn_out, (p.N, p.N), torch.bfloat16, "dProjw", stream)
     _lib.call("ma_projBackwarddW", _ptr(attn_out), _ptr(dZ), _ptr(dProjw), ctypes.byref(p), B,
               _stream(stream))
     return dProjw
@@ -143,7 +154,7 @@ def projBackwarddX(dZ: torch.Tensor, proj_w: torch.Tensor, p: AttentionParams, B
     act = (B, p.M, p.N)
     _check(dZ, "dZ", torch.bfloat16, act)
     _check(proj_w, "proj_w", torch.bfloat16, (p.N, p.N))
-    dAttn = _out(dAttn, dZ, act, torch.bfloat16, "dAttn")
+    dAttn = _out(dAttn, dZ, act, torch.bfloat16, "dAttn", stream)
     _lib.call("ma_projBackwarddX", _ptr(dZ), _ptr(proj_w), _ptr(dAttn), ctypes.byref(p), B,
               _stream(stream))
     return dAttn
@@ -159,8 +170,8 @@ def projBackwarddXComputeD(dZ: torch.Tensor, proj_w: torch.Tensor, attn_out: tor
     _check(dZ, "dZ", torch.bfloat16, act)
     _check(proj_w, "proj_w", torch.bfloat16, (p.N, p.N))
     _check(attn_out, "attn_out", torch.bfloat16, act)
-    dAttn = _out(dAttn, dZ, act, torch.bfloat16, "dAttn")
-    D = _out(D, dZ, (B, p.M, p.NH), torch.bfloat16, "D")
+    dAttn = _out(dAttn, dZ, act, torch.bfloat16, "dAttn", stream)
+    D = _out(D, dZ, (B, p.M, p.NH), torch.bfloat16, "D", stream)
     _lib.call("ma_projBackwarddXComputeD", _ptr(dZ), _ptr(proj_w), _ptr(dAttn), _ptr(attn_out), _ptr(D),
               ctypes.byref(p), B, _stream(stream))
     return dAttn, D
@@ -176,7 +187,7 @@ def computeGradDx(q_w: torch.Tensor, k_w: torch.Tensor, v_w: torch.Tensor, dQ: t
     _check(dQ, "dQ", torch.float32, act)
     _check(dK, "dK", torch.bfloat16, act)
     _check(dV, "dV", torch.bfloat16, act)
-    dX = _out(dX, dK, act, torch.float32, "dX")
+    dX = _out(dX, dK, act, torch.float32, "dX", stream)
     _lib.call("ma_computeGradDx", _ptr(dX), _ptr(q_w), _ptr(k_w), _ptr(v_w), _ptr(dQ), _ptr(dK),
               _ptr(dV), ctypes.byref(p), B, _stream(stream))
     return dX
@@ -194,9 +205,9 @@ def computeGradDw(x: torch.Tensor, dQ: torch.Tensor, dK: torch.Tensor, dV: torch
     _check(dK, "dK", torch.bfloat16, act)
     _check(dV, "dV", torch.bfloat16, act)
     w = (p.N, p.N)
-    dQw = _out(dQw, x, w, torch.float32, "dQw")
-    dKw = _out(dKw, x, w, torch.bfloat16, "dKw")
-    dVw = _out(dVw, x, w, torch.bfloat16, "dVw")
+    dQw = _out(dQw, x, w, torch.float32, "dQw", stream)
+    dKw = _out(dKw, x, w, torch.bfloat16, "dKw", stream)
+    dVw = _out(dVw, x, w, torch.bfloat16, "dVw", stream)
     _lib.call("ma_computeGradDw", _ptr(x), _ptr(dQ), _ptr(dK), _ptr(dV), _ptr(dQw), _ptr(dKw),
               _ptr(dVw), ctypes.byref(p), B, _stream(stream))
     return dQw, dKw, dVw
@@ -213,8 +224,8 @@ def flashAttentionForward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, p: 
     act = (B, p.M, p.N)
     for t, n in ((q, "q"), (k, "k"), (v, "v")):
         _check(t, n, torch.bfloat16, act)
-    out = _out(out, q, act, torch.bfloat16, "out")
-    l = _out(l, q, (B, p.M, p.NH), torch.float32, "l")
+    out = _out(out, q, act, torch.bfloat16, "out", stream)
+    l = _out(l, q, (B, p.M, p.NH), torch.float32, "l", stream)
     if shard is None:
         _lib.call("ma_flashAttentionForward", _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(l),
                   ctypes.byref(p), B, _stream(stream))
@@ -238,9 +249,9 @@ def flashAttentionForwardComputeD(q: torch.Tensor, k: torch.Tensor, v: torch.Ten
     act = (B, p.M, p.N)
     for t, n in ((q, "q"), (k, "k"), (v, "v"), (dO, "dO")):
         _check(t, n, torch.bfloat16, act)
-    out = _out(out, q, act, torch.bfloat16, "out")
-    l = _out(l, q, (B, p.M, p.NH), torch.float32, "l")
-    D = _out(D, q, (B, p.M, p.NH), torch.bfloat16, "D")
+    out = _out(out, q, act, torch.bfloat16, "out", stream)
+    l = _out(l, q, (B, p.M, p.NH), torch.float32, "l", stream)
+    D = _out(D, q, (B, p.M, p.NH), torch.bfloat16, "D", stream)
     if zero_dQ is not None:
         _check(zero_dQ, "zero_dQ", torch.float32, act)
         name = "ma_flashAttentionForwardComputeDZeroDQ"
@@ -266,7 +277,7 @@ def computeD(dO: torch.Tensor, O: torch.Tensor, p: AttentionParams, B: int,
     act = (B, p.M, p.N)
     _check(dO, "dO", torch.bfloat16, act)
     _check(O, "O", torch.bfloat16, act)
-    D = _out(D, dO, (B, p.M, p.NH), torch.bfloat16, "D")
+    D = _out(D, dO, (B, p.M, p.NH), torch.bfloat16, "D", stream)
     if shard is None:
         _lib.call("ma_computeD", _ptr(dO), _ptr(O), _ptr(D), ctypes.byref(p), B, _stream(stream))
     else:
@@ -291,9 +302,9 @@ def flashAttentionBackward(dZ: torch.Tensor, d: torch.Tensor, l: torch.Tensor, q
     _check(l, "l", torch.float32, (B, p.M, p.NH))
     if accumulate_dQ and dQ is None:
         raise ValueError("accumulate_dQ needs the dQ tensor to add into")
-    dQ = _out(dQ, q, act, torch.float32, "dQ")
-    dK = _out(dK, q, act, torch.bfloat16, "dK")
-    dV = _out(dV, q, act, torch.bfloat16, "dV")
+    dQ = _out(dQ, q, act, torch.float32, "dQ", stream)
+    dK = _out(dK, q, act, torch.bfloat16, "dK", stream)
+    dV = _out(dV, q, act, torch.bfloat16, "dV", stream)
     args = (_ptr(dZ), _ptr(d), _ptr(l), _ptr(q), _ptr(k), _ptr(v), _ptr(dQ), _ptr(dK), _ptr(dV),
             ctypes.byref(p), B)
     name = "ma_flashAttentionBackwardAccumulate" if accumulate_dQ else "ma_flashAttentionBackward"
@@ -403,8 +414,8 @@ def rotaryForward(q: torch.Tensor, k: torch.Tensor, inv_freq: torch.Tensor, p: A
     qs, ks = (B, p.M, p.N), (B, p.M, NKV * p.D)
     _check_all((q, "q", torch.bfloat16, qs), (k, "k", torch.bfloat16, ks))
     _check_optional(positions, "positions", torch.int32, (B, p.M))
-    q_out = _out(q_out, q, qs, torch.bfloat16, "q_out")
-    k_out = _out(k_out, k, ks, torch.bfloat16, "k_out")
+    q_out = _out(q_out, q, qs, torch.bfloat16, "q_out", stream)
+    k_out = _out(k_out, k, ks, torch.bfloat16, "k_out", stream)
     _lib.call("ma_rotaryForward", _ptr(q), _ptr(k), _ptr(q_out), _ptr(k_out), ctypes.byref(r), _ptr(positions),
               ctypes.byref(p), B, _stream(stream))
     return q_out, k_out
@@ -423,8 +434,8 @@ def rotaryBackward(dQ: torch.Tensor, dK: torch.Tensor, inv_freq: torch.Tensor, p
     t = torch.float32 if isinstance(dQ, torch.Tensor) and dQ.dtype == torch.float32 else torch.bfloat16
     _check_all((dQ, "dQ", t, qs), (dK, "dK", torch.bfloat16, ks))
     _check_optional(positions, "positions", torch.int32, (B, p.M))
-    dQ_out = _out(dQ_out, dQ, qs, t, "dQ_out")
-    dK_out = _out(dK_out, dK, ks, torch.bfloat16, "dK_out")
+    dQ_out = _out(dQ_out, dQ, qs, t, "dQ_out", stream)
+    dK_out = _out(dK_out, dK, ks, torch.bfloat16, "dK_out", stream)
     _lib.call("ma_rotaryBackward", _ptr(dQ), _ptr(dK), _ptr(dQ_out), _ptr(dK_out), int(t == torch.float32),
               ctypes.byref(r), _ptr(positions), ctypes.byref(p), B, _stream(stream))
     return dQ_out, dK_out
@@ -454,7 +465,7 @@ def rotaryCacheAppend(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache
                (k_cache, "k_cache", torch.bfloat16, cs), (v_cache, "v_cache", torch.bfloat16, cs),
                (start, "start", torch.int32, (B,)))
     _check_optional(lens, "lens", torch.int32, (B,))
-    q_out = _out(q_out, q, qs, torch.bfloat16, "q_out")
+    q_out = _out(q_out, q, qs, torch.bfloat16, "q_out", stream)
     _lib.call("ma_rotaryCacheAppend", _ptr(q), _ptr(k), _ptr(v), _ptr(q_out), _ptr(k_cache), _ptr(v_cache),
               _ptr(start), _ptr(lens), ctypes.byref(r), ctypes.byref(p), B, cap, _stream(stream))
     return q_out
@@ -472,8 +483,8 @@ def windowAttentionForward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, p:
     qs, ks = (B, p.M, p.N), (B, p.M, NKV * p.D)
     _check_all((q, "q", torch.bfloat16, qs), (k, "k", torch.bfloat16, ks), (v, "v", torch.bfloat16, ks))
     _check_optional(lens, "lens", torch.int32, (B,))
-    out = _out(out, q, qs, torch.bfloat16, "out")
-    l = _out(l, q, (B, p.M, p.NH), torch.float32, "l")
+    out = _out(out, q, qs, torch.bfloat16, "out", stream)
+    l = _out(l, q, (B, p.M, p.NH), torch.float32, "l", stream)
     _lib.call("ma_windowAttentionForward", _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(l), _ptr(lens),
               ctypes.byref(w), ctypes.byref(p), B, _stream(stream))
     return out, l
@@ -500,9 +511,9 @@ def windowAttentionBackward(dO: torch.Tensor, out: torch.Tensor, l: torch.Tensor
     if dQ_dtype not in (torch.float32, torch.bfloat16):
         raise TypeError(f"dQ must be float32 or bfloat16, got {dQ_dtype}")
     f32 = int(dQ_dtype == torch.float32)
-    dQ = _out(dQ, q, qs, dQ_dtype, "dQ")
-    dK = _out(dK, k, ks, torch.bfloat16, "dK")
-    dV = _out(dV, k, ks, torch.bfloat16, "dV")
+    dQ = _out(dQ, q, qs, dQ_dtype, "dQ", stream)
+    dK = _out(dK, k, ks, torch.bfloat16, "dK", stream)
+    dV = _out(dV, k, ks, torch.bfloat16, "dV", stream)
     ws = _workspace(q, stream, p, w, B)
     _lib.call("ma_windowAttentionBackward", _ptr(dO), _ptr(out), _ptr(l), _ptr(q), _ptr(k), _ptr(v), _ptr(dQ),
               _ptr(dK), _ptr(dV), f32, _ptr(lens), ctypes.byref(w), ctypes.byref(p), B, _ptr(ws), ws.numel(),
@@ -526,8 +537,8 @@ def windowAttentionCached(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch
     _check_all((q, "q", torch.bfloat16, qs), (k_cache, "k_cache", torch.bfloat16, cs),
                (v_cache, "v_cache", torch.bfloat16, cs), (start, "start", torch.int32, (B,)))
     _check_optional(lens, "lens", torch.int32, (B,))
-    out = _out(out, q, qs, torch.bfloat16, "out")
-    l = _out(l, q, (B, p.M, p.NH), torch.float32, "l")
+    out = _out(out, q, qs, torch.bfloat16, "out", stream)
+    l = _out(l, q, (B, p.M, p.NH), torch.float32, "l", stream)
     ws = _workspace(q, stream, p, w, B, cap=cap)
     _lib.call("ma_windowAttentionCached", _ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(out), _ptr(l), _ptr(start),
               _ptr(lens), ctypes.byref(w), ctypes.byref(p), B, cap, _ptr(ws), 0 if ws is None else ws.numel(),

@@ -298,6 +298,34 @@ def test_window_other_stream_and_graph(A, D):
             assert torch.equal(a, b), name
 
 
+def test_outputs_on_another_stream_take_no_block_of_this_one(A):
+    """A block freed on the current stream, whose work may still be queued, is not the output of a call on another
+    stream; a dropped output is not handed out on its own stream while the current one may read it."""
+    B, T, NH, D = 2, 300, 4, 64
+    p = A.make_params(T, NH, D)
+    q, k, v = (randn(B, T, NH * D, seed=s) for s in (1, 2, 3))
+    want = A.windowAttentionForward(q, k, v, p, B, 50)
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    side = torch.cuda.Stream()
+    x = torch.empty_like(q)
+    ptr = x.data_ptr()
+    del x
+    out, l = A.windowAttentionForward(q, k, v, p, B, 50, stream=side)
+    assert out.data_ptr() != ptr
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(out, want[0]) and torch.equal(l, want[1])
+    torch.cuda._sleep(200_000_000)  # the current stream is busy for about 0.1 s
+    got = out + 0.0
+    ptr = out.data_ptr()
+    del out
+    with torch.cuda.stream(side):
+        y = torch.empty_like(q)
+    assert y.data_ptr() != ptr
+    torch.cuda.synchronize()
+    assert torch.equal(got, want[0])
+
+
 def test_window_calls_at_once(A):
     """Two streams, each with its own backward and its own split attention over a cache, workspaces and all."""
     B, T, NH, NKV, D, W, S = 1, 2300, 4, 1, 64, 90, 3  # split sink tiles: partial sums in the workspace

@@ -244,3 +244,55 @@ def test_python_layer_refuses():
         A.windowAttentionCached(q, k[0], k[0], None, p, 1, 4, NKV=2)
     with pytest.raises(ValueError, match="even"):
         A.rotaryFrequencies(7)
+
+
+def test_outputs_of_a_call_on_another_stream(monkeypatch):
+    """They are allocated in that stream's order and recorded for the current one; on the current stream itself,
+    and without stream=, neither is done."""
+    from contextlib import contextmanager
+
+    from metalllm_b200 import attention as A
+    inside, made, recorded = [], [], []
+
+    @contextmanager
+    def on(stream):
+        inside.append(stream)
+        yield
+        inside.pop()
+
+    class Stream:
+        def __init__(self, handle):
+            self.cuda_stream = handle
+
+    here, side = Stream(5), Stream(9)
+    empty, empty_like = torch.empty, torch.empty_like
+    monkeypatch.setattr(torch.cuda, "stream", on)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda *a: here)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    monkeypatch.setattr(A, "_raw_stream", lambda device: here.cuda_stream)
+    monkeypatch.setattr(torch, "empty", lambda *a, **k: (made.append(tuple(inside)), empty(*a, **k))[1])
+    monkeypatch.setattr(torch, "empty_like", lambda *a, **k: (made.append(tuple(inside)), empty_like(*a, **k))[1])
+    monkeypatch.setattr(torch.Tensor, "record_stream", lambda t, s: recorded.append(s))
+    monkeypatch.setattr(A, "_check_all", lambda *a: None)
+    monkeypatch.setattr(A, "_check", lambda *a: None)
+    monkeypatch.setattr(A._lib, "call", lambda *a: None)
+    monkeypatch.setattr(A, "_workspace", lambda *a, **k: torch.zeros(1))
+    p, f = A.make_params(8, 4, 64), torch.ones(32, dtype=torch.float64)
+    q, k = torch.zeros(2, 8, 256, dtype=torch.bfloat16), torch.zeros(2, 8, 128, dtype=torch.bfloat16)
+    st = torch.zeros(2, dtype=torch.int32)
+    l = torch.zeros(2, 8, 4)
+    calls = {
+        2: [lambda s: A.rotaryForward(q, k, f, p, 2, 2, stream=s), lambda s: A.rotaryBackward(q, k, f, p, 2, 2, stream=s),
+            lambda s: A.windowAttentionForward(q, k, k, p, 2, 4, 0, 2, stream=s),
+            lambda s: A.windowAttentionCached(q, k, k, st, p, 2, 4, 0, 2, stream=s),
+            lambda s: A.flashAttentionForward(q, q, q, p, 2, stream=s)],
+        1: [lambda s: A.rotaryCacheAppend(q, k, k, k, k, st, f, p, 2, 2, stream=s)],
+        3: [lambda s: A.windowAttentionBackward(q, q, l, q, k, k, p, 2, 4, 0, 2, stream=s)],
+    }
+    for n, group in calls.items():
+        for call in group:
+            for stream, want in ((side, [(side,)] * n), (here, [()] * n), (None, [()] * n)):
+                made.clear(), recorded.clear()
+                call(stream)
+                assert made == want
+                assert recorded == ([here] * n if stream is side else [])
