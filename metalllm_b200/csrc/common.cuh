@@ -20,10 +20,12 @@ __device__ __forceinline__ void pdl_wait_and_release() {
 }
 
 // Kernel launch with programmatic dependent launch allowed: the kernel may be
-// scheduled while the previous kernel in the stream is still draining; every
-// kernel of this library starts with pdl_wait_and_release(), which waits for
-// that kernel's completion before any memory is touched, so stream order is
-// kept.  Errors are reported through cudaGetLastError as for <<<>>>.
+// scheduled while the previous kernel in the stream is still draining.  The
+// kernels of this library wait with pdl_wait_and_release() for that kernel's
+// completion before they touch global memory, so stream order is kept.  The one
+// that does not is the dQ pass of windowAttentionBackward, which waits at its end
+// (window_bwd_sm100.cu: it may follow the dK/dV pass only).  Errors are reported
+// through cudaGetLastError as for <<<>>>.
 template <typename... KArgs, typename... Args>
 inline void launch_pdl(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st,
                        Args&&... args) {

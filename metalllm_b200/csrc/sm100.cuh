@@ -133,8 +133,9 @@ __device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, vo
 }
 
 // mbar_wait in a third of the code, for kernels whose many waits would crowd the
-// instruction cache: at most 2^21 polls bound the wait.  Without a time of its
-// own a poll is suspended for up to 1.03 us (measured), 2 s in all; with one it
+// instruction cache: no clock is read, at most 2^21 polls bound the wait.  Without
+// a time of its own a poll is suspended for up to 1.03 us (measured), so that is
+// about 2 s, or less where the hardware ends a suspension early; with one it
 // returned at once, and the warps that wait took issue slots from those that work.
 __device__ __forceinline__ bool mbar_poll(uint32_t bar, uint32_t parity, volatile int* abort) {
   for (uint32_t i = 0;; ++i) {
@@ -153,15 +154,6 @@ __device__ __forceinline__ bool mbar_poll(uint32_t bar, uint32_t parity, volatil
 }
 __device__ __forceinline__ bool mbar_poll_warp(uint32_t bar, uint32_t parity, volatile int* abort) {
   return __all_sync(0xffffffffu, mbar_poll(bar, parity, abort));
-}
-
-template <bool SHORT>
-__device__ __forceinline__ bool wait_on(uint32_t bar, uint32_t parity, volatile int* abort) {
-  return SHORT ? mbar_poll(bar, parity, abort) : mbar_wait(bar, parity, abort);
-}
-template <bool SHORT>
-__device__ __forceinline__ bool wait_on_warp(uint32_t bar, uint32_t parity, volatile int* abort) {
-  return SHORT ? mbar_poll_warp(bar, parity, abort) : mbar_wait_warp(bar, parity, abort);
 }
 
 // Named barrier `id` over `nthreads` threads that also returns the AND of

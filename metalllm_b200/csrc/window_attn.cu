@@ -393,8 +393,14 @@ __global__ void __launch_bounds__(JOIN) window_join_kernel(const DecodeParams pr
   if (lane == 0) a.l[item] = valid ? (top + log2f(sum)) * LN2 : -INFINITY;
 }
 
-// Few query rows a K/V head take the kernel of this file, more the tiled
-// forward, whose tiles hold 128 rows of one head.
+// Few query rows a K/V head take the kernel of this file, more the tiled forward,
+// whose tiles hold 128 rows of one head: this one's time goes by the rows and the
+// other's by the heads.  Measured (us, this kernel / tiled, heads of 64, window
+// 4096): 8 requests, 32 / 8 heads: 16 rows 29 / 104, 64 rows 51 / 106, 68 rows
+// 88 / 106, 128 rows 96 / 106, 256 rows 182 / 106; 16 requests, 16 / 16 heads: 32
+// rows 98 / 104, 64 rows 184 / 104.  The times meet at about 32 new tokens whatever
+// the heads of a group; 64 rows are on the safe side of that from 2 heads a group on.
+// (The two also differ in P: hi + lo here, one bf16 operand there.)
 bool few_rows(const WindowArgs& a) { return (long long)a.M * (a.NH / a.NKV) <= 4 * ROWS; }
 
 struct DecodePlan {

@@ -48,7 +48,7 @@
 // any other unit's; what lies past its window is cut into units of their own
 // whose partial dV, dK a last kernel adds up in slot order (win_plan).
 //
-// All mbarrier waits are bounded (mbar_poll); on time-out the CTA winds down,
+// All mbarrier waits are bounded (mbar_poll, about 2 s); on time-out the CTA winds down,
 // frees its TMEM and sets STATUS_BWD_TIMEOUT.
 #include <algorithm>
 
@@ -100,7 +100,8 @@ struct Cfg {
   static constexpr uint32_t OFF_SCHED = OFF_STAT + SSTG * STAT;     // 16-byte responses
   static constexpr uint32_t OFF_DESC = OFF_SCHED + kSchedSlots * 16;
   static constexpr uint32_t OFF_BAR = OFF_DESC + NDESC * DESC;
-  // full and empty of R, X1, X2, stat; X1/X2 fixed; dp_full[DPB],
+  // full and empty of R, X1, X2, stat (EXT: its full is not used, X2 fixed says it
+  // too); X1/X2 fixed; dp_full[DPB],
   // p_ready[DPB], p_free[DPB]; s_full, s_free, done, acc_free, fin[2]; sched
   // full/empty, desc_full
   static constexpr int NBAR = 2 * (RST + X1ST + X2ST + SSTG) + X1ST + X2ST + 3 * DPB + 6 + 2 * (int)kSchedSlots + NDESC;
@@ -996,6 +997,9 @@ cudaError_t launch_all(const WindowArgs& a, const WindowGrads& g, cudaStream_t s
   prm.dQ = g.dQ;
   prm.dq_f32 = g.dq_f32;
   prm.nunits = prm.nfar_units + p.ntiles * a.B * a.NKV;
+  // The order of the two is fixed, with nothing between them: the dQ pass reads the
+  // statistics without a wait of its own, and may because every block of the dK/dV
+  // pass has waited for them before it lets the dQ pass start.
   e = launch_pass<HD, false>(tk, tv, tq, tdo, prm, st);
   if (e != cudaSuccess) return e;
   prm.nunits = p.ntiles * a.B * a.NH;

@@ -17,7 +17,7 @@
 // exponentials and product; 500 tokens over a cache, 16 heads of 64, window 2048
 // 26 us (SINGLE; in pairs 33).
 //
-// Every mbarrier wait is bounded (about 2 s); on time-out the CTA sets an
+// Every mbarrier wait is bounded (mbar_poll, about 2 s); on time-out the CTA sets an
 // abort flag that all roles poll, winds down, frees its TMEM and sets
 // STATUS_FWD_TIMEOUT in the device status word.
 #include <type_traits>
@@ -51,8 +51,10 @@ struct FwdCfg {
   static constexpr int KST = HD == 64 ? 3 : 2;  // K tile stages
   static constexpr int VST = HD == 64 ? 3 : 1;  // V tile stages
   // D=64: P_X lives in TMEM (bf16 pairs) and PV_X reads it from there, which
-  // halves the shared-memory traffic of the tensor core; D=128 has no TMEM
-  // columns left and stages P in shared memory
+  // halves the shared-memory traffic of the tensor core.  At D=128 S and O of both
+  // tiles fill TMEM, and P is staged in shared memory, so that S_X(j+1) need not
+  // wait for PV_X(j) as it would with P over S_X's own columns; its 64 KB leave
+  // two stages for K and one for V
   static constexpr bool P_TMEM = HD == 64;
   static constexpr uint32_t QT_BYTES = BM * HD * 2;  // one query tile
   static constexpr uint32_t KV_BYTES = BN * HD * 2;
@@ -347,148 +349,142 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       // ---------------------------------------------------- S, under a window
       // S_X(j) = Q_X K_j^T, as soon as softmax X has read S_X(j-1).  Another
       // warp issues the products with V, so neither waits for the other's tile.
-      {
-        constexpr uint32_t IDESC_S = idesc_bf16_f32(BM, BN, 0, 0);
-        constexpr uint32_t IDESC_SN = idesc_bf16_f32(BM, NARROW, 0, 0);
-        uint32_t qc = 0, kc = 0, sc[2] = {0, 0};
-        bool ok = true;
-        for (int g = 0; ok; ++g) {
-          const int k = sched_unit<false>(sch, g);
-          if (k < 0) break;
-          const auto un = unit(k);
-          if (un.nkv == 0) continue;  // only padding
-          const int qs = qc % C::QST;
-          if (!mbar_poll(BAR_QF(qs), (qc / C::QST) & 1, abort_p)) break;
-          for (int j = 0; ok && j < un.nkv; ++j, ++kc) {
-            const int ks = kc % C::KST;
-            ok = mbar_poll(BAR_KF(ks), (kc / C::KST) & 1, abort_p);
-            const uint32_t idesc = un.narrow(prm.win, j) ? IDESC_SN : IDESC_S;
-            const uint32_t dk = desc_lo(sbase + C::OFF_K + ks * C::KV_BYTES, 16);
+      constexpr uint32_t IDESC_S = idesc_bf16_f32(BM, BN, 0, 0);
+      constexpr uint32_t IDESC_SN = idesc_bf16_f32(BM, NARROW, 0, 0);
+      uint32_t qc = 0, kc = 0, sc[2] = {0, 0};
+      bool ok = true;
+      for (int g = 0; ok; ++g) {
+        const int k = sched_unit<false>(sch, g);
+        if (k < 0) break;
+        const auto un = unit(k);
+        if (un.nkv == 0) continue;  // only padding
+        const int qs = qc % C::QST;
+        if (!mbar_poll(BAR_QF(qs), (qc / C::QST) & 1, abort_p)) break;
+        for (int j = 0; ok && j < un.nkv; ++j, ++kc) {
+          const int ks = kc % C::KST;
+          ok = mbar_poll(BAR_KF(ks), (kc / C::KST) & 1, abort_p);
+          const uint32_t idesc = un.narrow(prm.win, j) ? IDESC_SN : IDESC_S;
+          const uint32_t dk = desc_lo(sbase + C::OFF_K + ks * C::KV_BYTES, 16);
 #pragma unroll
-            for (int x = 0; x < 2; ++x) {
-              if (!ok || !un.active(x, j)) continue;
-              if (sc[x] >= 1 && !mbar_poll(BAR_SE(x), (sc[x] - 1) & 1, abort_p)) {
-                ok = false;
-                continue;
-              }
-              tc_fence_after();
-              const uint32_t dq = desc_lo(sbase + C::OFF_Q + (qs * 2 + (SINGLE ? 0 : x)) * C::QT_BYTES, 16);
-#pragma unroll
-              for (int kk = 0; kk < HD / 16; ++kk) {
-                const uint32_t off = ((kk >> 2) * (BM * 128) + (kk & 3) * 32) >> 4;
-                umma_bf16_ss_lo(tmem + C::TCOL_S + x * BN, dq + off, dk + off, idesc, kk > 0 ? 1u : 0u);
-              }
-              umma_commit(BAR_SF(x));
-              ++sc[x];
+          for (int x = 0; x < 2; ++x) {
+            if (!ok || !un.active(x, j)) continue;
+            if (sc[x] >= 1 && !mbar_poll(BAR_SE(x), (sc[x] - 1) & 1, abort_p)) {
+              ok = false;
+              continue;
             }
-            if (ok) umma_commit(BAR_KE(ks));
+            tc_fence_after();
+            const uint32_t dq = desc_lo(sbase + C::OFF_Q + (qs * 2 + (SINGLE ? 0 : x)) * C::QT_BYTES, 16);
+#pragma unroll
+            for (int kk = 0; kk < HD / 16; ++kk) {
+              const uint32_t off = ((kk >> 2) * (BM * 128) + (kk & 3) * 32) >> 4;
+              umma_bf16_ss_lo(tmem + C::TCOL_S + x * BN, dq + off, dk + off, idesc, kk > 0 ? 1u : 0u);
+            }
+            umma_commit(BAR_SF(x));
+            ++sc[x];
           }
-          if (ok) umma_commit(BAR_QE(qs));
-          ++qc;
+          if (ok) umma_commit(BAR_KE(ks));
         }
-        if (*abort_p) {  // wind-down: every UMMA issued must complete before TMEM is freed
-          umma_commit(BAR_FIN);
-          mbar_wait_for(BAR_FIN, 0, kDrainLimitNs);
-        }
+        if (ok) umma_commit(BAR_QE(qs));
+        ++qc;
+      }
+      if (*abort_p) {  // wind-down: every UMMA issued must complete before TMEM is freed
+        umma_commit(BAR_FIN);
+        mbar_wait_for(BAR_FIN, 0, kDrainLimitNs);
       }
     } else if (warp == 3 && lane == 0) {
       // --------------------------------------------------- PV, under a window
       // O_X += P_X V_j, once softmax X has written P_X(j)
-      {
-        constexpr uint32_t IDESC_O = idesc_bf16_f32(BM, HD, 0, 1);
-        uint32_t vc = 0, pvc[2] = {0, 0}, uc[2] = {0, 0};
-        uint32_t vzp = 0;  // bit s = parity of v_fixed[s]'s next phase
-        // time-out test hook: while the first scores are formed, wait until its limit
-        // runs out on the barrier that nothing arrives at before the wind-down
-        if (prm.expire_ns) mbar_wait(BAR_FIN2, 0, abort_p, prm.expire_ns);
-        bool ok = true;
-        for (int g = 0; ok; ++g) {
-          const int k = sched_unit<false>(sch, g);
-          if (k < 0) break;
-          const auto un = unit(k);
-          for (int j = 0; ok && j < un.nkv; ++j, ++vc) {
-            const int vs = vc % C::VST;
-            ok = mbar_poll(BAR_VF(vs), (vc / C::VST) & 1, abort_p);
-            if (ok && un.fix(prm.win, un.key_tile(j) * BN)) {  // warp 2 has zeroed its unseen rows
-              ok = mbar_poll(BAR_VZ(vs), (vzp >> vs) & 1, abort_p);
-              vzp ^= 1u << vs;
-            }
-            const bool narrow = un.narrow(prm.win, j);
-            const uint32_t dv = desc_lo(sbase + C::OFF_V + vs * C::KV_BYTES, BN * 128);
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-              if (!ok || !un.active(x, j)) continue;
-              const bool first = j == un.first(x);
-              ok = mbar_poll(BAR_PF(x), pvc[x] & 1, abort_p);
-              // the tile's previous unit has been read out of O_X
-              if (ok && first && uc[x] >= 1) ok = mbar_poll(BAR_OE(x), (uc[x] - 1) & 1, abort_p);
-              if (!ok) continue;
-              tc_fence_after();
-              const uint32_t dp = desc_lo(sbase + C::OFF_P + x * C::STG_BYTES, 16);
-#pragma unroll
-              for (int kk = 0; kk < BN / 16; ++kk) {
-                if (narrow && kk >= NARROW / 16) break;
-                const uint32_t acc = !first || kk > 0 ? 1u : 0u;
-                if (C::P_TMEM)  // A = P_X from TMEM: 8 columns per 16 keys
-                  umma_bf16_ts_lo(tmem + C::TCOL_O + x * HD, tmem + C::TCOL_P + x * (BN / 2) + kk * 8,
-                                  dv + kk * (2048 >> 4), IDESC_O, acc);
-                else
-                  umma_bf16_ss_lo(tmem + C::TCOL_O + x * HD, dp + (((kk >> 2) * (BM * 128) + (kk & 3) * 32) >> 4),
-                                  dv + kk * (2048 >> 4), IDESC_O, acc);
-              }
-              umma_commit(BAR_PV(x));
-              ++pvc[x];
-            }
-            if (ok) umma_commit(BAR_VE(vs));
+      constexpr uint32_t IDESC_O = idesc_bf16_f32(BM, HD, 0, 1);
+      uint32_t vc = 0, pvc[2] = {0, 0}, uc[2] = {0, 0};
+      uint32_t vzp = 0;  // bit s = parity of v_fixed[s]'s next phase
+      // time-out test hook: while the first scores are formed, wait until its limit
+      // runs out on the barrier that nothing arrives at before the wind-down
+      if (prm.expire_ns) mbar_wait(BAR_FIN2, 0, abort_p, prm.expire_ns);
+      bool ok = true;
+      for (int g = 0; ok; ++g) {
+        const int k = sched_unit<false>(sch, g);
+        if (k < 0) break;
+        const auto un = unit(k);
+        for (int j = 0; ok && j < un.nkv; ++j, ++vc) {
+          const int vs = vc % C::VST;
+          ok = mbar_poll(BAR_VF(vs), (vc / C::VST) & 1, abort_p);
+          if (ok && un.fix(prm.win, un.key_tile(j) * BN)) {  // warp 2 has zeroed its unseen rows
+            ok = mbar_poll(BAR_VZ(vs), (vzp >> vs) & 1, abort_p);
+            vzp ^= 1u << vs;
           }
-          if (un.nA > 0) ++uc[0];
-          if (un.nB > 0) ++uc[1];
+          const bool narrow = un.narrow(prm.win, j);
+          const uint32_t dv = desc_lo(sbase + C::OFF_V + vs * C::KV_BYTES, BN * 128);
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            if (!ok || !un.active(x, j)) continue;
+            const bool first = j == un.first(x);
+            ok = mbar_poll(BAR_PF(x), pvc[x] & 1, abort_p);
+            // the tile's previous unit has been read out of O_X
+            if (ok && first && uc[x] >= 1) ok = mbar_poll(BAR_OE(x), (uc[x] - 1) & 1, abort_p);
+            if (!ok) continue;
+            tc_fence_after();
+            const uint32_t dp = desc_lo(sbase + C::OFF_P + x * C::STG_BYTES, 16);
+#pragma unroll
+            for (int kk = 0; kk < BN / 16; ++kk) {
+              if (narrow && kk >= NARROW / 16) break;
+              const uint32_t acc = !first || kk > 0 ? 1u : 0u;
+              if (C::P_TMEM)  // A = P_X from TMEM: 8 columns per 16 keys
+                umma_bf16_ts_lo(tmem + C::TCOL_O + x * HD, tmem + C::TCOL_P + x * (BN / 2) + kk * 8,
+                                dv + kk * (2048 >> 4), IDESC_O, acc);
+              else
+                umma_bf16_ss_lo(tmem + C::TCOL_O + x * HD, dp + (((kk >> 2) * (BM * 128) + (kk & 3) * 32) >> 4),
+                                dv + kk * (2048 >> 4), IDESC_O, acc);
+            }
+            umma_commit(BAR_PV(x));
+            ++pvc[x];
+          }
+          if (ok) umma_commit(BAR_VE(vs));
         }
-        if (*abort_p) {
-          umma_commit(BAR_FIN2);
-          mbar_wait_for(BAR_FIN2, 0, kDrainLimitNs);
-        }
+        if (un.nA > 0) ++uc[0];
+        if (un.nB > 0) ++uc[1];
+      }
+      if (*abort_p) {
+        umma_commit(BAR_FIN2);
+        mbar_wait_for(BAR_FIN2, 0, kDrainLimitNs);
       }
     } else if (warp == 2) {
       // ------------------------------------------------ unseen rows of V
-      {
-        uint32_t vc = 0;
-        bool ok = true;
-        for (int g = 0; ok; ++g) {
-          const int k = sched_unit<true>(sch, g);
-          if (k < 0) break;
-          const auto un = unit(k);
-          for (int j = 0; ok && j < un.nkv; ++j) {
-            // every tile is waited for and released, so that this warp stays
-            // within one phase of each slot's barriers
-            const int k0 = un.key_tile(j) * BN;
-            const uint32_t v = vc + j, vs = v % C::VST;
-            ok = mbar_poll_warp(BAR_VF(vs), (v / C::VST) & 1, abort_p);
-            if (!ok) break;
-            if (!un.fix(prm.win, k0)) {
-              if (lane == 0) mbar_arrive(BAR_VE(vs));
-              continue;
-            }
-            // rows [a, b) are contiguous in each 64-column block (the swizzle
-            // permutes the chunks of a row within its 128 bytes)
-            auto zero = [&](int a, int b) {
-              for (int kb = 0; kb < C::KB; ++kb) {
-                uint4* blk = reinterpret_cast<uint4*>(gbase + C::OFF_V + vs * C::KV_BYTES + kb * BN * 128);
-                for (int i = a * 8 + lane; i < b * 8; i += 32) blk[i] = make_uint4(0u, 0u, 0u, 0u);
-              }
-            };
-            int a, b;
-            if (un.past_end(prm.win, k0, &a)) zero(a, BN);
-            if (un.out_of_window(prm.win, k0, &a, &b)) zero(a, b);
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) {
-              mbar_arrive(BAR_VZ(vs));
-              mbar_arrive(BAR_VE(vs));
-            }
+      uint32_t vc = 0;
+      bool ok = true;
+      for (int g = 0; ok; ++g) {
+        const int k = sched_unit<true>(sch, g);
+        if (k < 0) break;
+        const auto un = unit(k);
+        for (int j = 0; ok && j < un.nkv; ++j) {
+          // every tile is waited for and released, so that this warp stays
+          // within one phase of each slot's barriers
+          const int k0 = un.key_tile(j) * BN;
+          const uint32_t v = vc + j, vs = v % C::VST;
+          ok = mbar_poll_warp(BAR_VF(vs), (v / C::VST) & 1, abort_p);
+          if (!ok) break;
+          if (!un.fix(prm.win, k0)) {
+            if (lane == 0) mbar_arrive(BAR_VE(vs));
+            continue;
           }
-          vc += un.nkv;
+          // rows [a, b) are contiguous in each 64-column block (the swizzle
+          // permutes the chunks of a row within its 128 bytes)
+          auto zero = [&](int a, int b) {
+            for (int kb = 0; kb < C::KB; ++kb) {
+              uint4* blk = reinterpret_cast<uint4*>(gbase + C::OFF_V + vs * C::KV_BYTES + kb * BN * 128);
+              for (int i = a * 8 + lane; i < b * 8; i += 32) blk[i] = make_uint4(0u, 0u, 0u, 0u);
+            }
+          };
+          int a, b;
+          if (un.past_end(prm.win, k0, &a)) zero(a, BN);
+          if (un.out_of_window(prm.win, k0, &a, &b)) zero(a, b);
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(BAR_VZ(vs));
+            mbar_arrive(BAR_VE(vs));
+          }
         }
+        vc += un.nkv;
       }
     }
   } else {
@@ -531,9 +527,10 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         if (store && grow < prm.T) prm.lse[((long long)un.b * prm.T + grow) * prm.NH + un.h] = -INFINITY;
       } else {
         float m_used = -INFINITY, l_sum = 0.0f;
-        // one key tile; DIAG: the diagonal tile (keys after the query masked).
-        // Instantiated twice so that the other tiles carry no masking code.
-        // NC: the tile's first columns that matter (all 128, or a sink tile's 32).
+        // one key tile; DIAG: some key of it is hidden from some row (past the
+        // diagonal, out of the window, not a sink).  NC: the tile's first columns that
+        // matter (all 128, or a sink tile's 32).  Three instances, so that the tiles
+        // which every row sees whole carry no masking code.
         auto tile = [&](auto diag_tag, auto nc_tag, int j) -> bool {
           constexpr bool DIAG = decltype(diag_tag)::value;
           constexpr int NC = decltype(nc_tag)::value;
@@ -562,21 +559,19 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
           }
           tc_fence_before();
           mbar_arrive(BAR_SE(x));
-          {
-            if constexpr (DIAG) {
-              // key k0 + i is visible up to the row's own position, and from its
-              // window's first key on or among the sinks; 32 keys to a word of
-              // bits, one test and one select a key
-              const int k0 = un.key_tile(j) * BN;
-              const int t = prm.win.pos(un.b, qtile * BM + row);
-              const int up = t - k0, from = t - prm.win.window + 1 - k0, sink = prm.win.sinks - k0;
+          if constexpr (DIAG) {
+            // key k0 + i is visible up to the row's own position, and from its
+            // window's first key on or among the sinks; 32 keys to a word of
+            // bits, one test and one select a key
+            const int k0 = un.key_tile(j) * BN;
+            const int t = prm.win.pos(un.b, qtile * BM + row);
+            const int up = t - k0, from = t - prm.win.window + 1 - k0, sink = prm.win.sinks - k0;
 #pragma unroll
-              for (int w = 0; w < NC; w += 32) {
-                const uint32_t see = bits_below(up + 1 - w) & (~bits_below(from - w) | bits_below(sink - w));
+            for (int w = 0; w < NC; w += 32) {
+              const uint32_t see = bits_below(up + 1 - w) & (~bits_below(from - w) | bits_below(sink - w));
 #pragma unroll
-                for (int i = 0; i < 32; ++i)
-                  if (!(see & (1u << i))) s[w + i] = -INFINITY;
-              }
+              for (int i = 0; i < 32; ++i)
+                if (!(see & (1u << i))) s[w + i] = -INFINITY;
             }
           }
           // row maximum: 8 independent partial maxima, 3-input max (short chains)
@@ -717,18 +712,16 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
             tmem_ld32(trow + tcol_o + c64, ra);
             tmem_ld32(trow + tcol_o + c64 + 32, rb);
             tmem_wait_ld_dep(ra, rb);
-            {
-              if (joined) {
-                uint32_t rc[32], rd[32];
-                tmem_ld32(trow + C::TCOL_O + HD + c64, rc);
-                tmem_ld32(trow + C::TCOL_O + HD + c64 + 32, rd);
-                tmem_wait_ld_dep(rc, rd);
-                auto join = [&](uint32_t a, uint32_t b) {
-                  return __float_as_uint(__uint_as_float(a) * fa + __uint_as_float(b) * fb);
-                };
+            if (joined) {
+              uint32_t rc[32], rd[32];
+              tmem_ld32(trow + C::TCOL_O + HD + c64, rc);
+              tmem_ld32(trow + C::TCOL_O + HD + c64 + 32, rd);
+              tmem_wait_ld_dep(rc, rd);
+              auto join = [&](uint32_t a, uint32_t b) {
+                return __float_as_uint(__uint_as_float(a) * fa + __uint_as_float(b) * fb);
+              };
 #pragma unroll
-                for (int i = 0; i < 32; ++i) ra[i] = join(ra[i], rc[i]), rb[i] = join(rb[i], rd[i]);
-              }
+              for (int i = 0; i < 32; ++i) ra[i] = join(ra[i], rc[i]), rb[i] = join(rb[i], rd[i]);
             }
 #pragma unroll
             for (int c16 = 0; c16 < 64; c16 += 16) {
