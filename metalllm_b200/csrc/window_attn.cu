@@ -18,7 +18,7 @@
 // end.  Few rows on a long axis leave most SMs idle, so the blocks are split
 // over CTAs until the GPU is full, and a second kernel joins the splits'
 // (m, l, O) in a fixed order.  Measured: 64 requests, 32 / 8 heads of 128, window
-// 4096: 165 us, 6.5 TB/s; one request over 131072 keys: 92 us, 83 of them the
+// 4096: 166 us, 6.5 TB/s; one request over 131072 keys: 93 us, 83 of them the
 // splits at 6.5 TB/s.
 //
 // Cache rows that no query sees may hold anything: their scores are replaced

@@ -12,7 +12,7 @@
 // past the end or out of the window): P is 0 there, but 0 * NaN is not.  Warp 1
 // issues S and warp 3 PV.  SINGLE: a unit is one query tile, not a pair, and the
 // two softmax warpgroups share its key tiles (few units, long windows).
-// Measured: 8192 tokens, 32 / 8 heads of 128, window 1024, 16 sinks 198 us, 660
+// Measured: 8192 tokens, 32 / 8 heads of 128, window 1024, 16 sinks 200 us, 653
 // TFLOP/s, bound like the causal form by the chain of a tile's scores,
 // exponentials and product; 500 tokens over a cache, 16 heads of 64, window 2048
 // 26 us (SINGLE; in pairs 33).
