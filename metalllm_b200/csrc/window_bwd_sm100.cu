@@ -25,7 +25,7 @@
 // a step where these spend 4 + 3, but it had to zero dQ, add 64 KB a step into
 // L2 and convert the sums: at B=2, 4096 tokens, 16 / 4 heads of 128, window 1000
 // it took 384 us, at up to 64 x 1024, 12 heads of 64, window 250 605 us; these
-// passes take 272 (571 TFLOP/s; the tensor pipe is busy 55 % of the time) and 420
+// passes take 272 (571 TFLOP/s; the tensor pipe is busy 56 % of the time) and 420
 // (units of three steps).  The chain from a step's scores over the row math to
 // its products bounds them, at D=64 the row math's instructions.)
 //
